@@ -109,6 +109,7 @@ def main(argv=None):
     ap.add_argument("--impl", default="dfccl", choices=["dfccl", "nccl"])
     ap.add_argument("--optimizer", default="sgd", choices=["sgd", "adamw"], help="fused optimizer of this library's arm")
     ap.add_argument("--graph", type=int, default=0, help="capture forward + backward of the whole step in one CUDA graph")
+    ap.add_argument("--fused-ends", type=int, default=0, help="embedding and head loss on this library's kernels (its arm only)")
     ap.add_argument("--out", default="")
     a = ap.parse_args(argv)
     faulthandler.dump_traceback_later(int(os.environ.get("BENCH_WATCHDOG_S", "600")), exit=True)
@@ -120,7 +121,7 @@ def main(argv=None):
     cfg = GPT2Config.medium() if a.model == "medium" else GPT2Config.tiny()
     mesh = build_mesh(d, a.tp, a.pp, a.dp)
     mesh.tp_group.library = "dfccl" if a.impl == "dfccl" else "torch"
-    stage = GPT2Stage(cfg, mesh.tp_group, mesh.pp_rank, a.pp, a.micro_batch)
+    stage = GPT2Stage(cfg, mesh.tp_group, mesh.pp_rank, a.pp, a.micro_batch, fused_ends=bool(a.fused_ends) and a.impl == "dfccl")
     tr = HybridTrainer(d, mesh, stage, n_micro=a.n_micro, lr=0.01 if a.optimizer == "sgd" else 3e-4, seed=5, use_graph=bool(a.graph), optimizer=a.optimizer)
     if a.impl == "nccl":
         tr.ddp.close()
@@ -212,6 +213,7 @@ def main(argv=None):
                "model_tflops_per_gpu": flops / (ms / 1e3) / 1e12 / w,
                "config": {"model": f"GPT-2 {a.model}", "parallelism": f"tp{a.tp} x pp{a.pp} x dp{a.dp}", "micro_batch": a.micro_batch,
                           "n_micro": a.n_micro, "global_batch": a.dp * a.n_micro * a.micro_batch, "seq_len": cfg.seq_len, "cuda_graph": bool(a.graph),
+                          "fused_ends": stage.fused_ends,
                           "schedule": "1F1B, receives posted one micro-batch ahead" if tr.schedule == "1f1b" else "GPipe",
                           "pipeline_link_ctas": hyb.PP_CTAS, "optimizer": "SGD momentum 0.9, fp32 master weights" if a.impl == "dfccl" else "SGD momentum 0.9 (bf16)"},
                "clocks": clk.summary(),

@@ -56,6 +56,11 @@ ncclResult_t gemmMakeMap(CUtensorMap* m, const void* base, uint64_t rows, uint64
 // The same for whole operands of a stage in one load: a K-major matrix [rows, k] as (64, rows, k / 64) with boxes of
 // 64 x boxRows x boxK / 64, an MN-major one ([k, rows] as stored) as (64, k, rows / 64) with boxes of 64 x boxK x boxRows / 64.
 ncclResult_t gemmMakeMap3(CUtensorMap* m, const void* base, uint64_t rows, uint64_t k, int mnMajor, uint32_t boxRows, uint32_t boxK);
+// The same two, made anew for every call: for operands that lie elsewhere each time.
+ncclResult_t gemmEncodeMap(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, uint32_t boxRows);
+ncclResult_t gemmEncodeMap3(CUtensorMap* m, const void* base, uint64_t rows, uint64_t k, int mnMajor, uint32_t boxRows, uint32_t boxK);
+// The current device's error word and its mirror in pinned host memory; dfcclTimeout where a kernel has given up on a bounded wait.
+ncclResult_t gemmErrorWords(uint32_t** dev, uint32_t** host);
 // True when a kernel of the current device gave up on a bounded wait (pinned word, no device access).
 bool gemmGaveUp();
 // SMs the fused launches leave to a co-resident persistent kernel: raised to at least `n`.

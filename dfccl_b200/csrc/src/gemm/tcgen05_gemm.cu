@@ -538,8 +538,23 @@ ncclResult_t launch(const void* A, const void* B, void* C, int M, int N, int K, 
 }  // namespace
 
 ncclResult_t gemmMakeMap(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, uint32_t boxRows, uint32_t boxCols) { return makeMap(m, base, rows, cols, boxRows, boxCols); }
+static MapKey map3Key(const void* base, uint64_t rows, uint64_t k, int mnMajor, uint32_t boxRows, uint32_t boxK) {
+  return mnMajor ? MapKey{base, k, rows / 64, rows * 2, 64, 64, boxK, boxRows / 64} : MapKey{base, rows, k / 64, k * 2, 64, 64, boxRows, boxK / 64};
+}
 ncclResult_t gemmMakeMap3(CUtensorMap* m, const void* base, uint64_t rows, uint64_t k, int mnMajor, uint32_t boxRows, uint32_t boxK) {
-  return cachedMap(m, mnMajor ? MapKey{base, k, rows / 64, rows * 2, 64, 64, boxK, boxRows / 64} : MapKey{base, rows, k / 64, k * 2, 64, 64, boxRows, boxK / 64});
+  return cachedMap(m, map3Key(base, rows, k, mnMajor, boxRows, boxK));
+}
+ncclResult_t gemmEncodeMap(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, uint32_t boxRows) {
+  return encodeMap(m, MapKey{base, rows, 0, cols * 2, (uint32_t)cols, BK, boxRows, 0});
+}
+ncclResult_t gemmEncodeMap3(CUtensorMap* m, const void* base, uint64_t rows, uint64_t k, int mnMajor, uint32_t boxRows, uint32_t boxK) {
+  return encodeMap(m, map3Key(base, rows, k, mnMajor, boxRows, boxK));
+}
+ncclResult_t gemmErrorWords(uint32_t** dev, uint32_t** host) {
+  const ErrWords ew = errWords();
+  if (*ew.host) { DF_WARN("an earlier tensor-core kernel on this device gave up on a bounded wait; call dfcclGemmCheck to clear"); return dfcclTimeout; }
+  *dev = ew.dev; *host = (uint32_t*)ew.host;
+  return ncclSuccess;
 }
 ncclResult_t gemmLaunch(const void* A, const void* B, void* C, int M, int N, int K, const FusedArgs* f, cudaStream_t stream, int aMn, int bMn) {
   return launch(A, B, C, M, N, K, f, stream, aMn, bMn);

@@ -1,0 +1,472 @@
+// Products over a large vocabulary for the losses of a language model's head, on CTA pairs (tcgen05 cta_group::2), bf16 with fp32
+// accumulators in tensor memory.  With z = x w^T, x [n, d] and the head w [v, d]:
+//   VOCAB_STATS     of every row the maximum and the sum of powers of each stretch of its logits, and the logits of its targets
+//   VOCAB_GRAD      dz = coef (softmax(z) - target): the logits are computed again, what is stored is their gradient, rounded once
+//   VOCAB_PRODUCTS  dx = dz w and dw = dz^T x, in one launch
+// A logit exists in tensor memory and registers only.  Computing the product again costs a third more than the two products
+// of the gradients do by themselves; keeping n v logits or powers of them would cost their rounding twice (1.7 times the error of one
+// rounding in dw) and n v 2 bytes between forward and backward.
+//
+// Tiles of 256 x 256, stages of 64 of the contraction, roles as in tcgen05_gemm_pair.cu (TMA producer, MMA issuer, eight epilogue warps,
+// two accumulators).  All of n, v are any number, d a multiple of 8: the tensor maps give zeros outside, the epilogues store inside.
+#include "tc_common.h"
+#include "gemm.h"
+#include "epilogue.h"
+#include "vocab.h"
+#include "../common/device_once.h"
+#include "../common/log.h"
+#include <algorithm>
+
+namespace dfccl {
+namespace {
+
+using namespace tc;
+
+constexpr int T = VOCAB_TILE, HALF = 128, BK = 64, UMMA_K = 16, STAGES = 6;
+constexpr int A_BYTES = HALF * BK * 2, STAGE_BYTES = 2 * A_BYTES;                 // per CTA: 128 rows of A, 128 of B
+constexpr int SMEM_BYTES = 227 * 1024;                                            // all of it: tensor memory for one CTA at a time (tcgen05_gemm_pair.cu)
+constexpr int EPI_WARPS = 4 * VOCAB_PARTS, THREADS = 64 + 32 * EPI_WARPS;
+constexpr uint64_t WAIT_NS = 4000000000ull;                                       // nothing here waits on another GPU
+static_assert(STAGES * STAGE_BYTES + 1024 + 256 <= SMEM_BYTES, "stages");
+
+enum VocabMode { VOCAB_STATS, VOCAB_GRAD, VOCAB_PRODUCTS };
+
+// One product: result [M, N], `kBlocks` blocks of 64 of the contraction cut into slices of `perSlice`.
+struct Product {
+  int M, N, mTiles, nTiles, kBlocks, slices, perSlice, items, groupM;
+  int aMn, bMn, bLoose;             // operand stored with the contraction index slow; loose: its blocks of 64 columns are loaded one by one
+  __nv_bfloat16* out;               // direct results, ld N
+  float* part;                      // or slices [slice][M][N]
+  int add, wide;
+};
+struct VocabArgs {
+  Product p[2];                     // items of the first, then of the second (items = 0: none)
+  int headStart;                    // rounds of the second product's items that pairs with one item less of the first take alone
+  VocabRows rows;
+  float2* parts;
+  float* picked;
+  VocabGrad grad;
+  __nv_bfloat16* dz;
+  int ld, first;                    // of dz; first column of the vocabulary
+  uint32_t* err;
+  uint32_t* errHost;
+};
+
+// The items of a pair.  Those of the first product go round; pairs that get one less of them (their time is several items' of the
+// second) start on the second product while the others finish, then its items go round too.  What a pair gets is a matter of time, not of results.
+struct Items {
+  int pair, pairs, r, k0, t1, t2, n1, n2, early;
+  __device__ Items(const VocabArgs& g, int pair_, int pairs_) : pair(pair_), pairs(pairs_) {
+    t1 = g.p[0].items; t2 = g.p[1].items;
+    r = t1 % pairs;
+    early = r && pair >= r ? 1 : 0;
+    k0 = r ? g.headStart : 0;
+    n1 = t1 > pair ? (t1 - pair + pairs - 1) / pairs : 0;
+    const int e = pairs - r, alone = k0 * e;
+    n2 = t2 - alone > pair ? (t2 - alone - pair + pairs - 1) / pairs : 0;
+    if (early) n2 += min(k0, t2 > pair - r ? (t2 - (pair - r) + e - 1) / e : 0);
+  }
+  __device__ int count() const { return n1 + n2; }
+  // Which product, and its item.
+  __device__ int at(int j, int& item) const {
+    if (j < n1) { item = pair + j * pairs; return 0; }
+    j -= n1;
+    const int e = pairs - r;
+    if (!early) item = k0 * e + pair + j * pairs;
+    else item = j < k0 ? j * e + pair - r : k0 * e + pair + (j - k0) * pairs;
+    return 1;
+  }
+};
+
+struct Tile { int mt, nt, slice, k0, k1; };
+__device__ __forceinline__ Tile tileOf(const Product& p, int item) {
+  Tile t;
+  const int tiles = p.mTiles * p.nTiles;
+  t.slice = item / tiles;
+  raster_tile(item - t.slice * tiles, p.mTiles, p.nTiles, p.groupM, t.mt, t.nt);
+  t.k0 = t.slice * p.perSlice;
+  t.k1 = min(p.kBlocks, t.k0 + p.perSlice);
+  return t;
+}
+
+// A row's list from the first entry at or behind a column on.
+struct List {
+  const int* tokens;
+  int k, pos, next;
+  __device__ __forceinline__ void seek(const int* t, int n, int col) {
+    tokens = t; k = n;
+    int lo = 0, hi = n;
+    while (lo < hi) { const int mid = (lo + hi) >> 1; if (tokens[mid] < col) lo = mid + 1; else hi = mid; }
+    pos = lo;
+    next = lo < k ? tokens[lo] : VOCAB_NO_TOKEN;
+  }
+  __device__ __forceinline__ void step() { ++pos; next = pos < k ? tokens[pos] : VOCAB_NO_TOKEN; }
+};
+
+template <int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtensorMap mapB0, const __grid_constant__ CUtensorMap mapA1,
+                 const __grid_constant__ CUtensorMap mapB1, const __grid_constant__ VocabArgs g) {
+  extern __shared__ uint8_t smemRaw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smemRaw + 1023) & ~(uintptr_t)1023);       // the same offset in both CTAs
+  uint64_t* fullBar = (uint64_t*)(smem + STAGES * STAGE_BYTES);      // used in the leader only
+  uint64_t* emptyBar = fullBar + STAGES;                             // in both CTAs (commit to both)
+  uint64_t* accFull = emptyBar + STAGES;                             // [2] in both CTAs
+  uint64_t* accEmpty = accFull + 2;                                  // [2] used in the leader only
+  uint32_t* tmemBaseSlot = (uint32_t*)(accEmpty + 2);
+  volatile uint32_t* giveUp = tmemBaseSlot + 1;
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t cr = cluster_ctarank();             // 0 = leader
+  const Items items(g, blockIdx.x >> 1, gridDim.x >> 1);
+  const int count = items.count();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&fullBar[s], 1); mbar_init(&emptyBar[s], 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(&accFull[a], 1); mbar_init(&accEmpty[a], 2 * EPI_WARPS); }
+    *giveUp = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&mapA0);
+    tma_prefetch_desc(&mapB0);
+  }
+  if (warp == 1) tmem_alloc_pair(tmemBaseSlot, 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                                // the partner's barriers exist before anything arrives on them
+  tc_fence_after();
+  const uint32_t tmemBase = *tmemBaseSlot;
+  grid_dependency_wait();
+  grid_launch_dependents();
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer (both CTAs; bytes counted in the leader)
+    if (elect_one()) {
+      const uint32_t bar0 = mapa_u32(smem_u32(fullBar), 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int j = 0; j < count && ok; ++j) {
+        int item;
+        const int which = MODE == VOCAB_PRODUCTS ? items.at(j, item) : (items.at(j, item), 0);
+        const Product& p = g.p[which];
+        const CUtensorMap* ma = which ? &mapA1 : &mapA0;
+        const CUtensorMap* mb = which ? &mapB1 : &mapB0;
+        const Tile t = tileOf(p, item);
+        const int rowA = t.mt * T + (int)cr * HALF, rowB = t.nt * T + (int)cr * HALF;
+        for (int k = t.k0; k < t.k1; ++k) {
+          if (!mbar_wait(&emptyBar[stage], phase ^ 1, giveUp, WAIT_NS)) { ok = false; break; }
+          if (cr == 0) mbar_expect_tx(&fullBar[stage], 2 * STAGE_BYTES);      // my bytes and the partner's
+          uint8_t* sa = smem + stage * STAGE_BYTES;
+          uint8_t* sb = sa + A_BYTES;
+          const uint32_t bar = bar0 + stage * 8;
+          // K-major: a box of 64 of the contraction x 128 rows.  MN-major: two blocks of 64 columns x 64 of the contraction,
+          // in one load where the matrix is cut into whole blocks.
+          if (MODE == VOCAB_PRODUCTS && p.aMn) tma_load_3d_pair(sa, ma, k * BK, rowA / 64, bar);
+          else tma_load_2d_pair(sa, ma, k * BK, rowA, bar);
+          if (MODE != VOCAB_PRODUCTS) tma_load_2d_pair(sb, mb, k * BK, rowB, bar);
+          else if (!p.bLoose) tma_load_3d_pair(sb, mb, k * BK, rowB / 64, bar);
+          else {
+            tma_load_2d_pair(sb, mb, rowB, k * BK, bar);
+            tma_load_2d_pair(sb + 64 * BK * 2, mb, rowB + 64, k * BK, bar);
+          }
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok) for (int i = 0; i < 20000; ++i) __nanosleep(200);     // copies already issued land before the CTA goes away
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (leader only)
+    if (cr == 0 && elect_one()) {
+      int stage = 0, blocks = 0;
+      uint32_t phase = 0;
+      for (int j = 0; j < count; ++j) {                // stages that are loaded again need their release
+        int item;
+        const Product& p = g.p[items.at(j, item)];
+        const Tile t = tileOf(p, item);
+        blocks += t.k1 - t.k0;
+      }
+      int loads = blocks - STAGES;
+      bool ok = true;
+      for (int j = 0; j < count && ok; ++j) {
+        int item;
+        const int which = MODE == VOCAB_PRODUCTS ? items.at(j, item) : (items.at(j, item), 0);
+        const Product& p = g.p[which];
+        const Tile t = tileOf(p, item);
+        const bool aMn = MODE == VOCAB_PRODUCTS && p.aMn, bMn = MODE == VOCAB_PRODUCTS && p.bMn;
+        const uint32_t idesc = umma_idesc_bf16(T, T, aMn, bMn);
+        // per instruction (16 of the contraction): 32 bytes along a K-major row, two groups of 8 rows of an MN-major block
+        const uint32_t stepA = aMn ? 128u : 2u, stepB = bMn ? 128u : 2u;
+        const int ab = j & 1;
+        if (!mbar_wait(&accEmpty[ab], ((j >> 1) & 1) ^ 1, giveUp, WAIT_NS)) break;
+        tc_fence_after();
+        const uint32_t d = tmemBase + ab * T;
+        for (int k = t.k0; k < t.k1; ++k) {
+          if (!mbar_wait(&fullBar[stage], phase, giveUp, WAIT_NS)) { ok = false; break; }
+          tc_fence_after();
+          const uint8_t* pa = smem + stage * STAGE_BYTES;
+          const uint64_t da = aMn ? umma_smem_desc_mn_sw128(pa, 64 * BK * 2) : umma_smem_desc_sw128(pa);
+          const uint64_t db = bMn ? umma_smem_desc_mn_sw128(pa + A_BYTES, 64 * BK * 2) : umma_smem_desc_sw128(pa + A_BYTES);
+#pragma unroll
+          for (int i = 0; i < BK / UMMA_K; ++i) umma_bf16_pair(d, da + stepA * i, db + stepB * i, idesc, k != t.k0 || i != 0);
+          if (loads-- > 0) umma_commit_pair(&emptyBar[stage]);      // both CTAs' stage is free once these MMAs have read it
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (ok) umma_commit_pair(&accFull[ab]);       // both halves of the accumulator complete
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue: a row of my 128 per lane, 32 columns at a time
+    const int quarter = warp & 3, part = (warp - 2) >> 2;
+    const uint32_t accEmptyLeader0 = mapa_u32(smem_u32(&accEmpty[0]), 0), accEmptyLeader1 = mapa_u32(smem_u32(&accEmpty[1]), 0);
+    for (int j = 0; j < count; ++j) {
+      int item;
+      const int which = MODE == VOCAB_PRODUCTS ? items.at(j, item) : (items.at(j, item), 0);
+      const Product& p = g.p[which];
+      const Tile t = tileOf(p, item);
+      const int ab = j & 1;
+      const int row0 = t.mt * T + (int)cr * HALF + quarter * 32, row = row0 + lane, col0 = t.nt * T;
+      const bool mine = row0 < p.M, here = row < p.M;
+      const uint32_t acc = tmemBase + ((uint32_t)(quarter * 32) << 16) + ab * T;
+      uint32_t r[32];
+
+      if (MODE != VOCAB_PRODUCTS) {
+        List list;
+        list.pos = list.k = 0; list.next = VOCAB_NO_TOKEN; list.tokens = nullptr;
+        const float scale = g.rows.scale;
+        float lse = 0.f, coef = 0.f;
+        if (here) {                                    // on its way while the accumulator is computed
+          if (MODE == VOCAB_GRAD) {
+            const int state = g.grad.state[row];
+            lse = g.grad.lse[row];
+            coef = g.grad.gout[(size_t)row * g.grad.goutStride] * g.grad.temperature;
+            if (g.grad.count) coef = coef / (float)max(1, *g.grad.count);
+            if (state != 1) coef = state ? __int_as_float(0x7fffffff) : 0.f;
+          }
+          list.seek(g.rows.tokens + (size_t)row * g.rows.k, g.rows.k, g.first + col0);
+        }
+        if (!mbar_wait(&accFull[ab], (j >> 1) & 1, giveUp, WAIT_NS)) break;
+        tc_fence_after();
+        float top = -INFINITY, sum = 0.f;
+        const int cols = MODE == VOCAB_GRAD ? g.ld : p.N, steps = (min(T, cols - col0) + 31) / 32;
+#pragma unroll 1
+        for (int i = part; i < steps; i += VOCAB_PARTS) {
+          if (!mine) break;
+          const int c = col0 + i * 32;
+          __syncwarp();
+          tmem_ld32(acc + i * 32, r);
+          tmem_ld_wait();
+          if (MODE == VOCAB_STATS) {
+            if (c + 32 > p.N) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) if (c + e >= p.N) r[e] = 0xff800000u;          // -inf
+            }
+            while (list.next < c + 32) {
+              if (list.next >= c) {
+                const int at = list.next - c;
+                float z = 0.f;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) if (e == at) z = __uint_as_float(r[e]);
+                g.picked[(size_t)row * g.rows.k + list.pos] = z;
+              }
+              list.step();
+            }
+            // running maximum and sum over the row's columns
+            float m0 = __uint_as_float(r[0]), m1 = __uint_as_float(r[1]);
+#pragma unroll
+            for (int e = 2; e < 32; e += 2) { m0 = fmaxf(m0, __uint_as_float(r[e])); m1 = fmaxf(m1, __uint_as_float(r[e + 1])); }
+            const float now = fmaxf(top, fmaxf(m0, m1) * scale), base = now == -INFINITY ? 0.f : now;
+            float s[4] = {sum * exp2Approx(top - base), 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 32; ++e) s[e & 3] += exp2Approx(fmaf(__uint_as_float(r[e]), scale, -base));
+            sum = (s[0] + s[1]) + (s[2] + s[3]);
+            top = now;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(exp2Approx(fmaf(__uint_as_float(r[e]), scale, -lse)));
+            while (list.next < g.first + c + 32) {
+              if (list.next >= g.first + c) {
+                const int at = list.next - g.first - c;
+                const float q = g.rows.weights ? g.rows.weights[(size_t)row * g.rows.k + list.pos] : 1.f;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) if (e == at) r[e] = __float_as_uint(__uint_as_float(r[e]) - q);
+              }
+              list.step();
+            }
+            if (c + 32 > p.N) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) if (c + e >= p.N) r[e] = 0u;
+            }
+            // (a row without a gradient may hold anything, infinities and NaN among it)
+            if (here) {
+              uint4 o[4];
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                uint32_t* ow = (uint32_t*)&o[v];
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                  const float lo = __uint_as_float(r[8 * v + 2 * w]) * coef, hi = __uint_as_float(r[8 * v + 2 * w + 1]) * coef;
+                  ow[w] = coef == 0.f ? 0u : pack_bf16x2(lo, hi);
+                }
+              }
+              __nv_bfloat16* dst = g.dz + (size_t)row * g.ld + c;
+              st_global32(dst, o, true);
+              st_global32(dst + 16, o + 2, true);
+            }
+          }
+        }
+        if (MODE == VOCAB_STATS && here) g.parts[(size_t)(t.nt * VOCAB_PARTS + part) * p.M + row] = make_float2(top, sum);
+      } else {
+        if (!mbar_wait(&accFull[ab], (j >> 1) & 1, giveUp, WAIT_NS)) break;
+        tc_fence_after();
+        const int steps = (min(T, p.N - col0) + 31) / 32;
+#pragma unroll 1
+        for (int i = part; i < steps; i += VOCAB_PARTS) {
+          if (!mine) break;
+          const int c = col0 + i * 32, packs = min(4, (p.N - c) / 8);
+          __syncwarp();
+          tmem_ld32(acc + i * 32, r);
+          tmem_ld_wait();
+          if (!here) continue;
+          if (p.part) {
+            float4* dst = (float4*)(p.part + ((size_t)t.slice * p.M + row) * p.N + c);
+#pragma unroll
+            for (int v = 0; v < 8; ++v) {
+              if (v / 2 >= packs) break;
+              float4 o = make_float4(__uint_as_float(r[4 * v]), __uint_as_float(r[4 * v + 1]), __uint_as_float(r[4 * v + 2]), __uint_as_float(r[4 * v + 3]));
+              if (p.add) { const float4 q = dst[v]; o.x += q.x; o.y += q.y; o.z += q.z; o.w += q.w; }
+              dst[v] = o;
+            }
+          } else {
+            uint4 o[4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              uint32_t* ow = (uint32_t*)&o[v];
+#pragma unroll
+              for (int w = 0; w < 4; ++w) ow[w] = pack_bf16x2(__uint_as_float(r[8 * v + 2 * w]), __uint_as_float(r[8 * v + 2 * w + 1]));
+            }
+            __nv_bfloat16* dst = p.out + (size_t)row * p.N + c;
+            if (packs == 4) { st_global32(dst, o, p.wide); st_global32(dst + 16, o + 2, p.wide); }
+            else {
+#pragma unroll
+              for (int v = 0; v < 4; ++v) if (v < packs) ((uint4*)dst)[v] = o[v];
+            }
+          }
+        }
+      }
+      if (j + 2 < count) {                             // released to the item after the next: every arrival is waited for
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(ab ? accEmptyLeader1 : accEmptyLeader0);
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------- leave: nothing of the pair may still use my shared or tensor memory
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_relaxed();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc_pair(tmemBase, 512);
+  if (threadIdx.x == 0 && *giveUp) { atomicExch(g.err, 1u); *(volatile uint32_t*)g.errHost = 1u; __threadfence_system(); }
+}
+
+template <int MODE>
+ncclResult_t launchVocab(const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1, const CUtensorMap& b1, VocabArgs& g, cudaStream_t stream) {
+  CUDACHECK(oncePerDevice([] { return allowSharedMemory(dfcclVocabKernel<MODE>, SMEM_BYTES); }));
+  DFCHECK(gemmErrorWords(&g.err, &g.errHost));
+  cudaLaunchConfig_t cfg = {};
+  const int pairs = std::min(g.p[0].items + g.p[1].items, gemmPairResident());
+  cfg.gridDim = dim3(2 * pairs); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM_BYTES; cfg.stream = stream;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization; at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at; cfg.numAttrs = 1;
+  // the head start of pairs with one item less of the first product: as many items of the second as that one takes
+  const int64_t c1 = g.p[0].items ? g.p[0].perSlice : 0, c2 = g.p[1].items ? std::max(1, g.p[1].perSlice) : 1;
+  g.headStart = g.p[1].items ? (int)((c1 + c2 / 2) / c2) : 0;
+  CUDACHECK(cudaLaunchKernelEx(&cfg, dfcclVocabKernel<MODE>, a0, b0, a1, b1, g));
+  return ncclSuccess;
+}
+
+Product productOf(int M, int N, int K, int per) {
+  Product p = {};
+  p.M = M; p.N = N; p.mTiles = (M + T - 1) / T; p.nTiles = (N + T - 1) / T;
+  p.kBlocks = (K + BK - 1) / BK;
+  p.perSlice = per;
+  p.slices = vocabSlices(K, per);
+  p.items = p.mTiles * p.nTiles * p.slices;
+  p.groupM = 8;
+  return p;
+}
+
+// The tiles of z: x and w both K-major.
+ncclResult_t logits(CUtensorMap* a, CUtensorMap* b, VocabArgs* g, const void* x, const void* w, int n, int v, int d, const VocabRows& rows) {
+  *g = VocabArgs{};
+  DFCHECK(gemmEncodeMap(a, x, (uint64_t)n, (uint64_t)d, HALF));
+  DFCHECK(gemmEncodeMap(b, w, (uint64_t)v, (uint64_t)d, HALF));
+  g->p[0] = productOf(n, v, d, (d + BK - 1) / BK);
+  g->rows = rows;
+  return ncclSuccess;
+}
+
+}  // namespace
+
+ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, float* picked, cudaStream_t stream) {
+  CUtensorMap a, b;
+  VocabArgs g;
+  DFCHECK(logits(&a, &b, &g, x, w, n, v, d, rows));
+  g.parts = parts; g.picked = picked;
+  return launchVocab<VOCAB_STATS>(a, b, a, b, g, stream);
+}
+
+ncclResult_t vocabGrad(const void* x, const void* w, int n, int v, int first, int d, const VocabRows& rows, const VocabGrad& grad, void* dz, cudaStream_t stream) {
+  CUtensorMap a, b;
+  VocabArgs g;
+  DFCHECK(logits(&a, &b, &g, x, w, n, v, d, rows));
+  g.grad = grad; g.dz = (__nv_bfloat16*)dz; g.ld = (v + 63) / 64 * 64; g.first = first;
+  return launchVocab<VOCAB_GRAD>(a, b, a, b, g, stream);
+}
+
+// A product is cut into slices of its contraction where its tiles alone would keep pairs waiting: until the longest item is no more
+// than a pair's share of all the work.
+VocabPlan vocabProductPlan(int n, int v, int d, bool wantX, bool wantW, int pairs) {
+  const int64_t tn = (n + T - 1) / T, tv = (v + T - 1) / T, td = (d + T - 1) / T, kn = (n + BK - 1) / BK, kv = (v + BK - 1) / BK;
+  const int64_t all = (wantX ? tn * td * kv : 0) + (wantW ? tv * td * kn : 0), share = std::max<int64_t>(1, all / pairs);
+  // A slice costs its sums a way to memory and back: none is cut below 16 blocks.
+  auto cut = [&](int64_t tiles, int64_t k) -> int {
+    if (k <= share || tiles >= 4 * pairs) return (int)k;
+    const int64_t slices = std::max<int64_t>(1, std::min<int64_t>((k + share - 1) / share, k / 16));
+    return (int)((k + slices - 1) / slices);
+  };
+  return VocabPlan{cut(tn * td, kv), cut(tv * td, kn)};
+}
+
+ncclResult_t vocabProducts(const void* dz, const void* x, const void* w, int n, int v, int d, const VocabPlan& plan, void* dx, float* partX, bool addX,
+                           void* dw, float* partW, cudaStream_t stream) {
+  const int ld = (v + 63) / 64 * 64;
+  CUtensorMap a[2], b[2];
+  VocabArgs g = {};
+  int k = 0;
+  auto narrow = [&](CUtensorMap* m, const void* base, int rows) {      // [rows of the contraction][d columns]
+    return d % 64 ? gemmEncodeMap(m, base, (uint64_t)rows, (uint64_t)d, BK) : gemmEncodeMap3(m, base, (uint64_t)d, (uint64_t)rows, 1, HALF, BK);
+  };
+  if (dx || partX) {
+    DFCHECK(gemmEncodeMap(&a[k], dz, (uint64_t)n, (uint64_t)ld, HALF));
+    DFCHECK(narrow(&b[k], w, v));
+    Product& p = g.p[k++] = productOf(n, d, v, plan.perX);
+    p.bMn = 1; p.bLoose = d % 64 != 0;
+    p.out = (__nv_bfloat16*)dx; p.part = partX; p.add = addX;
+  }
+  if (dw || partW) {
+    DFCHECK(gemmEncodeMap3(&a[k], dz, (uint64_t)ld, (uint64_t)n, 1, HALF, BK));
+    DFCHECK(narrow(&b[k], x, n));
+    Product& p = g.p[k++] = productOf(v, d, n, plan.perW);
+    p.aMn = p.bMn = 1; p.bLoose = d % 64 != 0;
+    p.out = (__nv_bfloat16*)dw; p.part = partW;
+  }
+  if (!k) return ncclInvalidArgument;
+  for (int i = 0; i < k; ++i) g.p[i].wide = d % 16 == 0 && ((uintptr_t)g.p[i].out & 31) == 0;
+  if (k == 1) { a[1] = a[0]; b[1] = b[0]; }
+  return launchVocab<VOCAB_PRODUCTS>(a[0], b[0], a[1], b[1], g, stream);
+}
+
+}  // namespace dfccl

@@ -9,7 +9,9 @@ layer norms, residuals and dropouts never repeat work; a block's two GEMM pairs 
     all-gather -> GEMM (4d up)   ... GELU ...                           GEMM -> reduce-scatter (down)
 
 each pair member one fused tcgen05 kernel (``dfccl_b200.parallel.tp``).  Attention itself is the
-library kernel behind ``scaled_dot_product_attention``.
+library kernel behind ``scaled_dot_product_attention``.  With ``fused_ends`` the model's ends run on this package's kernels too:
+the embedding with its gradients by sorted tokens (``dfccl_b200.ops.embedding``) and the loss of the head without its logits
+(``dfccl_b200.ops.loss``).
 
 The reference ships no model code; its simulator only knows the communication group structure of
 such a job (reference: simulator/simulator.py:434-493, simulator/configs/megatron.json).
@@ -24,7 +26,9 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ..ops.block import norm_residual, unhooked
+from ..ops.embedding import embedding
 from ..ops.fused_linear import TpGroup
+from ..ops.loss import linear_cross_entropy, linear_loss_supported
 from ..parallel.tp import ColumnParallelLinear, RowParallelLinear, gelu_mlp
 
 
@@ -94,12 +98,13 @@ class ParallelBlock(nn.Module):
 
 class GPT2Stage(nn.Module):
     """Blocks ``[first_layer, first_layer + n_layers)`` of the model for micro-batches of
-    ``micro_batch`` sequences."""
+    ``micro_batch`` sequences.  ``fused_ends``: token and position embedding in one kernel, and the loss without the logits,
+    whose rounding to bf16 it leaves out (on GPUs; elsewhere the stage computes as without it)."""
 
-    def __init__(self, cfg: GPT2Config, tp: TpGroup, stage: int, n_stages: int, micro_batch: int, seed: int = 1234):
+    def __init__(self, cfg: GPT2Config, tp: TpGroup, stage: int, n_stages: int, micro_batch: int, seed: int = 1234, fused_ends: bool = False):
         super().__init__()
         assert cfg.n_layer % n_stages == 0
-        self.cfg, self.tp = cfg, tp
+        self.cfg, self.tp, self.fused_ends = cfg, tp, fused_ends
         self.is_first, self.is_last = stage == 0, stage == n_stages - 1
         self.tokens = micro_batch * cfg.seq_len
         self.rows = self.tokens // tp.n
@@ -130,12 +135,17 @@ class GPT2Stage(nn.Module):
         to the micro-batch's loss); the others return their hidden rows."""
         if self.is_first:
             ids = self.my_rows(x.reshape(-1))
-            h = self.wte(ids) + self.wpe(self.pos)
+            if self.fused_ends and ids.is_cuda and unhooked(self.wte, nn.Embedding) and unhooked(self.wpe, nn.Embedding):
+                h = embedding(ids, self.wte.weight, positions=self.pos, position_weight=self.wpe.weight)
+            else:
+                h = self.wte(ids) + self.wpe(self.pos)
         else:
             h = x
         for blk in self.blocks:
             h = blk(h)
         if not self.is_last:
             return h
-        logits = norm_residual(self.ln_f, h)[1] @ self.head.t()
-        return F.cross_entropy(logits.float(), self.my_rows(targets.reshape(-1)), reduction="sum") / self.tokens
+        y, mine = norm_residual(self.ln_f, h)[1], self.my_rows(targets.reshape(-1))
+        if self.fused_ends and linear_loss_supported(y, self.head):
+            return linear_cross_entropy(y, self.head, mine, reduction="sum") / self.tokens
+        return F.cross_entropy((y @ self.head.t()).float(), mine, reduction="sum") / self.tokens

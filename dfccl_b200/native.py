@@ -119,7 +119,7 @@ def lib() -> C.CDLL:
         elif not path.exists() or os.environ.get("DFCCL_REBUILD") == "1":
             path = _build.build()
         L = C.CDLL(str(path))       # local scope: the nccl* names must not shadow another collective library's
-        vp, i, sz = C.c_void_p, C.c_int, C.c_size_t
+        vp, i, sz, i64 = C.c_void_p, C.c_int, C.c_size_t, C.c_int64
         sig = {
             "ncclGetVersion": [C.POINTER(i)],
             "ncclGetUniqueId": [C.POINTER(UniqueId)],
@@ -175,6 +175,12 @@ def lib() -> C.CDLL:
             "dfcclColumnSum": [vp, vp, vp, i, i, vp], "dfcclColumnSumWork": [i, i],
             "dfcclLayerNormForward": [vp, vp, vp, vp, vp, vp, i, i, C.c_float, vp],
             "dfcclLayerNormBackward": [vp] * 10 + [i, i, vp], "dfcclLayerNormWork": [i, i], "dfcclLayerNormMaxWidth": [],
+            "dfcclEmbeddingForward": [vp, i, i, vp, i64, i64, vp, i, vp, i64, i64, vp, i, i, C.c_float, vp],
+            "dfcclEmbeddingBackward": [vp, i, i, i, vp, i, i64, C.c_float, vp, i64, vp, i, vp, i64, vp, vp], "dfcclEmbeddingBackwardWork": [i, i, i],
+            "dfcclTargetRows": [vp, i, i, i, i64, vp, vp, vp], "dfcclTeacherRows": [vp, i, vp, i, i, i, i, C.c_float, vp, vp, vp, vp],
+            "dfcclLinearLossForward": [vp, vp, i, i, i, vp, vp, vp, i, C.c_float, i, vp, vp, vp, vp, vp, vp], "dfcclLinearLossForwardWork": [i, i, i],
+            "dfcclLinearLossBackward": [vp, vp, i, i, i, vp, vp, vp, i, C.c_float, vp, vp, i, vp, vp, vp, vp, sz, vp],
+            "dfcclLinearLossBackwardWork": [i, i, i, i, i], "dfcclLinearLossMaxList": [],
             "dfcclGemmCheck": [C.POINTER(i)],
             "dfcclGemmPairResident": [C.POINTER(i)], "dfcclGemmPlan": [i, i, i, i, i, i, C.POINTER(i)],
             "dfcclGemmFused": [vp, vp, vp, i, i, i, vp, sz, vp],
@@ -201,6 +207,7 @@ def lib() -> C.CDLL:
         L.dfcclTunerPredictUs.restype = C.c_double
         L.dfcclTopoReset.restype = None
         L.dfcclLayerNormWork.restype = L.dfcclColumnSumWork.restype = sz
+        L.dfcclEmbeddingBackwardWork.restype = L.dfcclLinearLossForwardWork.restype = L.dfcclLinearLossBackwardWork.restype = sz
         L.dfcclParam.argtypes = [C.c_char_p, C.c_longlong]
         L.dfcclParam.restype = C.c_longlong
         L.dfcclLogReset.argtypes = []

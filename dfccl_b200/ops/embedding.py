@@ -1,0 +1,107 @@
+"""Embedding of tokens with the gradients of its tables by sorted tokens (``csrc/src/ops/embed.cu``)."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import native as nv
+from ..utils.tensors import nccl_dtype, on_device, raw_stream
+
+TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _index(name: str, t: torch.Tensor) -> None:
+    if t.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"{name} are int64 or int32, got {t.dtype}")
+
+
+def _table(name: str, t: torch.Tensor) -> None:
+    if t.dim() != 2 or t.shape[0] == 0 or t.shape[1] == 0:
+        raise ValueError(f"{name} is [rows, columns], got {tuple(t.shape)}")
+    if t.dtype not in TYPES:
+        raise ValueError(f"{name} is bf16, fp16 or fp32, got {t.dtype}")
+    if t.shape[0] > 2 ** 31 - 16:
+        raise ValueError(f"{name} has {t.shape[0]} rows, more than 31 bits count")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """Rows of consecutive elements, however far apart."""
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+class _EmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, positions, position_weight, scale, padding):
+        n, d = ids.numel(), weight.shape[1]
+        out = torch.empty(*ids.shape, d, dtype=weight.dtype, device=weight.device)
+        ids = ids.contiguous()
+        w, p = _rows(weight), None
+        if positions is not None:
+            positions, p = positions.contiguous(), _rows(position_weight)
+        if n:
+            with on_device(weight.device):
+                nv.check(nv.lib().dfcclEmbeddingForward(ids.data_ptr(), int(ids.dtype == torch.int64), n, w.data_ptr(), w.shape[0], w.stride(0), _ptr(positions),
+                                                        int(positions is not None and positions.dtype == torch.int64), _ptr(p),
+                                                        0 if p is None else p.shape[0], 0 if p is None else p.stride(0), out.data_ptr(), d,
+                                                        nccl_dtype(w.dtype), scale, raw_stream(weight.device)), "dfcclEmbeddingForward")
+        ctx.save_for_backward(ids, positions)
+        ctx.rows, ctx.prows, ctx.scale, ctx.padding = weight.shape[0], 0 if p is None else p.shape[0], scale, padding
+        ctx.set_materialize_grads(False)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        ids, positions = ctx.saved_tensors
+        if g is None:
+            return None, None, None, None, None, None
+        n, d = ids.numel(), g.shape[-1]
+        g = g.contiguous()
+        want_w, want_p = ctx.needs_input_grad[1], positions is not None and ctx.needs_input_grad[3]
+        make = torch.empty if n else torch.zeros
+        gw = make(ctx.rows, d, dtype=g.dtype, device=g.device) if want_w else None
+        gp = make(ctx.prows, d, dtype=g.dtype, device=g.device) if want_p else None
+        if n and (want_w or want_p):
+            with on_device(g.device):
+                work = torch.empty(nv.lib().dfcclEmbeddingBackwardWork(n, d, int(want_w) + int(want_p)), dtype=torch.uint8, device=g.device)
+                nv.check(nv.lib().dfcclEmbeddingBackward(g.data_ptr(), n, d, nccl_dtype(g.dtype), ids.data_ptr(), int(ids.dtype == torch.int64), ctx.padding,
+                                                         ctx.scale, _ptr(gw), ctx.rows, _ptr(positions),
+                                                         int(positions is not None and positions.dtype == torch.int64), _ptr(gp), ctx.prows,
+                                                         work.data_ptr(), raw_stream(g.device)), "dfcclEmbeddingBackward")
+        return None, gw, None, gp, None, None
+
+
+def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, positions: Optional[torch.Tensor] = None,
+              position_weight: Optional[torch.Tensor] = None, padding_idx: Optional[int] = None) -> torch.Tensor:
+    """``scale * weight[ids] + position_weight[positions]``, computed in fp32 and rounded once; [*ids.shape, columns].
+
+    ``weight`` and ``position_weight`` (both or neither of the position arguments) are bf16, fp16 or fp32 of one type, ``ids``
+    and ``positions`` int64 or int32 of one shape.  The gradients of both tables are dense; each row of them is the fp32 sum over
+    its tokens in their order, rounded once, the same in every run.  Tokens ``padding_idx`` give none.  There is no check of the
+    ids' values on the host: a token outside its table gives a row of NaN and no gradient of that table."""
+    _index("ids", ids)
+    _table("weight", weight)
+    if (positions is None) != (position_weight is None):
+        raise ValueError("positions and position_weight belong together")
+    tensors = [ids, weight]
+    if positions is not None:
+        _index("positions", positions)
+        _table("position_weight", position_weight)
+        if positions.shape != ids.shape:
+            raise ValueError(f"positions of {tuple(positions.shape)} for ids of {tuple(ids.shape)}")
+        if position_weight.shape[1] != weight.shape[1] or position_weight.dtype != weight.dtype:
+            raise ValueError(f"position_weight of {tuple(position_weight.shape)} {position_weight.dtype} beside weight of {tuple(weight.shape)} {weight.dtype}")
+        tensors += [positions, position_weight]
+    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+        raise ValueError(f"padding_idx {padding_idx} outside a table of {weight.shape[0]} rows")
+    if ids.numel() > 2 ** 31 - 4096:
+        raise ValueError(f"{ids.numel()} tokens in one call, more than 31 bits count")
+    if not all(t.is_cuda and t.device == weight.device for t in tensors):
+        raise ValueError("the embedding runs on tensors of one GPU")
+    return _EmbeddingFn.apply(ids, weight, positions, position_weight, float(scale), -1 if padding_idx is None else int(padding_idx))

@@ -1,0 +1,146 @@
+"""Losses of a language model's head from the head's inputs and weights, without keeping the logits (``csrc/src/ops/loss.cu``,
+``csrc/src/gemm/tcgen05_vocab.cu``): cross entropy with a target per row, distillation from a teacher's top logits."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import native as nv
+from ..utils.tensors import nccl_dtype, on_device, raw_stream
+from .block import packed
+
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+MAX_LIST = 256                       # entries of a teacher's list
+
+
+def linear_loss_supported(x: torch.Tensor, weight: torch.Tensor) -> bool:
+    """True if the losses of this module take ``x`` [..., d] and ``weight`` [vocabulary, d]."""
+    return (x.is_cuda and x.device == weight.device and x.dtype == weight.dtype == torch.bfloat16 and x.dim() >= 1 and weight.dim() == 2
+            and weight.shape[0] > 0 and x.shape[-1] == weight.shape[1] and weight.shape[1] > 0 and weight.shape[1] % 8 == 0)
+
+
+def _check(x: torch.Tensor, weight: torch.Tensor, index: torch.Tensor, name: str, reduction: str) -> None:
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"reduction is one of {', '.join(REDUCTIONS)}, got {reduction!r}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x [..., d] and weight [vocabulary, d], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+        raise ValueError(f"x and weight are bf16, got {x.dtype} and {weight.dtype}")
+    v, d = weight.shape
+    if d == 0 or d % 8 or v == 0:
+        raise ValueError(f"the width is a multiple of 8 and the vocabulary not empty, got {v} x {d}")
+    if index.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"{name} are int64 or int32, got {index.dtype}")
+    if max(x.numel() // d, v) > 2 ** 31 - 4096:
+        raise ValueError("more rows or entries than 31 bits count")
+
+
+def _on_one_gpu(*tensors: torch.Tensor) -> None:
+    if not all(t.is_cuda and t.device == tensors[0].device for t in tensors):
+        raise ValueError("the losses run on tensors of one GPU")
+
+
+class _LinearLossFn(torch.autograd.Function):
+    """Rows are compared with lists of entries (``tokens``, ``weights``, ``state``: the C interface)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, tokens, weights, state, k, temperature, reduction):
+        n, (v, d) = x.numel() // weight.shape[1], weight.shape
+        xp, wp = packed(x.detach()), packed(weight.detach())
+        lse, losses = torch.empty(n, dtype=torch.float32, device=x.device), torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        count = torch.empty(1, dtype=torch.int32, device=x.device) if reduction else None
+        loss = torch.empty((), dtype=torch.float32, device=x.device) if reduction else losses
+        if n:
+            with on_device(x.device):
+                work = torch.empty(nv.lib().dfcclLinearLossForwardWork(n, v, k), dtype=torch.uint8, device=x.device)
+                nv.check(nv.lib().dfcclLinearLossForward(xp.data_ptr(), wp.data_ptr(), n, v, d, tokens.data_ptr(), None if weights is None else weights.data_ptr(),
+                                                         state.data_ptr(), k, temperature, reduction, work.data_ptr(), lse.data_ptr(), losses.data_ptr(),
+                                                         loss.data_ptr() if reduction else None, count.data_ptr() if reduction else None,
+                                                         raw_stream(x.device)), "dfcclLinearLossForward")
+        elif reduction:
+            loss.zero_()
+        # (what the kernels read is kept: the tensors themselves where they are packed, so that a change in place is noticed)
+        ctx.save_for_backward(x if xp.data_ptr() == x.data_ptr() else xp, weight if wp.data_ptr() == weight.data_ptr() else wp, tokens, weights, state, lse, count)
+        ctx.k, ctx.temperature, ctx.mean, ctx.shape = k, temperature, reduction == REDUCTIONS["mean"], x.shape
+        ctx.set_materialize_grads(False)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        nothing = (None,) * 8
+        want_x, want_w = ctx.needs_input_grad[:2]
+        if g is None or not (want_x or want_w):
+            return nothing
+        x, w, tokens, weights, state, lse, count = ctx.saved_tensors
+        (v, d), n = w.shape, lse.shape[0]
+        if n == 0:
+            return (torch.zeros(ctx.shape, dtype=x.dtype, device=x.device) if want_x else None, torch.zeros_like(w) if want_w else None) + nothing[2:]
+        g = g.reshape(-1) if g.dim() else g
+        dx = torch.empty(ctx.shape, dtype=x.dtype, device=x.device) if want_x else None
+        dw = torch.empty(v, d, dtype=x.dtype, device=x.device) if want_w else None
+        with on_device(x.device):
+            size = nv.lib().dfcclLinearLossBackwardWork(n, v, d, int(want_x), int(want_w))
+            work = torch.empty(size, dtype=torch.uint8, device=x.device)
+            nv.check(nv.lib().dfcclLinearLossBackward(x.data_ptr(), w.data_ptr(), n, v, d, tokens.data_ptr(), None if weights is None else weights.data_ptr(),
+                                                      state.data_ptr(), ctx.k, ctx.temperature, lse.data_ptr(), g.data_ptr(), g.stride(0) if g.dim() else 0,
+                                                      count.data_ptr() if ctx.mean else None, dx.data_ptr() if want_x else None, dw.data_ptr() if want_w else None,
+                                                      work.data_ptr(), size, raw_stream(x.device)), "dfcclLinearLossBackward")
+        return (dx, dw) + nothing[2:]
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    """Softmax cross entropy of the logits ``x @ weight.T`` with ``targets``, in fp32; the logits are never stored.
+
+    ``x`` [..., d] and ``weight`` [vocabulary, d] are bf16, d a multiple of 8; ``targets`` [...] int64 or int32.  Rows of target
+    ``ignore_index`` have no loss and give no gradient, whatever ``x`` holds there; ``"mean"`` is over the other rows, and 0 where
+    there is none.  Logits and sums are fp32; the gradient of a logit is rounded once, to bf16, on its way into the products that
+    make the gradients of ``x`` and ``weight``.  It exists for as many columns at a time as ``DFCCL_LOSS_WORKSPACE_BYTES`` (1 GiB)
+    hold.  There is no check of the targets' values on the host: one outside the vocabulary makes its row's loss and gradients NaN."""
+    _check(x, weight, targets, "targets", reduction)
+    if targets.shape != x.shape[:-1]:
+        raise ValueError(f"targets of {tuple(targets.shape)} for x of {tuple(x.shape)}")
+    _on_one_gpu(x, weight, targets)
+    n, v = targets.numel(), weight.shape[0]
+    lists = torch.empty(2, n, dtype=torch.int32, device=x.device)
+    targets = targets.contiguous()
+    if n:
+        with on_device(x.device):
+            nv.check(nv.lib().dfcclTargetRows(targets.data_ptr(), int(targets.dtype == torch.int64), n, v, ignore_index, lists.data_ptr(), lists.data_ptr() + 4 * n,
+                                              raw_stream(x.device)), "dfcclTargetRows")
+    return _LinearLossFn.apply(x, weight, lists[0], None, lists[1], 1, 1.0, REDUCTIONS[reduction])
+
+
+def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor, teacher_tokens: torch.Tensor, *, temperature: float = 1.0,
+                        reduction: str = "mean") -> torch.Tensor:
+    """Divergence of the student's distribution from the teacher's top logits, ``T^2 sum_k q_k (ln q_k - ln p_k)`` per row: q is the
+    softmax of ``teacher_logits / T`` over the row's entries, p that of ``x @ weight.T / T`` over the whole vocabulary, read at
+    ``teacher_tokens``.
+
+    ``x`` and ``weight`` as in ``linear_cross_entropy``; ``teacher_logits`` [..., k] fp32, bf16 or fp16 and ``teacher_tokens`` [..., k]
+    int64 or int32, k up to 256 in any order.  Entries of token -1 or of logit -inf are left out; a row without any has no loss and
+    gives no gradient.  A token that stands in a row twice counts as two entries.  ``"mean"`` is over the rows with entries, 0 where
+    there is none.  No gradient reaches the teacher.  Any other token outside the vocabulary makes its row NaN."""
+    _check(x, weight, teacher_tokens, "teacher_tokens", reduction)
+    if teacher_tokens.dim() != x.dim() or teacher_tokens.shape[:-1] != x.shape[:-1] or teacher_logits.shape != teacher_tokens.shape:
+        raise ValueError(f"teacher_logits of {tuple(teacher_logits.shape)} and teacher_tokens of {tuple(teacher_tokens.shape)} for x of {tuple(x.shape)}")
+    if teacher_logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"teacher_logits are fp32, bf16 or fp16, got {teacher_logits.dtype}")
+    k = teacher_tokens.shape[-1]
+    if not 1 <= k <= MAX_LIST:
+        raise ValueError(f"lists of 1 to {MAX_LIST} entries, got {k}")
+    if not (temperature > 0.0 and temperature < float("inf")):
+        raise ValueError(f"the temperature is positive, got {temperature}")
+    _on_one_gpu(x, weight, teacher_logits, teacher_tokens)
+    n, v = teacher_tokens.numel() // k, weight.shape[0]
+    tokens = torch.empty(n, k, dtype=torch.int32, device=x.device)
+    weights = torch.empty(n, k, dtype=torch.float32, device=x.device)
+    state = torch.empty(n, dtype=torch.int32, device=x.device)
+    logits, listed = teacher_logits.detach().contiguous(), teacher_tokens.contiguous()
+    if n:
+        with on_device(x.device):
+            nv.check(nv.lib().dfcclTeacherRows(logits.data_ptr(), nccl_dtype(logits.dtype), listed.data_ptr(), int(listed.dtype == torch.int64), n, k, v,
+                                               temperature, tokens.data_ptr(), weights.data_ptr(), state.data_ptr(), raw_stream(x.device)), "dfcclTeacherRows")
+    return _LinearLossFn.apply(x, weight, tokens, weights, state, k, float(temperature), REDUCTIONS[reduction])

@@ -1,0 +1,311 @@
+"""Cross entropy and distillation over a vocabulary without the logits, against 64 bits.
+
+What may be off, by arithmetic: a logit of d terms is added up in fp32 in steps of 16, each at most one step of its type (2**-23 of the
+magnitudes' sum) off; a power of two or logarithm is a few of those; a gradient of a logit is rounded once to bf16 (2**-8 at most, less
+than 2**-9 in the 2-norm over many), the gradients of x and weight once more."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+LN = 2.0 ** -18                      # of a loss's own size: powers, logarithms and sums in fp32
+
+
+def logit_error(x, w):
+    """Of every logit, [n, v]; with the largest of a row below."""
+    return (x.shape[1] / 16 + 4) * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t())
+
+
+def problem(n, v, d, seed, spread=0.5):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(n, d, generator=gen, device="cuda").to(torch.bfloat16)
+    w = (torch.randn(v, d, generator=gen, device="cuda") * (spread * 4 / d ** 0.5)).to(torch.bfloat16)
+    return x, w, gen
+
+
+def reference(x, w, tokens, q, temp):
+    """Row losses, gradient of the logits for a gradient of 1 of each row's loss, logits' errors; q [n, k] weights of the entries."""
+    z = x.double() @ w.double().t() / temp
+    logp = torch.log_softmax(z, dim=1)
+    keep = q > 0
+    picked = logp.gather(1, torch.where(keep, tokens, 0))
+    loss = temp * temp * torch.where(keep, torch.special.xlogy(q, q) - q * picked, 0.0).sum(dim=1)
+    dz = temp * (logp.exp() * q.sum(dim=1, keepdim=True)).scatter_add(1, torch.where(keep, tokens, 0), -q)
+    return loss, torch.where(keep.any(dim=1)[:, None], dz, 0.0)
+
+
+def check_gradients(got, x, w, dz, share, temp, limit=2.0 ** -8):
+    """Elementwise by the sums of magnitudes, and in the 2-norm: two roundings, each below 2**-9, are below 2**-8 together."""
+    err = logit_error(x, w)
+    rel = 2.0 ** -8 * (1 + 2.0 ** -8) + 2.0 ** -18 + 3 * err.max().item() / temp      # of p; p - q and its factor are rounded after it
+    dz = dz * share[:, None]
+    off = dz.abs() * rel + temp * share.abs()[:, None] * torch.minimum(torch.softmax(x.double() @ w.double().t() / temp, dim=1), torch.ones_like(dz)) * (rel - 2.0 ** -8)
+    xd, wd = x.double(), w.double()
+    depth = (max(x.shape[0], w.shape[0]) / 16 + 8) * 2.0 ** -23
+    for name, g, want, bound, size in (("dx", got[0], dz @ wd, off @ wd.abs(), dz.abs() @ wd.abs()),
+                                       ("dw", got[1], dz.t() @ xd, off.t() @ xd.abs(), dz.abs().t() @ xd.abs())):
+        if g is None:
+            continue
+        tol = bound * (1 + 2.0 ** -8) + want.abs() * 2.0 ** -8 + size * depth + 1e-38
+        assert bool(((g.double() - want).abs() <= tol).all()), name
+        norm = want.norm().item()
+        if norm > 0 and want.numel() >= 4096:
+            assert (g.double() - want).norm().item() <= limit * norm, name
+
+
+def check_loss(got, want, x, w, temp):
+    err = 2 * temp * logit_error(x, w).amax(dim=1)
+    assert bool(((got.double() - want).abs() <= err + LN * (want.abs() + temp * temp)).all())
+
+
+SIZES = [(1, 1, 8), (1, 2, 8), (1, 300, 16), (3, 257, 40), (77, 1000, 64), (128, 255, 72), (129, 256, 128), (255, 512, 136), (256, 513, 256), (257, 769, 264),
+         (300, 5000, 200), (1000, 3001, 320), (2049, 640, 1024), (33, 50257, 64), (2, 50257, 768)]
+
+
+@pytest.mark.parametrize("n,v,d", SIZES)
+def test_cross_entropy(n, v, d):
+    from dfccl_b200.ops.gemm import check_kernels
+    from dfccl_b200.ops.loss import linear_cross_entropy
+    x, w, gen = problem(n, v, d, n + 3 * v + 5 * d)
+    t = torch.randint(0, v, (n,), generator=gen, device="cuda")
+    drop = torch.rand(n, generator=gen, device="cuda") < 0.2
+    drop[0] = False
+    targets = torch.where(drop, -100, t)
+    loss, dz = reference(x, w, t[:, None], (~drop).double()[:, None], 1.0)
+    count = (~drop).sum().double()
+    x.requires_grad_(True), w.requires_grad_(True)
+    rows = linear_cross_entropy(x, w, targets, reduction="none")
+    check_loss(rows.detach(), loss, x.detach(), w.detach(), 1.0)
+    gout = torch.randn(n, generator=gen, device="cuda")
+    check_gradients(torch.autograd.grad(rows, [x, w], gout), x.detach(), w.detach(), dz, gout.double(), 1.0)
+    mean = linear_cross_entropy(x, w, targets)
+    assert abs(mean.item() - (loss.sum() / count).item()) <= (2 * logit_error(x.detach(), w.detach()).max().item() + 2 * LN * (1 + loss.abs().max().item()))
+    got = torch.autograd.grad(mean, [x, w], retain_graph=True)
+    check_gradients(got, x.detach(), w.detach(), dz, torch.ones(n, device="cuda").double() / count, 1.0)
+    again = torch.autograd.grad(mean, [x, w])
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    assert check_kernels()
+
+
+@pytest.mark.parametrize("n,v,d,k,temp", [(1, 1, 8, 1, 1.0), (1, 300, 16, 5, 2.0), (77, 1000, 64, 1, 0.5), (130, 515, 72, 32, 1.0), (257, 2049, 264, 33, 3.0),
+                                          (300, 256, 128, 256, 2.0), (500, 5001, 320, 100, 1.5), (33, 50257, 64, 64, 1.0)])
+def test_distillation(n, v, d, k, temp):
+    from dfccl_b200.ops.loss import linear_distillation
+    x, w, gen = problem(n, v, d, n + 3 * v + 5 * d + k)
+    tokens = torch.randint(0, v, (n, k), generator=gen, device="cuda")           # in any order, some twice
+    logits = torch.randn(n, k, generator=gen, device="cuda") * 3
+    tokens = torch.where(torch.rand(n, k, generator=gen, device="cuda") < 0.2, -1, tokens)
+    tokens[n // 2] = -1 if n > 1 else tokens[0]
+    logits = torch.where(torch.rand(n, k, generator=gen, device="cuda") < 0.05, float("-inf"), logits)
+    keep = (tokens >= 0) & (logits > float("-inf"))
+    valid = keep.any(dim=1)
+    q = torch.nan_to_num(torch.softmax((logits.double() / temp).masked_fill(~keep, float("-inf")), dim=1), nan=0.0)
+    loss, dz = reference(x, w, tokens.clamp(min=0), q, temp)
+    x.requires_grad_(True), w.requires_grad_(True)
+    rows = linear_distillation(x, w, torch.where(tokens < 0, float("nan"), logits), tokens, temperature=temp, reduction="none")
+    check_loss(rows.detach(), loss, x.detach(), w.detach(), temp)
+    assert bool((rows.detach()[~valid] == 0).all())
+    gout = torch.randn(n, generator=gen, device="cuda")
+    check_gradients(torch.autograd.grad(rows, [x, w], gout), x.detach(), w.detach(), dz, gout.double(), temp)
+    total = linear_distillation(x, w, logits.to(torch.float32), tokens.int(), temperature=temp)
+    got = torch.autograd.grad(total, [x, w])
+    check_gradients(got, x.detach(), w.detach(), dz, torch.ones(n, device="cuda").double() / max(1, int(valid.sum())), temp)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_teacher_types(dtype):
+    """A list's order does not matter, and logits of 16 bits are what they are in 32."""
+    from dfccl_b200.ops.loss import linear_distillation
+    x, w, gen = problem(100, 700, 64, 5)
+    tokens = torch.rand(100, 700, generator=gen, device="cuda").topk(24, dim=1).indices
+    logits = torch.randn(100, 24, generator=gen, device="cuda").to(dtype)
+    want = linear_distillation(x, w, logits.float(), tokens, reduction="none")
+    assert torch.equal(want, linear_distillation(x, w, logits, tokens, reduction="none"))
+    turned = linear_distillation(x, w, logits.flip(1), tokens.flip(1).int(), reduction="none")
+    assert bool(((turned - want).abs() <= LN * (1 + want.abs())).all())          # the teacher's softmax adds up in the order of the list
+
+
+@pytest.mark.parametrize("limit", [1 << 20, 3 << 20, 1 << 30])
+@pytest.mark.parametrize("n,v,d", [(700, 5003, 128), (1500, 3000, 264), (100, 50257, 64)])
+def test_pieces_of_the_vocabulary(n, v, d, limit, monkeypatch):
+    """The gradient of the logits in one piece or many, with and without either of the two results."""
+    from dfccl_b200.ops.loss import linear_cross_entropy
+    monkeypatch.setenv("DFCCL_LOSS_WORKSPACE_BYTES", str(limit))
+    x, w, gen = problem(n, v, d, n + v + d)
+    t = torch.randint(0, v, (n,), generator=gen, device="cuda")
+    _, dz = reference(x, w, t[:, None], torch.ones(n, 1, dtype=torch.float64, device="cuda"), 1.0)
+    for want_x, want_w in ((True, True), (True, False), (False, True)):
+        xl, wl = x.clone().requires_grad_(want_x), w.clone().requires_grad_(want_w)
+        linear_cross_entropy(xl, wl, t, reduction="sum").backward()
+        check_gradients((xl.grad, wl.grad), x, w, dz, torch.ones(n, dtype=torch.float64, device="cuda"), 1.0)
+
+
+def test_ignored_rows_hold_anything():
+    """Infinities and NaN in rows without a target reach nothing; a batch without any target costs nothing and gives zeros."""
+    from dfccl_b200.ops.loss import linear_cross_entropy, linear_distillation
+    x, w, gen = problem(300, 1000, 64, 9)
+    t = torch.randint(0, 1000, (300,), generator=gen, device="cuda")
+    hole = torch.arange(300, device="cuda") % 3 == 1
+    dirty = x.clone()
+    dirty[hole] = torch.tensor([float("inf"), float("nan"), float("-inf"), 1e38], device="cuda").to(torch.bfloat16).repeat(16)
+    t = torch.where(hole, -100, t)
+    lists = torch.where(hole[:, None], -1, torch.stack([t, (t + 1) % 1000], dim=1))
+    teacher = torch.zeros(300, 2, device="cuda")
+    for loss in (lambda a, b: linear_cross_entropy(a, b, t), lambda a, b: linear_distillation(a, b, teacher, lists)):
+        res = []
+        for rows in (x, dirty):
+            a, b = rows.clone().requires_grad_(True), w.clone().requires_grad_(True)
+            value = loss(a, b)
+            value.backward()
+            res.append((value.detach(), a.grad, b.grad))
+        clean, mixed = res
+        assert torch.equal(clean[0], mixed[0])
+        assert torch.equal(clean[1][~hole], mixed[1][~hole]) and bool((mixed[1][hole] == 0).all())
+        # the rows' zeros stand beside x's NaN in the product of the weight's gradient: they must not meet
+        assert torch.equal(clean[2], mixed[2])
+    a, b = dirty.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    for value in (linear_cross_entropy(a, b, torch.full_like(t, -100)), linear_distillation(a, b, teacher, torch.full_like(lists, -1))):
+        assert value.item() == 0.0
+        ga, gb = torch.autograd.grad(value, [a, b])
+        assert bool((ga == 0).all()) and bool((gb == 0).all())
+
+
+def test_large_and_infinite_logits():
+    """Logits of hundreds, a head with a row of the type's lowest value or of -inf logits, equal logits; a row of NaN is NaN by itself."""
+    from dfccl_b200.ops.loss import linear_cross_entropy
+    x, w, gen = problem(200, 900, 64, 21, spread=40.0)
+    t = torch.randint(0, 900, (200,), generator=gen, device="cuda")
+    loss, dz = reference(x, w, t[:, None], torch.ones(200, 1, dtype=torch.float64, device="cuda"), 1.0)
+    rows = linear_cross_entropy(x, w, t, reduction="none")
+    check_loss(rows, loss, x, w, 1.0)
+    ones = torch.ones(200, 64, device="cuda").to(torch.bfloat16)
+    w2 = w.clone()
+    w2[7] = torch.finfo(torch.bfloat16).min / 128
+    w2[8] = float("-inf")
+    t = torch.where((t == 7) | (t == 8), 9, t)
+    got = linear_cross_entropy(ones, w2, t, reduction="none")
+    kept = torch.cat([w[:7], w[9:]])
+    want, _ = reference(ones, kept, torch.where(t > 8, t - 2, t)[:, None], torch.ones(200, 1, dtype=torch.float64, device="cuda"), 1.0)
+    check_loss(got, want, ones, kept, 1.0)
+    assert linear_cross_entropy(ones[:1], w2, torch.tensor([8], device="cuda")).item() == float("inf")
+    flat = linear_cross_entropy(ones, torch.zeros_like(w), t, reduction="none")
+    assert bool(((flat - torch.log(torch.tensor(900.0))).abs() < 1e-5).all())
+    x[5, 3] = float("nan")
+    rows = linear_cross_entropy(x, w, t, reduction="none")
+    assert rows.isnan().nonzero()[:, 0].tolist() == [5]
+
+
+def test_targets_outside_the_vocabulary():
+    from dfccl_b200.ops.loss import linear_cross_entropy, linear_distillation
+    x, w, gen = problem(64, 300, 32, 23)
+    t = torch.randint(0, 300, (64,), generator=gen, device="cuda")
+    t[3], t[40], t[50] = 300, -1, 2 ** 33
+    rows = linear_cross_entropy(x, w, t, reduction="none")
+    assert rows.isnan().nonzero()[:, 0].tolist() == [3, 40, 50]
+    lists = t[:, None].clamp(min=-1)
+    lists[41] = -2
+    rows = linear_distillation(x, w, torch.zeros(64, 1, device="cuda"), lists, reduction="none")
+    assert rows.isnan().nonzero()[:, 0].tolist() == [3, 41, 50] and rows[40].item() == 0.0
+    a = x.clone().requires_grad_(True)
+    linear_distillation(a, w, torch.zeros(64, 1, device="cuda"), lists, reduction="sum").backward()
+    assert a.grad.isnan().any(dim=1).nonzero()[:, 0].tolist() == [3, 41, 50]
+
+
+def test_strides_shapes_and_gradients_of_one_value():
+    from dfccl_b200.ops.loss import linear_cross_entropy
+    x, w, gen = problem(60, 500, 72, 31)
+    t = torch.randint(0, 500, (60,), generator=gen, device="cuda")
+    want = linear_cross_entropy(x, w, t, reduction="none")
+    wide = torch.zeros(60, 80, device="cuda", dtype=torch.bfloat16)
+    wide[:, 3:75] = x
+    assert torch.equal(want, linear_cross_entropy(wide[:, 3:75], w.t().contiguous().t(), t.int(), reduction="none"))
+    shaped = linear_cross_entropy(x.view(3, 20, 72), w, t.view(3, 20), reduction="none")
+    assert shaped.shape == (3, 20) and torch.equal(shaped.view(-1), want)
+    a, b = wide.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    linear_cross_entropy(a[:, 3:75].view(4, 15, 72), b, t.view(4, 15), reduction="none").sum().backward()
+    c, d = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    linear_cross_entropy(c, d, t, reduction="sum").backward()
+    assert torch.equal(a.grad[:, 3:75], c.grad) and torch.equal(b.grad, d.grad) and bool((a.grad[:, :3] == 0).all())
+    none = linear_cross_entropy(x[:0].requires_grad_(True), d, t[:0])
+    assert none.item() == 0.0
+    assert bool((torch.autograd.grad(none, [d])[0] == 0).all())
+    one = linear_cross_entropy(x[0], w, t[0], reduction="none")
+    assert one.shape == () and torch.equal(one, want[0])
+
+
+def test_gradient_against_differences():
+    """The loss, in 64 bits, along the gradient: central differences of the reference against what the kernels give."""
+    from dfccl_b200.ops.loss import linear_cross_entropy
+    x, w, gen = problem(96, 700, 64, 37)
+    t = torch.randint(0, 700, (96,), generator=gen, device="cuda")
+    a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    ga, gb = torch.autograd.grad(linear_cross_entropy(a, b, t), [a, b])
+
+    def value(step):
+        z = (x.double() + step * ga.double()) @ (w.double() + step * gb.double()).t()
+        return torch.nn.functional.cross_entropy(z, t).item()
+
+    slope = (value(1e-4) - value(-1e-4)) / 2e-4
+    size = (ga.double().square().sum() + gb.double().square().sum()).item()
+    assert abs(slope - size) <= 2.0 ** -8 * size                      # the gradients' error in the 2-norm, along themselves
+
+
+def test_other_stream_and_graphs():
+    """On a stream of its own; forward and backward captured and replayed for other data, two graphs in turns."""
+    from dfccl_b200.ops.gemm import check_kernels
+    from dfccl_b200.ops.loss import linear_cross_entropy, linear_distillation
+    x, w, gen = problem(300, 3001, 128, 41)
+    w.requires_grad_(True)
+    xs = [torch.randn(300, 128, generator=gen, device="cuda").to(torch.bfloat16) for _ in range(3)]
+    ts = [torch.randint(-1, 3001, (300, 4), generator=gen, device="cuda") for _ in range(3)]
+    teacher = torch.randn(300, 4, generator=gen, device="cuda")
+
+    def step(x, t):
+        x = x.detach().requires_grad_(True)
+        loss = linear_cross_entropy(x, w, t[:, 0], ignore_index=-1) + linear_distillation(x, w, teacher, t, temperature=2.0)
+        return (loss.detach(),) + torch.autograd.grad(loss, [x, w])
+
+    want = [step(a, b) for a, b in zip(xs, ts)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(xs[1], ts[1])
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want[1]))
+    graphs = []
+    for _ in range(2):
+        a, b = xs[0].clone(), ts[0].clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(a, b)
+        graphs.append((a, b, graph, out))
+    for turn in range(3):
+        for k, (a, b, graph, _) in enumerate(graphs):
+            a.copy_(xs[(turn + k) % 3]), b.copy_(ts[(turn + k) % 3])
+            graph.replay()
+        for k, (_, _, _, out) in enumerate(graphs):
+            assert all(torch.equal(p, q) for p, q in zip(out, want[(turn + k) % 3]))
+    assert check_kernels()
+
+
+def test_a_models_two_ends():
+    """A stage of GPT-2 with its ends on these kernels against the same weights without: the embedding's rows are the same, the loss is
+    off by the rounding of the logits to bf16 (2**-9 of logits of a few units, over many rows), every gradient by roundings to bf16."""
+    from dfccl_b200 import native as nv
+    from dfccl_b200.models.gpt2 import GPT2Config, GPT2Stage
+    from dfccl_b200.ops.fused_linear import TpGroup
+    (comm,) = nv.Comm.init_loopback(1, torch.cuda.current_device())
+    cfg = GPT2Config(n_layer=1, d_model=256, n_head=4, seq_len=128, vocab=1111)
+    tp = TpGroup(comm, None, torch.device("cuda", torch.cuda.current_device()))
+    plain, fused = GPT2Stage(cfg, tp, 0, 1, 4), GPT2Stage(cfg, tp, 0, 1, 4, fused_ends=True)
+    tokens = torch.randint(0, 1111, (4, 129), device="cuda")
+    losses, grads = [], []
+    for stage in (plain, fused):
+        loss = stage(tokens[:, :-1], tokens[:, 1:])
+        loss.backward()
+        losses.append(loss.item())
+        grads.append([p.grad.double() for p in stage.parameters()])
+    assert abs(losses[0] - losses[1]) <= 2.0 ** -9 * losses[0]
+    for a, b in zip(*grads):
+        assert (a - b).norm().item() <= 0.03 * a.norm().item()       # several roundings of 2**-9 on either side, through a block
+    comm.destroy()

@@ -1,0 +1,107 @@
+"""What the embedding and the losses over a vocabulary refuse, before anything reaches a GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+BF = torch.bfloat16
+
+
+def x(*shape, dtype=BF):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def i(*shape, dtype=torch.int64):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("args,kw,what", [
+    ((x(4, 16), x(9, 16), i(4)), {"reduction": "average"}, "reduction"),
+    ((x(4, 16), x(9, 24), i(4)), {}, "x \\[..., d\\]"),
+    ((x(4, 16), x(16), i(4)), {}, "x \\[..., d\\]"),
+    ((x(4, 16, dtype=torch.float32), x(9, 16, dtype=torch.float32), i(4)), {}, "bf16"),
+    ((x(4, 16), x(9, 16, dtype=torch.float16), i(4)), {}, "bf16"),
+    ((x(4, 12), x(9, 12), i(4)), {}, "multiple of 8"),
+    ((x(4, 0), x(9, 0), i(4)), {}, "multiple of 8"),
+    ((x(4, 16), x(0, 16), i(4)), {}, "not empty"),
+    ((x(4, 16), x(9, 16), i(4, dtype=torch.int16)), {}, "int64 or int32"),
+    ((x(4, 16), x(9, 16), i(5)), {}, "targets of"),
+    ((x(4, 16), x(9, 16), i(4, 1)), {}, "targets of"),
+    ((x(4, 16), x(9, 16), i(4)), {}, "GPU")])
+def test_cross_entropy_refuses(args, kw, what):
+    from dfccl_b200.ops.loss import linear_cross_entropy
+    with pytest.raises(ValueError, match=what):
+        linear_cross_entropy(*args, **kw)
+
+
+@pytest.mark.parametrize("args,kw,what", [
+    ((x(4, 16), x(9, 16), x(4, 3), i(4, 2)), {}, "teacher_logits of"),
+    ((x(4, 16), x(9, 16), x(4), i(4)), {}, "teacher_logits of"),
+    ((x(4, 16), x(9, 16), x(5, 2), i(5, 2)), {}, "teacher_logits of"),
+    ((x(4, 16), x(9, 16), i(4, 2), i(4, 2)), {}, "fp32, bf16 or fp16"),
+    ((x(4, 16), x(9, 16), x(4, 2), x(4, 2)), {}, "int64 or int32"),
+    ((x(4, 16), x(9, 16), x(4, 0), i(4, 0)), {}, "1 to 256"),
+    ((x(4, 16), x(9, 16), x(4, 257), i(4, 257)), {}, "1 to 256"),
+    ((x(4, 16), x(9, 16), x(4, 2), i(4, 2)), {"temperature": 0.0}, "temperature"),
+    ((x(4, 16), x(9, 16), x(4, 2), i(4, 2)), {"temperature": float("nan")}, "temperature"),
+    ((x(4, 16), x(9, 16), x(4, 2), i(4, 2)), {"temperature": float("inf")}, "temperature"),
+    ((x(4, 16), x(9, 16), x(4, 2), i(4, 2)), {}, "GPU")])
+def test_distillation_refuses(args, kw, what):
+    from dfccl_b200.ops.loss import linear_distillation
+    with pytest.raises(ValueError, match=what):
+        linear_distillation(*args, **kw)
+
+
+@pytest.mark.parametrize("args,kw,what", [
+    ((i(4, dtype=torch.uint8), x(9, 16)), {}, "int64 or int32"),
+    ((i(4), x(16)), {}, "weight is"),
+    ((i(4), x(0, 16)), {}, "weight is"),
+    ((i(4), x(9, 0)), {}, "weight is"),
+    ((i(4), x(9, 16, dtype=torch.float64)), {}, "bf16, fp16 or fp32"),
+    ((i(4), x(9, 16)), {"positions": i(4)}, "belong together"),
+    ((i(4), x(9, 16)), {"position_weight": x(9, 16)}, "belong together"),
+    ((i(4), x(9, 16)), {"positions": i(5), "position_weight": x(9, 16)}, "positions of"),
+    ((i(4), x(9, 16)), {"positions": x(4), "position_weight": x(9, 16)}, "int64 or int32"),
+    ((i(4), x(9, 16)), {"positions": i(4), "position_weight": x(9, 24)}, "beside weight"),
+    ((i(4), x(9, 16)), {"positions": i(4), "position_weight": x(9, 16, dtype=torch.float32)}, "beside weight"),
+    ((i(4), x(9, 16)), {"padding_idx": 9}, "padding_idx"),
+    ((i(4), x(9, 16)), {"padding_idx": -1}, "padding_idx"),
+    ((i(4), x(9, 16)), {}, "GPU")])
+def test_embedding_refuses(args, kw, what):
+    from dfccl_b200.ops.embedding import embedding
+    with pytest.raises(ValueError, match=what):
+        embedding(*args, **kw)
+
+
+def test_entries_refuse(native):
+    """The C entry points answer with a status: no null pointers, no odd widths, no lists beyond the limit, no misaligned operands."""
+    L, bad, p, q = native.lib(), native.INVALID_ARGUMENT, 4096, 4100
+    assert L.dfcclLinearLossMaxList() == 256
+    ok = [p, p, 4, 9, 16, p, None, p, 1, 1.0, 0, p, p, p, None, None, None]
+    for at, value in ((0, None), (1, q), (2, 0), (3, 0), (4, 12), (5, None), (7, None), (8, 0), (8, 257), (9, 0.0), (10, 3), (10, 1), (11, None), (12, None), (13, None)):
+        args = list(ok)
+        args[at] = value
+        assert L.dfcclLinearLossForward(*args) == bad, (at, value)
+    ok = [p, p, 4, 9, 16, p, None, p, 1, 1.0, p, p, 0, None, p, p, p, 1 << 30, None]
+    for at, value in ((0, None), (1, q), (2, -1), (4, 4), (8, 300), (9, -1.0), (10, None), (11, None), (12, -1), (14, q), (15, q), (16, None), (17, 16)):
+        args = list(ok)
+        args[at] = value
+        assert L.dfcclLinearLossBackward(*args) == bad, (at, value)
+    args = list(ok)
+    args[14] = args[15] = None
+    assert L.dfcclLinearLossBackward(*args) == bad
+    assert L.dfcclLinearLossForwardWork(4, 9, 0) == 0 and L.dfcclLinearLossBackwardWork(4, 9, 16, 0, 0) == 0
+    assert L.dfcclTargetRows(None, 1, 4, 9, -100, p, p, None) == bad and L.dfcclTargetRows(p, 1, 0, 9, -100, p, p, None) == bad
+    assert L.dfcclTeacherRows(p, native.INT32, p, 1, 4, 2, 9, 1.0, p, p, p, None) == bad and L.dfcclTeacherRows(p, native.FLOAT32, p, 1, 4, 257, 9, 1.0, p, p, p, None) == bad
+    ok = [p, 1, 4, p, 9, 16, None, 0, None, 0, 0, p, 16, native.BFLOAT16, 1.0, None]
+    for at, value in ((0, None), (2, 0), (3, None), (4, 0), (5, 8), (6, p), (11, None), (12, 0), (13, native.FLOAT64)):
+        args = list(ok)
+        args[at] = value
+        assert L.dfcclEmbeddingForward(*args) == bad, (at, value)
+    ok = [p, 4, 16, native.BFLOAT16, p, 1, -1, 1.0, p, 9, None, 0, None, 0, p, None]
+    for at, value in ((0, None), (1, 0), (2, 0), (3, native.INT64), (4, None), (8, None), (8, q), (9, 0), (9, 2 ** 31), (12, p), (14, None)):
+        args = list(ok)
+        args[at] = value
+        assert L.dfcclEmbeddingBackward(*args) == bad, (at, value)
+    assert L.dfcclEmbeddingBackwardWork(4, 16, 3) == 0 and L.dfcclEmbeddingBackwardWork(4, 16, 2) > 0
+    assert isinstance(L.dfcclLinearLossBackwardWork(1000, 50257, 1024, 1, 1), int) and C.sizeof(C.c_size_t) == 8
