@@ -23,8 +23,8 @@ namespace dfccl {
 namespace {
 
 constexpr int SORT_CTAS = 8, SORT_THREADS = 1024, SORT_WARPS = SORT_CTAS * SORT_THREADS / 32;
-constexpr int CLEAR_CLUSTERS = 16;             // beside the sorting ones: 128 blocks of 1024 threads
-constexpr int SUM_GROUPS = 8;                  // of threads that share a row's stretches in the last step
+constexpr int CLEAR_BLOCKS = 128;
+constexpr int JOIN_WARPS = 8;
 constexpr int MAX_TABLES = 2;
 
 template <typename... P, typename... A>
@@ -60,42 +60,96 @@ struct Forward {
   void* out;
   int wideIds, widePositions;
   int n, packs;                                  // packs of E elements per row
+  int lanes, turns;                              // of a warp that share a row (a power of two); rows one after the other
   long long rows, prows, ldw, ldp;               // in elements
   float scale;
 };
 
-// A thread takes U packs, a block apart, so that its loads overlap.
-template <typename T, int E, int U>
+// Two elements of 16 bits at a time, rounded by one instruction.
+template <typename T> struct Pair;
+template <> struct Pair<__nv_bfloat16> {
+  using Type = __nv_bfloat162;
+  static __device__ __forceinline__ float2 wide(Type v) { return __bfloat1622float2(v); }
+  static __device__ __forceinline__ Type narrow(float a, float b) { return __floats2bfloat162_rn(a, b); }
+};
+template <> struct Pair<__half> {
+  using Type = __half2;
+  static __device__ __forceinline__ float2 wide(Type v) { return __half22float2(v); }
+  static __device__ __forceinline__ Type narrow(float a, float b) { return __floats2half2_rn(a, b); }
+};
+
+// What becomes of a row: copied (scale 1), the position's row added (scale 1), or scaled in general.
+enum EmbedForm { EMBED_COPY, EMBED_ADD, EMBED_SCALE, EMBED_SCALE_ADD };
+template <typename T, int E, int FORM>
+__device__ __forceinline__ void combine(const Pack<T, E>& x, const Pack<T, E>& y, float scale, Pack<T, E>& o) {
+  if (FORM == EMBED_COPY) { o = x; return; }
+  if constexpr (sizeof(T) == 2 && E > 1) {
+    using P2 = typename Pair<T>::Type;
+    const P2* a = (const P2*)x.v; const P2* b = (const P2*)y.v;
+    P2* r = (P2*)o.v;
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) {
+      // (a sum of two elements in 32 bits, rounded to 16, is the sum rounded once: 24 bits are twice those of the type and two)
+      if (FORM == EMBED_ADD) { r[e] = __hadd2(a[e], b[e]); continue; }
+      const float2 f = Pair<T>::wide(a[e]);
+      if (FORM == EMBED_SCALE) { r[e] = Pair<T>::narrow(f.x * scale, f.y * scale); continue; }
+      const float2 h = Pair<T>::wide(b[e]);
+      r[e] = Pair<T>::narrow(fmaf(f.x, scale, h.x), fmaf(f.y, scale, h.y));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) o.v[e] = fromFloat<T>(FORM == EMBED_SCALE ? toFloat(x.v[e]) * scale : fmaf(toFloat(x.v[e]), scale, toFloat(y.v[e])));
+  }
+}
+
+// A warp takes `turns` rows one after the other (`turns` times as many side by side where rows are short), 32 at most: their tokens are one
+// load in front, and four packs of a lane are on their way at a time (a row of 1024 bf16 is four).
+template <typename T, int E, int FORM>
 __global__ void __launch_bounds__(256) embedForwardKernel(const Forward a) {
+  constexpr int U = 4;
+  constexpr bool POS = FORM == EMBED_ADD || FORM == EMBED_SCALE_ADD;
   tc::grid_dependency_wait();
   tc::grid_launch_dependents();
   using P = Pack<T, E>;
-  const long long total = (long long)a.n * a.packs, base = (long long)blockIdx.x * 256 * U + threadIdx.x;
-  P w[U], p[U];
-  bool bad[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const long long i = base + u * 256;
-    if (i >= total) break;
-    const int row = (int)(i / a.packs), c = (int)(i - (long long)row * a.packs);
-    const long long id = intAt(a.ids, a.wideIds, row), at = a.positions ? intAt(a.positions, a.widePositions, row) : 0;
-    bad[u] = id < 0 || id >= a.rows || (a.positions && (at < 0 || at >= a.prows));
-    if (bad[u]) continue;
-    w[u] = *(const P*)((const T*)a.w + id * a.ldw + (long long)c * E);
-    if (a.positions) p[u] = *(const P*)((const T*)a.p + at * a.ldp + (long long)c * E);
+  const int lane = threadIdx.x & 31, perWarp = 32 / a.lanes, sub = lane / a.lanes, own = lane & (a.lanes - 1);
+  const long long row0 = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * perWarp * a.turns;
+  const int rows = (int)max(0ll, min((long long)perWarp * a.turns, a.n - row0));
+  long long mine = 0, minePos = 0;
+  if (lane < rows) {
+    mine = intAt(a.ids, a.wideIds, row0 + lane);
+    if (POS) minePos = intAt(a.positions, a.widePositions, row0 + lane);
+    if (mine < 0 || mine >= a.rows || (POS && (minePos < 0 || minePos >= a.prows))) mine = -1;
   }
+  for (int k = 0; k < rows; k += perWarp) {
+    const long long id = __shfl_sync(0xffffffffu, mine, k + sub), at = POS ? __shfl_sync(0xffffffffu, minePos, k + sub) : 0;
+    if (k + sub >= rows) continue;
+    P* out = (P*)a.out + (row0 + k + sub) * a.packs;
+    if (id < 0) {                                            // a token outside the table: not a number
+      P o;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const long long i = base + u * 256;
-    if (i >= total) break;
-    P o;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      float y = __int_as_float(0x7fffffff);            // a token outside the table: not a number
-      if (!bad[u]) y = a.positions ? fmaf(toFloat(w[u].v[e]), a.scale, toFloat(p[u].v[e])) : toFloat(w[u].v[e]) * a.scale;
-      o.v[e] = fromFloat<T>(y);
+      for (int e = 0; e < E; ++e) o.v[e] = fromFloat<T>(__int_as_float(0x7fffffff));
+      for (int c = own; c < a.packs; c += a.lanes) out[c] = o;
+      continue;
     }
-    ((P*)a.out)[i] = o;
+    const P* w = (const P*)((const T*)a.w + id * a.ldw);
+    const P* p = (const P*)((const T*)a.p + at * a.ldp);
+    for (int c = own; c < a.packs; c += U * a.lanes) {
+      P x[U], y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = min(c + u * a.lanes, a.packs - 1);     // (no branch between the loads)
+        x[u] = w[i];
+        if (POS) y[u] = p[i];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = c + u * a.lanes;
+        if (i >= a.packs) break;
+        P o;
+        combine<T, E, FORM>(x[u], y[u], a.scale, o);
+        out[i] = o;
+      }
+    }
   }
 }
 
@@ -117,92 +171,128 @@ struct Backward {
   const void* g;
 };
 
-__device__ __forceinline__ uint2 itemAt(const Table& t, int pass, int i) {
-  if (pass) return __ldcg(&t.buf[pass & 1][i]);
-  const long long id = intAt(t.ids, t.wide, i);
-  return make_uint2(id >= 0 && id < t.rows && id != t.padding ? (uint32_t)id : (uint32_t)t.rows, (uint32_t)i);
+// The lanes with an item of the same digit, bit by bit.
+__device__ __forceinline__ uint32_t sameDigit(int digit, bool in) {
+  uint32_t same = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+  for (int b = 0; b < 8; ++b) {
+    const uint32_t set = __ballot_sync(0xffffffffu, digit >> b & 1);
+    same &= digit >> b & 1 ? set : ~set;
+  }
+  return same;
 }
 
-// Every warp has a range of the items of its own; its counts of the digits, summed over the ranges in front, are where its items go.
+// Every warp has a range of the items of its own; the counts of its digits, behind those of smaller digits and of the ranges in front,
+// are where its items go.  Eight items of a lane are on their way at a time.
 __device__ void sortCluster(const Table& t, int n) {
   namespace cg = cooperative_groups;
+  constexpr int AHEAD = 8;
   __shared__ int hist[32][256];
-  __shared__ int total[256], scan[8];
+  __shared__ int quarter[4][256], total[256], scan[8];
   cg::cluster_group cluster = cg::this_cluster();
-  const int cta = cluster.block_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cta = cluster.block_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, digit = threadIdx.x & 255, part = threadIdx.x >> 8;
   const int range = ((n + SORT_WARPS - 1) / SORT_WARPS + 31) / 32 * 32;
   const long long begin = (long long)(cta * 32 + warp) * range;
   const int first = (int)min((long long)n, begin), last = (int)min((long long)n, begin + range);
   for (int pass = 0; pass < t.passes; ++pass) {
     const int shift = pass * 8;
+    const uint2* src = t.buf[pass & 1];
     uint2* dst = t.buf[(pass + 1) & 1];
+    auto load = [&](int base, uint2 (&item)[AHEAD]) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int i = base + u * 32 + lane;
+        if (i >= last) break;
+        if (pass) { item[u] = __ldcg(&src[i]); continue; }
+        const long long id = intAt(t.ids, t.wide, i);
+        item[u] = make_uint2(id >= 0 && id < t.rows && id != t.padding ? (uint32_t)id : (uint32_t)t.rows, (uint32_t)i);
+      }
+    };
     for (int i = lane; i < 256; i += 32) hist[warp][i] = 0;
     __syncwarp();
-    for (int i = first; i < last; i += 32) {
-      const bool in = i + lane < last;
-      const int digit = in ? (int)(itemAt(t, pass, i + lane).x >> shift & 255) : 256;
-      const uint32_t same = __match_any_sync(0xffffffffu, digit);
-      if (in && (same & ((1u << lane) - 1)) == 0) hist[warp][digit] += __popc(same);
-      __syncwarp();
-    }
-    __syncthreads();
-    if (threadIdx.x < 256) {                             // this block's ranges, in order
-      int run = 0;
-      for (int w = 0; w < 32; ++w) { const int c = hist[w][threadIdx.x]; hist[w][threadIdx.x] = run; run += c; }
-      total[threadIdx.x] = run;
-    }
-    cluster.sync();
-    int offset = 0;
-    if (threadIdx.x < 256) {                             // the blocks in front, and all smaller digits
-      int before = 0, all = 0;
-      for (int c = 0; c < SORT_CTAS; ++c) {
-        const int x = *cluster.map_shared_rank(&total[threadIdx.x], c);
-        if (c < cta) before += x;
-        all += x;
-      }
-      int inc = all;
+    for (int i = first; i < last; i += 32 * AHEAD) {
+      uint2 item[AHEAD];
+      load(i, item);
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += x; }
-      if (lane == 31) scan[warp] = inc;
-      offset = before + inc - all;
+      for (int u = 0; u < AHEAD; ++u)
+        if (i + u * 32 + lane < last) atomicAdd(&hist[warp][item[u].x >> shift & 255], 1);
     }
     __syncthreads();
-    if (threadIdx.x < 256) {
-      for (int w = 0; w < warp; ++w) offset += scan[w];
-      for (int w = 0; w < 32; ++w) hist[w][threadIdx.x] += offset;
-    }
+    // the warps in front (a quarter of them per thread), the blocks in front, all smaller digits
+    int own[8], run = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) own[w] = hist[part * 8 + w][digit];
+#pragma unroll
+    for (int w = 0; w < 8; ++w) { const int c = own[w]; own[w] = run; run += c; }
+    quarter[part][digit] = run;
     __syncthreads();
-    for (int i = first; i < last; i += 32) {
-      const bool in = i + lane < last;
-      const uint2 item = in ? itemAt(t, pass, i + lane) : make_uint2(0u, 0u);
-      const int digit = in ? (int)(item.x >> shift & 255) : 256;
-      const uint32_t same = __match_any_sync(0xffffffffu, digit), before = same & ((1u << lane) - 1);
-      if (in) dst[hist[warp][digit] + __popc(before)] = item;
-      __syncwarp();
-      if (in && before == 0) hist[warp][digit] += __popc(same);
-      __syncwarp();
+    int inFront = 0, sum = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) { const int c = quarter[q][digit]; inFront += q < part ? c : 0; sum += c; }
+    if (part == 0) total[digit] = sum;
+    cluster.sync();
+    int all = 0;
+    {
+      int c[SORT_CTAS];
+#pragma unroll
+      for (int k = 0; k < SORT_CTAS; ++k) c[k] = *cluster.map_shared_rank(&total[digit], k);
+#pragma unroll
+      for (int k = 0; k < SORT_CTAS; ++k) { inFront += k < cta ? c[k] : 0; all += c[k]; }
+    }
+    int inc = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += x; }
+    if (part == 0 && lane == 31) scan[warp] = inc;
+    __syncthreads();
+    inFront += inc - all;
+#pragma unroll
+    for (int w = 0; w < 7; ++w) inFront += w < (warp & 7) ? scan[w] : 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) hist[part * 8 + w][digit] = inFront + own[w];
+    __syncthreads();
+    for (int i = first; i < last; i += 32 * AHEAD) {
+      uint2 item[AHEAD];
+      load(i, item);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        if (i + u * 32 >= last) break;
+        const bool in = i + u * 32 + lane < last;
+        const int d = (int)(item[u].x >> shift & 255);
+        const uint32_t same = sameDigit(d, in), before = same & ((1u << lane) - 1);
+        int at = 0;
+        if (in) at = hist[warp][d];
+        __syncwarp();
+        if (in && before == 0) hist[warp][d] = at + __popc(same);
+        __syncwarp();
+        if (in) dst[at + __popc(before)] = item[u];
+      }
     }
     __threadfence();
     cluster.sync();                                      // all items in place; all counts read
   }
 }
 
-__global__ void __launch_bounds__(SORT_THREADS) sortAndClearKernel(const Backward a) {
+__global__ void __launch_bounds__(SORT_THREADS) sortTokensKernel(const Backward a) {
   tc::grid_dependency_wait();
+  tc::grid_launch_dependents();                          // the clearing starts now
+  sortCluster(a.t[blockIdx.x / SORT_CTAS], a.n);
+}
+
+// Runs beside the sort, which has seen the kernels in front of both end before it let this one start; ends behind it.  128 blocks: a
+// power of two of them clears 103 MB in 16.6 us, 148 in 18.6.
+__global__ void __launch_bounds__(256) clearKernel(const Backward a) {
   tc::grid_launch_dependents();
-  const int cluster = blockIdx.x / SORT_CTAS;
-  if (cluster < a.tables) { sortCluster(a.t[cluster], a.n); return; }
-  const size_t thread = (size_t)(blockIdx.x - a.tables * SORT_CTAS) * SORT_THREADS + threadIdx.x;
-  const size_t threads = (size_t)(gridDim.x - a.tables * SORT_CTAS) * SORT_THREADS;
+  const size_t thread = (size_t)blockIdx.x * 256 + threadIdx.x, threads = (size_t)gridDim.x * 256;
   for (int k = 0; k < a.tables; ++k) {
     uint4* dst = (uint4*)a.t[k].grad;
     const size_t packs = a.t[k].gradBytes / 16;
     for (size_t i = thread; i < packs; i += threads) dst[i] = make_uint4(0u, 0u, 0u, 0u);
     for (size_t i = packs * 16 + thread; i < a.t[k].gradBytes; i += threads) ((uint8_t*)a.t[k].grad)[i] = 0;
   }
+  tc::grid_dependency_wait();
 }
 
-// A block sums the tokens of a stretch for its columns (E per thread), row after row.
+// A block sums the tokens of a stretch for its columns (E per thread), row after row; eight rows are on their way at a time.
 template <typename T, int E>
 __global__ void __launch_bounds__(128) sumStretchKernel(const Backward a) {
   constexpr int MAX = 128, AHEAD = 8;
@@ -231,7 +321,7 @@ __global__ void __launch_bounds__(128) sumStretchKernel(const Backward a) {
   for (int i = 0; i < count; i += AHEAD) {
     P p[AHEAD];
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) if (i + u < count && keys[i + u + 1] != none) p[u] = *(const P*)(g + (size_t)tokens[i + u] * a.d);
+    for (int u = 0; u < AHEAD; ++u) p[u] = *(const P*)(g + (size_t)tokens[min(i + u, count - 1)] * a.d);
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       const int j = i + u;
@@ -241,9 +331,10 @@ __global__ void __launch_bounds__(128) sumStretchKernel(const Backward a) {
       const bool goesOn = keys[j + 2] == keys[j + 1];
       if (goesOn && j + 1 < count) continue;
       if (head || goesOn) {                                              // not all of the row
-        float* s = t.sums + ((size_t)blockIdx.x * 2 + (head ? 0 : 1)) * a.d + col;
+        Pack<float, E> s;
 #pragma unroll
-        for (int e = 0; e < E; ++e) s[e] = acc[e];
+        for (int e = 0; e < E; ++e) s.v[e] = acc[e];
+        *(Pack<float, E>*)(t.sums + ((size_t)blockIdx.x * 2 + (head ? 0 : 1)) * a.d + col) = s;
       } else {
         P o;
 #pragma unroll
@@ -257,58 +348,95 @@ __global__ void __launch_bounds__(128) sumStretchKernel(const Backward a) {
   }
 }
 
-// Rows that go on behind the stretch in which they begin: a block per such stretch and 32 packs of columns; SUM_GROUPS groups of threads
-// add up a part of the row's stretches each.
+// acc += the sums of stretches [from, to) of a row that goes through them.
+template <int E>
+__device__ __forceinline__ void addStretches(const float* s, size_t step, int from, int to, float (&acc)[E]) {
+#pragma unroll 4
+  for (int i = from; i < to; ++i) {
+    const Pack<float, E> x = *(const Pack<float, E>*)(s + i * step);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] += x.v[e];
+  }
+}
+
+// Rows that go on behind the stretch in which they begin, 32 packs of columns per block.  A warp looks whether its stretch has such a row
+// and adds up what few stretches it goes through; one that goes through more than eight, the block's warps add up together.  (With all rows
+// added up by one warp each, a row of 12000 tokens of 131072 took 35 us.)
 template <typename T, int E>
-__global__ void __launch_bounds__(32 * SUM_GROUPS) joinStretchKernel(const Backward a) {
-  __shared__ float part[SUM_GROUPS][32 * E];
+__global__ void __launch_bounds__(32 * JOIN_WARPS) joinStretchKernel(const Backward a) {
+  constexpr int FEW = 8;
+  __shared__ float part[JOIN_WARPS][32 * E];
+  __shared__ int rowKey[JOIN_WARPS], rowCount[JOIN_WARPS];
   tc::grid_dependency_wait();
   tc::grid_launch_dependents();
   const Table& t = a.t[blockIdx.z];
   const uint2* items = t.buf[t.passes & 1];
-  const int start = blockIdx.x * a.stretch, end = start + a.stretch;     // the last stretch has nothing behind it
-  const uint32_t key = __ldcg(&items[end - 1]).x;
-  if (key == (uint32_t)t.rows || __ldcg(&items[end]).x != key) return;
-  if (start > 0 && __ldcg(&items[start]).x == key && __ldcg(&items[start - 1]).x == key) return;      // it began further in front
-  int lo = end, hi = a.n;                                                // the first item behind the row
-  while (lo < hi) { const int mid = (lo + hi) >> 1; if (__ldcg(&items[mid]).x <= key) lo = mid + 1; else hi = mid; }
-  const int first = blockIdx.x + 1, count = (lo - 1) / a.stretch - first + 1;      // stretches that begin with it
-  const int group = threadIdx.x >> 5, lane = threadIdx.x & 31, col = (blockIdx.y * 32 + lane) * E;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = (blockIdx.y * 32 + lane) * E;
+  const int own = blockIdx.x * JOIN_WARPS + warp, start = own * a.stretch, end = start + a.stretch;
+  uint32_t key = 0;
+  int count = 0;                                                         // stretches that begin with the row
+  if (own + 1 < a.stretches) {                                           // (the last one has nothing behind it)
+    key = __ldcg(&items[end - 1]).x;
+    const uint32_t behind = __ldcg(&items[end]).x, front = __ldcg(&items[start]).x, before = start > 0 ? __ldcg(&items[start - 1]).x : 0xffffffffu;
+    if (key != (uint32_t)t.rows && behind == key && !(front == key && before == key)) {      // goes on, and did not begin further in front
+      int next = own + 1;                                                // the first that does not end with it
+      for (;;) {
+        const int at = next + lane;
+        const bool through = at < a.stretches && __ldcg(&items[min((at + 1) * a.stretch, a.n) - 1]).x == key;
+        const uint32_t stops = ~__ballot_sync(0xffffffffu, through);
+        if (stops) { next += __ffs(stops) - 1; break; }
+        next += 32;
+      }
+      count = next - own - 1 + (next < a.stretches && __ldcg(&items[next * a.stretch]).x == key ? 1 : 0);
+    }
+  }
+  if (lane == 0) { rowKey[warp] = (int)key; rowCount[warp] = count; }
+  const size_t step = (size_t)2 * a.d;
   float acc[E];
+  auto begin = [&](int stretch) {                                        // what the row has in the stretch in which it begins
+    const Pack<float, E> x = *(const Pack<float, E>*)(t.sums + stretch * step + a.d + col);
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  if (col < a.d) {
-    if (group == 0) {
-      const float* s = t.sums + ((size_t)blockIdx.x * 2 + 1) * a.d + col;
+    for (int e = 0; e < E; ++e) acc[e] = x.v[e];
+  };
+  auto store = [&](uint32_t row) {
+    Pack<T, E> o;
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = s[e];
-    }
-    const int per = (count + SUM_GROUPS - 1) / SUM_GROUPS, from = group * per, to = min(count, from + per);
-    const float* s = t.sums + (size_t)first * 2 * a.d + col;
-#pragma unroll 4
-    for (int i = from; i < to; ++i) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += s[(size_t)i * 2 * a.d + e];
-    }
+    for (int e = 0; e < E; ++e) o.v[e] = fromFloat<T>(acc[e] * t.scale);
+    *(Pack<T, E>*)((T*)t.grad + (size_t)row * a.d + col) = o;
+  };
+  if (count && count <= FEW && col < a.d) {
+    begin(own);
+    addStretches<E>(t.sums + (own + 1) * step + col, step, 0, count, acc);
+    store(key);
   }
-#pragma unroll
-  for (int e = 0; e < E; ++e) part[group][lane * E + e] = acc[e];
   __syncthreads();
-  if (group || col >= a.d) return;
-  Pack<T, E> o;
+  for (int w = 0; w < JOIN_WARPS; ++w) {
+    const int many = rowCount[w], first = blockIdx.x * JOIN_WARPS + w;
+    if (many <= FEW) continue;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    float s = 0.f;
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    const int per = (many + JOIN_WARPS - 1) / JOIN_WARPS;
+    if (col < a.d) {
+      if (warp == 0) begin(first);
+      addStretches<E>(t.sums + (first + 1) * step + col, step, min(many, warp * per), min(many, warp * per + per), acc);
+    }
+    __syncthreads();
 #pragma unroll
-    for (int k = 0; k < SUM_GROUPS; ++k) s += part[k][lane * E + e];
-    o.v[e] = fromFloat<T>(s * t.scale);
+    for (int e = 0; e < E; ++e) part[warp][lane * E + e] = acc[e];
+    __syncthreads();
+    if (warp || col >= a.d) continue;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int k = 1; k < JOIN_WARPS; ++k) acc[e] += part[k][lane * E + e];
+    store((uint32_t)rowKey[w]);
   }
-  *(Pack<T, E>*)((T*)t.grad + (size_t)key * a.d + col) = o;
 }
 
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
-// Tokens of a stretch: 16, more (up to 128) once there are more than 4096 stretches.
-int stretchOf(int n) { return std::min(128, std::max(16, (n + 4095) / 4096)); }
+// Tokens of a stretch: 16, more (up to 128) once there are more than 2048 stretches.
+int stretchOf(int n) { return std::min(128, std::max(16, (n + 2047) / 2048)); }
+int lanesOf(int packs, int most) { int l = 1; while (l < packs && l < most) l *= 2; return l; }
 struct Layout { size_t items, sums; };
 Layout layoutOf(int n, int d) {
   const int s = stretchOf(n);
@@ -317,23 +445,21 @@ Layout layoutOf(int n, int d) {
 
 template <typename T, int E>
 ncclResult_t forward(const Forward& a, cudaStream_t stream) {
-  const long long total = (long long)a.n * a.packs;
-  // Four packs a thread where that still leaves every SM two blocks.
-  if (total >= 4ll * 256 * 296) {
-    CUDACHECK(launchBehind(embedForwardKernel<T, E, 4>, dim3((unsigned)((total + 1023) / 1024)), 256, 1, stream, a));
-  } else {
-    CUDACHECK(launchBehind(embedForwardKernel<T, E, 1>, dim3((unsigned)((total + 255) / 256)), 256, 1, stream, a));
-  }
+  const long long perBlock = 8ll * (32 / a.lanes) * a.turns;
+  const bool plain = a.scale == 1.f;
+  auto* kernel = a.positions ? plain ? embedForwardKernel<T, E, EMBED_ADD> : embedForwardKernel<T, E, EMBED_SCALE_ADD>
+                             : plain ? embedForwardKernel<T, E, EMBED_COPY> : embedForwardKernel<T, E, EMBED_SCALE>;
+  CUDACHECK(launchBehind(kernel, dim3((unsigned)((a.n + perBlock - 1) / perBlock)), 256, 1, stream, a));
   return ncclSuccess;
 }
 
 template <typename T, int E>
 ncclResult_t backward(const Backward& a, cudaStream_t stream) {
-  CUDACHECK(launchBehind(sortAndClearKernel, dim3(SORT_CTAS * (a.tables + CLEAR_CLUSTERS)), SORT_THREADS, SORT_CTAS, stream, a));
+  CUDACHECK(launchBehind(sortTokensKernel, dim3(SORT_CTAS * a.tables), SORT_THREADS, SORT_CTAS, stream, a));
+  CUDACHECK(launchBehind(clearKernel, dim3(CLEAR_BLOCKS), 256, 1, stream, a));
   const int packs = a.d / E;
   CUDACHECK(launchBehind(sumStretchKernel<T, E>, dim3(a.stretches, (packs + 127) / 128, a.tables), 128, 1, stream, a));
-  if (a.stretches > 1)
-    CUDACHECK(launchBehind(joinStretchKernel<T, E>, dim3(a.stretches - 1, (packs + 31) / 32, a.tables), 32 * SUM_GROUPS, 1, stream, a));
+  if (a.stretches > 1) CUDACHECK(launchBehind(joinStretchKernel<T, E>, dim3((a.stretches + JOIN_WARPS - 2) / JOIN_WARPS, (packs + 31) / 32, a.tables), 32 * JOIN_WARPS, 1, stream, a));
   return ncclSuccess;
 }
 
@@ -349,12 +475,14 @@ DF_API ncclResult_t dfcclEmbeddingForward(const void* ids, int wideIds, int n, c
                                           const void* p, int64_t prows, int64_t ldp, void* out, int d, int type, float scale, cudaStream_t stream) {
   const int bytes = typeBytes(type);
   if (n <= 0 || d <= 0 || rows <= 0 || !bytes || !ids || !w || !out || ldw < d || (positions && (!p || prows <= 0 || ldp < d))) return ncclInvalidArgument;
-  Forward a{ids, positions, w, p, out, wideIds, widePositions, n, 0, rows, prows, ldw, ldp, scale};
+  Forward a{ids, positions, w, p, out, wideIds, widePositions, n, 0, 0, 0, rows, prows, ldw, ldp, scale};
   const uintptr_t grid = (uintptr_t)w | (uintptr_t)out | (uintptr_t)(ldw * bytes) | (uintptr_t)((size_t)d * bytes) |
                          (positions ? (uintptr_t)p | (uintptr_t)(ldp * bytes) : 0);
   const bool whole = (grid & 15) == 0;
   a.packs = whole ? d / (16 / bytes) : d;
-  if ((long long)n * a.packs > 0x7fffffffll * 256) return ncclInvalidArgument;
+  a.lanes = lanesOf(a.packs, 32);
+  // rows one after the other, 8 at most, once there are more than 64 warps of them per SM
+  { const int64_t warps = 148 * 64, side = 32 / a.lanes; a.turns = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(8, a.lanes), n / (warps * side))); }
   if (type == ncclFloat32) return whole ? forward<float, 4>(a, stream) : forward<float, 1>(a, stream);
   if (type == ncclBfloat16) return whole ? forward<__nv_bfloat16, 8>(a, stream) : forward<__nv_bfloat16, 1>(a, stream);
   return whole ? forward<__half, 8>(a, stream) : forward<__half, 1>(a, stream);
