@@ -70,25 +70,25 @@ ncclResult_t dfcclEmbeddingBackward(const void* g, int n, int d, int type, const
 size_t dfcclEmbeddingBackwardWork(int n, int d, int tables);
 
 /* ---- losses of z = x w^T, x [n, d], w [v, d] (bf16, contiguous, 16-byte aligned, d % 8 == 0), without keeping z.
- * Every row has a list of k vocabulary entries with weights q that add up to 1; loss = T^2 sum q (ln q - ln softmax(z / T)).  The lists
- * come from targets (k = 1, weights null) or from a teacher's logits (k <= dfcclLinearLossMaxList()).  state [n]: 0 a row without a list
- * (loss 0, no gradient), 1 a row with one, 2 a row with a token outside the vocabulary (loss and gradients NaN). */
-ncclResult_t dfcclTargetRows(const void* targets, int wide, int n, int v, int64_t ignore, void* tokens /* int32 [n] */, void* state /* int32 [n] */,
-                             cudaStream_t stream);
-/* q = softmax(logits / temperature) over the entries of a row whose token is not -1 and whose logit is not -inf, in the order of their tokens.
- * logitType: ncclFloat32, ncclBfloat16 or ncclFloat16. */
+ * Every row is compared with a target (`targets`: 64-bit integers where `wide` is set, 32-bit otherwise; `ignore`: no target; k = 1) or,
+ * with targets null, with a list of k <= dfcclLinearLossMaxList() vocabulary entries whose weights q add up to 1 (dfcclTeacherRows):
+ * loss = T^2 sum q (ln q - ln softmax(z / T)).  A target outside the vocabulary makes its row's loss and gradients NaN. */
+/* Lists from a teacher's logits: q = softmax(logits / temperature) over the entries of a row whose token is not -1 and whose logit is not
+ * -inf, in the order of their tokens.  logitType: ncclFloat32, ncclBfloat16 or ncclFloat16.  state: 0 a row without an entry (loss 0, no
+ * gradient), 1 a row with some, 2 a row with a token outside the vocabulary (NaN). */
 ncclResult_t dfcclTeacherRows(const void* logits, int logitType, const void* tokens, int wide, int n, int k, int v, float temperature,
-                              void* outTokens /* int32 [n, k] */, void* outWeights /* fp32 [n, k] */, void* state, cudaStream_t stream);
-/* lse [n]: log2 of the sum of 2^(z log2(e) / T), kept for the backward pass; rowLoss [n]; reduction 1 (mean over the rows whose state is
- * not 0; 0 where there is none) or 2 (sum): loss and count (int32), one each; 0: neither.  All fp32. */
-ncclResult_t dfcclLinearLossForward(const void* x, const void* w, int n, int v, int d, const void* tokens, const void* weights, const void* state, int k,
-                                    float temperature, int reduction, void* work, void* lse, void* rowLoss, void* loss, void* count, cudaStream_t stream);
+                              void* outTokens /* int32 [n, k] */, void* outWeights /* fp32 [n, k] */, void* state /* int32 [n] */, cudaStream_t stream);
+/* lse [n]: log2 of the sum of 2^(z log2(e) / T), kept for the backward pass; reduction 0: rowLoss [n]; 1 (mean over the rows with a target
+ * or list; 0 where there is none) or 2 (sum): loss and count (int32), one each.  All fp32. */
+ncclResult_t dfcclLinearLossForward(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, const void* tokens,
+                                    const void* weights, const void* state, int k, float temperature, int reduction, void* work, void* lse, void* rowLoss,
+                                    void* loss, void* count, cudaStream_t stream);
 size_t dfcclLinearLossForwardWork(int n, int v, int k);
 /* dx and dw (either may be null) for the gradient gout of the loss: one value (goutStride 0) or one per row; count: of a mean, else null.
  * The gradient of the logits exists for as many columns at a time as DFCCL_LOSS_WORKSPACE_BYTES (1 GiB) hold. */
-ncclResult_t dfcclLinearLossBackward(const void* x, const void* w, int n, int v, int d, const void* tokens, const void* weights, const void* state, int k,
-                                     float temperature, const void* lse, const void* gout, int goutStride, const void* count, void* dx, void* dw, void* work,
-                                     size_t workBytes, cudaStream_t stream);
+ncclResult_t dfcclLinearLossBackward(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, const void* tokens,
+                                     const void* weights, const void* state, int k, float temperature, const void* lse, const void* gout, int goutStride,
+                                     const void* count, void* dx, void* dw, void* work, size_t workBytes, cudaStream_t stream);
 size_t dfcclLinearLossBackwardWork(int n, int v, int d, int wantX, int wantW);
 int dfcclLinearLossMaxList(void);
 

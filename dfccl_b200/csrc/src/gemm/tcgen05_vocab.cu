@@ -1,7 +1,7 @@
 // Products over a large vocabulary for the losses of a language model's head, on CTA pairs (tcgen05 cta_group::2), bf16 with fp32
 // accumulators in tensor memory.  With z = x w^T, x [n, d] and the head w [v, d]:
 //   VOCAB_STATS     of every row the maximum and the sum of powers of each stretch of its logits, and the logits of its targets
-//   VOCAB_GRAD      dz = coef (softmax(z) - target): the logits are computed again, what is stored is their gradient, rounded once
+//   VOCAB_GRAD      dz = g (softmax(z) - target): the logits are computed again, what is stored is their gradient, rounded once
 //   VOCAB_PRODUCTS  dx = dz w and dw = dz^T x, in one launch
 // A logit exists in tensor memory and registers only.  Computing the product again costs a third more than the two products
 // of the gradients do by themselves; keeping n v logits or powers of them would cost their rounding twice (1.7 times the error of one
@@ -45,7 +45,9 @@ struct VocabArgs {
   VocabRows rows;
   float2* parts;
   float* picked;
+  int* ticket;
   VocabGrad grad;
+  VocabFactor factor;
   __nv_bfloat16* dz;
   int ld, first;                    // of dz; first column of the vocabulary
   uint32_t* err;
@@ -93,12 +95,14 @@ __device__ __forceinline__ Tile tileOf(const Product& p, int item) {
 struct List {
   const int* tokens;
   int k, pos, next;
-  __device__ __forceinline__ void seek(const int* t, int n, int col) {
-    tokens = t; k = n;
-    int lo = 0, hi = n;
-    while (lo < hi) { const int mid = (lo + hi) >> 1; if (tokens[mid] < col) lo = mid + 1; else hi = mid; }
-    pos = lo;
-    next = lo < k ? tokens[lo] : VOCAB_NO_TOKEN;
+  __device__ __forceinline__ void seek(const VocabRows& r, int row, int token, int col) {
+    pos = 0; k = 1; tokens = nullptr;
+    next = token >= col ? token : VOCAB_NO_TOKEN;
+    if (r.targets) return;
+    k = r.k; tokens = r.tokens + (size_t)row * k;
+    int hi = k;
+    while (pos < hi) { const int mid = (pos + hi) >> 1; if (tokens[mid] < col) pos = mid + 1; else hi = mid; }
+    next = pos < k ? tokens[pos] : VOCAB_NO_TOKEN;
   }
   __device__ __forceinline__ void step() { ++pos; next = pos < k ? tokens[pos] : VOCAB_NO_TOKEN; }
 };
@@ -137,6 +141,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
   const uint32_t tmemBase = *tmemBaseSlot;
   grid_dependency_wait();
   grid_launch_dependents();
+  if (MODE == VOCAB_STATS && g.ticket && blockIdx.x == 0 && threadIdx.x == 0) *g.ticket = 0;
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs; bytes counted in the leader)
@@ -218,6 +223,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
     // ------------------------------------------------------------ epilogue: a row of my 128 per lane, 32 columns at a time
     const int quarter = warp & 3, part = (warp - 2) >> 2;
     const uint32_t accEmptyLeader0 = mapa_u32(smem_u32(&accEmpty[0]), 0), accEmptyLeader1 = mapa_u32(smem_u32(&accEmpty[1]), 0);
+    const float factor = MODE == VOCAB_PRODUCTS ? vocabFactor(g.factor) : 1.f;
     for (int j = 0; j < count; ++j) {
       int item;
       const int which = MODE == VOCAB_PRODUCTS ? items.at(j, item) : (items.at(j, item), 0);
@@ -235,14 +241,14 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
         const float scale = g.rows.scale;
         float lse = 0.f, coef = 0.f;
         if (here) {                                    // on its way while the accumulator is computed
+          int token;
+          const int state = rowState(g.rows, row, token);
           if (MODE == VOCAB_GRAD) {
-            const int state = g.grad.state[row];
             lse = g.grad.lse[row];
-            coef = g.grad.gout[(size_t)row * g.grad.goutStride] * g.grad.temperature;
-            if (g.grad.count) coef = coef / (float)max(1, *g.grad.count);
-            if (state != 1) coef = state ? __int_as_float(0x7fffffff) : 0.f;
+            coef = g.grad.gout ? g.grad.gout[(size_t)row * g.grad.goutStride] : 1.f;
+            if (state != ROW_LIST) coef = state == ROW_BAD ? __int_as_float(0x7fffffff) : 0.f;
           }
-          list.seek(g.rows.tokens + (size_t)row * g.rows.k, g.rows.k, g.first + col0);
+          list.seek(g.rows, row, token, g.first + col0);
         }
         if (!mbar_wait(&accFull[ab], (j >> 1) & 1, giveUp, WAIT_NS)) break;
         tc_fence_after();
@@ -286,7 +292,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
             while (list.next < g.first + c + 32) {
               if (list.next >= g.first + c) {
                 const int at = list.next - g.first - c;
-                const float q = g.rows.weights ? g.rows.weights[(size_t)row * g.rows.k + list.pos] : 1.f;
+                const float q = g.rows.targets ? 1.f : g.rows.weights[(size_t)row * g.rows.k + list.pos];
 #pragma unroll
                 for (int e = 0; e < 32; ++e) if (e == at) r[e] = __float_as_uint(__uint_as_float(r[e]) - q);
               }
@@ -342,7 +348,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
             for (int v = 0; v < 4; ++v) {
               uint32_t* ow = (uint32_t*)&o[v];
 #pragma unroll
-              for (int w = 0; w < 4; ++w) ow[w] = pack_bf16x2(__uint_as_float(r[8 * v + 2 * w]), __uint_as_float(r[8 * v + 2 * w + 1]));
+              for (int w = 0; w < 4; ++w) ow[w] = pack_bf16x2(__uint_as_float(r[8 * v + 2 * w]) * factor, __uint_as_float(r[8 * v + 2 * w + 1]) * factor);
             }
             __nv_bfloat16* dst = p.out + (size_t)row * p.N + c;
             if (packs == 4) { st_global32(dst, o, p.wide); st_global32(dst + 16, o + 2, p.wide); }
@@ -410,11 +416,11 @@ ncclResult_t logits(CUtensorMap* a, CUtensorMap* b, VocabArgs* g, const void* x,
 
 }  // namespace
 
-ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, float* picked, cudaStream_t stream) {
+ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, float* picked, int* ticket, cudaStream_t stream) {
   CUtensorMap a, b;
   VocabArgs g;
   DFCHECK(logits(&a, &b, &g, x, w, n, v, d, rows));
-  g.parts = parts; g.picked = picked;
+  g.parts = parts; g.picked = picked; g.ticket = ticket;
   return launchVocab<VOCAB_STATS>(a, b, a, b, g, stream);
 }
 
@@ -440,11 +446,12 @@ VocabPlan vocabProductPlan(int n, int v, int d, bool wantX, bool wantW, int pair
   return VocabPlan{cut(tn * td, kv), cut(tv * td, kn)};
 }
 
-ncclResult_t vocabProducts(const void* dz, const void* x, const void* w, int n, int v, int d, const VocabPlan& plan, void* dx, float* partX, bool addX,
-                           void* dw, float* partW, cudaStream_t stream) {
+ncclResult_t vocabProducts(const void* dz, const void* x, const void* w, int n, int v, int d, const VocabPlan& plan, const VocabFactor& factor, void* dx, float* partX,
+                           bool addX, void* dw, float* partW, cudaStream_t stream) {
   const int ld = (v + 63) / 64 * 64;
   CUtensorMap a[2], b[2];
   VocabArgs g = {};
+  g.factor = factor;
   int k = 0;
   auto narrow = [&](CUtensorMap* m, const void* base, int rows) {      // [rows of the contraction][d columns]
     return d % 64 ? gemmEncodeMap(m, base, (uint64_t)rows, (uint64_t)d, BK) : gemmEncodeMap3(m, base, (uint64_t)d, (uint64_t)rows, 1, HALF, BK);

@@ -12,41 +12,69 @@ constexpr int VOCAB_TILE = 256;              // rows and columns of a tile
 constexpr int VOCAB_PARTS = 2;               // epilogue warps that share 32 rows of a tile: each leaves a maximum and a sum of its own
 constexpr int VOCAB_NO_TOKEN = 0x7fffffff;   // behind the last entry of a row's list
 
-// What a row of logits is compared with: a list of vocabulary entries in ascending order (VOCAB_NO_TOKEN behind the last one) with the
-// weight of each.  One entry of weight 1 is a target of the cross entropy.
+// What the rows of logits are compared with: a target each (`targets`), or a list of vocabulary entries in ascending order (VOCAB_NO_TOKEN
+// behind the last one) with the weight of each.  A target is a list of one entry of weight 1.
 struct VocabRows {
+  const void* targets;          // [n] 64-bit integers (wide) or 32-bit, or null: lists
+  int wide, v;                  // v: of the whole vocabulary
+  long long ignore;
   const int* tokens;            // [n][k]
-  const float* weights;         // [n][k], or null: 1
-  int k;
+  const float* weights;         // [n][k]
+  const int* state;             // [n]
+  int k;                        // 1 beside targets
   float scale;                  // logits -> exponents of two: log2(e) / temperature
 };
+enum RowState { ROW_NONE = 0, ROW_LIST = 1, ROW_BAD = 2 };      // nothing to compare with; something; a token outside the vocabulary
+
+#if defined(__CUDACC__)
+__device__ __forceinline__ int rowState(const VocabRows& r, int row, int& token) {
+  if (!r.targets) { token = VOCAB_NO_TOKEN; return r.state[row]; }
+  const long long t = r.wide ? ((const long long*)r.targets)[row] : ((const int*)r.targets)[row];
+  const bool in = t >= 0 && t < r.v && t != r.ignore;
+  token = in ? (int)t : VOCAB_NO_TOKEN;
+  return in ? ROW_LIST : t == r.ignore ? ROW_NONE : ROW_BAD;
+}
+__device__ __forceinline__ int rowState(const VocabRows& r, int row) { int token; return rowState(r, row, token); }
+#endif
 
 inline int vocabParts(int v) { return (v + VOCAB_TILE - 1) / VOCAB_TILE * VOCAB_PARTS; }
 
 // z = x [n, d] w[v, d]^T, tile by tile and never stored.  Of every row: for each of the vocabParts(v) stretches of its columns
-// {largest z scale, sum of 2^(z scale - that)} -> parts [stretch][n], and the z of its list's entries -> picked [n][k].
-ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, float* picked, cudaStream_t stream);
+// {largest z scale, sum of 2^(z scale - that)} -> parts [stretch][n], and the z of its list's entries -> picked [n][k].  `ticket`, where given, is set to 0.
+ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, float* picked, int* ticket, cudaStream_t stream);
 
-// dz = coef (2^(z scale - lse) - weight where an entry is in the list) for the columns [0, v) of w, which start at column `first` of the
-// vocabulary: bf16, [n][ld], ld = v rounded up to 64 (zeros behind v).
-struct VocabGrad {
-  const float* lse;             // [n] log2 of the sum of 2^(z scale)
-  const float* gout;            // gradient of the loss: [n] or, with goutStride 0, one
-  int goutStride;
+// What all rows' gradients share: the gradient of the reduced loss, a mean's count, the temperature.  It does not go into dz, where its
+// rounding to bf16 would be the same for all of them (a mean over 32113 rows: dx 3.1e-3 off, 1.7e-3 without), but into the results.
+struct VocabFactor {
+  const float* gout;            // one value, or null: the rows have their own
   const int* count;             // rows that share a mean, or null
-  const int* state;             // [n] 0: no gradient, 1: a row with a list, 2: a row with a token outside the vocabulary (NaN)
   float temperature;
 };
+// dz = g (2^(z scale - lse) - weight where an entry is in the list), 0 in rows without a list and NaN in those with a token outside the
+// vocabulary, for the columns [0, v) of w, which start at column `first` of the vocabulary: bf16, [n][ld], ld = v rounded up to 64 (zeros behind v).
+struct VocabGrad {
+  const float* lse;             // [n] log2 of the sum of 2^(z scale)
+  const float* gout;            // g [n], or null: 1
+  int goutStride;
+};
 ncclResult_t vocabGrad(const void* x, const void* w, int n, int v, int first, int d, const VocabRows& rows, const VocabGrad& grad, void* dz, cudaStream_t stream);
+
+#if defined(__CUDACC__)
+__device__ __forceinline__ float vocabFactor(const VocabFactor& f) {
+  float s = f.gout ? *f.gout * f.temperature : f.temperature;
+  if (f.count) s /= (float)max(1, *f.count);
+  return s;
+}
+#endif
 
 // How the contractions of the two products are cut: blocks of 64 in a slice.
 struct VocabPlan { int perX, perW; };
 VocabPlan vocabProductPlan(int n, int v, int d, bool wantX, bool wantW, int pairs);
 inline int vocabSlices(int k, int per) { return ((k + 63) / 64 + per - 1) / per; }
 
-// dx [n, d] = dz w and dw [v, d] = dz^T x in one launch; either may be left out (null).  dx is bf16 where `partX` is null, otherwise
-// an fp32 sum [slice][n][d] of each slice of the vocabulary, added to what is there with `addX`; dw likewise with partW.
-ncclResult_t vocabProducts(const void* dz, const void* x, const void* w, int n, int v, int d, const VocabPlan& plan, void* dx, float* partX, bool addX,
-                           void* dw, float* partW, cudaStream_t stream);
+// dx [n, d] = factor dz w and dw [v, d] = factor dz^T x in one launch; either may be left out (null).  dx is bf16 where `partX` is null, otherwise
+// an fp32 sum [slice][n][d] of each slice of the vocabulary, without the factor, added to what is there with `addX`; dw likewise with partW.
+ncclResult_t vocabProducts(const void* dz, const void* x, const void* w, int n, int v, int d, const VocabPlan& plan, const VocabFactor& factor, void* dx, float* partX,
+                           bool addX, void* dw, float* partW, cudaStream_t stream);
 
 }  // namespace dfccl

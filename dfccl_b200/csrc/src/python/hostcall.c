@@ -28,6 +28,38 @@ static PyObject* call(PyObject* self, PyObject* const* args, Py_ssize_t n) {
   return PyLong_FromLong(r);
 }
 
-static PyMethodDef methods[] = {{"call", (PyCFunction)(void (*)(void))call, METH_FASTCALL, "call(address, arguments...) -> int"}, {NULL, NULL, 0, NULL}};
+/* The same for longer lists, with floats among them (both conventions pass those in registers of their own, in their order, wherever
+ * they stand): up to 24 integers, addresses or None and one float, which the entry point takes as a C float. */
+#define MAX_LONG 24
+typedef int (*LongEntry)(uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t,
+                         uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, float);
+static PyObject* call_long(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  uint64_t v[MAX_LONG + 1] = {0};
+  float f = 0.0f;
+  int ints = 0, floats = 0;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    if (PyFloat_Check(args[i])) {
+      if (i == 0 || ++floats > 1) { PyErr_SetString(PyExc_TypeError, "one float at most"); return NULL; }
+      f = (float)PyFloat_AsDouble(args[i]);
+      continue;
+    }
+    if (ints > MAX_LONG) break;
+    if (args[i] != Py_None) {
+      v[ints] = PyLong_AsUnsignedLongLongMask(args[i]);
+      if (v[ints] == (uint64_t)-1 && PyErr_Occurred()) return NULL;
+    }
+    ++ints;
+  }
+  if (ints < 1 || ints + floats != n) { PyErr_SetString(PyExc_TypeError, "an address and at most 24 arguments beside a float"); return NULL; }
+  if (v[0] == 0) { PyErr_SetString(PyExc_TypeError, "no address"); return NULL; }
+  int r;
+  Py_BEGIN_ALLOW_THREADS
+  r = ((LongEntry)(uintptr_t)v[0])(v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15], v[16], v[17], v[18], v[19], v[20],
+                                   v[21], v[22], v[23], v[24], f);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(r);
+}
+
+static PyMethodDef methods[] = {{"call_long", (PyCFunction)(void (*)(void))call_long, METH_FASTCALL, "call_long(address, arguments...) -> int"}, {"call", (PyCFunction)(void (*)(void))call, METH_FASTCALL, "call(address, arguments...) -> int"}, {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "dfccl_hostcall", NULL, -1, methods, NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit_dfccl_hostcall(void) { return PyModule_Create(&module); }

@@ -74,11 +74,16 @@ class DfcclError(RuntimeError):
 _lib = None
 _lock = threading.Lock()
 _entries: Dict[str, Callable[..., int]] = {}
+_long_entries: Dict[str, Callable[..., int]] = {}
+
+
+_hostcall_module = None
 
 
 @functools.lru_cache(maxsize=None)
 def _hostcall():
     """The extension's ``call``, or None where it is missing and cannot be compiled (no compiler, no interpreter headers)."""
+    global _hostcall_module
     path = _build.try_hostcall()
     if path is None:
         return None
@@ -86,6 +91,7 @@ def _hostcall():
         loader = importlib.machinery.ExtensionFileLoader("dfccl_hostcall", str(path))
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("dfccl_hostcall", loader))
         loader.exec_module(module)
+        _hostcall_module = module
         return module.call
     except (ImportError, OSError):
         return None
@@ -102,6 +108,17 @@ def entry(name: str) -> Callable[..., int]:
         else:
             f = lambda *a: slow(*(NO_CALLBACK if t is CALLBACK and x is None else x for x, t in zip(a, slow.argtypes)))        # noqa: E731
         _entries[name] = f
+    return f
+
+
+def long_entry(name: str) -> Callable[..., int]:
+    """The same for entry points with up to 24 such arguments and one float."""
+    f = _long_entries.get(name)
+    if f is None:
+        slow = getattr(lib(), name)
+        fast = _hostcall() is not None
+        f = functools.partial(_hostcall_module.call_long, C.cast(slow, C.c_void_p).value) if fast else slow
+        _long_entries[name] = f
     return f
 
 
@@ -177,9 +194,9 @@ def lib() -> C.CDLL:
             "dfcclLayerNormBackward": [vp] * 10 + [i, i, vp], "dfcclLayerNormWork": [i, i], "dfcclLayerNormMaxWidth": [],
             "dfcclEmbeddingForward": [vp, i, i, vp, i64, i64, vp, i, vp, i64, i64, vp, i, i, C.c_float, vp],
             "dfcclEmbeddingBackward": [vp, i, i, i, vp, i, i64, C.c_float, vp, i64, vp, i, vp, i64, vp, vp], "dfcclEmbeddingBackwardWork": [i, i, i],
-            "dfcclTargetRows": [vp, i, i, i, i64, vp, vp, vp], "dfcclTeacherRows": [vp, i, vp, i, i, i, i, C.c_float, vp, vp, vp, vp],
-            "dfcclLinearLossForward": [vp, vp, i, i, i, vp, vp, vp, i, C.c_float, i, vp, vp, vp, vp, vp, vp], "dfcclLinearLossForwardWork": [i, i, i],
-            "dfcclLinearLossBackward": [vp, vp, i, i, i, vp, vp, vp, i, C.c_float, vp, vp, i, vp, vp, vp, vp, sz, vp],
+            "dfcclTeacherRows": [vp, i, vp, i, i, i, i, C.c_float, vp, vp, vp, vp],
+            "dfcclLinearLossForward": [vp, vp, i, i, i, vp, i, i64, vp, vp, vp, i, C.c_float, i, vp, vp, vp, vp, vp, vp], "dfcclLinearLossForwardWork": [i, i, i],
+            "dfcclLinearLossBackward": [vp, vp, i, i, i, vp, i, i64, vp, vp, vp, i, C.c_float, vp, vp, i, vp, vp, vp, vp, sz, vp],
             "dfcclLinearLossBackwardWork": [i, i, i, i, i], "dfcclLinearLossMaxList": [],
             "dfcclGemmCheck": [C.POINTER(i)],
             "dfcclGemmPairResident": [C.POINTER(i)], "dfcclGemmPlan": [i, i, i, i, i, i, C.POINTER(i)],

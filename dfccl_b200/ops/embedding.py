@@ -1,13 +1,14 @@
 """Embedding of tokens with the gradients of its tables by sorted tokens (``csrc/src/ops/embed.cu``)."""
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from .. import native as nv
-from ..utils.tensors import nccl_dtype, on_device, raw_stream
+from ..utils.tensors import nccl_dtype, on_device, stream_of
 
 TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -31,49 +32,55 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _forward(ids, weight, positions, position_weight, scale):
+    n, d = ids.numel(), weight.shape[1]
+    out = torch.empty(*ids.shape, d, dtype=weight.dtype, device=weight.device)
+    if n == 0:
+        return out
+    w = _rows(weight)
+    if positions is None:
+        second = (None, 0, None, 0, 0)
+    else:
+        p = _rows(position_weight)
+        second = (positions.data_ptr(), int(positions.dtype == torch.int64), p.data_ptr(), p.shape[0], p.stride(0))
+    with on_device(w.device):
+        nv.check(nv.long_entry("dfcclEmbeddingForward")(ids.data_ptr(), int(ids.dtype == torch.int64), n, w.data_ptr(), w.shape[0], w.stride(0), *second, out.data_ptr(),
+                                                        d, nccl_dtype(w.dtype), scale, stream_of(w)), "dfcclEmbeddingForward")
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _backward_work(n: int, d: int, tables: int) -> int:
+    return nv.lib().dfcclEmbeddingBackwardWork(n, d, tables)
 
 
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, positions, position_weight, scale, padding):
-        n, d = ids.numel(), weight.shape[1]
-        out = torch.empty(*ids.shape, d, dtype=weight.dtype, device=weight.device)
-        ids = ids.contiguous()
-        w, p = _rows(weight), None
-        if positions is not None:
-            positions, p = positions.contiguous(), _rows(position_weight)
-        if n:
-            with on_device(weight.device):
-                nv.check(nv.lib().dfcclEmbeddingForward(ids.data_ptr(), int(ids.dtype == torch.int64), n, w.data_ptr(), w.shape[0], w.stride(0), _ptr(positions),
-                                                        int(positions is not None and positions.dtype == torch.int64), _ptr(p),
-                                                        0 if p is None else p.shape[0], 0 if p is None else p.stride(0), out.data_ptr(), d,
-                                                        nccl_dtype(w.dtype), scale, raw_stream(weight.device)), "dfcclEmbeddingForward")
         ctx.save_for_backward(ids, positions)
-        ctx.rows, ctx.prows, ctx.scale, ctx.padding = weight.shape[0], 0 if p is None else p.shape[0], scale, padding
+        ctx.rows, ctx.prows, ctx.scale, ctx.padding = weight.shape[0], 0 if positions is None else position_weight.shape[0], scale, padding
         ctx.set_materialize_grads(False)
-        return out
+        return _forward(ids, weight, positions, position_weight, scale)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        ids, positions = ctx.saved_tensors
-        if g is None:
+        want_w, want_p = ctx.needs_input_grad[1], ctx.needs_input_grad[3]
+        if g is None or not (want_w or want_p):
             return None, None, None, None, None, None
-        n, d = ids.numel(), g.shape[-1]
-        g = g.contiguous()
-        want_w, want_p = ctx.needs_input_grad[1], positions is not None and ctx.needs_input_grad[3]
+        ids, positions = ctx.saved_tensors
+        n, d, device = ids.numel(), g.shape[-1], g.device
         make = torch.empty if n else torch.zeros
-        gw = make(ctx.rows, d, dtype=g.dtype, device=g.device) if want_w else None
-        gp = make(ctx.prows, d, dtype=g.dtype, device=g.device) if want_p else None
-        if n and (want_w or want_p):
-            with on_device(g.device):
-                work = torch.empty(nv.lib().dfcclEmbeddingBackwardWork(n, d, int(want_w) + int(want_p)), dtype=torch.uint8, device=g.device)
-                nv.check(nv.lib().dfcclEmbeddingBackward(g.data_ptr(), n, d, nccl_dtype(g.dtype), ids.data_ptr(), int(ids.dtype == torch.int64), ctx.padding,
-                                                         ctx.scale, _ptr(gw), ctx.rows, _ptr(positions),
-                                                         int(positions is not None and positions.dtype == torch.int64), _ptr(gp), ctx.prows,
-                                                         work.data_ptr(), raw_stream(g.device)), "dfcclEmbeddingBackward")
+        gw = make(ctx.rows, d, dtype=g.dtype, device=device) if want_w else None
+        gp = make(ctx.prows, d, dtype=g.dtype, device=device) if want_p else None
+        if n:
+            g = g.contiguous()
+            second = (None, 0, None, 0) if gp is None else (positions.data_ptr(), int(positions.dtype == torch.int64), gp.data_ptr(), ctx.prows)
+            with on_device(device):
+                work = torch.empty(_backward_work(n, d, want_w + want_p), dtype=torch.uint8, device=device)
+                nv.check(nv.long_entry("dfcclEmbeddingBackward")(g.data_ptr(), n, d, nccl_dtype(g.dtype), ids.data_ptr(), int(ids.dtype == torch.int64), ctx.padding,
+                                                                 ctx.scale, None if gw is None else gw.data_ptr(), ctx.rows, *second, work.data_ptr(), stream_of(g)),
+                         "dfcclEmbeddingBackward")
         return None, gw, None, gp, None, None
 
 
@@ -89,7 +96,8 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, po
     _table("weight", weight)
     if (positions is None) != (position_weight is None):
         raise ValueError("positions and position_weight belong together")
-    tensors = [ids, weight]
+    device = weight.device
+    here = device.type == "cuda" and ids.device == device
     if positions is not None:
         _index("positions", positions)
         _table("position_weight", position_weight)
@@ -97,11 +105,15 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, po
             raise ValueError(f"positions of {tuple(positions.shape)} for ids of {tuple(ids.shape)}")
         if position_weight.shape[1] != weight.shape[1] or position_weight.dtype != weight.dtype:
             raise ValueError(f"position_weight of {tuple(position_weight.shape)} {position_weight.dtype} beside weight of {tuple(weight.shape)} {weight.dtype}")
-        tensors += [positions, position_weight]
+        here = here and positions.device == device and position_weight.device == device
+        positions = positions.contiguous()
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"padding_idx {padding_idx} outside a table of {weight.shape[0]} rows")
     if ids.numel() > 2 ** 31 - 4096:
         raise ValueError(f"{ids.numel()} tokens in one call, more than 31 bits count")
-    if not all(t.is_cuda and t.device == weight.device for t in tensors):
+    if not here:
         raise ValueError("the embedding runs on tensors of one GPU")
-    return _EmbeddingFn.apply(ids, weight, positions, position_weight, float(scale), -1 if padding_idx is None else int(padding_idx))
+    ids, scale = ids.contiguous(), float(scale)
+    if torch.is_grad_enabled() and (weight.requires_grad or (position_weight is not None and position_weight.requires_grad)):
+        return _EmbeddingFn.apply(ids, weight, positions, position_weight, scale, -1 if padding_idx is None else int(padding_idx))
+    return _forward(ids, weight, positions, position_weight, scale)

@@ -2,13 +2,13 @@
 ``csrc/src/gemm/tcgen05_vocab.cu``): cross entropy with a target per row, distillation from a teacher's top logits."""
 from __future__ import annotations
 
-from typing import Optional
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from .. import native as nv
-from ..utils.tensors import nccl_dtype, on_device, raw_stream
+from ..utils.tensors import nccl_dtype, on_device, stream_of
 from .block import packed
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -37,58 +37,89 @@ def _check(x: torch.Tensor, weight: torch.Tensor, index: torch.Tensor, name: str
         raise ValueError("more rows or entries than 31 bits count")
 
 
-def _on_one_gpu(*tensors: torch.Tensor) -> None:
-    if not all(t.is_cuda and t.device == tensors[0].device for t in tensors):
+def _on_one_gpu(device: torch.device, *tensors: torch.Tensor) -> None:
+    if device.type != "cuda" or any(t.device != device for t in tensors):
         raise ValueError("the losses run on tensors of one GPU")
 
 
-class _LinearLossFn(torch.autograd.Function):
-    """Rows are compared with lists of entries (``tokens``, ``weights``, ``state``: the C interface)."""
+@functools.lru_cache(maxsize=1024)
+def _forward_work(n: int, v: int, k: int) -> int:
+    return nv.lib().dfcclLinearLossForwardWork(n, v, k)
 
+
+class _Rows:
+    """What the rows are compared with, as the C interface takes it: a target each, or lists of ``k`` entries."""
+    __slots__ = ("targets", "ignore", "lists", "k", "temperature")
+
+    def __init__(self, targets, ignore, lists, k, temperature):
+        self.targets, self.ignore, self.lists, self.k, self.temperature = targets, ignore, lists, k, temperature
+
+    def tensors(self):
+        return (self.targets,) if self.lists is None else self.lists
+
+    def args(self):
+        if self.lists is None:
+            return self.targets.data_ptr(), int(self.targets.dtype == torch.int64), self.ignore, None, None, None, 1, 1.0
+        tokens, weights, state = self.lists
+        return None, 0, 0, tokens.data_ptr(), weights.data_ptr(), state.data_ptr(), self.k, self.temperature
+
+
+def _forward(x, weight, rows, reduction):
+    """(loss, x and weight as the kernels read them, what the backward pass needs of the sums)."""
+    v, d = weight.shape
+    n, device = x.numel() // d, x.device
+    xp, wp = packed(x), packed(weight)
+    # log2 of the sums, the number of rows that count
+    kept = torch.empty(n + 1, dtype=torch.float32, device=device)
+    loss = torch.empty(() if reduction else x.shape[:-1], dtype=torch.float32, device=device)
+    if n:
+        at, out = kept.data_ptr(), loss.data_ptr()
+        with on_device(device):
+            work = torch.empty(_forward_work(n, v, rows.k), dtype=torch.uint8, device=device)
+            nv.check(nv.long_entry("dfcclLinearLossForward")(xp.data_ptr(), wp.data_ptr(), n, v, d, *rows.args(), reduction, work.data_ptr(), at,
+                                                             None if reduction else out, out if reduction else None, at + 4 * n if reduction else None,
+                                                             stream_of(x)), "dfcclLinearLossForward")
+    elif reduction:
+        loss.zero_()
+    return loss, xp, wp, kept
+
+
+class _LinearLossFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, tokens, weights, state, k, temperature, reduction):
-        n, (v, d) = x.numel() // weight.shape[1], weight.shape
-        xp, wp = packed(x.detach()), packed(weight.detach())
-        lse, losses = torch.empty(n, dtype=torch.float32, device=x.device), torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        count = torch.empty(1, dtype=torch.int32, device=x.device) if reduction else None
-        loss = torch.empty((), dtype=torch.float32, device=x.device) if reduction else losses
-        if n:
-            with on_device(x.device):
-                work = torch.empty(nv.lib().dfcclLinearLossForwardWork(n, v, k), dtype=torch.uint8, device=x.device)
-                nv.check(nv.lib().dfcclLinearLossForward(xp.data_ptr(), wp.data_ptr(), n, v, d, tokens.data_ptr(), None if weights is None else weights.data_ptr(),
-                                                         state.data_ptr(), k, temperature, reduction, work.data_ptr(), lse.data_ptr(), losses.data_ptr(),
-                                                         loss.data_ptr() if reduction else None, count.data_ptr() if reduction else None,
-                                                         raw_stream(x.device)), "dfcclLinearLossForward")
-        elif reduction:
-            loss.zero_()
-        # (what the kernels read is kept: the tensors themselves where they are packed, so that a change in place is noticed)
-        ctx.save_for_backward(x if xp.data_ptr() == x.data_ptr() else xp, weight if wp.data_ptr() == weight.data_ptr() else wp, tokens, weights, state, lse, count)
-        ctx.k, ctx.temperature, ctx.mean, ctx.shape = k, temperature, reduction == REDUCTIONS["mean"], x.shape
+    def forward(ctx, x, weight, rows, reduction):
+        loss, xp, wp, kept = _forward(x, weight, rows, reduction)
+        ctx.save_for_backward(xp, wp, kept, *rows.tensors())
+        ctx.rows, ctx.mean, ctx.shape = rows, reduction == 1, x.shape
         ctx.set_materialize_grads(False)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        nothing = (None,) * 8
         want_x, want_w = ctx.needs_input_grad[:2]
         if g is None or not (want_x or want_w):
-            return nothing
-        x, w, tokens, weights, state, lse, count = ctx.saved_tensors
-        (v, d), n = w.shape, lse.shape[0]
+            return None, None, None, None
+        x, w, kept = ctx.saved_tensors[:3]                  # (asking for them notices a change in place, of the targets too)
+        (v, d), n, device = w.shape, kept.shape[0] - 1, x.device
         if n == 0:
-            return (torch.zeros(ctx.shape, dtype=x.dtype, device=x.device) if want_x else None, torch.zeros_like(w) if want_w else None) + nothing[2:]
+            return torch.zeros_like(x) if want_x else None, torch.zeros_like(w) if want_w else None, None, None
         g = g.reshape(-1) if g.dim() else g
-        dx = torch.empty(ctx.shape, dtype=x.dtype, device=x.device) if want_x else None
-        dw = torch.empty(v, d, dtype=x.dtype, device=x.device) if want_w else None
-        with on_device(x.device):
-            size = nv.lib().dfcclLinearLossBackwardWork(n, v, d, int(want_x), int(want_w))
-            work = torch.empty(size, dtype=torch.uint8, device=x.device)
-            nv.check(nv.lib().dfcclLinearLossBackward(x.data_ptr(), w.data_ptr(), n, v, d, tokens.data_ptr(), None if weights is None else weights.data_ptr(),
-                                                      state.data_ptr(), ctx.k, ctx.temperature, lse.data_ptr(), g.data_ptr(), g.stride(0) if g.dim() else 0,
-                                                      count.data_ptr() if ctx.mean else None, dx.data_ptr() if want_x else None, dw.data_ptr() if want_w else None,
-                                                      work.data_ptr(), size, raw_stream(x.device)), "dfcclLinearLossBackward")
-        return (dx, dw) + nothing[2:]
+        dx = torch.empty(ctx.shape, dtype=x.dtype, device=device) if want_x else None
+        dw = torch.empty(v, d, dtype=x.dtype, device=device) if want_w else None
+        with on_device(device):
+            size = nv.lib().dfcclLinearLossBackwardWork(n, v, d, want_x, want_w)
+            work = torch.empty(size, dtype=torch.uint8, device=device)
+            at = kept.data_ptr()
+            nv.check(nv.long_entry("dfcclLinearLossBackward")(x.data_ptr(), w.data_ptr(), n, v, d, *ctx.rows.args(), at, g.data_ptr(), g.stride(0) if g.dim() else 0,
+                                                              at + 4 * n if ctx.mean else None, dx.data_ptr() if want_x else None,
+                                                              dw.data_ptr() if want_w else None, work.data_ptr(), size, stream_of(x)), "dfcclLinearLossBackward")
+        return dx, dw, None, None
+
+
+def _loss(x, weight, rows, reduction):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _LinearLossFn.apply(x, weight, rows, REDUCTIONS[reduction])
+    return _forward(x, weight, rows, REDUCTIONS[reduction])[0]
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
@@ -102,15 +133,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     _check(x, weight, targets, "targets", reduction)
     if targets.shape != x.shape[:-1]:
         raise ValueError(f"targets of {tuple(targets.shape)} for x of {tuple(x.shape)}")
-    _on_one_gpu(x, weight, targets)
-    n, v = targets.numel(), weight.shape[0]
-    lists = torch.empty(2, n, dtype=torch.int32, device=x.device)
-    targets = targets.contiguous()
-    if n:
-        with on_device(x.device):
-            nv.check(nv.lib().dfcclTargetRows(targets.data_ptr(), int(targets.dtype == torch.int64), n, v, ignore_index, lists.data_ptr(), lists.data_ptr() + 4 * n,
-                                              raw_stream(x.device)), "dfcclTargetRows")
-    return _LinearLossFn.apply(x, weight, lists[0], None, lists[1], 1, 1.0, REDUCTIONS[reduction])
+    _on_one_gpu(x.device, weight, targets)
+    return _loss(x, weight, _Rows(targets.contiguous(), ignore_index, None, 1, 1.0), reduction)
 
 
 def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor, teacher_tokens: torch.Tensor, *, temperature: float = 1.0,
@@ -133,14 +157,14 @@ def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_logits: t
         raise ValueError(f"lists of 1 to {MAX_LIST} entries, got {k}")
     if not (temperature > 0.0 and temperature < float("inf")):
         raise ValueError(f"the temperature is positive, got {temperature}")
-    _on_one_gpu(x, weight, teacher_logits, teacher_tokens)
+    device, temperature = x.device, float(temperature)
+    _on_one_gpu(device, weight, teacher_logits, teacher_tokens)
     n, v = teacher_tokens.numel() // k, weight.shape[0]
-    tokens = torch.empty(n, k, dtype=torch.int32, device=x.device)
-    weights = torch.empty(n, k, dtype=torch.float32, device=x.device)
-    state = torch.empty(n, dtype=torch.int32, device=x.device)
+    lists = torch.empty(2 * n * k + n, dtype=torch.int32, device=device)
+    tokens, weights, state = lists[:n * k], lists[n * k:2 * n * k].view(torch.float32), lists[2 * n * k:]
     logits, listed = teacher_logits.detach().contiguous(), teacher_tokens.contiguous()
     if n:
-        with on_device(x.device):
-            nv.check(nv.lib().dfcclTeacherRows(logits.data_ptr(), nccl_dtype(logits.dtype), listed.data_ptr(), int(listed.dtype == torch.int64), n, k, v,
-                                               temperature, tokens.data_ptr(), weights.data_ptr(), state.data_ptr(), raw_stream(x.device)), "dfcclTeacherRows")
-    return _LinearLossFn.apply(x, weight, tokens, weights, state, k, float(temperature), REDUCTIONS[reduction])
+        with on_device(device):
+            nv.check(nv.long_entry("dfcclTeacherRows")(logits.data_ptr(), nccl_dtype(logits.dtype), listed.data_ptr(), int(listed.dtype == torch.int64), n, k, v,
+                                               temperature, tokens.data_ptr(), weights.data_ptr(), state.data_ptr(), stream_of(x)), "dfcclTeacherRows")
+    return _loss(x, weight, _Rows(None, 0, (tokens, weights, state), k, temperature), reduction)

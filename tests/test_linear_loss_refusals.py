@@ -77,21 +77,25 @@ def test_entries_refuse(native):
     """The C entry points answer with a status: no null pointers, no odd widths, no lists beyond the limit, no misaligned operands."""
     L, bad, p, q = native.lib(), native.INVALID_ARGUMENT, 4096, 4100
     assert L.dfcclLinearLossMaxList() == 256
-    ok = [p, p, 4, 9, 16, p, None, p, 1, 1.0, 0, p, p, p, None, None, None]
-    for at, value in ((0, None), (1, q), (2, 0), (3, 0), (4, 12), (5, None), (7, None), (8, 0), (8, 257), (9, 0.0), (10, 3), (10, 1), (11, None), (12, None), (13, None)):
+    ok = [p, p, 4, 9, 16, p, 1, -100, None, None, None, 1, 1.0, 0, p, p, p, None, None, None]
+    for at, value in ((0, None), (1, q), (2, 0), (3, 0), (4, 12), (5, None), (11, 0), (11, 2), (12, 0.0), (13, 3), (13, 1), (14, None), (15, None), (16, None)):
         args = list(ok)
         args[at] = value
         assert L.dfcclLinearLossForward(*args) == bad, (at, value)
-    ok = [p, p, 4, 9, 16, p, None, p, 1, 1.0, p, p, 0, None, p, p, p, 1 << 30, None]
-    for at, value in ((0, None), (1, q), (2, -1), (4, 4), (8, 300), (9, -1.0), (10, None), (11, None), (12, -1), (14, q), (15, q), (16, None), (17, 16)):
+    lists = ok[:5] + [None, 0, 0, p, p, p, 8] + ok[12:]
+    for at, value in ((8, None), (9, None), (10, None), (11, 257)):
+        args = list(lists)
+        args[at] = value
+        assert L.dfcclLinearLossForward(*args) == bad, (at, value)
+    ok = [p, p, 4, 9, 16, p, 1, -100, None, None, None, 1, 1.0, p, p, 0, None, p, p, p, 1 << 30, None]
+    for at, value in ((0, None), (1, q), (2, -1), (4, 4), (5, None), (11, 300), (12, -1.0), (13, None), (14, None), (15, -1), (17, q), (18, q), (19, None), (20, 16)):
         args = list(ok)
         args[at] = value
         assert L.dfcclLinearLossBackward(*args) == bad, (at, value)
     args = list(ok)
-    args[14] = args[15] = None
+    args[17] = args[18] = None
     assert L.dfcclLinearLossBackward(*args) == bad
     assert L.dfcclLinearLossForwardWork(4, 9, 0) == 0 and L.dfcclLinearLossBackwardWork(4, 9, 16, 0, 0) == 0
-    assert L.dfcclTargetRows(None, 1, 4, 9, -100, p, p, None) == bad and L.dfcclTargetRows(p, 1, 0, 9, -100, p, p, None) == bad
     assert L.dfcclTeacherRows(p, native.INT32, p, 1, 4, 2, 9, 1.0, p, p, p, None) == bad and L.dfcclTeacherRows(p, native.FLOAT32, p, 1, 4, 257, 9, 1.0, p, p, p, None) == bad
     ok = [p, 1, 4, p, 9, 16, None, 0, None, 0, 0, p, 16, native.BFLOAT16, 1.0, None]
     for at, value in ((0, None), (2, 0), (3, None), (4, 0), (5, 8), (6, p), (11, None), (12, 0), (13, native.FLOAT64)):
@@ -105,3 +109,24 @@ def test_entries_refuse(native):
         assert L.dfcclEmbeddingBackward(*args) == bad, (at, value)
     assert L.dfcclEmbeddingBackwardWork(4, 16, 3) == 0 and L.dfcclEmbeddingBackwardWork(4, 16, 2) > 0
     assert isinstance(L.dfcclLinearLossBackwardWork(1000, 50257, 1024, 1, 1), int) and C.sizeof(C.c_size_t) == 8
+
+
+def test_long_entries(native):
+    """Entry points of many arguments: integers, None and a float wherever it stands, as ctypes passes them; nothing else."""
+    import numpy as np
+    f, g = native.long_entry("dfcclEmbeddingBackward"), native.lib().dfcclEmbeddingBackward
+    assert native.long_entry("dfcclEmbeddingBackward") is f
+    ok = [4096, 4, 16, native.BFLOAT16, 4096, 1, -1, 1.0, 4100, 9, None, 0, None, 0, 4096, None]          # (misaligned: refused)
+    assert f(*ok) == g(*ok) == native.INVALID_ARGUMENT
+    if native._hostcall() is None:
+        return
+    call = native._hostcall_module.call_long
+    libc = C.CDLL(None)
+    assert call(C.cast(libc.abs, C.c_void_p).value, -7) == 7
+    assert call(C.cast(libc.lrintf, C.c_void_p).value, 41.6) == 42 and call(C.cast(libc.ilogbf, C.c_void_p).value, None, 8.5, 3) == 3
+    text = [C.create_string_buffer(t) for t in (b"abcd", b"abxy")]
+    where = C.cast(libc.strncmp, C.c_void_p).value
+    assert call(where, *(C.addressof(t) for t in text), np.int64(2)) == 0 and call(where, *(C.addressof(t) for t in text), 3) < 0
+    for bad in ((1.5,), (None,), (1, 1.0, 2.0), (1, "x"), tuple([1] * 26), ()):
+        with pytest.raises(TypeError):
+            call(*bad)
