@@ -2,10 +2,10 @@
 // accumulators in tensor memory.  With z = x w^T, x [n, d] and the head w [v, d]:
 //   VOCAB_STATS     of every row the maximum and the sum of powers of each stretch of its logits, and the logits of its targets
 //   VOCAB_GRAD      dz = g (softmax(z) - target): the logits are computed again, what is stored is their gradient, rounded once
+//   VOCAB_POWERS    powers of the logits relative to a number known in front of the product (a target's logit), and their sums: the
+//                   logits are not computed again, for rows whose gradients are wanted with the loss
 //   VOCAB_PRODUCTS  dx = dz w and dw = dz^T x, in one launch
-// A logit exists in tensor memory and registers only.  Computing the product again costs a third more than the two products
-// of the gradients do by themselves; keeping n v logits or powers of them would cost their rounding twice (1.7 times the error of one
-// rounding in dw) and n v 2 bytes between forward and backward.
+// A logit exists in tensor memory and registers only.
 //
 // Tiles of 256 x 256, stages of 64 of the contraction, roles as in tcgen05_gemm_pair.cu (TMA producer, MMA issuer, eight epilogue warps,
 // two accumulators).  All of n, v are any number, d a multiple of 8: the tensor maps give zeros outside, the epilogues store inside.
@@ -29,7 +29,7 @@ constexpr int EPI_WARPS = 4 * VOCAB_PARTS, THREADS = 64 + 32 * EPI_WARPS;
 constexpr uint64_t WAIT_NS = 4000000000ull;                                       // nothing here waits on another GPU
 static_assert(STAGES * STAGE_BYTES + 1024 + 256 <= SMEM_BYTES, "stages");
 
-enum VocabMode { VOCAB_STATS, VOCAB_GRAD, VOCAB_PRODUCTS };
+enum VocabMode { VOCAB_STATS, VOCAB_GRAD, VOCAB_POWERS, VOCAB_PRODUCTS };
 
 // One product: result [M, N], `kBlocks` blocks of 64 of the contraction cut into slices of `perSlice`.
 struct Product {
@@ -38,6 +38,7 @@ struct Product {
   __nv_bfloat16* out;               // direct results, ld N
   float* part;                      // or slices [slice][M][N]
   int add, wide;
+  int exact;                        // what VocabExact adds to a direct result: 1 of dx, 2 of dw, 0 nothing
 };
 struct VocabArgs {
   Product p[2];                     // items of the first, then of the second (items = 0: none)
@@ -47,7 +48,10 @@ struct VocabArgs {
   float* picked;
   int* ticket;
   VocabGrad grad;
+  const float* base;                // of the powers
   VocabFactor factor;
+  VocabExact exact;
+  const int* only;                  // null, or a word without which there is nothing to do
   __nv_bfloat16* dz;
   int ld, first;                    // of dz; first column of the vocabulary
   uint32_t* err;
@@ -123,7 +127,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t cr = cluster_ctarank();             // 0 = leader
   const Items items(g, blockIdx.x >> 1, gridDim.x >> 1);
-  const int count = items.count();
+  int count = items.count();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&fullBar[s], 1); mbar_init(&emptyBar[s], 1); }
@@ -141,6 +145,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
   const uint32_t tmemBase = *tmemBaseSlot;
   grid_dependency_wait();
   grid_launch_dependents();
+  if ((MODE == VOCAB_STATS || MODE == VOCAB_POWERS) && g.only && *g.only == 0) count = 0;
   if (MODE == VOCAB_STATS && g.ticket && blockIdx.x == 0 && threadIdx.x == 0) *g.ticket = 0;
 
   if (warp == 0) {
@@ -243,17 +248,21 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
         if (here) {                                    // on its way while the accumulator is computed
           int token;
           const int state = rowState(g.rows, row, token);
+          if (MODE == VOCAB_POWERS) {
+            lse = g.base[row];
+            coef = state == ROW_LIST ? 1.f : 0.f;
+          }
           if (MODE == VOCAB_GRAD) {
             lse = g.grad.lse[row];
             coef = g.grad.gout ? g.grad.gout[(size_t)row * g.grad.goutStride] : 1.f;
             if (state != ROW_LIST) coef = state == ROW_BAD ? __int_as_float(0x7fffffff) : 0.f;
           }
-          list.seek(g.rows, row, token, g.first + col0);
+          if (MODE != VOCAB_POWERS) list.seek(g.rows, row, token, g.first + col0);
         }
         if (!mbar_wait(&accFull[ab], (j >> 1) & 1, giveUp, WAIT_NS)) break;
         tc_fence_after();
         float top = -INFINITY, sum = 0.f;
-        const int cols = MODE == VOCAB_GRAD ? g.ld : p.N, steps = (min(T, cols - col0) + 31) / 32;
+        const int cols = MODE == VOCAB_STATS ? p.N : g.ld, steps = (min(T, cols - col0) + 31) / 32;
 #pragma unroll 1
         for (int i = part; i < steps; i += VOCAB_PARTS) {
           if (!mine) break;
@@ -286,6 +295,23 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
             for (int e = 0; e < 32; ++e) s[e & 3] += exp2Approx(fmaf(__uint_as_float(r[e]), scale, -base));
             sum = (s[0] + s[1]) + (s[2] + s[3]);
             top = now;
+          } else if (MODE == VOCAB_POWERS) {
+            if (c + 32 > p.N) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) if (c + e >= p.N) r[e] = 0xff800000u;          // -inf
+            }
+            float m0 = __uint_as_float(r[0]), m1 = __uint_as_float(r[1]);
+#pragma unroll
+            for (int e = 2; e < 32; e += 2) { m0 = fmaxf(m0, __uint_as_float(r[e])); m1 = fmaxf(m1, __uint_as_float(r[e + 1])); }
+            top = fmaxf(top, fmaf(fmaxf(m0, m1), scale, -lse));
+            float s[4] = {sum, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float v = exp2Approx(fmaf(__uint_as_float(r[e]), scale, -lse));
+              s[e & 3] += v;
+              r[e] = __float_as_uint(v);
+            }
+            sum = (s[0] + s[1]) + (s[2] + s[3]);
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(exp2Approx(fmaf(__uint_as_float(r[e]), scale, -lse)));
@@ -302,7 +328,9 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
 #pragma unroll
               for (int e = 0; e < 32; ++e) if (c + e >= p.N) r[e] = 0u;
             }
-            // (a row without a gradient may hold anything, infinities and NaN among it)
+          }
+          // (a row without a gradient may hold anything, infinities and NaN among it)
+          if (MODE != VOCAB_STATS) {
             if (here) {
               uint4 o[4];
 #pragma unroll
@@ -310,7 +338,8 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
                 uint32_t* ow = (uint32_t*)&o[v];
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                  const float lo = __uint_as_float(r[8 * v + 2 * w]) * coef, hi = __uint_as_float(r[8 * v + 2 * w + 1]) * coef;
+                  float lo = __uint_as_float(r[8 * v + 2 * w]), hi = __uint_as_float(r[8 * v + 2 * w + 1]);
+                  if (MODE == VOCAB_GRAD) { lo *= coef; hi *= coef; }
                   ow[w] = coef == 0.f ? 0u : pack_bf16x2(lo, hi);
                 }
               }
@@ -320,11 +349,16 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
             }
           }
         }
-        if (MODE == VOCAB_STATS && here) g.parts[(size_t)(t.nt * VOCAB_PARTS + part) * p.M + row] = make_float2(top, sum);
+        if (MODE != VOCAB_GRAD && here) g.parts[(size_t)(t.nt * VOCAB_PARTS + part) * p.M + row] = make_float2(top, sum);
       } else {
         if (!mbar_wait(&accFull[ab], (j >> 1) & 1, giveUp, WAIT_NS)) break;
         tc_fence_after();
         const int steps = (min(T, p.N - col0) + 31) / 32;
+        int state = ROW_NONE, token = 0;
+        float scale = 0.f;
+        const float* sums = nullptr;
+        if (here && p.exact == 1) { state = rowState(g.exact.rows, row, token); scale = g.exact.scale[row]; }
+        if (here && p.exact == 2) { const int at = g.exact.where[row]; if (at >= 0) sums = g.exact.sums + (size_t)at * p.N; }
 #pragma unroll 1
         for (int i = part; i < steps; i += VOCAB_PARTS) {
           if (!mine) break;
@@ -346,9 +380,16 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
             uint4 o[4];
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
+              float f[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(r[8 * v + e]);
+              if (v < packs) {
+                if (p.exact == 1) vocabExactX(f, state, scale, (const uint4*)(g.exact.w + (size_t)(state == ROW_LIST ? token : 0) * p.N + c) + v);
+                else if (sums) vocabMinus(f, (const float4*)(sums + c) + 2 * v);
+              }
               uint32_t* ow = (uint32_t*)&o[v];
 #pragma unroll
-              for (int w = 0; w < 4; ++w) ow[w] = pack_bf16x2(__uint_as_float(r[8 * v + 2 * w]) * factor, __uint_as_float(r[8 * v + 2 * w + 1]) * factor);
+              for (int w = 0; w < 4; ++w) ow[w] = pack_bf16x2(f[2 * w] * factor, f[2 * w + 1] * factor);
             }
             __nv_bfloat16* dst = p.out + (size_t)row * p.N + c;
             if (packs == 4) { st_global32(dst, o, p.wide); st_global32(dst + 16, o + 2, p.wide); }
@@ -416,12 +457,22 @@ ncclResult_t logits(CUtensorMap* a, CUtensorMap* b, VocabArgs* g, const void* x,
 
 }  // namespace
 
-ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, float* picked, int* ticket, cudaStream_t stream) {
+ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, float* picked, int* ticket, const int* only,
+                        cudaStream_t stream) {
   CUtensorMap a, b;
   VocabArgs g;
   DFCHECK(logits(&a, &b, &g, x, w, n, v, d, rows));
-  g.parts = parts; g.picked = picked; g.ticket = ticket;
+  g.parts = parts; g.picked = picked; g.ticket = ticket; g.only = only;
   return launchVocab<VOCAB_STATS>(a, b, a, b, g, stream);
+}
+
+ncclResult_t vocabPowers(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, const float* base, float2* parts, void* powers, const int* only,
+                         cudaStream_t stream) {
+  CUtensorMap a, b;
+  VocabArgs g;
+  DFCHECK(logits(&a, &b, &g, x, w, n, v, d, rows));
+  g.parts = parts; g.base = base; g.dz = (__nv_bfloat16*)powers; g.ld = (v + 63) / 64 * 64; g.only = only;
+  return launchVocab<VOCAB_POWERS>(a, b, a, b, g, stream);
 }
 
 ncclResult_t vocabGrad(const void* x, const void* w, int n, int v, int first, int d, const VocabRows& rows, const VocabGrad& grad, void* dz, cudaStream_t stream) {
@@ -446,32 +497,38 @@ VocabPlan vocabProductPlan(int n, int v, int d, bool wantX, bool wantW, int pair
   return VocabPlan{cut(tn * td, kv), cut(tv * td, kn)};
 }
 
-ncclResult_t vocabProducts(const void* dz, const void* x, const void* w, int n, int v, int d, const VocabPlan& plan, const VocabFactor& factor, void* dx, float* partX,
-                           bool addX, void* dw, float* partW, cudaStream_t stream) {
+ncclResult_t vocabProducts(const void* dz, const void* x, const void* w, int n, int v, int d, const VocabPlan& plan, const VocabFactor& factor, const VocabExact* exact,
+                           const VocabResult& dx, const VocabResult& dw, cudaStream_t stream) {
   const int ld = (v + 63) / 64 * 64;
   CUtensorMap a[2], b[2];
   VocabArgs g = {};
   g.factor = factor;
+  if (exact) g.exact = *exact;
   int k = 0;
   auto narrow = [&](CUtensorMap* m, const void* base, int rows) {      // [rows of the contraction][d columns]
     return d % 64 ? gemmEncodeMap(m, base, (uint64_t)rows, (uint64_t)d, BK) : gemmEncodeMap3(m, base, (uint64_t)d, (uint64_t)rows, 1, HALF, BK);
   };
-  if (dx || partX) {
+  auto result = [&](const VocabResult& r, int which) {
+    Product& p = g.p[k++];
+    p.bMn = 1; p.bLoose = d % 64 != 0;
+    p.out = (__nv_bfloat16*)r.out; p.part = r.part; p.add = r.add;
+    p.exact = exact && r.out ? which : 0;
+    p.wide = d % 16 == 0 && ((uintptr_t)r.out & 31) == 0;
+  };
+  if (dx.out || dx.part) {
     DFCHECK(gemmEncodeMap(&a[k], dz, (uint64_t)n, (uint64_t)ld, HALF));
     DFCHECK(narrow(&b[k], w, v));
-    Product& p = g.p[k++] = productOf(n, d, v, plan.perX);
-    p.bMn = 1; p.bLoose = d % 64 != 0;
-    p.out = (__nv_bfloat16*)dx; p.part = partX; p.add = addX;
+    g.p[k] = productOf(n, d, v, plan.perX);
+    result(dx, 1);
   }
-  if (dw || partW) {
+  if (dw.out || dw.part) {
     DFCHECK(gemmEncodeMap3(&a[k], dz, (uint64_t)ld, (uint64_t)n, 1, HALF, BK));
     DFCHECK(narrow(&b[k], x, n));
-    Product& p = g.p[k++] = productOf(v, d, n, plan.perW);
-    p.aMn = p.bMn = 1; p.bLoose = d % 64 != 0;
-    p.out = (__nv_bfloat16*)dw; p.part = partW;
+    g.p[k] = productOf(v, d, n, plan.perW);
+    g.p[k].aMn = 1;
+    result(dw, 2);
   }
   if (!k) return ncclInvalidArgument;
-  for (int i = 0; i < k; ++i) g.p[i].wide = d % 16 == 0 && ((uintptr_t)g.p[i].out & 31) == 0;
   if (k == 1) { a[1] = a[0]; b[1] = b[0]; }
   return launchVocab<VOCAB_PRODUCTS>(a[0], b[0], a[1], b[1], g, stream);
 }

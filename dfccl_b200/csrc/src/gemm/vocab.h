@@ -41,7 +41,14 @@ inline int vocabParts(int v) { return (v + VOCAB_TILE - 1) / VOCAB_TILE * VOCAB_
 
 // z = x [n, d] w[v, d]^T, tile by tile and never stored.  Of every row: for each of the vocabParts(v) stretches of its columns
 // {largest z scale, sum of 2^(z scale - that)} -> parts [stretch][n], and the z of its list's entries -> picked [n][k].  `ticket`, where given, is set to 0.
-ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, float* picked, int* ticket, cudaStream_t stream);
+// `only`, where given: nothing happens unless it holds something other than 0.
+ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, float* picked, int* ticket, const int* only,
+                        cudaStream_t stream);
+
+// powers = 2^(z scale - base) of every row with a target, 0 elsewhere: bf16, [n][ld], ld = v rounded up to 64 (zeros behind v).  Of each stretch
+// of a row's columns {largest exponent, sum of the powers in fp32} -> parts [stretch][n].
+ncclResult_t vocabPowers(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, const float* base, float2* parts, void* powers, const int* only,
+                         cudaStream_t stream);
 
 // What all rows' gradients share: the gradient of the reduced loss, a mean's count, the temperature.  It does not go into dz, where its
 // rounding to bf16 would be the same for all of them (a mean over 32113 rows: dx 3.1e-3 off, 1.7e-3 without), but into the results.
@@ -72,9 +79,49 @@ struct VocabPlan { int perX, perW; };
 VocabPlan vocabProductPlan(int n, int v, int d, bool wantX, bool wantW, int pairs);
 inline int vocabSlices(int k, int per) { return ((k + 63) / 64 + per - 1) / per; }
 
-// dx [n, d] = factor dz w and dw [v, d] = factor dz^T x in one launch; either may be left out (null).  dx is bf16 where `partX` is null, otherwise
-// an fp32 sum [slice][n][d] of each slice of the vocabulary, without the factor, added to what is there with `addX`; dw likewise with partW.
-ncclResult_t vocabProducts(const void* dz, const void* x, const void* w, int n, int v, int d, const VocabPlan& plan, const VocabFactor& factor, void* dx, float* partX,
-                           bool addX, void* dw, float* partW, cudaStream_t stream);
+// Where dz is not the gradient of the logits but their powers (vocabPowers, targets only): what is missing of both results, in fp32.
+//   dx_n = factor (scale_n (powers w)_n - w_target(n)),   dw_t = factor ((powers^T x')_t - sums_where(t))
+// with x' = scale_n x_n as the right operand, sums_where(t) the sum of the x_n whose target is t.
+struct VocabExact {
+  VocabRows rows;               // of the n rows
+  const float* scale;           // [n]
+  const __nv_bfloat16* w;       // [v, d]
+  const float* sums;            // rows of d
+  const int* where;             // [v] a row of sums, or -1
+};
+
+// dx [n, d] = factor dz w and dw [v, d] = factor dz^T x in one launch.  A result is bf16 where `out` is given; otherwise `part` gets an fp32
+// sum [slice][rows][d] of each slice of the contraction, without the factor and without what `exact` (may be null) adds, on top of what is
+// there with `add`.  A result with neither is left out.
+struct VocabResult {
+  void* out;
+  float* part;
+  bool add;
+};
+ncclResult_t vocabProducts(const void* dz, const void* x, const void* w, int n, int v, int d, const VocabPlan& plan, const VocabFactor& factor, const VocabExact* exact,
+                           const VocabResult& dx, const VocabResult& dw, cudaStream_t stream);
+
+#if defined(__CUDACC__)
+// Eight elements of a row of dx or dw from their sums.
+__device__ __forceinline__ void vocabMinus(float (&f)[8], const float4* p) {
+  const float4 a = p[0], b = p[1];
+  f[0] -= a.x; f[1] -= a.y; f[2] -= a.z; f[3] -= a.w; f[4] -= b.x; f[5] -= b.y; f[6] -= b.z; f[7] -= b.w;
+}
+__device__ __forceinline__ void vocabExactX(float (&f)[8], int state, float scale, const uint4* target) {
+  if (state != ROW_LIST) {
+    const float none = state == ROW_BAD ? __int_as_float(0x7fffffff) : 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = none;
+    return;
+  }
+  const uint4 t = *target;
+  const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    f[2 * e] = fmaf(f[2 * e], scale, -__uint_as_float(w[e] << 16));
+    f[2 * e + 1] = fmaf(f[2 * e + 1], scale, -__uint_as_float(w[e] & 0xffff0000u));
+  }
+}
+#endif
 
 }  // namespace dfccl

@@ -18,6 +18,7 @@
 #include "dfccl_ops.h"
 #include "../common/log.h"
 #include "../gemm/tc_common.h"
+#include "embed.h"
 
 namespace dfccl {
 namespace {
@@ -164,6 +165,9 @@ struct Table {
   size_t gradBytes;
   float scale;
   float* sums;                    // [stretches][2][d]: of the row that goes on from the stretch in front, of the one that goes on behind
+  // sums by themselves instead of a gradient: fp32 rows [n][d], used where `where` [rows] says
+  float* compact;
+  int* where;
 };
 struct Backward {
   Table t[MAX_TABLES];
@@ -292,8 +296,25 @@ __global__ void __launch_bounds__(256) clearKernel(const Backward a) {
   tc::grid_dependency_wait();
 }
 
+// Stores the sum of a row whose last token (of the stretch in which the row begins) is the `at`-th of the sorted ones.
+template <typename T, int E, bool COMPACT>
+__device__ __forceinline__ void storeRow(const Table& t, uint32_t row, int at, int d, int col, const float (&acc)[E]) {
+  if (COMPACT) {
+    Pack<float, E> o;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o.v[e] = acc[e];
+    *(Pack<float, E>*)(t.compact + (size_t)at * d + col) = o;
+    if (col == 0) t.where[row] = at;
+  } else {
+    Pack<T, E> o;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o.v[e] = fromFloat<T>(acc[e] * t.scale);
+    *(Pack<T, E>*)((T*)t.grad + (size_t)row * d + col) = o;
+  }
+}
+
 // A block sums the tokens of a stretch for its columns (E per thread), row after row; eight rows are on their way at a time.
-template <typename T, int E>
+template <typename T, int E, bool COMPACT>
 __global__ void __launch_bounds__(128) sumStretchKernel(const Backward a) {
   constexpr int MAX = 128, AHEAD = 8;
   __shared__ uint32_t keys[MAX + 2], tokens[MAX];
@@ -336,10 +357,7 @@ __global__ void __launch_bounds__(128) sumStretchKernel(const Backward a) {
         for (int e = 0; e < E; ++e) s.v[e] = acc[e];
         *(Pack<float, E>*)(t.sums + ((size_t)blockIdx.x * 2 + (head ? 0 : 1)) * a.d + col) = s;
       } else {
-        P o;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o.v[e] = fromFloat<T>(acc[e] * t.scale);
-        *(P*)((T*)t.grad + (size_t)keys[j + 1] * a.d + col) = o;
+        storeRow<T, E, COMPACT>(t, keys[j + 1], start + j, a.d, col, acc);
       }
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] = 0.f;
@@ -362,7 +380,7 @@ __device__ __forceinline__ void addStretches(const float* s, size_t step, int fr
 // Rows that go on behind the stretch in which they begin, 32 packs of columns per block.  A warp looks whether its stretch has such a row
 // and adds up what few stretches it goes through; one that goes through more than eight, the block's warps add up together.  (With all rows
 // added up by one warp each, a row of 12000 tokens of 131072 took 35 us.)
-template <typename T, int E>
+template <typename T, int E, bool COMPACT>
 __global__ void __launch_bounds__(32 * JOIN_WARPS) joinStretchKernel(const Backward a) {
   constexpr int FEW = 8;
   __shared__ float part[JOIN_WARPS][32 * E];
@@ -398,16 +416,10 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) joinStretchKernel(const Backw
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = x.v[e];
   };
-  auto store = [&](uint32_t row) {
-    Pack<T, E> o;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o.v[e] = fromFloat<T>(acc[e] * t.scale);
-    *(Pack<T, E>*)((T*)t.grad + (size_t)row * a.d + col) = o;
-  };
   if (count && count <= FEW && col < a.d) {
     begin(own);
     addStretches<E>(t.sums + (own + 1) * step + col, step, 0, count, acc);
-    store(key);
+    storeRow<T, E, COMPACT>(t, key, end - 1, a.d, col, acc);
   }
   __syncthreads();
   for (int w = 0; w < JOIN_WARPS; ++w) {
@@ -429,7 +441,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) joinStretchKernel(const Backw
     for (int e = 0; e < E; ++e)
 #pragma unroll
       for (int k = 1; k < JOIN_WARPS; ++k) acc[e] += part[k][lane * E + e];
-    store((uint32_t)rowKey[w]);
+    storeRow<T, E, COMPACT>(t, (uint32_t)rowKey[w], (first + 1) * a.stretch - 1, a.d, col, acc);
   }
 }
 
@@ -453,19 +465,42 @@ ncclResult_t forward(const Forward& a, cudaStream_t stream) {
   return ncclSuccess;
 }
 
-template <typename T, int E>
+template <typename T, int E, bool COMPACT>
 ncclResult_t backward(const Backward& a, cudaStream_t stream) {
   CUDACHECK(launchBehind(sortTokensKernel, dim3(SORT_CTAS * a.tables), SORT_THREADS, SORT_CTAS, stream, a));
-  CUDACHECK(launchBehind(clearKernel, dim3(CLEAR_BLOCKS), 256, 1, stream, a));
+  if (!COMPACT) CUDACHECK(launchBehind(clearKernel, dim3(CLEAR_BLOCKS), 256, 1, stream, a));
   const int packs = a.d / E;
-  CUDACHECK(launchBehind(sumStretchKernel<T, E>, dim3(a.stretches, (packs + 127) / 128, a.tables), 128, 1, stream, a));
-  if (a.stretches > 1) CUDACHECK(launchBehind(joinStretchKernel<T, E>, dim3((a.stretches + JOIN_WARPS - 2) / JOIN_WARPS, (packs + 31) / 32, a.tables), 32 * JOIN_WARPS, 1, stream, a));
+  CUDACHECK(launchBehind(sumStretchKernel<T, E, COMPACT>, dim3(a.stretches, (packs + 127) / 128, a.tables), 128, 1, stream, a));
+  if (a.stretches > 1)
+    CUDACHECK(launchBehind(joinStretchKernel<T, E, COMPACT>, dim3((a.stretches + JOIN_WARPS - 2) / JOIN_WARPS, (packs + 31) / 32, a.tables), 32 * JOIN_WARPS, 1,
+                           stream, a));
   return ncclSuccess;
+}
+
+void setKeys(Table* t, const void* idx, int wide, int64_t rows, int64_t padding, uint8_t* at, const Layout& l) {
+  t->ids = idx; t->wide = wide; t->rows = (int)rows; t->padding = padding;
+  t->passes = 1;
+  while (t->passes < 4 && (uint64_t)rows >> (8 * t->passes)) ++t->passes;
+  t->buf[0] = (uint2*)at; t->buf[1] = (uint2*)(at + l.items); t->sums = (float*)(at + 2 * l.items);
 }
 
 int typeBytes(int t) { return t == ncclFloat32 ? 4 : t == ncclBfloat16 || t == ncclFloat16 ? 2 : 0; }
 
 }  // namespace
+
+size_t tokenSumsWork(int n, int d) {
+  const Layout l = layoutOf(n, d);
+  return 2 * l.items + l.sums;
+}
+ncclResult_t tokenSums(const void* x, int n, int d, const void* ids, int wide, int64_t ignore, int v, float* sums, int* where, void* work, cudaStream_t stream) {
+  if (d % 8) return ncclInvalidArgument;
+  Backward a = {};
+  a.tables = 1; a.n = n; a.d = d; a.stretch = stretchOf(n); a.stretches = (n + a.stretch - 1) / a.stretch; a.g = x;
+  setKeys(&a.t[0], ids, wide, v, ignore, (uint8_t*)work, layoutOf(n, d));
+  a.t[0].compact = sums; a.t[0].where = where;
+  return backward<__nv_bfloat16, 8, true>(a, stream);
+}
+
 }  // namespace dfccl
 
 using namespace dfccl;
@@ -501,21 +536,19 @@ DF_API ncclResult_t dfcclEmbeddingBackward(const void* g, int n, int d, int type
       (gp && (!positions || prows <= 0 || prows > 0x7ffffff0ll)) || (((uintptr_t)gw | (uintptr_t)gp | (uintptr_t)work) & 15))
     return ncclInvalidArgument;
   const Layout l = layoutOf(n, d);
-  Backward a;
-  a.tables = 0; a.n = n; a.d = d; a.stretch = stretchOf(n); a.stretches = (n + a.stretch - 1) / a.stretch; a.g = g;
+  Backward a = {};
+  a.n = n; a.d = d; a.stretch = stretchOf(n); a.stretches = (n + a.stretch - 1) / a.stretch; a.g = g;
   uint8_t* at = (uint8_t*)work;
   auto add = [&](const void* idx, int wide, int64_t count, int64_t pad, void* grad, float s) {
     Table& t = a.t[a.tables++];
-    t.ids = idx; t.wide = wide; t.rows = (int)count; t.padding = pad; t.grad = grad; t.gradBytes = (size_t)count * d * bytes; t.scale = s;
-    t.passes = 1;
-    while (t.passes < 4 && (uint64_t)count >> (8 * t.passes)) ++t.passes;
-    t.buf[0] = (uint2*)at; t.buf[1] = (uint2*)(at + l.items); t.sums = (float*)(at + 2 * l.items);
+    setKeys(&t, idx, wide, count, pad, at, l);
+    t.grad = grad; t.gradBytes = (size_t)count * d * bytes; t.scale = s;
     at += 2 * l.items + l.sums;
   };
   if (gw) add(ids, wideIds, rows, padding, gw, scale);
   if (gp) add(positions, widePositions, prows, -1, gp, 1.f);
   const bool whole = (((uintptr_t)g | (uintptr_t)((size_t)d * bytes)) & 15) == 0;
-  if (type == ncclFloat32) return whole ? backward<float, 4>(a, stream) : backward<float, 1>(a, stream);
-  if (type == ncclBfloat16) return whole ? backward<__nv_bfloat16, 8>(a, stream) : backward<__nv_bfloat16, 1>(a, stream);
-  return whole ? backward<__half, 8>(a, stream) : backward<__half, 1>(a, stream);
+  if (type == ncclFloat32) return whole ? backward<float, 4, false>(a, stream) : backward<float, 1, false>(a, stream);
+  if (type == ncclBfloat16) return whole ? backward<__nv_bfloat16, 8, false>(a, stream) : backward<__nv_bfloat16, 1, false>(a, stream);
+  return whole ? backward<__half, 8, false>(a, stream) : backward<__half, 1, false>(a, stream);
 }

@@ -17,6 +17,7 @@
 #include "../gemm/gemm.h"
 #include "../gemm/tc_common.h"
 #include "../gemm/vocab.h"
+#include "embed.h"
 
 namespace dfccl {
 namespace {
@@ -131,6 +132,12 @@ struct JoinArgs {
   float t2;
   float* lse;
   float* loss;
+  // behind vocabPowers: the powers' bases and, to be written, the powers' share of a probability, 2^base / sum; rows whose sums say that
+  // their base was no good raise `again`
+  float* base;
+  float* share;
+  int* again;
+  const int* only;              // nothing but the sum over all rows unless this holds something (null: always)
   // the sum over all rows, by the block of the last launch that comes last; null: none
   VocabRows allRows;
   const float* allLoss;
@@ -140,47 +147,66 @@ struct JoinArgs {
   int* count;
 };
 
+// A base is good while no power is above 2^60 (the sums of powers times x or w stay far from the end of fp32) and the target's own power,
+// 1 but for rounding, is in the sum.
+constexpr float MOST_POWER = 60.f;
+
 // 32 rows per block: warp g takes every 32nd stretch of all of them (a line of 256 bytes each), then warp r finishes row r.
+// POWERS: the stretches' sums are relative to the rows' bases.  Otherwise, with `base`, the logarithms of the sums become the bases.
+template <bool POWERS>
 __global__ void __launch_bounds__(1024) joinRowsKernel(const JoinArgs a) {
   __shared__ float2 part[32][33];
   __shared__ int last;
   tc::grid_dependency_wait();
   tc::grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row0 = blockIdx.x * 32;
-  float2 acc = make_float2(-INFINITY, 0.f);
-  if (row0 + lane < a.n) {
-    int i = warp;
-    for (; i + 96 < a.stretches; i += 128) {
-      float2 p[4];
+  auto join = [](float2 x, float2 y) { return POWERS ? make_float2(fmaxf(x.x, y.x), x.y + y.y) : joined(x, y); };
+  if (!a.only || *a.only) {
+    float2 acc = make_float2(-INFINITY, 0.f);
+    if (row0 + lane < a.n) {
+      int i = warp;
+      for (; i + 96 < a.stretches; i += 128) {
+        float2 p[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) p[u] = a.parts[(size_t)(i + 32 * u) * a.n + row0 + lane];
+        for (int u = 0; u < 4; ++u) p[u] = a.parts[(size_t)(i + 32 * u) * a.n + row0 + lane];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) acc = joined(acc, p[u]);
-    }
-    for (; i < a.stretches; i += 32) acc = joined(acc, a.parts[(size_t)i * a.n + row0 + lane]);
-  }
-  part[warp][lane] = acc;
-  __syncthreads();
-  const int row = row0 + warp;
-  if (row < a.n) {
-    acc = part[lane][warp];
-#pragma unroll
-    for (int o = 16; o; o >>= 1) acc = joined(acc, make_float2(__shfl_xor_sync(0xffffffffu, acc.x, o), __shfl_xor_sync(0xffffffffu, acc.y, o)));
-    const float l = acc.x + log2f(acc.y);
-    float sum = 0.f;
-    const int st = rowState(a.rows, row);
-    if (st == ROW_LIST)
-      for (int i = lane; i < a.rows.k; i += 32) {
-        const size_t at = (size_t)row * a.rows.k + i;
-        if (!a.rows.targets && a.rows.tokens[at] == VOCAB_NO_TOKEN) continue;
-        const float q = a.rows.targets ? 1.f : a.rows.weights[at];
-        if (q == 0.f) continue;                         // 0 ln 0
-        sum += q * (logf(q) - (a.picked[at] * a.rows.scale - l) * LN2);
+        for (int u = 0; u < 4; ++u) acc = join(acc, p[u]);
       }
-    sum = warpSum(sum);
-    if (lane == 0) {
-      a.lse[row] = l;
-      a.loss[row] = st == ROW_LIST ? sum * a.t2 : st == ROW_NONE ? 0.f : __int_as_float(0x7fffffff);
+      for (; i < a.stretches; i += 32) acc = join(acc, a.parts[(size_t)i * a.n + row0 + lane]);
+    }
+    part[warp][lane] = acc;
+    __syncthreads();
+    const int row = row0 + warp;
+    if (row < a.n) {
+      acc = part[lane][warp];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) acc = join(acc, make_float2(__shfl_xor_sync(0xffffffffu, acc.x, o), __shfl_xor_sync(0xffffffffu, acc.y, o)));
+      const int st = rowState(a.rows, row);
+      float l, sum = 0.f;
+      if (POWERS) {
+        l = a.base[row] + log2f(acc.y);
+        sum = log2f(fmaxf(acc.y, 1.f)) * LN2;           // the target's power alone is 1
+        if (lane == 0) {
+          a.share[row] = st == ROW_LIST ? 1.f / acc.y : st == ROW_NONE ? 0.f : __int_as_float(0x7fffffff);
+          if (st == ROW_LIST && !(acc.x <= MOST_POWER && acc.y >= 0.5f)) *a.again = 1;
+        }
+      } else {
+        l = acc.x + log2f(acc.y);
+        if (st == ROW_LIST)
+          for (int i = lane; i < a.rows.k; i += 32) {
+            const size_t at = (size_t)row * a.rows.k + i;
+            if (!a.rows.targets && a.rows.tokens[at] == VOCAB_NO_TOKEN) continue;
+            const float q = a.rows.targets ? 1.f : a.rows.weights[at];
+            if (q == 0.f) continue;                     // 0 ln 0
+            sum += q * (logf(q) - (a.picked[at] * a.rows.scale - l) * LN2);
+          }
+        sum = warpSum(sum);
+        if (a.base && lane == 0) { a.base[row] = l; if (st == ROW_LIST) a.share[row] = 1.f; }
+      }
+      if (lane == 0) {
+        a.lse[row] = l;
+        a.loss[row] = st == ROW_LIST ? sum * a.t2 : st == ROW_NONE ? 0.f : __int_as_float(0x7fffffff);
+      }
     }
   }
   if (!a.ticket) return;
@@ -191,6 +217,73 @@ __global__ void __launch_bounds__(1024) joinRowsKernel(const JoinArgs a) {
   if (!last) return;
   __threadfence();
   reduceLoss(a.allLoss, a.allRows, a.all, a.mean, a.out, a.count);
+}
+
+// In front of the powers: the targets' logits, by a warp each, as the rows' bases; the number of rows that count; words set to their start.
+__global__ void __launch_bounds__(256) targetLogitsKernel(const uint4* x, const uint4* w, const VocabRows rows, int n, int packs, float* base, int* count, int* where,
+                                                          int v, int* words, int nWords) {
+  __shared__ int counts[8];
+  tc::grid_dependency_wait();
+  tc::grid_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (blockIdx.x == 0) {
+    int c = 0;
+    for (int i = threadIdx.x; i < n; i += 256) c += rowState(rows, i) != ROW_NONE;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+    if (lane == 0) counts[warp] = c;
+    __syncthreads();
+    if (threadIdx.x == 0) { for (int k = 1; k < 8; ++k) c += counts[k]; *count = c; }
+    for (int i = threadIdx.x; i < nWords; i += 256) words[i] = 0;
+  }
+  if (where) for (int i = blockIdx.x * 256 + threadIdx.x; i < v; i += gridDim.x * 256) where[i] = -1;
+  for (int row = blockIdx.x * 8 + warp; row < n; row += gridDim.x * 8) {
+    int token;
+    const int st = rowState(rows, row, token);
+    float sum = 0.f;
+    if (st == ROW_LIST)
+      for (int i = lane; i < packs; i += 32) {
+        const uint4 a = x[(size_t)row * packs + i], b = w[(size_t)token * packs + i];
+        const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum = fmaf(bf16Lo(aw[e]), bf16Lo(bw[e]), fmaf(bf16Hi(aw[e]), bf16Hi(bw[e]), sum));
+      }
+    sum = warpSum(sum);
+    if (lane == 0) base[row] = sum * rows.scale;
+  }
+}
+
+// x scale, a row's share each, rounded to bf16: the right operand of the powers' product.  Rows without a target are zeros whatever they hold.
+__global__ void __launch_bounds__(256) shareRowsKernel(const uint4* x, const VocabRows rows, const float* share, int n, int packs, uint4* out) {
+  tc::grid_dependency_wait();
+  tc::grid_launch_dependents();
+  for (int row = blockIdx.x; row < n; row += gridDim.x) {
+    const bool keep = rowState(rows, row) != ROW_NONE;
+    const float f = share[row];
+    for (int i = threadIdx.x; i < packs; i += 256) {
+      uint4 o = make_uint4(0u, 0u, 0u, 0u);
+      if (keep) {
+        const uint4 p = x[(size_t)row * packs + i];
+        o = make_uint4(tc::pack_bf16x2(bf16Lo(p.x) * f, bf16Hi(p.x) * f), tc::pack_bf16x2(bf16Lo(p.y) * f, bf16Hi(p.y) * f),
+                       tc::pack_bf16x2(bf16Lo(p.z) * f, bf16Hi(p.z) * f), tc::pack_bf16x2(bf16Lo(p.w) * f, bf16Hi(p.w) * f));
+      }
+      out[(size_t)row * packs + i] = o;
+    }
+  }
+}
+
+// Two results times one number on the device, in place; nothing is read or written where it is 1.
+__global__ void __launch_bounds__(256) scaleResultsKernel(uint4* a, size_t na, uint4* b, size_t nb, const float* scale) {
+  tc::grid_dependency_wait();
+  tc::grid_launch_dependents();
+  const float f = *scale;
+  if (f == 1.f) return;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < na + nb; i += (size_t)gridDim.x * 256) {
+    uint4* p = i < na ? a + i : b + (i - na);
+    const uint4 v = *p;
+    *p = make_uint4(tc::pack_bf16x2(bf16Lo(v.x) * f, bf16Hi(v.x) * f), tc::pack_bf16x2(bf16Lo(v.y) * f, bf16Hi(v.y) * f),
+                    tc::pack_bf16x2(bf16Lo(v.z) * f, bf16Hi(v.z) * f), tc::pack_bf16x2(bf16Lo(v.w) * f, bf16Hi(v.w) * f));
+  }
 }
 
 // x with zeros in the rows without a list: in the product of the weights' gradient they meet the zeros of the logits' gradient, and nothing
@@ -204,26 +297,40 @@ __global__ void __launch_bounds__(256) keepRowsKernel(const uint4* x, const Voca
   }
 }
 
-// out = factor times the sum of the slices, rounded once; `packs` of 8 elements.
-__global__ void __launch_bounds__(256) joinSlicesKernel(const float* part, int slices, size_t packs, const VocabFactor factor, __nv_bfloat16* out) {
+// out = factor times the sum of the slices, rounded once; `packs` of 8 elements, `rowPacks` to a row.  which: what `exact` adds, as in the products'
+// own epilogue: 1 of dx, 2 of dw, 0 nothing.
+__global__ void __launch_bounds__(256) joinSlicesKernel(const float* part, int slices, size_t packs, int rowPacks, const VocabFactor factor, const VocabExact exact,
+                                                        int which, __nv_bfloat16* out) {
   tc::grid_dependency_wait();
   tc::grid_launch_dependents();
-  const float f = vocabFactor(factor);
+  const float scale = vocabFactor(factor);
   for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < packs; i += (size_t)gridDim.x * 256) {
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < slices; ++s) {
       const float4* src = (const float4*)part + ((size_t)s * packs + i) * 2;
       const float4 x = src[0], y = src[1];
-      a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
-      b.x += y.x; b.y += y.y; b.z += y.z; b.w += y.w;
+      f[0] += x.x; f[1] += x.y; f[2] += x.z; f[3] += x.w; f[4] += y.x; f[5] += y.y; f[6] += y.z; f[7] += y.w;
     }
-    ((uint4*)out)[i] = make_uint4(tc::pack_bf16x2(a.x * f, a.y * f), tc::pack_bf16x2(a.z * f, a.w * f), tc::pack_bf16x2(b.x * f, b.y * f), tc::pack_bf16x2(b.z * f, b.w * f));
+    if (which) {
+      const int row = (int)(i / rowPacks), c = (int)(i - (size_t)row * rowPacks);
+      if (which == 1) {
+        int token;
+        const int st = rowState(exact.rows, row, token);
+        vocabExactX(f, st, exact.scale[row], (const uint4*)exact.w + (size_t)(st == ROW_LIST ? token : 0) * rowPacks + c);
+      } else {
+        const int at = exact.where[row];
+        if (at >= 0) vocabMinus(f, (const float4*)exact.sums + ((size_t)at * rowPacks + c) * 2);
+      }
+    }
+    ((uint4*)out)[i] = make_uint4(tc::pack_bf16x2(f[0] * scale, f[1] * scale), tc::pack_bf16x2(f[2] * scale, f[3] * scale), tc::pack_bf16x2(f[4] * scale, f[5] * scale),
+                                  tc::pack_bf16x2(f[6] * scale, f[7] * scale));
   }
 }
 
-ncclResult_t joinSlices(const float* part, int slices, size_t elements, const VocabFactor& factor, void* out, cudaStream_t stream) {
-  const size_t packs = elements / 8;
-  CUDACHECK(launchBehind(joinSlicesKernel, dim3((unsigned)std::min<size_t>((packs + 255) / 256, 148 * 8)), 256, stream, part, slices, packs, factor, (__nv_bfloat16*)out));
+ncclResult_t joinSlices(const float* part, int slices, int rows, int d, const VocabFactor& factor, const VocabExact* exact, int which, void* out, cudaStream_t stream) {
+  const size_t packs = (size_t)rows * d / 8;
+  CUDACHECK(launchBehind(joinSlicesKernel, dim3((unsigned)std::min<size_t>((packs + 255) / 256, 148 * 8)), 256, stream, part, slices, packs, d / 8, factor,
+                         exact ? *exact : VocabExact{}, exact ? which : 0, (__nv_bfloat16*)out));
   return ncclSuccess;
 }
 
@@ -317,8 +424,8 @@ DF_API ncclResult_t dfcclLinearLossForward(const void* x, const void* w, int n, 
     j.n = std::min(ROWS, n - r);
     j.rows = rowsOf(targets, wide, v, ignore, tokens, weights, state, k, temperature, r);
     j.lse = (float*)lse + r; j.loss = losses + r;
-    DFCHECK(vocabStats((const __nv_bfloat16*)x + (size_t)r * d, w, j.n, v, d, j.rows, (float2*)j.parts, (float*)j.picked, r ? nullptr : j.ticket, stream));
-    CUDACHECK(launchBehind(joinRowsKernel, (j.n + 31) / 32, 1024, stream, j));
+    DFCHECK(vocabStats((const __nv_bfloat16*)x + (size_t)r * d, w, j.n, v, d, j.rows, (float2*)j.parts, (float*)j.picked, r ? nullptr : j.ticket, nullptr, stream));
+    CUDACHECK(launchBehind(joinRowsKernel<false>, (j.n + 31) / 32, 1024, stream, j));
   }
   return ncclSuccess;
 }
@@ -349,9 +456,109 @@ DF_API ncclResult_t dfcclLinearLossBackward(const void* x, const void* w, int n,
     const __nv_bfloat16* wc = (const __nv_bfloat16*)w + (size_t)c * d;
     __nv_bfloat16* dwc = dw ? (__nv_bfloat16*)dw + (size_t)c * d : nullptr;
     DFCHECK(vocabGrad(x, wc, n, cols, c, d, rows, grad, dz, stream));
-    DFCHECK(vocabProducts(dz, kept, wc, n, cols, d, p.cut, factor, p.sumX ? nullptr : dx, partX, c != 0, p.sumW ? nullptr : dwc, partW, stream));
-    if (p.sumW) DFCHECK(joinSlices(partW, p.slicesW, (size_t)cols * d, factor, dwc, stream));
+    DFCHECK(vocabProducts(dz, kept, wc, n, cols, d, p.cut, factor, nullptr, VocabResult{p.sumX ? nullptr : dx, partX, c != 0}, VocabResult{p.sumW ? nullptr : dwc, partW, false}, stream));
+    if (p.sumW) DFCHECK(joinSlices(partW, p.slicesW, cols, d, factor, nullptr, 0, dwc, stream));
   }
-  if (p.sumX) DFCHECK(joinSlices(partX, p.slicesX, (size_t)n * d, factor, dx, stream));
+  if (p.sumX) DFCHECK(joinSlices(partX, p.slicesX, n, d, factor, nullptr, 0, dx, stream));
+  return ncclSuccess;
+}
+
+namespace {
+// How a pass with gradients goes over the rows, and where its parts of the workspace begin.
+struct OneGoPlan {
+  int rows;                       // of a piece (all of them, or a multiple of the tile)
+  VocabPlan cut;
+  int slicesX, slicesW;
+  bool sumX, sumW;
+  size_t powers, parts, partX, partW, shared, base, share, losses, words, where, sums, tokens, picked, bytes;
+};
+OneGoPlan oneGoPlan(int n, int v, int d, bool wantX, bool wantW) {
+  OneGoPlan p = {};
+  const size_t ld = (size_t)(v + 63) / 64 * 64;
+  const int64_t limit = std::max<int64_t>(1 << 20, paramI64("LOSS_WORKSPACE_BYTES", 1ll << 30));
+  const int64_t most = std::max<int64_t>(1, limit / (int64_t)(2 * ld) / VOCAB_TILE) * VOCAB_TILE;
+  const int64_t pieces = (n + most - 1) / most;
+  p.rows = pieces == 1 ? n : (int)(((n + pieces - 1) / pieces + VOCAB_TILE - 1) / VOCAB_TILE * VOCAB_TILE);
+  p.cut = vocabProductPlan(p.rows, v, d, wantX, wantW, gemmPairResident());
+  p.slicesX = vocabSlices(v, p.cut.perX);
+  p.slicesW = vocabSlices(p.rows, p.cut.perW);
+  p.sumX = wantX && p.slicesX > 1;
+  p.sumW = wantW && (pieces > 1 || p.slicesW > 1);
+  auto take = [&](size_t bytes) { const size_t at = p.bytes; p.bytes += up256(bytes); return at; };
+  p.powers = take(p.rows * ld * 2);
+  p.parts = take((size_t)p.rows * vocabParts(v) * sizeof(float2));
+  p.partX = take(p.sumX ? (size_t)p.slicesX * p.rows * d * 4 : 0);
+  p.partW = take(p.sumW ? (size_t)p.slicesW * v * d * 4 : 0);
+  p.shared = take(wantW ? (size_t)p.rows * d * 2 : 0);
+  p.base = take((size_t)n * 4); p.share = take((size_t)n * 4); p.losses = take((size_t)n * 4); p.picked = take((size_t)p.rows * 4);
+  p.words = take((size_t)(pieces + 1) * 4);
+  p.where = take(wantW ? (size_t)v * 4 : 0);
+  p.sums = take(wantW ? (size_t)n * d * 4 : 0);
+  p.tokens = take(wantW ? tokenSumsWork(n, d) : 0);
+  return p;
+}
+}  // namespace
+
+DF_API size_t dfcclCrossEntropyWithGradientsWork(int n, int v, int d, int wantX, int wantW) {
+  return sizesOk(n, v, d, 1) && (wantX || wantW) ? oneGoPlan(n, v, d, wantX != 0, wantW != 0).bytes : 0;
+}
+
+// Per piece of rows: powers of the logits relative to the targets' (vocabPowers), their sums, x times the rows' shares, the two products.  What the
+// targets themselves add to the gradients is most of their size and does not go through bf16 (VocabExact).  Rows with a power that is too
+// large send their piece through statistics and powers once more, with the logarithms of the sums as bases: launches that find nothing
+// to do otherwise (2 us each).
+DF_API ncclResult_t dfcclCrossEntropyWithGradients(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, int reduction,
+                                                   void* work, size_t workBytes, void* lse, void* loss, void* count, void* dx, void* dw, cudaStream_t stream) {
+  if (!sizesOk(n, v, d, 1) || !x || !w || !targets || !work || !lse || !loss || !count || !(dx || dw) || reduction < 1 || reduction > 2) return ncclInvalidArgument;
+  if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw) & 15) return ncclInvalidArgument;
+  const OneGoPlan p = oneGoPlan(n, v, d, dx != nullptr, dw != nullptr);
+  if (p.bytes > workBytes) return ncclInvalidArgument;           // (the setting has changed since the size was asked for)
+  uint8_t* at = (uint8_t*)work;
+  void* powers = at + p.powers;
+  float2* parts = (float2*)(at + p.parts);
+  float* partX = p.sumX ? (float*)(at + p.partX) : nullptr;
+  float* partW = p.sumW ? (float*)(at + p.partW) : nullptr;
+  float *base = (float*)(at + p.base), *share = (float*)(at + p.share), *losses = (float*)(at + p.losses);
+  int *words = (int*)(at + p.words), *where = (int*)(at + p.where);
+  const VocabRows all = rowsOf(targets, wide, v, ignore, nullptr, nullptr, nullptr, 1, 1.f, 0);
+  const int pieces = (n + p.rows - 1) / p.rows, packs = d / 8;
+  CUDACHECK(launchBehind(targetLogitsKernel, std::min((n + 7) / 8, 148 * 8), 256, stream, (const uint4*)x, (const uint4*)w, all, n, packs, base, (int*)count,
+                         dw ? where : nullptr, v, words, pieces + 1));
+  if (dw) DFCHECK(tokenSums(x, n, d, targets, wide, ignore, v, (float*)(at + p.sums), where, at + p.tokens, stream));
+  const VocabFactor factor{nullptr, reduction == 1 ? (const int*)count : nullptr, 1.f};
+  JoinArgs j = {};
+  j.parts = parts; j.picked = (const float*)(at + p.picked); j.stretches = vocabParts(v); j.t2 = 1.f;
+  j.allRows = all; j.allLoss = losses; j.all = n; j.mean = reduction == 1;
+  j.out = (float*)loss; j.count = (int*)count;
+  for (int r = 0; r < n; r += p.rows) j.blocks += (std::min(p.rows, n - r) + 31) / 32;
+  for (int i = 0; i < pieces; ++i) {
+    const int r = i * p.rows, m = std::min(p.rows, n - r);
+    const __nv_bfloat16* xr = (const __nv_bfloat16*)x + (size_t)r * d;
+    j.rows = rowsOf(targets, wide, v, ignore, nullptr, nullptr, nullptr, 1, 1.f, r);
+    j.n = m; j.lse = (float*)lse + r; j.loss = losses + r; j.base = base + r; j.share = share + r;
+    DFCHECK(vocabPowers(xr, w, m, v, d, j.rows, base + r, parts, powers, nullptr, stream));
+    j.again = words + 1 + i; j.only = nullptr; j.ticket = nullptr;
+    CUDACHECK(launchBehind(joinRowsKernel<true>, (m + 31) / 32, 1024, stream, j));
+    DFCHECK(vocabStats(xr, w, m, v, d, j.rows, parts, (float*)j.picked, nullptr, j.again, stream));
+    j.only = j.again; j.ticket = words;
+    CUDACHECK(launchBehind(joinRowsKernel<false>, (m + 31) / 32, 1024, stream, j));
+    DFCHECK(vocabPowers(xr, w, m, v, d, j.rows, base + r, parts, powers, j.again, stream));
+    if (dw) CUDACHECK(launchBehind(shareRowsKernel, std::min(m, 148 * 8), 256, stream, (const uint4*)xr, j.rows, (const float*)share + r, m, packs, (uint4*)(at + p.shared)));
+    const VocabExact exact{j.rows, share + r, (const __nv_bfloat16*)w, (const float*)(at + p.sums), where};
+    __nv_bfloat16* dxr = dx ? (__nv_bfloat16*)dx + (size_t)r * d : nullptr;
+    // (a shorter last piece has fewer slices of dw: it adds to the first of them)
+    DFCHECK(vocabProducts(powers, at + p.shared, w, m, v, d, p.cut, factor, &exact, VocabResult{p.sumX ? nullptr : dxr, partX, false},
+                          VocabResult{p.sumW ? nullptr : dw, partW, i != 0}, stream));
+    if (p.sumX) DFCHECK(joinSlices(partX, p.slicesX, m, d, factor, &exact, 1, dxr, stream));
+    if (p.sumW && i == pieces - 1) DFCHECK(joinSlices(partW, p.slicesW, v, d, factor, &exact, 2, dw, stream));
+  }
+  return ncclSuccess;
+}
+
+DF_API ncclResult_t dfcclScaleResults(void* a, size_t na, void* b, size_t nb, const void* scale, cudaStream_t stream) {
+  if (!scale || na % 8 || nb % 8 || (na && !a) || (nb && !b) || !(na || nb) || (((uintptr_t)a | (uintptr_t)b) & 15)) return ncclInvalidArgument;
+  const size_t packs = (na + nb) / 8;
+  CUDACHECK(launchBehind(scaleResultsKernel, dim3((unsigned)std::min<size_t>((packs + 255) / 256, 148 * 8)), 256, stream, (uint4*)a, na / 8, (uint4*)b, nb / 8,
+                         (const float*)scale));
   return ncclSuccess;
 }

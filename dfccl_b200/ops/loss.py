@@ -13,6 +13,8 @@ from .block import packed
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 MAX_LIST = 256                       # entries of a teacher's list
+# Rows x vocabulary x width from which a reduced cross entropy makes its gradients with the loss.
+ONE_GO_FROM = 2 ** 35
 
 
 def linear_loss_supported(x: torch.Tensor, weight: torch.Tensor) -> bool:
@@ -84,10 +86,47 @@ def _forward(x, weight, rows, reduction):
     return loss, xp, wp, kept
 
 
+def _forward_with_gradients(x, weight, rows, reduction, want_x, want_w):
+    """What ``_forward`` returns, and the gradients of x and weight for a gradient of 1 of the loss."""
+    v, d = weight.shape
+    n, device = x.numel() // d, x.device
+    xp, wp = packed(x), packed(weight)
+    kept = torch.empty(n + 1, dtype=torch.float32, device=device)
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=device) if want_x else None
+    dw = torch.empty(v, d, dtype=x.dtype, device=device) if want_w else None
+    targets, at = rows.targets, kept.data_ptr()
+    with on_device(device):
+        size = nv.lib().dfcclCrossEntropyWithGradientsWork(n, v, d, want_x, want_w)
+        work = torch.empty(size, dtype=torch.uint8, device=device)
+        nv.check(nv.long_entry("dfcclCrossEntropyWithGradients")(xp.data_ptr(), wp.data_ptr(), n, v, d, targets.data_ptr(), int(targets.dtype == torch.int64), rows.ignore,
+                                                                 reduction, work.data_ptr(), size, at, loss.data_ptr(), at + 4 * n,
+                                                                 dx.data_ptr() if want_x else None, dw.data_ptr() if want_w else None, stream_of(x)),
+                 "dfcclCrossEntropyWithGradients")
+    return loss, xp, wp, kept, (dx, dw)
+
+
+def _scaled(grads, g):
+    """The gradients times that of the loss, in place: nothing else holds them."""
+    dx, dw = grads
+    with on_device(g.device):
+        nv.check(nv.entry("dfcclScaleResults")(None if dx is None else dx.data_ptr(), 0 if dx is None else dx.numel(), None if dw is None else dw.data_ptr(),
+                                               0 if dw is None else dw.numel(), g.data_ptr(), stream_of(g)), "dfcclScaleResults")
+    return dx, dw, None, None
+
+
 class _LinearLossFn(torch.autograd.Function):
+    """A reduced cross entropy of some size makes its gradients with the loss, which saves computing the logits a second time: the
+    first backward pass scales them.  Another pass over the same graph, and every other loss, computes the logits again."""
+
     @staticmethod
     def forward(ctx, x, weight, rows, reduction):
-        loss, xp, wp, kept = _forward(x, weight, rows, reduction)
+        want_x, want_w = ctx.needs_input_grad[:2]
+        ctx.grads = None
+        if reduction and rows.lists is None and x.numel() * weight.shape[0] >= ONE_GO_FROM and (want_x or want_w):
+            loss, xp, wp, kept, ctx.grads = _forward_with_gradients(x, weight, rows, reduction, want_x, want_w)
+        else:
+            loss, xp, wp, kept = _forward(x, weight, rows, reduction)
         ctx.save_for_backward(xp, wp, kept, *rows.tensors())
         ctx.rows, ctx.mean, ctx.shape = rows, reduction == 1, x.shape
         ctx.set_materialize_grads(False)
@@ -100,6 +139,9 @@ class _LinearLossFn(torch.autograd.Function):
         if g is None or not (want_x or want_w):
             return None, None, None, None
         x, w, kept = ctx.saved_tensors[:3]                  # (asking for them notices a change in place, of the targets too)
+        grads, ctx.grads = ctx.grads, None
+        if grads is not None:
+            return _scaled(grads, g)
         (v, d), n, device = w.shape, kept.shape[0] - 1, x.device
         if n == 0:
             return torch.zeros_like(x) if want_x else None, torch.zeros_like(w) if want_w else None, None, None
