@@ -45,8 +45,6 @@ struct VocabArgs {
   int headStart;                    // rounds of the second product's items that pairs with one item less of the first take alone
   VocabRows rows;
   float2* parts;
-  float* picked;
-  int* ticket;
   VocabGrad grad;
   const float* base;                // of the powers
   VocabFactor factor;
@@ -146,7 +144,6 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
   grid_dependency_wait();
   grid_launch_dependents();
   if ((MODE == VOCAB_STATS || MODE == VOCAB_POWERS) && g.only && *g.only == 0) count = 0;
-  if (MODE == VOCAB_STATS && g.ticket && blockIdx.x == 0 && threadIdx.x == 0) *g.ticket = 0;
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs; bytes counted in the leader)
@@ -257,7 +254,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
             coef = g.grad.gout ? g.grad.gout[(size_t)row * g.grad.goutStride] : 1.f;
             if (state != ROW_LIST) coef = state == ROW_BAD ? __int_as_float(0x7fffffff) : 0.f;
           }
-          if (MODE != VOCAB_POWERS) list.seek(g.rows, row, token, g.first + col0);
+          list.seek(g.rows, row, token, g.first + col0);
         }
         if (!mbar_wait(&accFull[ab], (j >> 1) & 1, giveUp, WAIT_NS)) break;
         tc_fence_after();
@@ -278,10 +275,8 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
             while (list.next < c + 32) {
               if (list.next >= c) {
                 const int at = list.next - c;
-                float z = 0.f;
 #pragma unroll
-                for (int e = 0; e < 32; ++e) if (e == at) z = __uint_as_float(r[e]);
-                g.picked[(size_t)row * g.rows.k + list.pos] = z;
+                for (int e = 0; e < 32; ++e) if (e == at) r[e] = 0xff800000u;
               }
               list.step();
             }
@@ -300,6 +295,12 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
 #pragma unroll
               for (int e = 0; e < 32; ++e) if (c + e >= p.N) r[e] = 0xff800000u;          // -inf
             }
+            const int own = list.next - c;               // the target's column, out of the sum
+            float target = 0.f;
+            if (own >= 0 && own < 32) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) if (e == own) { target = __uint_as_float(r[e]); r[e] = 0xff800000u; }
+            }
             float m0 = __uint_as_float(r[0]), m1 = __uint_as_float(r[1]);
 #pragma unroll
             for (int e = 2; e < 32; e += 2) { m0 = fmaxf(m0, __uint_as_float(r[e])); m1 = fmaxf(m1, __uint_as_float(r[e + 1])); }
@@ -312,6 +313,11 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
               r[e] = __float_as_uint(v);
             }
             sum = (s[0] + s[1]) + (s[2] + s[3]);
+            if (own >= 0 && own < 32) {
+              target = exp2Approx(fmaf(target, scale, -lse));
+#pragma unroll
+              for (int e = 0; e < 32; ++e) if (e == own) r[e] = __float_as_uint(target);
+            }
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(exp2Approx(fmaf(__uint_as_float(r[e]), scale, -lse)));
@@ -457,12 +463,11 @@ ncclResult_t logits(CUtensorMap* a, CUtensorMap* b, VocabArgs* g, const void* x,
 
 }  // namespace
 
-ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, float* picked, int* ticket, const int* only,
-                        cudaStream_t stream) {
+ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, const int* only, cudaStream_t stream) {
   CUtensorMap a, b;
   VocabArgs g;
   DFCHECK(logits(&a, &b, &g, x, w, n, v, d, rows));
-  g.parts = parts; g.picked = picked; g.ticket = ticket; g.only = only;
+  g.parts = parts; g.only = only;
   return launchVocab<VOCAB_STATS>(a, b, a, b, g, stream);
 }
 

@@ -39,14 +39,14 @@ __device__ __forceinline__ int rowState(const VocabRows& r, int row) { int token
 
 inline int vocabParts(int v) { return (v + VOCAB_TILE - 1) / VOCAB_TILE * VOCAB_PARTS; }
 
-// z = x [n, d] w[v, d]^T, tile by tile and never stored.  Of every row: for each of the vocabParts(v) stretches of its columns
-// {largest z scale, sum of 2^(z scale - that)} -> parts [stretch][n], and the z of its list's entries -> picked [n][k].  `ticket`, where given, is set to 0.
-// `only`, where given: nothing happens unless it holds something other than 0.
-ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, float* picked, int* ticket, const int* only,
-                        cudaStream_t stream);
+// z = x [n, d] w[v, d]^T, tile by tile and never stored.  Of every row, for each of the vocabParts(v) stretches of its columns and without the
+// entries of its list: {largest z scale, sum of 2^(z scale - that)} -> parts [stretch][n].  (The tensor cores cut off what does not fit an
+// accumulator, step by step: a logit of 20 from 1024 products of one sign is 2.5e-5 too small, one of 4096 products 9e-5.  The logits that stand
+// out, and that a loss is the difference to, are computed apart.)  `only`, where given: nothing happens unless it holds something other than 0.
+ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, const int* only, cudaStream_t stream);
 
 // powers = 2^(z scale - base) of every row with a target, 0 elsewhere: bf16, [n][ld], ld = v rounded up to 64 (zeros behind v).  Of each stretch
-// of a row's columns {largest exponent, sum of the powers in fp32} -> parts [stretch][n].
+// of a row's columns, without its target: {largest exponent, sum of the powers in fp32} -> parts [stretch][n].
 ncclResult_t vocabPowers(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, const float* base, float2* parts, void* powers, const int* only,
                          cudaStream_t stream);
 

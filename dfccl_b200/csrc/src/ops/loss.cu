@@ -147,8 +147,7 @@ struct JoinArgs {
   int* count;
 };
 
-// A base is good while no power is above 2^60 (the sums of powers times x or w stay far from the end of fp32) and the target's own power,
-// 1 but for rounding, is in the sum.
+// A base is good if it is a number and no power is above 2^60: the sums of powers times x or w stay far from the end of fp32.
 constexpr float MOST_POWER = 60.f;
 
 // 32 rows per block: warp g takes every 32nd stretch of all of them (a line of 256 bytes each), then warp r finishes row r.
@@ -184,13 +183,24 @@ __global__ void __launch_bounds__(1024) joinRowsKernel(const JoinArgs a) {
       const int st = rowState(a.rows, row);
       float l, sum = 0.f;
       if (POWERS) {
-        l = a.base[row] + log2f(acc.y);
-        sum = log2f(fmaxf(acc.y, 1.f)) * LN2;           // the target's power alone is 1
+        l = a.base[row] + log2f(1.f + acc.y);           // the target's own power is 1
+        sum = log1pf(acc.y);
         if (lane == 0) {
-          a.share[row] = st == ROW_LIST ? 1.f / acc.y : st == ROW_NONE ? 0.f : __int_as_float(0x7fffffff);
-          if (st == ROW_LIST && !(acc.x <= MOST_POWER && acc.y >= 0.5f)) *a.again = 1;
+          a.share[row] = st == ROW_LIST ? 1.f / (1.f + acc.y) : st == ROW_NONE ? 0.f : __int_as_float(0x7fffffff);
+          if (st == ROW_LIST && !(acc.x <= MOST_POWER && acc.y < INFINITY && fabsf(a.base[row]) < INFINITY)) *a.again = 1;
         }
       } else {
+        if (st == ROW_LIST) {                           // the list's own powers, each entry once
+          float2 own = make_float2(-INFINITY, 0.f);
+          for (int i = lane; i < a.rows.k; i += 32) {
+            const size_t at = (size_t)row * a.rows.k + i;
+            if (!a.rows.targets && (a.rows.tokens[at] == VOCAB_NO_TOKEN || (i && a.rows.tokens[at] == a.rows.tokens[at - 1]))) continue;
+            own = joined(own, make_float2(a.picked[at] * a.rows.scale, 1.f));
+          }
+#pragma unroll
+          for (int o = 16; o; o >>= 1) own = joined(own, make_float2(__shfl_xor_sync(0xffffffffu, own.x, o), __shfl_xor_sync(0xffffffffu, own.y, o)));
+          acc = joined(acc, own);
+        }
         l = acc.x + log2f(acc.y);
         if (st == ROW_LIST)
           for (int i = lane; i < a.rows.k; i += 32) {
@@ -219,38 +229,80 @@ __global__ void __launch_bounds__(1024) joinRowsKernel(const JoinArgs a) {
   reduceLoss(a.allLoss, a.allRows, a.all, a.mean, a.out, a.count);
 }
 
-// In front of the powers: the targets' logits, by a warp each, as the rows' bases; the number of rows that count; words set to their start.
-__global__ void __launch_bounds__(256) targetLogitsKernel(const uint4* x, const uint4* w, const VocabRows rows, int n, int packs, float* base, int* count, int* where,
-                                                          int v, int* words, int nWords) {
+// In front of the products: the logits of the rows' lists by fp32 sums, a warp for four entries of a row, -> picked [n][k] (and times `scale`, as
+// the bases of powers, where `base` is given; k = 1 there).  On the way, words set to their start and the number of rows that count.
+struct PickArgs {
+  const uint4* x; const uint4* w;
+  VocabRows rows;
+  int n, packs;                  // of 8 columns
+  float* picked;
+  float* base;
+  int* count;                    // or null
+  int* where; int v;             // [v] to be -1, or null
+  int* words; int nWords;        // to be 0
+};
+__global__ void __launch_bounds__(256) pickLogitsKernel(const PickArgs a) {
   __shared__ int counts[8];
   tc::grid_dependency_wait();
   tc::grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (blockIdx.x == 0) {
-    int c = 0;
-    for (int i = threadIdx.x; i < n; i += 256) c += rowState(rows, i) != ROW_NONE;
+    if (a.count) {
+      int c = 0;
+      for (int i = threadIdx.x; i < a.n; i += 256) c += rowState(a.rows, i) != ROW_NONE;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-    if (lane == 0) counts[warp] = c;
-    __syncthreads();
-    if (threadIdx.x == 0) { for (int k = 1; k < 8; ++k) c += counts[k]; *count = c; }
-    for (int i = threadIdx.x; i < nWords; i += 256) words[i] = 0;
+      for (int o = 16; o; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+      if (lane == 0) counts[warp] = c;
+      __syncthreads();
+      if (threadIdx.x == 0) { for (int k = 1; k < 8; ++k) c += counts[k]; *a.count = c; }
+    }
+    for (int i = threadIdx.x; i < a.nWords; i += 256) a.words[i] = 0;
   }
-  if (where) for (int i = blockIdx.x * 256 + threadIdx.x; i < v; i += gridDim.x * 256) where[i] = -1;
-  for (int row = blockIdx.x * 8 + warp; row < n; row += gridDim.x * 8) {
+  if (a.where) for (int i = blockIdx.x * 256 + threadIdx.x; i < a.v; i += gridDim.x * 256) a.where[i] = -1;
+  const int k = a.rows.k, fours = (k + 3) / 4;
+  for (long long item = (long long)blockIdx.x * 8 + warp; item < (long long)a.n * fours; item += (long long)gridDim.x * 8) {
+    const int row = (int)(item / fours), first = (int)(item - (long long)row * fours) * 4;
     int token;
-    const int st = rowState(rows, row, token);
-    float sum = 0.f;
-    if (st == ROW_LIST)
-      for (int i = lane; i < packs; i += 32) {
-        const uint4 a = x[(size_t)row * packs + i], b = w[(size_t)token * packs + i];
-        const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+    const bool list = rowState(a.rows, row, token) == ROW_LIST;
+    const uint4* w[4];
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    bool some = false;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum = fmaf(bf16Lo(aw[e]), bf16Lo(bw[e]), fmaf(bf16Hi(aw[e]), bf16Hi(bw[e]), sum));
+    for (int e = 0; e < 4; ++e) {
+      int t = VOCAB_NO_TOKEN;
+      if (list) t = a.rows.targets ? e ? VOCAB_NO_TOKEN : token : first + e < k ? a.rows.tokens[(size_t)row * k + first + e] : VOCAB_NO_TOKEN;
+      w[e] = t == VOCAB_NO_TOKEN ? nullptr : a.w + (size_t)t * a.packs;
+      some = some || w[e];
+    }
+    if (some)
+      for (int i = lane; i < a.packs; i += 32) {
+        const uint4 x = a.x[(size_t)row * a.packs + i];
+        const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
+        uint4 y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = w[e] ? w[e][i] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t yw[4] = {y[e].x, y[e].y, y[e].z, y[e].w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) sum[e] = fmaf(bf16Lo(xw[q]), bf16Lo(yw[q]), fmaf(bf16Hi(xw[q]), bf16Hi(yw[q]), sum[e]));
+        }
       }
-    sum = warpSum(sum);
-    if (lane == 0) base[row] = sum * rows.scale;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (first + e >= k) break;
+      const float z = warpSum(sum[e]);
+      if (lane == 0) {
+        a.picked[(size_t)row * k + first + e] = z;
+        if (a.base) a.base[row] = z * a.rows.scale;
+      }
+    }
   }
+}
+ncclResult_t pickLogits(const PickArgs& a, cudaStream_t stream) {
+  const long long items = (long long)a.n * ((a.rows.k + 3) / 4);
+  CUDACHECK(launchBehind(pickLogitsKernel, dim3((unsigned)std::min<long long>((items + 7) / 8, 148 * 8)), 256, stream, a));
+  return ncclSuccess;
 }
 
 // x scale, a row's share each, rounded to bf16: the right operand of the powers' product.  Rows without a target are zeros whatever they hold.
@@ -385,8 +437,7 @@ DF_API ncclResult_t dfcclTeacherRows(const void* logits, int logitType, const vo
 namespace {
 struct ForwardLayout { size_t parts, picked, loss; };
 ForwardLayout forwardLayout(int n, int v, int k) {
-  const size_t rows = std::min(n, ROWS);
-  return ForwardLayout{up256(rows * vocabParts(v) * sizeof(float2)), up256(rows * k * 4), up256((size_t)n * 4)};
+  return ForwardLayout{up256((size_t)std::min(n, ROWS) * vocabParts(v) * sizeof(float2)), up256((size_t)n * k * 4), up256((size_t)n * 4)};
 }
 // A target per row, or lists; from row `r` on.
 VocabRows rowsOf(const void* targets, int wide, int v, int64_t ignore, const void* tokens, const void* weights, const void* state, int k, float temperature, int r) {
@@ -412,19 +463,22 @@ DF_API ncclResult_t dfcclLinearLossForward(const void* x, const void* w, int n, 
   if ((((uintptr_t)x | (uintptr_t)w) & 15) || (reduction ? !loss || !count : !rowLoss)) return ncclInvalidArgument;
   const ForwardLayout l = forwardLayout(n, v, k);
   JoinArgs j = {};
-  j.parts = (const float2*)work; j.picked = (const float*)((uint8_t*)work + l.parts);
+  j.parts = (const float2*)work;
+  float* picked = (float*)((uint8_t*)work + l.parts);
   j.stretches = vocabParts(v); j.t2 = temperature * temperature;
   float* losses = rowLoss ? (float*)rowLoss : (float*)((uint8_t*)work + l.parts + l.picked);
   j.allRows = rowsOf(targets, wide, v, ignore, tokens, weights, state, k, temperature, 0);
   j.allLoss = losses; j.all = n; j.mean = reduction == 1;
   j.ticket = reduction ? (int*)((uint8_t*)work + l.parts + l.picked + l.loss) : nullptr;
   j.out = (float*)loss; j.count = (int*)count;
+  DFCHECK(pickLogits(PickArgs{(const uint4*)x, (const uint4*)w, j.allRows, n, d / 8, picked, nullptr, nullptr, nullptr, 0, j.ticket, j.ticket ? 1 : 0}, stream));
   for (int r = 0; r < n; r += ROWS) j.blocks += (std::min(ROWS, n - r) + 31) / 32;
   for (int r = 0; r < n; r += ROWS) {
     j.n = std::min(ROWS, n - r);
+    j.picked = picked + (size_t)r * k;
     j.rows = rowsOf(targets, wide, v, ignore, tokens, weights, state, k, temperature, r);
     j.lse = (float*)lse + r; j.loss = losses + r;
-    DFCHECK(vocabStats((const __nv_bfloat16*)x + (size_t)r * d, w, j.n, v, d, j.rows, (float2*)j.parts, (float*)j.picked, r ? nullptr : j.ticket, nullptr, stream));
+    DFCHECK(vocabStats((const __nv_bfloat16*)x + (size_t)r * d, w, j.n, v, d, j.rows, (float2*)j.parts, nullptr, stream));
     CUDACHECK(launchBehind(joinRowsKernel<false>, (j.n + 31) / 32, 1024, stream, j));
   }
   return ncclSuccess;
@@ -490,7 +544,7 @@ OneGoPlan oneGoPlan(int n, int v, int d, bool wantX, bool wantW) {
   p.partX = take(p.sumX ? (size_t)p.slicesX * p.rows * d * 4 : 0);
   p.partW = take(p.sumW ? (size_t)p.slicesW * v * d * 4 : 0);
   p.shared = take(wantW ? (size_t)p.rows * d * 2 : 0);
-  p.base = take((size_t)n * 4); p.share = take((size_t)n * 4); p.losses = take((size_t)n * 4); p.picked = take((size_t)p.rows * 4);
+  p.base = take((size_t)n * 4); p.share = take((size_t)n * 4); p.losses = take((size_t)n * 4); p.picked = take((size_t)n * 4);
   p.words = take((size_t)(pieces + 1) * 4);
   p.where = take(wantW ? (size_t)v * 4 : 0);
   p.sums = take(wantW ? (size_t)n * d * 4 : 0);
@@ -522,12 +576,12 @@ DF_API ncclResult_t dfcclCrossEntropyWithGradients(const void* x, const void* w,
   int *words = (int*)(at + p.words), *where = (int*)(at + p.where);
   const VocabRows all = rowsOf(targets, wide, v, ignore, nullptr, nullptr, nullptr, 1, 1.f, 0);
   const int pieces = (n + p.rows - 1) / p.rows, packs = d / 8;
-  CUDACHECK(launchBehind(targetLogitsKernel, std::min((n + 7) / 8, 148 * 8), 256, stream, (const uint4*)x, (const uint4*)w, all, n, packs, base, (int*)count,
-                         dw ? where : nullptr, v, words, pieces + 1));
+  float* picked = (float*)(at + p.picked);
+  DFCHECK(pickLogits(PickArgs{(const uint4*)x, (const uint4*)w, all, n, packs, picked, base, (int*)count, dw ? where : nullptr, v, words, pieces + 1}, stream));
   if (dw) DFCHECK(tokenSums(x, n, d, targets, wide, ignore, v, (float*)(at + p.sums), where, at + p.tokens, stream));
   const VocabFactor factor{nullptr, reduction == 1 ? (const int*)count : nullptr, 1.f};
   JoinArgs j = {};
-  j.parts = parts; j.picked = (const float*)(at + p.picked); j.stretches = vocabParts(v); j.t2 = 1.f;
+  j.parts = parts; j.stretches = vocabParts(v); j.t2 = 1.f;
   j.allRows = all; j.allLoss = losses; j.all = n; j.mean = reduction == 1;
   j.out = (float*)loss; j.count = (int*)count;
   for (int r = 0; r < n; r += p.rows) j.blocks += (std::min(p.rows, n - r) + 31) / 32;
@@ -535,11 +589,11 @@ DF_API ncclResult_t dfcclCrossEntropyWithGradients(const void* x, const void* w,
     const int r = i * p.rows, m = std::min(p.rows, n - r);
     const __nv_bfloat16* xr = (const __nv_bfloat16*)x + (size_t)r * d;
     j.rows = rowsOf(targets, wide, v, ignore, nullptr, nullptr, nullptr, 1, 1.f, r);
-    j.n = m; j.lse = (float*)lse + r; j.loss = losses + r; j.base = base + r; j.share = share + r;
+    j.n = m; j.lse = (float*)lse + r; j.loss = losses + r; j.base = base + r; j.share = share + r; j.picked = picked + r;
     DFCHECK(vocabPowers(xr, w, m, v, d, j.rows, base + r, parts, powers, nullptr, stream));
     j.again = words + 1 + i; j.only = nullptr; j.ticket = nullptr;
     CUDACHECK(launchBehind(joinRowsKernel<true>, (m + 31) / 32, 1024, stream, j));
-    DFCHECK(vocabStats(xr, w, m, v, d, j.rows, parts, (float*)j.picked, nullptr, j.again, stream));
+    DFCHECK(vocabStats(xr, w, m, v, d, j.rows, parts, j.again, stream));
     j.only = j.again; j.ticket = words;
     CUDACHECK(launchBehind(joinRowsKernel<false>, (m + 31) / 32, 1024, stream, j));
     DFCHECK(vocabPowers(xr, w, m, v, d, j.rows, base + r, parts, powers, j.again, stream));

@@ -34,16 +34,20 @@ def reference(x, w, tokens, q, temp):
     return loss, torch.where(keep.any(dim=1)[:, None], dz, 0.0)
 
 
-def check_gradients(got, x, w, dz, share, temp, limit=2.0 ** -8):
-    """Elementwise by the sums of magnitudes, and in the 2-norm: two roundings, each below 2**-9, are below 2**-8 together."""
+def check_gradients(got, x, w, dz, share, temp, limit=2.0 ** -8, more=0.0):
+    """Elementwise by the sums of magnitudes, and in the 2-norm: two roundings, each below 2**-9, are below 2**-8 together.
+    ``more``: of a probability, in the gradient of w."""
     err = logit_error(x, w)
     rel = 2.0 ** -8 * (1 + 2.0 ** -8) + 2.0 ** -18 + 3 * err.max().item() / temp      # of p; p - q and its factor are rounded after it
     dz = dz * share[:, None]
-    off = dz.abs() * rel + temp * share.abs()[:, None] * torch.minimum(torch.softmax(x.double() @ w.double().t() / temp, dim=1), torch.ones_like(dz)) * (rel - 2.0 ** -8)
+    p = temp * share.abs()[:, None] * torch.softmax(x.double() @ w.double().t() / temp, dim=1)
+    off = dz.abs() * rel + p * (rel - 2.0 ** -8)
     xd, wd = x.double(), w.double()
     depth = (max(x.shape[0], w.shape[0]) / 16 + 8) * 2.0 ** -23
-    for name, g, want, bound, size in (("dx", got[0], dz @ wd, off @ wd.abs(), dz.abs() @ wd.abs()),
-                                       ("dw", got[1], dz.t() @ xd, off.t() @ xd.abs(), dz.abs().t() @ xd.abs())):
+    # a probability below the smallest normal number, 2**-126, is 0: of every term of a sum that much times the other factor
+    least = 2.0 ** -126 * max(1.0, temp * share.abs().max().item())
+    for name, g, want, bound, size in (("dx", got[0], dz @ wd, off @ wd.abs() + least * wd.abs().sum(dim=0), dz.abs() @ wd.abs()),
+                                       ("dw", got[1], dz.t() @ xd, (off + more * p).t() @ xd.abs() + least * xd.abs().sum(dim=0), dz.abs().t() @ xd.abs())):
         if g is None:
             continue
         tol = bound * (1 + 2.0 ** -8) + want.abs() * 2.0 ** -8 + size * depth + 1e-38
@@ -138,6 +142,105 @@ def test_pieces_of_the_vocabulary(n, v, d, limit, monkeypatch):
         xl, wl = x.clone().requires_grad_(want_x), w.clone().requires_grad_(want_w)
         linear_cross_entropy(xl, wl, t, reduction="sum").backward()
         check_gradients((xl.grad, wl.grad), x, w, dz, torch.ones(n, dtype=torch.float64, device="cuda"), 1.0)
+
+
+ONE_GO = [(1, 1, 8), (1, 300, 16), (77, 1000, 64), (255, 513, 136), (256, 512, 256), (300, 5000, 200), (1000, 3001, 320), (2049, 640, 1024), (40, 50257, 64)]
+
+
+@pytest.mark.parametrize("limit", [1 << 20, 1 << 30])
+@pytest.mark.parametrize("n,v,d", ONE_GO)
+def test_gradients_with_the_loss(n, v, d, limit, monkeypatch):
+    """The form that large losses take, in one piece of rows or several: the powers are rounded once for both gradients (the target's share of
+    them is not), and x times a row's share once more for that of w.  Scaled by what comes from behind, one more rounding."""
+    from dfccl_b200.ops import loss as module
+    from dfccl_b200.ops.gemm import check_kernels
+    monkeypatch.setattr(module, "ONE_GO_FROM", 0)
+    monkeypatch.setenv("DFCCL_LOSS_WORKSPACE_BYTES", str(limit))
+    x, w, gen = problem(n, v, d, n + 3 * v + 5 * d)
+    t = torch.randint(0, v, (n,), generator=gen, device="cuda")
+    drop = torch.rand(n, generator=gen, device="cuda") < 0.2
+    drop[0] = False
+    targets = torch.where(drop, -100, t)
+    loss, dz = reference(x, w, t[:, None], (~drop).double()[:, None], 1.0)
+    count = (~drop).sum().double()
+    two = 2.0 ** -8 * (1 + 2.0 ** -8)
+    for reduction, share in (("mean", 1.0 / count), ("sum", torch.ones_like(count))):
+        for want_x, want_w in ((True, True), (True, False), (False, True)):
+            a, b = x.clone().requires_grad_(want_x), w.clone().requires_grad_(want_w)
+            value = module.linear_cross_entropy(a, b, targets, reduction=reduction)
+            err = 2 * logit_error(x, w).max().item() + 2 * LN * (1 + loss.abs().max().item())
+            assert abs(value.item() - (loss.sum() * share).item()) <= err * (1 if reduction == "mean" else n)
+            value.backward(retain_graph=True)
+            each = share.expand(n)
+            check_gradients((a.grad, b.grad), x, w, dz, each, 1.0, more=two)
+            first = [None if g is None else g.clone() for g in (a.grad, b.grad)]
+            a.grad = b.grad = None
+            (value * 3).backward()                       # the same graph again: the logits are computed again
+            check_gradients((a.grad, b.grad), x, w, dz, 3 * each, 1.0)
+            a.grad = b.grad = None
+            other = module.linear_cross_entropy(a, b, targets, reduction=reduction)
+            (other * 0.3).backward()
+            for g, f in zip((a.grad, b.grad), first):    # one rounding of 0.3 times the same values
+                if g is not None:
+                    assert torch.equal(g, (f.float() * 0.3).to(torch.bfloat16))
+    assert check_kernels()
+
+
+def test_gradients_with_the_loss_of_odd_rows(monkeypatch):
+    """Targets far below their row's largest logit (powers above 2**60, which send the piece through once more), ignored rows that hold
+    anything, a target of probability one; infinities, NaN and targets outside give what they give otherwise."""
+    from dfccl_b200.ops import loss as module
+    monkeypatch.setattr(module, "ONE_GO_FROM", 0)
+    n, v, d = 400, 900, 64
+    for spread in (0.5, 40.0):
+        x, w, gen = problem(n, v, d, 77, spread=spread)
+        t = torch.randint(0, v, (n,), generator=gen, device="cuda")
+        t[::7] = (x[::7].double() @ w.double().t()).argmax(dim=1)
+        hole = torch.arange(n, device="cuda") % 5 == 2
+        targets = torch.where(hole, -100, t)
+        loss, dz = reference(x, w, t[:, None], (~hole).double()[:, None], 1.0)
+        dirty = x.clone()
+        dirty[hole] = torch.tensor([float("inf"), float("nan"), float("-inf"), 1e38], device="cuda").to(torch.bfloat16).repeat(16)
+        a, b = dirty.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        value = module.linear_cross_entropy(a, b, targets, reduction="sum")
+        assert abs(value.item() - loss.sum().item()) <= n * 2 * logit_error(x, w).max().item() + 2 * LN * (n + loss.sum().item())
+        value.backward()
+        a.grad[hole] += 0                                # (zeros stay)
+        check_gradients((a.grad, b.grad), x, w, dz, torch.ones(n, device="cuda").double(), 1.0, more=2.0 ** -8)
+        assert bool((a.grad[hole] == 0).all())
+    zero, b = dirty.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    value = module.linear_cross_entropy(zero, b, torch.full_like(t, -100))
+    value.backward()
+    assert value.item() == 0.0 and bool((zero.grad == 0).all()) and bool((b.grad == 0).all())
+    for bad in (v, -1):
+        a = x.clone().requires_grad_(True)
+        value = module.linear_cross_entropy(a, w, torch.where(torch.arange(n, device="cuda") == 3, bad, t))
+        value.backward()
+        assert value.isnan().item() and a.grad.isnan().any(dim=1).nonzero()[:, 0].tolist() == [3]
+    for k, value in ((8, float("-inf")), (9, float("inf")), (10, float("nan"))):
+        w2, ones = w.clone(), torch.ones_like(x)
+        w2[k] = value
+        with torch.no_grad():
+            plain = [module.linear_cross_entropy(ones, w2, torch.full_like(t, c), reduction="sum") for c in (k, 20)]
+        odd = [module.linear_cross_entropy(ones.clone().requires_grad_(True), w2, torch.full_like(t, c), reduction="sum") for c in (k, 20)]
+        for p, q in zip(plain, odd):
+            assert torch.equal(p.isnan(), q.isnan()) and (p.isnan().item() or abs(p.item() - q.item()) <= 1e-5 * abs(p.item()) or p.item() == q.item())
+
+
+def test_small_losses_and_large_logits():
+    """The logits of the targets are not what the tensor cores cut off, whichever way the loss goes: rows whose target stands out by 20, from
+    2048 products of one sign, have a loss of 2e-9 relative to 900 others, and those of the others one of 20."""
+    from dfccl_b200.ops.loss import linear_cross_entropy, linear_distillation
+    n, v, d = 64, 900, 2048
+    w = torch.zeros(v, d, device="cuda", dtype=torch.bfloat16)
+    w[5] = 2.0 ** -7
+    x = torch.full((n, d), 1.25, device="cuda", dtype=torch.bfloat16)            # logits of 20 exactly, and of 0
+    for token, want in ((5, 899 * 2.061153622438558e-09), (6, 20 + 899 * 2.061153622438558e-09)):
+        t = torch.full((n,), token, device="cuda")
+        got = linear_cross_entropy(x, w, t, reduction="none").double()
+        assert bool(((got - want).abs() <= 2.0 ** -22 * 20 + 2.0 ** -22).all())
+        again = linear_distillation(x, w, torch.zeros(n, 1, device="cuda"), t[:, None], reduction="none")
+        assert bool(((again.double() - want).abs() <= 2.0 ** -22 * 20 + 2.0 ** -22).all())
 
 
 def test_ignored_rows_hold_anything():
