@@ -50,6 +50,7 @@ struct VocabArgs {
   VocabFactor factor;
   VocabExact exact;
   const int* only;                  // null, or a word without which there is nothing to do
+  int early;                        // the kernel in front is nothing to this one: it is waited for at the end
   __nv_bfloat16* dz;
   int ld, first;                    // of dz; first column of the vocabulary
   uint32_t* err;
@@ -94,19 +95,29 @@ __device__ __forceinline__ Tile tileOf(const Product& p, int item) {
 }
 
 // A row's list from the first entry at or behind a column on.
+// A row's list from the first entry at or behind a column on.  The entry behind the present one is on its way too: a step does not wait
+// for memory (without it 32 entries a row cost 60 us of the 640 that dz of 8192 x 50257 x 1024 takes).
 struct List {
   const int* tokens;
-  int k, pos, next;
-  __device__ __forceinline__ void seek(const VocabRows& r, int row, int token, int col) {
-    pos = 0; k = 1; tokens = nullptr;
-    next = token >= col ? token : VOCAB_NO_TOKEN;
-    if (r.targets) return;
-    k = r.k; tokens = r.tokens + (size_t)row * k;
-    int hi = k;
-    while (pos < hi) { const int mid = (pos + hi) >> 1; if (tokens[mid] < col) pos = mid + 1; else hi = mid; }
-    next = pos < k ? tokens[pos] : VOCAB_NO_TOKEN;
+  const float* weights;
+  int k, behind, next, next2;
+  float q, q2;
+  __device__ __forceinline__ void load(int at, int& token, float& weight) {
+    token = at < k ? tokens[at] : VOCAB_NO_TOKEN;
+    weight = at < k ? weights[at] : 0.f;
   }
-  __device__ __forceinline__ void step() { ++pos; next = pos < k ? tokens[pos] : VOCAB_NO_TOKEN; }
+  __device__ __forceinline__ void none() { tokens = nullptr; weights = nullptr; k = behind = 0; next = next2 = VOCAB_NO_TOKEN; q = q2 = 1.f; }
+  __device__ __forceinline__ void seek(const VocabRows& r, int row, int token, int col) {
+    none();
+    if (r.targets) { if (token >= col) next = token; return; }
+    k = r.k; tokens = r.tokens + (size_t)row * k; weights = r.weights + (size_t)row * k;
+    int lo = 0, hi = k;
+    while (lo < hi) { const int mid = (lo + hi) >> 1; if (tokens[mid] < col) lo = mid + 1; else hi = mid; }
+    load(lo, next, q);
+    load(lo + 1, next2, q2);
+    behind = lo + 2;
+  }
+  __device__ __forceinline__ void step() { next = next2; q = q2; load(behind++, next2, q2); }
 };
 
 template <int MODE>
@@ -141,7 +152,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
   cluster_sync_all();                                // the partner's barriers exist before anything arrives on them
   tc_fence_after();
   const uint32_t tmemBase = *tmemBaseSlot;
-  grid_dependency_wait();
+  if (!g.early) grid_dependency_wait();
   grid_launch_dependents();
   if ((MODE == VOCAB_STATS || MODE == VOCAB_POWERS) && g.only && *g.only == 0) count = 0;
 
@@ -239,7 +250,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
 
       if (MODE != VOCAB_PRODUCTS) {
         List list;
-        list.pos = list.k = 0; list.next = VOCAB_NO_TOKEN; list.tokens = nullptr;
+        list.none();
         const float scale = g.rows.scale;
         float lse = 0.f, coef = 0.f;
         if (here) {                                    // on its way while the accumulator is computed
@@ -324,9 +335,8 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
             while (list.next < g.first + c + 32) {
               if (list.next >= g.first + c) {
                 const int at = list.next - g.first - c;
-                const float q = g.rows.targets ? 1.f : g.rows.weights[(size_t)row * g.rows.k + list.pos];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) if (e == at) r[e] = __float_as_uint(__uint_as_float(r[e]) - q);
+                for (int e = 0; e < 32; ++e) if (e == at) r[e] = __float_as_uint(__uint_as_float(r[e]) - list.q);
               }
               list.step();
             }
@@ -414,6 +424,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
     }
   }
 
+  if (g.early) grid_dependency_wait();               // what comes behind this kernel comes behind the one in front too
   // ---------------------------------------------------------------- leave: nothing of the pair may still use my shared or tensor memory
   tc_fence_before();
   __syncthreads();
@@ -463,11 +474,11 @@ ncclResult_t logits(CUtensorMap* a, CUtensorMap* b, VocabArgs* g, const void* x,
 
 }  // namespace
 
-ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, const int* only, cudaStream_t stream) {
+ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, const int* only, bool early, cudaStream_t stream) {
   CUtensorMap a, b;
   VocabArgs g;
   DFCHECK(logits(&a, &b, &g, x, w, n, v, d, rows));
-  g.parts = parts; g.only = only;
+  g.parts = parts; g.only = only; g.early = early;
   return launchVocab<VOCAB_STATS>(a, b, a, b, g, stream);
 }
 
@@ -480,11 +491,12 @@ ncclResult_t vocabPowers(const void* x, const void* w, int n, int v, int d, cons
   return launchVocab<VOCAB_POWERS>(a, b, a, b, g, stream);
 }
 
-ncclResult_t vocabGrad(const void* x, const void* w, int n, int v, int first, int d, const VocabRows& rows, const VocabGrad& grad, void* dz, cudaStream_t stream) {
+ncclResult_t vocabGrad(const void* x, const void* w, int n, int v, int first, int d, const VocabRows& rows, const VocabGrad& grad, void* dz, bool early,
+                       cudaStream_t stream) {
   CUtensorMap a, b;
   VocabArgs g;
   DFCHECK(logits(&a, &b, &g, x, w, n, v, d, rows));
-  g.grad = grad; g.dz = (__nv_bfloat16*)dz; g.ld = (v + 63) / 64 * 64; g.first = first;
+  g.grad = grad; g.early = early; g.dz = (__nv_bfloat16*)dz; g.ld = (v + 63) / 64 * 64; g.first = first;
   return launchVocab<VOCAB_GRAD>(a, b, a, b, g, stream);
 }
 

@@ -43,7 +43,9 @@ inline int vocabParts(int v) { return (v + VOCAB_TILE - 1) / VOCAB_TILE * VOCAB_
 // entries of its list: {largest z scale, sum of 2^(z scale - that)} -> parts [stretch][n].  (The tensor cores cut off what does not fit an
 // accumulator, step by step: a logit of 20 from 1024 products of one sign is 2.5e-5 too small, one of 4096 products 9e-5.  The logits that stand
 // out, and that a loss is the difference to, are computed apart.)  `only`, where given: nothing happens unless it holds something other than 0.
-ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, const int* only, cudaStream_t stream);
+// `early`: the launch in front of this one writes nothing that this one reads or writes, and lets it start when everything further in front
+// has ended; the two run side by side.
+ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, const int* only, bool early, cudaStream_t stream);
 
 // powers = 2^(z scale - base) of every row with a target, 0 elsewhere: bf16, [n][ld], ld = v rounded up to 64 (zeros behind v).  Of each stretch
 // of a row's columns, without its target: {largest exponent, sum of the powers in fp32} -> parts [stretch][n].
@@ -64,7 +66,8 @@ struct VocabGrad {
   const float* gout;            // g [n], or null: 1
   int goutStride;
 };
-ncclResult_t vocabGrad(const void* x, const void* w, int n, int v, int first, int d, const VocabRows& rows, const VocabGrad& grad, void* dz, cudaStream_t stream);
+ncclResult_t vocabGrad(const void* x, const void* w, int n, int v, int first, int d, const VocabRows& rows, const VocabGrad& grad, void* dz, bool early,
+                       cudaStream_t stream);
 
 #if defined(__CUDACC__)
 __device__ __forceinline__ float vocabFactor(const VocabFactor& f) {

@@ -112,6 +112,7 @@ __device__ void reduceLoss(const float* loss, const VocabRows& rows, int n, int 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   double s = 0.0;
   int c = 0;
+#pragma unroll 4
   for (int i = threadIdx.x; i < n; i += 1024) { s += __ldcg(loss + i); c += rowState(rows, i) != ROW_NONE; }
 #pragma unroll
   for (int o = 16; o; o >>= 1) { s += __shfl_xor_sync(0xffffffffu, s, o); c += __shfl_xor_sync(0xffffffffu, c, o); }
@@ -136,6 +137,9 @@ struct JoinArgs {
   // their base was no good raise `again`
   float* base;
   float* share;
+  const uint4* x;               // and x times that, where `shared` is given; `packs` of 8 elements in a row
+  uint4* shared;
+  int packs;
   int* again;
   const int* only;              // nothing but the sum over all rows unless this holds something (null: always)
   // the sum over all rows, by the block of the last launch that comes last; null: none
@@ -163,15 +167,13 @@ __global__ void __launch_bounds__(1024) joinRowsKernel(const JoinArgs a) {
   if (!a.only || *a.only) {
     float2 acc = make_float2(-INFINITY, 0.f);
     if (row0 + lane < a.n) {
-      int i = warp;
-      for (; i + 96 < a.stretches; i += 128) {
-        float2 p[4];
+      for (int i = warp; i < a.stretches; i += 32 * 8) {
+        float2 p[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) p[u] = a.parts[(size_t)(i + 32 * u) * a.n + row0 + lane];
+        for (int u = 0; u < 8; ++u) p[u] = i + 32 * u < a.stretches ? a.parts[(size_t)(i + 32 * u) * a.n + row0 + lane] : make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) acc = join(acc, p[u]);
+        for (int u = 0; u < 8; ++u) acc = join(acc, p[u]);
       }
-      for (; i < a.stretches; i += 32) acc = join(acc, a.parts[(size_t)i * a.n + row0 + lane]);
     }
     part[warp][lane] = acc;
     __syncthreads();
@@ -181,12 +183,13 @@ __global__ void __launch_bounds__(1024) joinRowsKernel(const JoinArgs a) {
 #pragma unroll
       for (int o = 16; o; o >>= 1) acc = join(acc, make_float2(__shfl_xor_sync(0xffffffffu, acc.x, o), __shfl_xor_sync(0xffffffffu, acc.y, o)));
       const int st = rowState(a.rows, row);
-      float l, sum = 0.f;
+      float l, sum = 0.f, share = st == ROW_BAD ? __int_as_float(0x7fffffff) : 1.f;
       if (POWERS) {
         l = a.base[row] + log2f(1.f + acc.y);           // the target's own power is 1
         sum = log1pf(acc.y);
+        if (st == ROW_LIST) share = 1.f / (1.f + acc.y);
         if (lane == 0) {
-          a.share[row] = st == ROW_LIST ? 1.f / (1.f + acc.y) : st == ROW_NONE ? 0.f : __int_as_float(0x7fffffff);
+          a.share[row] = st == ROW_NONE ? 0.f : share;
           if (st == ROW_LIST && !(acc.x <= MOST_POWER && acc.y < INFINITY && fabsf(a.base[row]) < INFINITY)) *a.again = 1;
         }
       } else {
@@ -213,6 +216,17 @@ __global__ void __launch_bounds__(1024) joinRowsKernel(const JoinArgs a) {
         sum = warpSum(sum);
         if (a.base && lane == 0) { a.base[row] = l; if (st == ROW_LIST) a.share[row] = 1.f; }
       }
+      // x times the row's share, rounded to bf16: the right operand of the powers' product.  A row without a target is zeros whatever it holds.
+      if (a.shared)
+        for (int i = lane; i < a.packs; i += 32) {
+          uint4 o = make_uint4(0u, 0u, 0u, 0u);
+          if (st != ROW_NONE) {
+            const uint4 p = a.x[(size_t)row * a.packs + i];
+            o = make_uint4(tc::pack_bf16x2(bf16Lo(p.x) * share, bf16Hi(p.x) * share), tc::pack_bf16x2(bf16Lo(p.y) * share, bf16Hi(p.y) * share),
+                           tc::pack_bf16x2(bf16Lo(p.z) * share, bf16Hi(p.z) * share), tc::pack_bf16x2(bf16Lo(p.w) * share, bf16Hi(p.w) * share));
+          }
+          a.shared[(size_t)row * a.packs + i] = o;
+        }
       if (lane == 0) {
         a.lse[row] = l;
         a.loss[row] = st == ROW_LIST ? sum * a.t2 : st == ROW_NONE ? 0.f : __int_as_float(0x7fffffff);
@@ -303,25 +317,6 @@ ncclResult_t pickLogits(const PickArgs& a, cudaStream_t stream) {
   const long long items = (long long)a.n * ((a.rows.k + 3) / 4);
   CUDACHECK(launchBehind(pickLogitsKernel, dim3((unsigned)std::min<long long>((items + 7) / 8, 148 * 8)), 256, stream, a));
   return ncclSuccess;
-}
-
-// x scale, a row's share each, rounded to bf16: the right operand of the powers' product.  Rows without a target are zeros whatever they hold.
-__global__ void __launch_bounds__(256) shareRowsKernel(const uint4* x, const VocabRows rows, const float* share, int n, int packs, uint4* out) {
-  tc::grid_dependency_wait();
-  tc::grid_launch_dependents();
-  for (int row = blockIdx.x; row < n; row += gridDim.x) {
-    const bool keep = rowState(rows, row) != ROW_NONE;
-    const float f = share[row];
-    for (int i = threadIdx.x; i < packs; i += 256) {
-      uint4 o = make_uint4(0u, 0u, 0u, 0u);
-      if (keep) {
-        const uint4 p = x[(size_t)row * packs + i];
-        o = make_uint4(tc::pack_bf16x2(bf16Lo(p.x) * f, bf16Hi(p.x) * f), tc::pack_bf16x2(bf16Lo(p.y) * f, bf16Hi(p.y) * f),
-                       tc::pack_bf16x2(bf16Lo(p.z) * f, bf16Hi(p.z) * f), tc::pack_bf16x2(bf16Lo(p.w) * f, bf16Hi(p.w) * f));
-      }
-      out[(size_t)row * packs + i] = o;
-    }
-  }
 }
 
 // Two results times one number on the device, in place; nothing is read or written where it is 1.
@@ -478,7 +473,8 @@ DF_API ncclResult_t dfcclLinearLossForward(const void* x, const void* w, int n, 
     j.picked = picked + (size_t)r * k;
     j.rows = rowsOf(targets, wide, v, ignore, tokens, weights, state, k, temperature, r);
     j.lse = (float*)lse + r; j.loss = losses + r;
-    DFCHECK(vocabStats((const __nv_bfloat16*)x + (size_t)r * d, w, j.n, v, d, j.rows, (float2*)j.parts, nullptr, stream));
+    // (the first beside pickLogitsKernel)
+    DFCHECK(vocabStats((const __nv_bfloat16*)x + (size_t)r * d, w, j.n, v, d, j.rows, (float2*)j.parts, nullptr, r == 0, stream));
     CUDACHECK(launchBehind(joinRowsKernel<false>, (j.n + 31) / 32, 1024, stream, j));
   }
   return ncclSuccess;
@@ -509,7 +505,7 @@ DF_API ncclResult_t dfcclLinearLossBackward(const void* x, const void* w, int n,
     const int cols = std::min(p.cols, v - c);
     const __nv_bfloat16* wc = (const __nv_bfloat16*)w + (size_t)c * d;
     __nv_bfloat16* dwc = dw ? (__nv_bfloat16*)dw + (size_t)c * d : nullptr;
-    DFCHECK(vocabGrad(x, wc, n, cols, c, d, rows, grad, dz, stream));
+    DFCHECK(vocabGrad(x, wc, n, cols, c, d, rows, grad, dz, dw && c == 0, stream));      // (beside keepRowsKernel)
     DFCHECK(vocabProducts(dz, kept, wc, n, cols, d, p.cut, factor, nullptr, VocabResult{p.sumX ? nullptr : dx, partX, c != 0}, VocabResult{p.sumW ? nullptr : dwc, partW, false}, stream));
     if (p.sumW) DFCHECK(joinSlices(partW, p.slicesW, cols, d, factor, nullptr, 0, dwc, stream));
   }
@@ -590,14 +586,14 @@ DF_API ncclResult_t dfcclCrossEntropyWithGradients(const void* x, const void* w,
     const __nv_bfloat16* xr = (const __nv_bfloat16*)x + (size_t)r * d;
     j.rows = rowsOf(targets, wide, v, ignore, nullptr, nullptr, nullptr, 1, 1.f, r);
     j.n = m; j.lse = (float*)lse + r; j.loss = losses + r; j.base = base + r; j.share = share + r; j.picked = picked + r;
+    j.x = (const uint4*)xr; j.shared = dw ? (uint4*)(at + p.shared) : nullptr; j.packs = packs;
     DFCHECK(vocabPowers(xr, w, m, v, d, j.rows, base + r, parts, powers, nullptr, stream));
     j.again = words + 1 + i; j.only = nullptr; j.ticket = nullptr;
     CUDACHECK(launchBehind(joinRowsKernel<true>, (m + 31) / 32, 1024, stream, j));
-    DFCHECK(vocabStats(xr, w, m, v, d, j.rows, parts, j.again, stream));
+    DFCHECK(vocabStats(xr, w, m, v, d, j.rows, parts, j.again, false, stream));
     j.only = j.again; j.ticket = words;
     CUDACHECK(launchBehind(joinRowsKernel<false>, (m + 31) / 32, 1024, stream, j));
     DFCHECK(vocabPowers(xr, w, m, v, d, j.rows, base + r, parts, powers, j.again, stream));
-    if (dw) CUDACHECK(launchBehind(shareRowsKernel, std::min(m, 148 * 8), 256, stream, (const uint4*)xr, j.rows, (const float*)share + r, m, packs, (uint4*)(at + p.shared)));
     const VocabExact exact{j.rows, share + r, (const __nv_bfloat16*)w, (const float*)(at + p.sums), where};
     __nv_bfloat16* dxr = dx ? (__nv_bfloat16*)dx + (size_t)r * d : nullptr;
     // (a shorter last piece has fewer slices of dw: it adds to the first of them)
