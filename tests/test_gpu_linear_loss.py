@@ -179,6 +179,11 @@ def test_gradients_with_the_loss(n, v, d, limit, monkeypatch):
             check_gradients((a.grad, b.grad), x, w, dz, 3 * each, 1.0)
             a.grad = b.grad = None
             other = module.linear_cross_entropy(a, b, targets, reduction=reduction)
+            if want_x and want_w:                        # one after the other: the second is computed again
+                pair = [torch.autograd.grad(other, [leaf], retain_graph=True)[0] for leaf in (a, b)]
+                assert torch.equal(pair[0], first[0])
+                check_gradients((None, pair[1]), x, w, dz, each, 1.0, more=two)
+                other = module.linear_cross_entropy(a, b, targets, reduction=reduction)
             (other * 0.3).backward()
             for g, f in zip((a.grad, b.grad), first):    # one rounding of 0.3 times the same values
                 if g is not None:
@@ -353,10 +358,13 @@ def test_gradient_against_differences():
     assert abs(slope - size) <= 2.0 ** -8 * size                      # the gradients' error in the 2-norm, along themselves
 
 
-def test_other_stream_and_graphs():
+@pytest.mark.parametrize("one_go", [False, True])
+def test_other_stream_and_graphs(one_go, monkeypatch):
     """On a stream of its own; forward and backward captured and replayed for other data, two graphs in turns."""
+    from dfccl_b200.ops import loss as module
     from dfccl_b200.ops.gemm import check_kernels
     from dfccl_b200.ops.loss import linear_cross_entropy, linear_distillation
+    monkeypatch.setattr(module, "ONE_GO_FROM", 0 if one_go else 1 << 60)
     x, w, gen = problem(300, 3001, 128, 41)
     w.requires_grad_(True)
     xs = [torch.randn(300, 128, generator=gen, device="cuda").to(torch.bfloat16) for _ in range(3)]
@@ -389,6 +397,55 @@ def test_other_stream_and_graphs():
         for k, (_, _, _, out) in enumerate(graphs):
             assert all(torch.equal(p, q) for p, q in zip(out, want[(turn + k) % 3]))
     assert check_kernels()
+
+
+def test_many_rows_and_wide_ones():
+    """More rows than the statistics take at a time, a width of many stages, row numbers beyond 16 bits."""
+    from dfccl_b200.ops.gemm import check_kernels
+    from dfccl_b200.ops.loss import linear_cross_entropy, linear_distillation
+    for n, v, d in ((40001, 300, 16), (16385, 40, 8), (70000, 9, 24), (130, 700, 8192)):
+        x, w, gen = problem(n, v, d, n + v + d)
+        t = torch.randint(0, v, (n,), generator=gen, device="cuda")
+        t[n // 3] = -100
+        keep = (t >= 0).double()[:, None]
+        loss, dz = reference(x, w, t.clamp(min=0)[:, None], keep, 1.0)
+        x.requires_grad_(True), w.requires_grad_(True)
+        value = linear_cross_entropy(x, w, t, reduction="sum")
+        err = 2 * logit_error(x.detach(), w.detach()).amax(dim=1).sum().item() + 2 * LN * (n + loss.sum().item())
+        assert abs(value.item() - loss.sum().item()) <= err
+        check_gradients(torch.autograd.grad(value, [x, w]), x.detach(), w.detach(), dz, torch.ones(n, device="cuda").double(), 1.0)
+        rows = linear_distillation(x, w, torch.zeros(n, 1, device="cuda"), t.clamp(min=-1)[:, None], reduction="none")
+        check_loss(rows.detach(), loss, x.detach(), w.detach(), 1.0)
+    assert check_kernels()
+
+
+def test_calls_on_two_streams_at_once():
+    """Two losses and an embedding on streams of their own, in flight together, each as by itself."""
+    from dfccl_b200.ops.embedding import embedding
+    from dfccl_b200.ops.loss import linear_cross_entropy
+    data = []
+    for k in range(2):
+        x, w, gen = problem(600 + 100 * k, 4000, 256, 50 + k)
+        data.append((x.requires_grad_(True), w.requires_grad_(True), torch.randint(0, 4000, (x.shape[0],), generator=gen, device="cuda")))
+
+    def step(k):
+        x, w, t = data[k]
+        h = embedding(t, w)
+        loss = linear_cross_entropy(x, w, t)
+        return (h.detach(), loss.detach()) + torch.autograd.grad([loss, h], [x, w], [torch.ones((), device="cuda"), torch.ones_like(h)])
+
+    want = [step(k) for k in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(5):
+        got = []
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append(step(k))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
 def test_a_models_two_ends():
