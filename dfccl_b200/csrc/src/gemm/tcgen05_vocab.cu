@@ -25,15 +25,19 @@ using namespace tc;
 constexpr int T = VOCAB_TILE, HALF = 128, BK = 64, UMMA_K = 16, STAGES = 6;
 constexpr int A_BYTES = HALF * BK * 2, STAGE_BYTES = 2 * A_BYTES;                 // per CTA: 128 rows of A, 128 of B
 constexpr int SMEM_BYTES = 227 * 1024;                                            // all of it: tensor memory for one CTA at a time (tcgen05_gemm_pair.cu)
-constexpr int EPI_WARPS = 4 * VOCAB_PARTS, THREADS = 64 + 32 * EPI_WARPS;
-constexpr uint64_t WAIT_NS = 4000000000ull;                                       // nothing here waits on another GPU
-static_assert(STAGES * STAGE_BYTES + 1024 + 256 <= SMEM_BYTES, "stages");
-
 enum VocabMode { VOCAB_STATS, VOCAB_GRAD, VOCAB_POWERS, VOCAB_PRODUCTS };
+// Epilogue warps that share 32 rows of a tile: four where every element is a power of two, two where it is only rounded and stored.
+__host__ __device__ constexpr int partsOf(int mode) { return mode == VOCAB_PRODUCTS ? 2 : 4; }
+__host__ __device__ constexpr int epiWarps(int mode) { return 4 * partsOf(mode); }
+__host__ __device__ constexpr int threadsOf(int mode) { return 64 + 32 * epiWarps(mode); }
+constexpr int JOIN_BYTES = 2 * 3 * HALF * 8;                                      // what the parts of a tile's rows leave for the first of them, two tiles' worth
+constexpr uint64_t WAIT_NS = 4000000000ull;                                       // nothing here waits on another GPU
+static_assert(STAGES * STAGE_BYTES + JOIN_BYTES + 1024 + 512 <= SMEM_BYTES, "stages");
 
 // One product: result [M, N], `kBlocks` blocks of 64 of the contraction cut into slices of `perSlice`.
 struct Product {
   int M, N, mTiles, nTiles, kBlocks, slices, perSlice, items, groupM;
+  int tn, stageBytes;               // columns of a tile (a multiple of 32, 128 to 256); bytes that a stage of a CTA is loaded with
   int aMn, bMn, bLoose;             // operand stored with the contraction index slow; loose: its blocks of 64 columns are loaded one by one
   __nv_bfloat16* out;               // direct results, ld N
   float* part;                      // or slices [slice][M][N]
@@ -121,16 +125,19 @@ struct List {
 };
 
 template <int MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threadsOf(MODE), 1)
 dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtensorMap mapB0, const __grid_constant__ CUtensorMap mapA1,
                  const __grid_constant__ CUtensorMap mapB1, const __grid_constant__ VocabArgs g) {
   extern __shared__ uint8_t smemRaw[];
+  constexpr int PARTS = partsOf(MODE), EPI_WARPS = epiWarps(MODE);
   uint8_t* smem = (uint8_t*)(((uintptr_t)smemRaw + 1023) & ~(uintptr_t)1023);       // the same offset in both CTAs
-  uint64_t* fullBar = (uint64_t*)(smem + STAGES * STAGE_BYTES);      // used in the leader only
+  float2* joinBuf = (float2*)(smem + STAGES * STAGE_BYTES);          // [2 tiles][3 parts][HALF rows]
+  uint64_t* fullBar = (uint64_t*)(smem + STAGES * STAGE_BYTES + JOIN_BYTES);      // used in the leader only
   uint64_t* emptyBar = fullBar + STAGES;                             // in both CTAs (commit to both)
   uint64_t* accFull = emptyBar + STAGES;                             // [2] in both CTAs
   uint64_t* accEmpty = accFull + 2;                                  // [2] used in the leader only
-  uint32_t* tmemBaseSlot = (uint32_t*)(accEmpty + 2);
+  uint64_t* joinBar = accEmpty + 2;                                  // [4 quarters][2 tiles] the other parts of 32 rows are in place
+  uint32_t* tmemBaseSlot = (uint32_t*)(joinBar + 8);
   volatile uint32_t* giveUp = tmemBaseSlot + 1;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -141,6 +148,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&fullBar[s], 1); mbar_init(&emptyBar[s], 1); }
     for (int a = 0; a < 2; ++a) { mbar_init(&accFull[a], 1); mbar_init(&accEmpty[a], 2 * EPI_WARPS); }
+    for (int a = 0; a < 8; ++a) mbar_init(&joinBar[a], PARTS - 1);
     *giveUp = 0;
     mbar_fence_init();
     tma_prefetch_desc(&mapA0);
@@ -170,23 +178,21 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
         const CUtensorMap* ma = which ? &mapA1 : &mapA0;
         const CUtensorMap* mb = which ? &mapB1 : &mapB0;
         const Tile t = tileOf(p, item);
-        const int rowA = t.mt * T + (int)cr * HALF, rowB = t.nt * T + (int)cr * HALF;
+        const int bHalf = MODE == VOCAB_PRODUCTS ? p.tn / 2 : HALF;
+        const int rowA = t.mt * T + (int)cr * HALF, rowB = t.nt * 2 * bHalf + (int)cr * bHalf;
         for (int k = t.k0; k < t.k1; ++k) {
           if (!mbar_wait(&emptyBar[stage], phase ^ 1, giveUp, WAIT_NS)) { ok = false; break; }
-          if (cr == 0) mbar_expect_tx(&fullBar[stage], 2 * STAGE_BYTES);      // my bytes and the partner's
+          if (cr == 0) mbar_expect_tx(&fullBar[stage], 2 * (MODE == VOCAB_PRODUCTS ? p.stageBytes : STAGE_BYTES));       // my bytes and the partner's
           uint8_t* sa = smem + stage * STAGE_BYTES;
           uint8_t* sb = sa + A_BYTES;
           const uint32_t bar = bar0 + stage * 8;
-          // K-major: a box of 64 of the contraction x 128 rows.  MN-major: two blocks of 64 columns x 64 of the contraction,
-          // in one load where the matrix is cut into whole blocks.
+          // K-major: a box of 64 of the contraction x 128 rows.  MN-major: blocks of 64 columns x 64 of the contraction, in one load
+          // where the matrix and the tile are cut into whole blocks, else block by block from any multiple of 16 columns.
           if (MODE == VOCAB_PRODUCTS && p.aMn) tma_load_3d_pair(sa, ma, k * BK, rowA / 64, bar);
           else tma_load_2d_pair(sa, ma, k * BK, rowA, bar);
           if (MODE != VOCAB_PRODUCTS) tma_load_2d_pair(sb, mb, k * BK, rowB, bar);
           else if (!p.bLoose) tma_load_3d_pair(sb, mb, k * BK, rowB / 64, bar);
-          else {
-            tma_load_2d_pair(sb, mb, rowB, k * BK, bar);
-            tma_load_2d_pair(sb + 64 * BK * 2, mb, rowB + 64, k * BK, bar);
-          }
+          else for (int i = 0; i * 64 < bHalf; ++i) tma_load_2d_pair(sb + i * 64 * BK * 2, mb, rowB + 64 * i, k * BK, bar);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
@@ -211,7 +217,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
         const Product& p = g.p[which];
         const Tile t = tileOf(p, item);
         const bool aMn = MODE == VOCAB_PRODUCTS && p.aMn, bMn = MODE == VOCAB_PRODUCTS && p.bMn;
-        const uint32_t idesc = umma_idesc_bf16(T, T, aMn, bMn);
+        const uint32_t idesc = umma_idesc_bf16(T, MODE == VOCAB_PRODUCTS ? p.tn : T, aMn, bMn);
         // per instruction (16 of the contraction): 32 bytes along a K-major row, two groups of 8 rows of an MN-major block
         const uint32_t stepA = aMn ? 128u : 2u, stepB = bMn ? 128u : 2u;
         const int ab = j & 1;
@@ -243,7 +249,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
       const Product& p = g.p[which];
       const Tile t = tileOf(p, item);
       const int ab = j & 1;
-      const int row0 = t.mt * T + (int)cr * HALF + quarter * 32, row = row0 + lane, col0 = t.nt * T;
+      const int row0 = t.mt * T + (int)cr * HALF + quarter * 32, row = row0 + lane, tn = MODE == VOCAB_PRODUCTS ? p.tn : T, col0 = t.nt * tn;
       const bool mine = row0 < p.M, here = row < p.M;
       const uint32_t acc = tmemBase + ((uint32_t)(quarter * 32) << 16) + ab * T;
       uint32_t r[32];
@@ -272,7 +278,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
         float top = -INFINITY, sum = 0.f;
         const int cols = MODE == VOCAB_STATS ? p.N : g.ld, steps = (min(T, cols - col0) + 31) / 32;
 #pragma unroll 1
-        for (int i = part; i < steps; i += VOCAB_PARTS) {
+        for (int i = part; i < steps; i += PARTS) {
           if (!mine) break;
           const int c = col0 + i * 32;
           __syncwarp();
@@ -365,18 +371,39 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
             }
           }
         }
-        if (MODE != VOCAB_GRAD && here) g.parts[(size_t)(t.nt * VOCAB_PARTS + part) * p.M + row] = make_float2(top, sum);
+        if (MODE != VOCAB_GRAD) {
+          // The parts of a row meet in the first one's warp.  (Its arrival on accEmpty, behind this, keeps the others from the tile after the next.)
+          uint64_t* bar = joinBar + quarter * 2 + ab;
+          if (part) {
+            joinBuf[(ab * 3 + part - 1) * HALF + quarter * 32 + lane] = make_float2(top, sum);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+          } else {
+            if (!mbar_wait(bar, (j >> 1) & 1, giveUp, WAIT_NS)) break;
+            float2 q[PARTS];
+            q[0] = make_float2(top, sum);
+#pragma unroll
+            for (int k = 1; k < PARTS; ++k) q[k] = joinBuf[(ab * 3 + k - 1) * HALF + quarter * 32 + lane];
+#pragma unroll
+            for (int k = 1; k < PARTS; ++k) top = fmaxf(top, q[k].x);
+            sum = 0.f;
+            const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k) sum += MODE == VOCAB_POWERS ? q[k].y : q[k].y * exp2Approx(q[k].x - base);
+            if (here) g.parts[(size_t)t.nt * p.M + row] = make_float2(top, sum);
+          }
+        }
       } else {
         if (!mbar_wait(&accFull[ab], (j >> 1) & 1, giveUp, WAIT_NS)) break;
         tc_fence_after();
-        const int steps = (min(T, p.N - col0) + 31) / 32;
+        const int steps = (min(tn, p.N - col0) + 31) / 32;
         int state = ROW_NONE, token = 0;
         float scale = 0.f;
         const float* sums = nullptr;
         if (here && p.exact == 1) { state = rowState(g.exact.rows, row, token); scale = g.exact.scale[row]; }
         if (here && p.exact == 2) { const int at = g.exact.where[row]; if (at >= 0) sums = g.exact.sums + (size_t)at * p.N; }
 #pragma unroll 1
-        for (int i = part; i < steps; i += VOCAB_PARTS) {
+        for (int i = part; i < steps; i += PARTS) {
           if (!mine) break;
           const int c = col0 + i * 32, packs = min(4, (p.N - c) / 8);
           __syncwarp();
@@ -440,7 +467,7 @@ ncclResult_t launchVocab(const CUtensorMap& a0, const CUtensorMap& b0, const CUt
   DFCHECK(gemmErrorWords(&g.err, &g.errHost));
   cudaLaunchConfig_t cfg = {};
   const int pairs = std::min(g.p[0].items + g.p[1].items, gemmPairResident());
-  cfg.gridDim = dim3(2 * pairs); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM_BYTES; cfg.stream = stream;
+  cfg.gridDim = dim3(2 * pairs); cfg.blockDim = dim3(threadsOf(MODE)); cfg.dynamicSmemBytes = SMEM_BYTES; cfg.stream = stream;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization; at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at; cfg.numAttrs = 1;
@@ -451,9 +478,10 @@ ncclResult_t launchVocab(const CUtensorMap& a0, const CUtensorMap& b0, const CUt
   return ncclSuccess;
 }
 
-Product productOf(int M, int N, int K, int per) {
+Product productOf(int M, int N, int K, int per, int tn) {
   Product p = {};
-  p.M = M; p.N = N; p.mTiles = (M + T - 1) / T; p.nTiles = (N + T - 1) / T;
+  p.M = M; p.N = N; p.mTiles = (M + T - 1) / T; p.nTiles = (N + tn - 1) / tn;
+  p.tn = tn; p.stageBytes = STAGE_BYTES;
   p.kBlocks = (K + BK - 1) / BK;
   p.perSlice = per;
   p.slices = vocabSlices(K, per);
@@ -467,7 +495,7 @@ ncclResult_t logits(CUtensorMap* a, CUtensorMap* b, VocabArgs* g, const void* x,
   *g = VocabArgs{};
   DFCHECK(gemmEncodeMap(a, x, (uint64_t)n, (uint64_t)d, HALF));
   DFCHECK(gemmEncodeMap(b, w, (uint64_t)v, (uint64_t)d, HALF));
-  g->p[0] = productOf(n, v, d, (d + BK - 1) / BK);
+  g->p[0] = productOf(n, v, d, (d + BK - 1) / BK, T);
   g->rows = rows;
   return ncclSuccess;
 }
@@ -500,10 +528,16 @@ ncclResult_t vocabGrad(const void* x, const void* w, int n, int v, int first, in
   return launchVocab<VOCAB_GRAD>(a, b, a, b, g, stream);
 }
 
+// Columns of a tile of dx and dw: as few tiles as 256 columns make them, no wider than they need be (d = 640: 3 x 224; at 4096 x 50257 TODO).
+static int productWidth(int d) {
+  const int tiles = (d + T - 1) / T;
+  return std::max(128, ((d + tiles - 1) / tiles + 31) / 32 * 32);
+}
+
 // A product is cut into slices of its contraction where its tiles alone would keep pairs waiting: until the longest item is no more
 // than a pair's share of all the work.
 VocabPlan vocabProductPlan(int n, int v, int d, bool wantX, bool wantW, int pairs) {
-  const int64_t tn = (n + T - 1) / T, tv = (v + T - 1) / T, td = (d + T - 1) / T, kn = (n + BK - 1) / BK, kv = (v + BK - 1) / BK;
+  const int64_t tn = (n + T - 1) / T, tv = (v + T - 1) / T, td = (d + productWidth(d) - 1) / productWidth(d), kn = (n + BK - 1) / BK, kv = (v + BK - 1) / BK;
   const int64_t all = (wantX ? tn * td * kv : 0) + (wantW ? tv * td * kn : 0), share = std::max<int64_t>(1, all / pairs);
   // A slice costs its sums a way to memory and back: none is cut below 16 blocks.
   auto cut = [&](int64_t tiles, int64_t k) -> int {
@@ -522,12 +556,15 @@ ncclResult_t vocabProducts(const void* dz, const void* x, const void* w, int n, 
   g.factor = factor;
   if (exact) g.exact = *exact;
   int k = 0;
+  const int tn = productWidth(d);
+  const bool loose = d % 64 != 0 || tn % 128 != 0;
   auto narrow = [&](CUtensorMap* m, const void* base, int rows) {      // [rows of the contraction][d columns]
-    return d % 64 ? gemmEncodeMap(m, base, (uint64_t)rows, (uint64_t)d, BK) : gemmEncodeMap3(m, base, (uint64_t)d, (uint64_t)rows, 1, HALF, BK);
+    return loose ? gemmEncodeMap(m, base, (uint64_t)rows, (uint64_t)d, BK) : gemmEncodeMap3(m, base, (uint64_t)d, (uint64_t)rows, 1, tn / 2, BK);
   };
   auto result = [&](const VocabResult& r, int which) {
     Product& p = g.p[k++];
-    p.bMn = 1; p.bLoose = d % 64 != 0;
+    p.bMn = 1; p.bLoose = loose;
+    p.stageBytes = A_BYTES + (tn / 2 + 63) / 64 * 64 * BK * 2;
     p.out = (__nv_bfloat16*)r.out; p.part = r.part; p.add = r.add;
     p.exact = exact && r.out ? which : 0;
     p.wide = d % 16 == 0 && ((uintptr_t)r.out & 31) == 0;
@@ -535,13 +572,13 @@ ncclResult_t vocabProducts(const void* dz, const void* x, const void* w, int n, 
   if (dx.out || dx.part) {
     DFCHECK(gemmEncodeMap(&a[k], dz, (uint64_t)n, (uint64_t)ld, HALF));
     DFCHECK(narrow(&b[k], w, v));
-    g.p[k] = productOf(n, d, v, plan.perX);
+    g.p[k] = productOf(n, d, v, plan.perX, tn);
     result(dx, 1);
   }
   if (dw.out || dw.part) {
     DFCHECK(gemmEncodeMap3(&a[k], dz, (uint64_t)ld, (uint64_t)n, 1, HALF, BK));
     DFCHECK(narrow(&b[k], x, n));
-    g.p[k] = productOf(v, d, n, plan.perW);
+    g.p[k] = productOf(v, d, n, plan.perW, tn);
     g.p[k].aMn = 1;
     result(dw, 2);
   }

@@ -9,7 +9,6 @@
 namespace dfccl {
 
 constexpr int VOCAB_TILE = 256;              // rows and columns of a tile
-constexpr int VOCAB_PARTS = 2;               // epilogue warps that share 32 rows of a tile: each leaves a maximum and a sum of its own
 constexpr int VOCAB_NO_TOKEN = 0x7fffffff;   // behind the last entry of a row's list
 
 // What the rows of logits are compared with: a target each (`targets`), or a list of vocabulary entries in ascending order (VOCAB_NO_TOKEN
@@ -37,7 +36,7 @@ __device__ __forceinline__ int rowState(const VocabRows& r, int row, int& token)
 __device__ __forceinline__ int rowState(const VocabRows& r, int row) { int token; return rowState(r, row, token); }
 #endif
 
-inline int vocabParts(int v) { return (v + VOCAB_TILE - 1) / VOCAB_TILE * VOCAB_PARTS; }
+inline int vocabParts(int v) { return (v + VOCAB_TILE - 1) / VOCAB_TILE; }
 
 // z = x [n, d] w[v, d]^T, tile by tile and never stored.  Of every row, for each of the vocabParts(v) stretches of its columns and without the
 // entries of its list: {largest z scale, sum of 2^(z scale - that)} -> parts [stretch][n].  (The tensor cores cut off what does not fit an

@@ -3,7 +3,7 @@
 // Both are a divergence from a distribution q over a row's list of entries (one entry of weight 1: a target),
 //     loss = T^2 sum_k q_k (ln q_k - ln p_k),   p = softmax(z / T),   dz = T g (p - q),
 // so both run on the same products (gemm/tcgen05_vocab.cu); here are the passes around them.  They move n (k + 1) words and, behind the
-// forward product, 8 bytes per row and stretch of 128 columns: microseconds beside the products'.
+// forward product, 8 bytes per row and stretch of 256 columns: microseconds beside the products'.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -23,7 +23,7 @@ namespace dfccl {
 namespace {
 
 constexpr int MAX_LIST = 256;          // entries of a teacher's list
-constexpr int ROWS = 16384;            // rows of a forward product at a time: bounds its partial sums (52 MB at 50257 columns)
+constexpr int ROWS = 16384;            // rows of a forward product at a time: bounds its partial sums (26 MB at 50257 columns)
 constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
 
 template <typename... P, typename... A>
