@@ -26,11 +26,12 @@ constexpr int T = VOCAB_TILE, HALF = 128, BK = 64, UMMA_K = 16, STAGES = 6;
 constexpr int A_BYTES = HALF * BK * 2, STAGE_BYTES = 2 * A_BYTES;                 // per CTA: 128 rows of A, 128 of B
 constexpr int SMEM_BYTES = 227 * 1024;                                            // all of it: tensor memory for one CTA at a time (tcgen05_gemm_pair.cu)
 enum VocabMode { VOCAB_STATS, VOCAB_GRAD, VOCAB_POWERS, VOCAB_PRODUCTS };
-// Epilogue warps that share 32 rows of a tile: four where every element is a power of two, two where it is only rounded and stored.
-__host__ __device__ constexpr int partsOf(int mode) { return mode == VOCAB_PRODUCTS ? 2 : 4; }
-__host__ __device__ constexpr int epiWarps(int mode) { return 4 * partsOf(mode); }
-__host__ __device__ constexpr int threadsOf(int mode) { return 64 + 32 * epiWarps(mode); }
-constexpr int JOIN_BYTES = 2 * 3 * HALF * 8;                                      // what the parts of a tile's rows leave for the first of them, two tiles' worth
+// Eight epilogue warps work on a tile, two (PARTS) on 32 rows of it.  Where every element is a power of two there are two groups of eight,
+// one for each accumulator: the waits of one tile (for its rows' targets, tensor memory, powers) lie beside the other's.
+constexpr int PARTS = 2, EPI_WARPS = 4 * PARTS;
+__host__ __device__ constexpr int groupsOf(int mode) { return mode == VOCAB_PRODUCTS ? 1 : 2; }
+__host__ __device__ constexpr int threadsOf(int mode) { return 64 + 32 * EPI_WARPS * groupsOf(mode); }
+constexpr int JOIN_BYTES = 2 * HALF * 8;                                          // what one part of a tile's rows leaves for the other, of either group
 constexpr uint64_t WAIT_NS = 4000000000ull;                                       // nothing here waits on another GPU
 static_assert(STAGES * STAGE_BYTES + JOIN_BYTES + 1024 + 512 <= SMEM_BYTES, "stages");
 
@@ -129,14 +130,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threadsOf(MODE), 1)
 dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtensorMap mapB0, const __grid_constant__ CUtensorMap mapA1,
                  const __grid_constant__ CUtensorMap mapB1, const __grid_constant__ VocabArgs g) {
   extern __shared__ uint8_t smemRaw[];
-  constexpr int PARTS = partsOf(MODE), EPI_WARPS = epiWarps(MODE);
+  constexpr int GROUPS = groupsOf(MODE);
   uint8_t* smem = (uint8_t*)(((uintptr_t)smemRaw + 1023) & ~(uintptr_t)1023);       // the same offset in both CTAs
-  float2* joinBuf = (float2*)(smem + STAGES * STAGE_BYTES);          // [2 tiles][3 parts][HALF rows]
+  float2* joinBuf = (float2*)(smem + STAGES * STAGE_BYTES);          // [2 groups][HALF rows]
   uint64_t* fullBar = (uint64_t*)(smem + STAGES * STAGE_BYTES + JOIN_BYTES);      // used in the leader only
   uint64_t* emptyBar = fullBar + STAGES;                             // in both CTAs (commit to both)
   uint64_t* accFull = emptyBar + STAGES;                             // [2] in both CTAs
   uint64_t* accEmpty = accFull + 2;                                  // [2] used in the leader only
-  uint64_t* joinBar = accEmpty + 2;                                  // [4 quarters][2 tiles] the other parts of 32 rows are in place
+  uint64_t* joinBar = accEmpty + 2;                                  // [4 quarters][2 groups] the other part of 32 rows is in place
   uint32_t* tmemBaseSlot = (uint32_t*)(joinBar + 8);
   volatile uint32_t* giveUp = tmemBaseSlot + 1;
 
@@ -148,7 +149,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&fullBar[s], 1); mbar_init(&emptyBar[s], 1); }
     for (int a = 0; a < 2; ++a) { mbar_init(&accFull[a], 1); mbar_init(&accEmpty[a], 2 * EPI_WARPS); }
-    for (int a = 0; a < 8; ++a) mbar_init(&joinBar[a], PARTS - 1);
+    for (int a = 0; a < 8; ++a) mbar_init(&joinBar[a], 1);
     *giveUp = 0;
     mbar_fence_init();
     tma_prefetch_desc(&mapA0);
@@ -240,10 +241,10 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
     }
   } else {
     // ------------------------------------------------------------ epilogue: a row of my 128 per lane, 32 columns at a time
-    const int quarter = warp & 3, part = (warp - 2) >> 2;
+    const int quarter = warp & 3, part = (warp - 2) >> 2 & 1, group = (warp - 2) >> 3;
     const uint32_t accEmptyLeader0 = mapa_u32(smem_u32(&accEmpty[0]), 0), accEmptyLeader1 = mapa_u32(smem_u32(&accEmpty[1]), 0);
     const float factor = MODE == VOCAB_PRODUCTS ? vocabFactor(g.factor) : 1.f;
-    for (int j = 0; j < count; ++j) {
+    for (int j = group; j < count; j += GROUPS) {
       int item;
       const int which = MODE == VOCAB_PRODUCTS ? items.at(j, item) : (items.at(j, item), 0);
       const Product& p = g.p[which];
@@ -372,25 +373,19 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
           }
         }
         if (MODE != VOCAB_GRAD) {
-          // The parts of a row meet in the first one's warp.  (Its arrival on accEmpty, behind this, keeps the others from the tile after the next.)
+          // The parts of a row meet in the first one's warp.  (Its arrival on accEmpty, behind this, keeps the other from the group's next tile.)
           uint64_t* bar = joinBar + quarter * 2 + ab;
+          float2* at = joinBuf + ab * HALF + quarter * 32 + lane;
           if (part) {
-            joinBuf[(ab * 3 + part - 1) * HALF + quarter * 32 + lane] = make_float2(top, sum);
+            *at = make_float2(top, sum);
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
           } else {
             if (!mbar_wait(bar, (j >> 1) & 1, giveUp, WAIT_NS)) break;
-            float2 q[PARTS];
-            q[0] = make_float2(top, sum);
-#pragma unroll
-            for (int k = 1; k < PARTS; ++k) q[k] = joinBuf[(ab * 3 + k - 1) * HALF + quarter * 32 + lane];
-#pragma unroll
-            for (int k = 1; k < PARTS; ++k) top = fmaxf(top, q[k].x);
-            sum = 0.f;
-            const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-            for (int k = 0; k < PARTS; ++k) sum += MODE == VOCAB_POWERS ? q[k].y : q[k].y * exp2Approx(q[k].x - base);
-            if (here) g.parts[(size_t)t.nt * p.M + row] = make_float2(top, sum);
+            const float2 q = *at;
+            const float m = fmaxf(top, q.x), base = m == -INFINITY ? 0.f : m;
+            sum = MODE == VOCAB_POWERS ? sum + q.y : sum * exp2Approx(top - base) + q.y * exp2Approx(q.x - base);
+            if (here) g.parts[(size_t)t.nt * p.M + row] = make_float2(m, sum);
           }
         }
       } else {
