@@ -47,6 +47,7 @@ struct Product {
 };
 struct VocabArgs {
   Product p[2];                     // items of the first, then of the second (items = 0: none)
+  int kStep, stages, stride;        // of the products: blocks of 64 of the contraction in a stage (1 or 2), stages, their bytes per CTA
   int headStart;                    // rounds of the second product's items that pairs with one item less of the first take alone
   VocabRows rows;
   float2* parts;
@@ -145,6 +146,8 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
   const uint32_t cr = cluster_ctarank();             // 0 = leader
   const Items items(g, blockIdx.x >> 1, gridDim.x >> 1);
   int count = items.count();
+  const int kStep = MODE == VOCAB_PRODUCTS ? g.kStep : 1, stages = MODE == VOCAB_PRODUCTS ? g.stages : STAGES;
+  const int stride = MODE == VOCAB_PRODUCTS ? g.stride : STAGE_BYTES, aBytes = A_BYTES * kStep, mnBlock = 64 * BK * 2 * kStep;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&fullBar[s], 1); mbar_init(&emptyBar[s], 1); }
@@ -181,20 +184,23 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
         const Tile t = tileOf(p, item);
         const int bHalf = MODE == VOCAB_PRODUCTS ? p.tn / 2 : HALF;
         const int rowA = t.mt * T + (int)cr * HALF, rowB = t.nt * 2 * bHalf + (int)cr * bHalf;
-        for (int k = t.k0; k < t.k1; ++k) {
+        for (int k = t.k0; k < t.k1; k += kStep) {       // (the second half of a slice's last stage may be another's, or outside: it is not multiplied)
           if (!mbar_wait(&emptyBar[stage], phase ^ 1, giveUp, WAIT_NS)) { ok = false; break; }
           if (cr == 0) mbar_expect_tx(&fullBar[stage], 2 * (MODE == VOCAB_PRODUCTS ? p.stageBytes : STAGE_BYTES));       // my bytes and the partner's
-          uint8_t* sa = smem + stage * STAGE_BYTES;
-          uint8_t* sb = sa + A_BYTES;
+          uint8_t* sa = smem + stage * stride;
+          uint8_t* sb = sa + aBytes;
           const uint32_t bar = bar0 + stage * 8;
-          // K-major: a box of 64 of the contraction x 128 rows.  MN-major: blocks of 64 columns x 64 of the contraction, in one load
+          // K-major: boxes of 64 of the contraction x 128 rows.  MN-major: blocks of 64 columns x 64 kStep of the contraction, in one load
           // where the matrix and the tile are cut into whole blocks, else block by block from any multiple of 16 columns.
-          if (MODE == VOCAB_PRODUCTS && p.aMn) tma_load_3d_pair(sa, ma, k * BK, rowA / 64, bar);
-          else tma_load_2d_pair(sa, ma, k * BK, rowA, bar);
-          if (MODE != VOCAB_PRODUCTS) tma_load_2d_pair(sb, mb, k * BK, rowB, bar);
-          else if (!p.bLoose) tma_load_3d_pair(sb, mb, k * BK, rowB / 64, bar);
-          else for (int i = 0; i * 64 < bHalf; ++i) tma_load_2d_pair(sb + i * 64 * BK * 2, mb, rowB + 64 * i, k * BK, bar);
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          if (MODE != VOCAB_PRODUCTS) {
+            tma_load_2d_pair(sa, ma, k * BK, rowA, bar);
+            tma_load_2d_pair(sb, mb, k * BK, rowB, bar);
+          } else {
+            tma_load_3d_pair(sa, ma, p.aMn ? k * BK : rowA, p.aMn ? rowA / 64 : k, bar);
+            if (!p.bLoose) tma_load_3d_pair(sb, mb, k * BK, rowB / 64, bar);
+            else for (int i = 0; i * 64 < bHalf; ++i) tma_load_2d_pair(sb + i * mnBlock, mb, rowB + 64 * i, k * BK, bar);
+          }
+          if (++stage == stages) { stage = 0; phase ^= 1; }
         }
       }
       if (!ok) for (int i = 0; i < 20000; ++i) __nanosleep(200);     // copies already issued land before the CTA goes away
@@ -208,9 +214,9 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
         int item;
         const Product& p = g.p[items.at(j, item)];
         const Tile t = tileOf(p, item);
-        blocks += t.k1 - t.k0;
+        blocks += (t.k1 - t.k0 + kStep - 1) / kStep;
       }
-      int loads = blocks - STAGES;
+      int loads = blocks - stages;
       bool ok = true;
       for (int j = 0; j < count && ok; ++j) {
         int item;
@@ -219,22 +225,27 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
         const Tile t = tileOf(p, item);
         const bool aMn = MODE == VOCAB_PRODUCTS && p.aMn, bMn = MODE == VOCAB_PRODUCTS && p.bMn;
         const uint32_t idesc = umma_idesc_bf16(T, MODE == VOCAB_PRODUCTS ? p.tn : T, aMn, bMn);
-        // per instruction (16 of the contraction): 32 bytes along a K-major row, two groups of 8 rows of an MN-major block
-        const uint32_t stepA = aMn ? 128u : 2u, stepB = bMn ? 128u : 2u;
+        // per instruction (16 of the contraction): 32 bytes along a K-major row, two groups of 8 rows of an MN-major block.  Per 64: the next
+        // box, or further down the same blocks.
+        const uint32_t stepA = aMn ? 128u : 2u, stepB = bMn ? 128u : 2u, hopA = aMn ? 512u : A_BYTES / 16, hopB = 512u;
         const int ab = j & 1;
         if (!mbar_wait(&accEmpty[ab], ((j >> 1) & 1) ^ 1, giveUp, WAIT_NS)) break;
         tc_fence_after();
         const uint32_t d = tmemBase + ab * T;
-        for (int k = t.k0; k < t.k1; ++k) {
+        for (int k = t.k0; k < t.k1; k += kStep) {
           if (!mbar_wait(&fullBar[stage], phase, giveUp, WAIT_NS)) { ok = false; break; }
           tc_fence_after();
-          const uint8_t* pa = smem + stage * STAGE_BYTES;
-          const uint64_t da = aMn ? umma_smem_desc_mn_sw128(pa, 64 * BK * 2) : umma_smem_desc_sw128(pa);
-          const uint64_t db = bMn ? umma_smem_desc_mn_sw128(pa + A_BYTES, 64 * BK * 2) : umma_smem_desc_sw128(pa + A_BYTES);
+          const uint8_t* pa = smem + stage * stride;
+          const uint64_t da = aMn ? umma_smem_desc_mn_sw128(pa, mnBlock) : umma_smem_desc_sw128(pa);
+          const uint64_t db = bMn ? umma_smem_desc_mn_sw128(pa + aBytes, mnBlock) : umma_smem_desc_sw128(pa + aBytes);
 #pragma unroll
-          for (int i = 0; i < BK / UMMA_K; ++i) umma_bf16_pair(d, da + stepA * i, db + stepB * i, idesc, k != t.k0 || i != 0);
+          for (int h = 0; h < (MODE == VOCAB_PRODUCTS ? 2 : 1); ++h) {
+            if (h == 1 && (kStep == 1 || k + 1 == t.k1)) break;
+#pragma unroll
+            for (int i = 0; i < BK / UMMA_K; ++i) umma_bf16_pair(d, da + hopA * h + stepA * i, db + hopB * h + stepB * i, idesc, k != t.k0 || (h | i) != 0);
+          }
           if (loads-- > 0) umma_commit_pair(&emptyBar[stage]);      // both CTAs' stage is free once these MMAs have read it
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          if (++stage == stages) { stage = 0; phase ^= 1; }
         }
         if (ok) umma_commit_pair(&accFull[ab]);       // both halves of the accumulator complete
       }
@@ -551,27 +562,31 @@ ncclResult_t vocabProducts(const void* dz, const void* x, const void* w, int n, 
   g.factor = factor;
   if (exact) g.exact = *exact;
   int k = 0;
-  const int tn = productWidth(d);
+  // Stages of 128 of the contraction under narrower tiles: the tensor cores are through with one of 64 before its loads are issued.
+  const int tn = productWidth(d), kStep = tn < T ? 2 : 1, box = BK * kStep;
   const bool loose = d % 64 != 0 || tn % 128 != 0;
+  g.kStep = kStep;
+  g.stride = A_BYTES * kStep + (tn / 2 + 63) / 64 * 64 * BK * 2 * kStep;
+  g.stages = std::min(STAGES, STAGES * STAGE_BYTES / g.stride);
   auto narrow = [&](CUtensorMap* m, const void* base, int rows) {      // [rows of the contraction][d columns]
-    return loose ? gemmEncodeMap(m, base, (uint64_t)rows, (uint64_t)d, BK) : gemmEncodeMap3(m, base, (uint64_t)d, (uint64_t)rows, 1, tn / 2, BK);
+    return loose ? gemmEncodeMap(m, base, (uint64_t)rows, (uint64_t)d, box) : gemmEncodeMap3(m, base, (uint64_t)d, (uint64_t)rows, 1, tn / 2, box);
   };
   auto result = [&](const VocabResult& r, int which) {
     Product& p = g.p[k++];
     p.bMn = 1; p.bLoose = loose;
-    p.stageBytes = A_BYTES + (tn / 2 + 63) / 64 * 64 * BK * 2;
+    p.stageBytes = g.stride;
     p.out = (__nv_bfloat16*)r.out; p.part = r.part; p.add = r.add;
     p.exact = exact && r.out ? which : 0;
     p.wide = d % 16 == 0 && ((uintptr_t)r.out & 31) == 0;
   };
   if (dx.out || dx.part) {
-    DFCHECK(gemmEncodeMap(&a[k], dz, (uint64_t)n, (uint64_t)ld, HALF));
+    DFCHECK(gemmEncodeMap3(&a[k], dz, (uint64_t)n, (uint64_t)ld, 0, HALF, box));
     DFCHECK(narrow(&b[k], w, v));
     g.p[k] = productOf(n, d, v, plan.perX, tn);
     result(dx, 1);
   }
   if (dw.out || dw.part) {
-    DFCHECK(gemmEncodeMap3(&a[k], dz, (uint64_t)ld, (uint64_t)n, 1, HALF, BK));
+    DFCHECK(gemmEncodeMap3(&a[k], dz, (uint64_t)ld, (uint64_t)n, 1, HALF, box));
     DFCHECK(narrow(&b[k], x, n));
     g.p[k] = productOf(v, d, n, plan.perW, tn);
     g.p[k].aMn = 1;
