@@ -78,24 +78,25 @@ size_t dfcclEmbeddingBackwardWork(int n, int d, int tables);
  * gradient), 1 a row with some, 2 a row with a token outside the vocabulary (NaN). */
 ncclResult_t dfcclTeacherRows(const void* logits, int logitType, const void* tokens, int wide, int n, int k, int v, float temperature,
                               void* outTokens /* int32 [n, k] */, void* outWeights /* fp32 [n, k] */, void* state /* int32 [n] */, cudaStream_t stream);
-/* lse [n]: log2 of the sum of 2^(z log2(e) / T), kept for the backward pass; reduction 0: rowLoss [n]; 1 (mean over the rows with a target
+/* lse [n]: log2 of the sum of 2^(z log2(e) / T); rest [n, k]: what of the entries' weights their probabilities leave; both are kept for the backward pass.  reduction 0: rowLoss [n]; 1 (mean over the rows with a target
  * or list; 0 where there is none) or 2 (sum): loss and count (int32), one each.  All fp32. */
 ncclResult_t dfcclLinearLossForward(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, const void* tokens,
-                                    const void* weights, const void* state, int k, float temperature, int reduction, void* work, void* lse, void* rowLoss,
-                                    void* loss, void* count, cudaStream_t stream);
+                                    const void* weights, const void* state, int k, float temperature, int reduction, void* work, void* lse, void* rest,
+                                    void* rowLoss, void* loss, void* count, cudaStream_t stream);
 size_t dfcclLinearLossForwardWork(int n, int v, int k);
 /* dx and dw (either may be null) for the gradient gout of the loss: one value (goutStride 0) or one per row; count: of a mean, else null.
  * The gradient of the logits exists for as many columns at a time as DFCCL_LOSS_WORKSPACE_BYTES (1 GiB) hold. */
 ncclResult_t dfcclLinearLossBackward(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, const void* tokens,
-                                     const void* weights, const void* state, int k, float temperature, const void* lse, const void* gout, int goutStride,
-                                     const void* count, void* dx, void* dw, void* work, size_t workBytes, cudaStream_t stream);
-size_t dfcclLinearLossBackwardWork(int n, int v, int d, int wantX, int wantW);
+                                     const void* weights, const void* state, int k, float temperature, const void* lse, const void* rest,
+                                     const void* gout, int goutStride, const void* count, void* dx, void* dw, void* work, size_t workBytes, cudaStream_t stream);
+size_t dfcclLinearLossBackwardWork(int n, int v, int d, int k /* 0: targets */, int wantX, int wantW);
 int dfcclLinearLossMaxList(void);
 /* The cross entropy (reduction 1 or 2) and its gradients for a gradient of 1 in one go: the product of the logits is computed once instead of
- * twice.  dx or dw may be null.  lse, loss and count as above.  The powers of the logits exist for as many rows at a time as
+ * twice.  dx or dw may be null.  lse, rest, loss and count as above.  The powers of the logits exist for as many rows at a time as
  * DFCCL_LOSS_WORKSPACE_BYTES hold. */
 ncclResult_t dfcclCrossEntropyWithGradients(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, int reduction,
-                                            void* work, size_t workBytes, void* lse, void* loss, void* count, void* dx, void* dw, cudaStream_t stream);
+                                            void* work, size_t workBytes, void* lse, void* rest, void* loss, void* count, void* dx, void* dw,
+                                            cudaStream_t stream);
 size_t dfcclCrossEntropyWithGradientsWork(int n, int v, int d, int wantX, int wantW);
 /* Two bf16 arrays (na and nb elements, multiples of 8; either may be empty) times *scale (fp32), in place; left alone where it is 1. */
 ncclResult_t dfcclScaleResults(void* a, size_t na, void* b, size_t nb, const void* scale, cudaStream_t stream);

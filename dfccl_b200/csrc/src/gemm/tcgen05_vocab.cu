@@ -100,23 +100,22 @@ __device__ __forceinline__ Tile tileOf(const Product& p, int item) {
   return t;
 }
 
-// A row's list from the first entry at or behind a column on.
 // A row's list from the first entry at or behind a column on.  The entry behind the present one is on its way too: a step does not wait
-// for memory (without it 32 entries a row cost 60 us of the 640 that dz of 8192 x 50257 x 1024 takes).
+// for memory (without it 32 entries a row cost 60 us of the 640 that dz of 8192 x 50257 x 1024 took).
 struct List {
   const int* tokens;
-  const float* weights;
+  const float* rest;
   int k, behind, next, next2;
   float q, q2;
-  __device__ __forceinline__ void load(int at, int& token, float& weight) {
+  __device__ __forceinline__ void load(int at, int& token, float& q) {
     token = at < k ? tokens[at] : VOCAB_NO_TOKEN;
-    weight = at < k ? weights[at] : 0.f;
+    q = at < k && rest ? rest[at] : 0.f;
   }
-  __device__ __forceinline__ void none() { tokens = nullptr; weights = nullptr; k = behind = 0; next = next2 = VOCAB_NO_TOKEN; q = q2 = 1.f; }
-  __device__ __forceinline__ void seek(const VocabRows& r, int row, int token, int col) {
+  __device__ __forceinline__ void none() { tokens = nullptr; rest = nullptr; k = behind = 0; next = next2 = VOCAB_NO_TOKEN; q = q2 = 0.f; }
+  __device__ __forceinline__ void seek(const VocabRows& r, const float* allRest, int row, int token, int col) {
     none();
-    if (r.targets) { if (token >= col) next = token; return; }
-    k = r.k; tokens = r.tokens + (size_t)row * k; weights = r.weights + (size_t)row * k;
+    if (r.targets) { if (token >= col) next = token; if (allRest) q = allRest[row]; return; }
+    k = r.k; tokens = r.tokens + (size_t)row * k; rest = allRest ? allRest + (size_t)row * k : nullptr;
     int lo = 0, hi = k;
     while (lo < hi) { const int mid = (lo + hi) >> 1; if (tokens[mid] < col) lo = mid + 1; else hi = mid; }
     load(lo, next, q);
@@ -283,7 +282,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
             coef = g.grad.gout ? g.grad.gout[(size_t)row * g.grad.goutStride] : 1.f;
             if (state != ROW_LIST) coef = state == ROW_BAD ? __int_as_float(0x7fffffff) : 0.f;
           }
-          list.seek(g.rows, row, token, g.first + col0);
+          list.seek(g.rows, MODE == VOCAB_GRAD ? g.grad.rest : nullptr, row, token, g.first + col0);
         }
         if (!mbar_wait(&accFull[ab], (j >> 1) & 1, giveUp, WAIT_NS)) break;
         tc_fence_after();
@@ -324,11 +323,10 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
 #pragma unroll
               for (int e = 0; e < 32; ++e) if (c + e >= p.N) r[e] = 0xff800000u;          // -inf
             }
-            const int own = list.next - c;               // the target's column, out of the sum
-            float target = 0.f;
+            const int own = list.next - c;               // the target: no power
             if (own >= 0 && own < 32) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) if (e == own) { target = __uint_as_float(r[e]); r[e] = 0xff800000u; }
+              for (int e = 0; e < 32; ++e) if (e == own) r[e] = 0xff800000u;
             }
             float m0 = __uint_as_float(r[0]), m1 = __uint_as_float(r[1]);
 #pragma unroll
@@ -342,19 +340,18 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
               r[e] = __float_as_uint(v);
             }
             sum = (s[0] + s[1]) + (s[2] + s[3]);
-            if (own >= 0 && own < 32) {
-              target = exp2Approx(fmaf(target, scale, -lse));
-#pragma unroll
-              for (int e = 0; e < 32; ++e) if (e == own) r[e] = __float_as_uint(target);
-            }
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(exp2Approx(fmaf(__uint_as_float(r[e]), scale, -lse)));
+            int before = -1;
             while (list.next < g.first + c + 32) {
               if (list.next >= g.first + c) {
                 const int at = list.next - g.first - c;
+                if (at != before) {                      // (the first entry of a token has all of it)
 #pragma unroll
-                for (int e = 0; e < 32; ++e) if (e == at) r[e] = __float_as_uint(__uint_as_float(r[e]) - list.q);
+                  for (int e = 0; e < 32; ++e) if (e == at) r[e] = __float_as_uint(-list.q);
+                }
+                before = at;
               }
               list.step();
             }
@@ -400,14 +397,10 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
           }
         }
       } else {
+        const float* sums = here && p.exact == 2 ? vocabSumsOf(g.exact, g.exact.first + row, p.N) : nullptr;      // (while the accumulator is computed)
         if (!mbar_wait(&accFull[ab], (j >> 1) & 1, giveUp, WAIT_NS)) break;
         tc_fence_after();
         const int steps = (min(tn, p.N - col0) + 31) / 32;
-        int state = ROW_NONE, token = 0;
-        float scale = 0.f;
-        const float* sums = nullptr;
-        if (here && p.exact == 1) { state = rowState(g.exact.rows, row, token); scale = g.exact.scale[row]; }
-        if (here && p.exact == 2) { const int at = g.exact.where[row]; if (at >= 0) sums = g.exact.sums + (size_t)at * p.N; }
 #pragma unroll 1
         for (int i = part; i < steps; i += PARTS) {
           if (!mine) break;
@@ -426,19 +419,24 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
               dst[v] = o;
             }
           } else {
+            float f[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(r[e]);
+            if (p.exact == 1) vocabExactX<4>(f, g.exact, row, p.N, c, packs);
+            else if (sums) {
+#pragma unroll
+              for (int v = 0; v < 8; ++v) {
+                if (v / 2 >= packs) break;
+                const float4 q = *((const float4*)(sums + c) + v);
+                f[4 * v] -= q.x; f[4 * v + 1] -= q.y; f[4 * v + 2] -= q.z; f[4 * v + 3] -= q.w;
+              }
+            }
             uint4 o[4];
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-              float f[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(r[8 * v + e]);
-              if (v < packs) {
-                if (p.exact == 1) vocabExactX(f, state, scale, (const uint4*)(g.exact.w + (size_t)(state == ROW_LIST ? token : 0) * p.N + c) + v);
-                else if (sums) vocabMinus(f, (const float4*)(sums + c) + 2 * v);
-              }
               uint32_t* ow = (uint32_t*)&o[v];
 #pragma unroll
-              for (int w = 0; w < 4; ++w) ow[w] = pack_bf16x2(f[2 * w] * factor, f[2 * w + 1] * factor);
+              for (int w = 0; w < 4; ++w) ow[w] = pack_bf16x2(f[8 * v + 2 * w] * factor, f[8 * v + 2 * w + 1] * factor);
             }
             __nv_bfloat16* dst = p.out + (size_t)row * p.N + c;
             if (packs == 4) { st_global32(dst, o, p.wide); st_global32(dst + 16, o + 2, p.wide); }

@@ -58,12 +58,14 @@ struct VocabFactor {
   const int* count;             // rows that share a mean, or null
   float temperature;
 };
-// dz = g (2^(z scale - lse) - weight where an entry is in the list), 0 in rows without a list and NaN in those with a token outside the
-// vocabulary, for the columns [0, v) of w, which start at column `first` of the vocabulary: bf16, [n][ld], ld = v rounded up to 64 (zeros behind v).
+// dz = g 2^(z scale - lse), for the entries of a row's list -g rest instead (0 where `rest` is null), 0 in rows without a list and NaN in those with a token
+// outside the vocabulary, for the columns [0, v) of w, which start at column `first` of the vocabulary: bf16, [n][ld], ld = v rounded up to 64
+// (zeros behind v).
 struct VocabGrad {
   const float* lse;             // [n] log2 of the sum of 2^(z scale)
   const float* gout;            // g [n], or null: 1
   int goutStride;
+  const float* rest;            // [n][k] an entry's weight less its probability; of entries of one token all of it in the first
 };
 ncclResult_t vocabGrad(const void* x, const void* w, int n, int v, int first, int d, const VocabRows& rows, const VocabGrad& grad, void* dz, bool early,
                        cudaStream_t stream);
@@ -81,15 +83,22 @@ struct VocabPlan { int perX, perW; };
 VocabPlan vocabProductPlan(int n, int v, int d, bool wantX, bool wantW, int pairs);
 inline int vocabSlices(int k, int per) { return ((k + 63) / 64 + per - 1) / per; }
 
-// Where dz is not the gradient of the logits but their powers (vocabPowers, targets only): what is missing of both results, in fp32.
-//   dx_n = factor (scale_n (powers w)_n - w_target(n)),   dw_t = factor ((powers^T x')_t - sums_where(t))
-// with x' = scale_n x_n as the right operand, sums_where(t) the sum of the x_n whose target is t.
+// What the entries of the rows' lists add to both results, in fp32, where dz has zeros in their places.  It is most of both: of few rows
+// its rounding in dz would be as large as that of the results.
+//   dx_n = factor (scale_n (dz w)_n - g_n sum_k rest_nk w_token(n,k)),   dw_t = factor ((dz^T x)_t - sums_where(t))
+// sums_where(t): the sum of g_n rest_nk x_n over the entries of token t.
 struct VocabExact {
   VocabRows rows;               // of the n rows
-  const float* scale;           // [n]
-  const __nv_bfloat16* w;       // [v, d]
+  const float* scale;           // [n], or null: 1
+  const float* rest;            // [n][k]
+  const float* gout;            // g [n], or null: 1
+  int goutStride;
+  const __nv_bfloat16* w;       // [v, d], the whole vocabulary
   const float* sums;            // rows of d
-  const int* where;             // [v] a row of sums, or -1
+  const int* where;             // [v] a row of sums; of a token that no list has it may be anything:
+  const uint2* items;           // it counts where items[that].x is the token, or where, with items null, the rows' entry of that number is
+  int entries;                  // of items or of the rows
+  int first;                    // token of dw's first row
 };
 
 // dx [n, d] = factor dz w and dw [v, d] = factor dz^T x in one launch.  A result is bf16 where `out` is given; otherwise `part` gets an fp32
@@ -104,24 +113,62 @@ ncclResult_t vocabProducts(const void* dz, const void* x, const void* w, int n, 
                            const VocabResult& dx, const VocabResult& dw, cudaStream_t stream);
 
 #if defined(__CUDACC__)
-// Eight elements of a row of dx or dw from their sums.
-__device__ __forceinline__ void vocabMinus(float (&f)[8], const float4* p) {
-  const float4 a = p[0], b = p[1];
-  f[0] -= a.x; f[1] -= a.y; f[2] -= a.z; f[3] -= a.w; f[4] -= b.x; f[5] -= b.y; f[6] -= b.z; f[7] -= b.w;
+// The row of sums of a token, or null.
+__device__ __forceinline__ const float* vocabSumsOf(const VocabExact& x, int token, int d) {
+  const int at = x.where[token];
+  if (at < 0 || at >= x.entries) return nullptr;
+  int own;
+  if (x.items) own = (int)x.items[at].x;
+  else if (x.rows.targets) rowState(x.rows, at, own);
+  else own = x.rows.tokens[at];
+  return own == token ? x.sums + (size_t)at * d : nullptr;
 }
-__device__ __forceinline__ void vocabExactX(float (&f)[8], int state, float scale, const uint4* target) {
+__device__ __forceinline__ void vocabMinus(float* f, float weight, const uint4& w) {
+  const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    f[2 * e] = fmaf(-weight, __uint_as_float(p[e] << 16), f[2 * e]);
+    f[2 * e + 1] = fmaf(-weight, __uint_as_float(p[e] & 0xffff0000u), f[2 * e + 1]);
+  }
+}
+// P packs of eight columns of a row of dx from their sums, from column c of d on (the first `packs` of them).
+template <int P>
+__device__ __forceinline__ void vocabExactX(float (&f)[8 * P], const VocabExact& x, int row, int d, int c, int packs) {
+  int token;
+  const int state = rowState(x.rows, row, token);
   if (state != ROW_LIST) {
     const float none = state == ROW_BAD ? __int_as_float(0x7fffffff) : 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = none;
+    for (int e = 0; e < 8 * P; ++e) f[e] = none;
     return;
   }
-  const uint4 t = *target;
-  const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+  if (x.scale) {
+    const float s = x.scale[row];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    f[2 * e] = fmaf(f[2 * e], scale, -__uint_as_float(w[e] << 16));
-    f[2 * e + 1] = fmaf(f[2 * e + 1], scale, -__uint_as_float(w[e] & 0xffff0000u));
+    for (int e = 0; e < 8 * P; ++e) f[e] *= s;
+  }
+  const float g = x.gout ? x.gout[(size_t)row * x.goutStride] : 1.f;
+  const size_t at = (size_t)row * x.rows.k;
+  for (int i = 0; i < x.rows.k; i += 2) {
+    const uint4* src[2];
+    float weight[2];
+    uint4 w[2][P];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int t = x.rows.targets ? u ? VOCAB_NO_TOKEN : token : i + u < x.rows.k ? x.rows.tokens[at + i + u] : VOCAB_NO_TOKEN;
+      weight[u] = t == VOCAB_NO_TOKEN ? 0.f : g * x.rest[at + i + u];
+      src[u] = (const uint4*)(x.w + (size_t)(t == VOCAB_NO_TOKEN ? 0 : t) * d + c);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int v = 0; v < P; ++v) w[u][v] = weight[u] != 0.f && v < packs ? src[u][v] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (weight[u] == 0.f) continue;
+#pragma unroll
+      for (int v = 0; v < P; ++v) vocabMinus(f + 8 * v, weight[u], w[u][v]);
+    }
   }
 }
 #endif

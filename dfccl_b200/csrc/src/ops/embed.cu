@@ -168,6 +168,9 @@ struct Table {
   // sums by themselves instead of a gradient: fp32 rows [n][d], used where `where` [rows] says
   float* compact;
   int* where;
+  const float* weights;           // [n] of the tokens there, times gout[n] where given
+  const float* gout;
+  int goutStride;
 };
 struct Backward {
   Table t[MAX_TABLES];
@@ -318,6 +321,7 @@ template <typename T, int E, bool COMPACT>
 __global__ void __launch_bounds__(128) sumStretchKernel(const Backward a) {
   constexpr int MAX = 128, AHEAD = 8;
   __shared__ uint32_t keys[MAX + 2], tokens[MAX];
+  __shared__ float weights[MAX];
   tc::grid_dependency_wait();
   tc::grid_launch_dependents();
   const Table& t = a.t[blockIdx.z];
@@ -327,7 +331,10 @@ __global__ void __launch_bounds__(128) sumStretchKernel(const Backward a) {
     const int at = start + i;
     const uint2 item = at >= 0 && at < a.n ? __ldcg(&items[at]) : make_uint2(0xffffffffu, 0u);
     keys[i + 1] = item.x;
-    if (i >= 0 && i < count) tokens[i] = item.y;
+    if (i >= 0 && i < count) {
+      tokens[i] = item.y;
+      if (COMPACT) weights[i] = item.x < (uint32_t)t.rows ? t.weights[item.y] * (t.gout ? t.gout[(size_t)item.y * t.goutStride] : 1.f) : 0.f;
+    }
   }
   __syncthreads();
   const int col = (blockIdx.y * 128 + threadIdx.x) * E;
@@ -348,7 +355,7 @@ __global__ void __launch_bounds__(128) sumStretchKernel(const Backward a) {
       const int j = i + u;
       if (j >= count || keys[j + 1] == none) return;                     // (tokens without a gradient are the last)
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += toFloat(p[u].v[e]);
+      for (int e = 0; e < E; ++e) acc[e] = COMPACT ? fmaf(weights[j], toFloat(p[u].v[e]), acc[e]) : acc[e] + toFloat(p[u].v[e]);
       const bool goesOn = keys[j + 2] == keys[j + 1];
       if (goesOn && j + 1 < count) continue;
       if (head || goesOn) {                                              // not all of the row
@@ -467,7 +474,7 @@ ncclResult_t forward(const Forward& a, cudaStream_t stream) {
 
 template <typename T, int E, bool COMPACT>
 ncclResult_t backward(const Backward& a, cudaStream_t stream) {
-  CUDACHECK(launchBehind(sortTokensKernel, dim3(SORT_CTAS * a.tables), SORT_THREADS, SORT_CTAS, stream, a));
+  if (!COMPACT) CUDACHECK(launchBehind(sortTokensKernel, dim3(SORT_CTAS * a.tables), SORT_THREADS, SORT_CTAS, stream, a));
   if (!COMPACT) CUDACHECK(launchBehind(clearKernel, dim3(CLEAR_BLOCKS), 256, 1, stream, a));
   const int packs = a.d / E;
   CUDACHECK(launchBehind(sumStretchKernel<T, E, COMPACT>, dim3(a.stretches, (packs + 127) / 128, a.tables), 128, 1, stream, a));
@@ -492,12 +499,25 @@ size_t tokenSumsWork(int n, int d) {
   const Layout l = layoutOf(n, d);
   return 2 * l.items + l.sums;
 }
-ncclResult_t tokenSums(const void* x, int n, int d, const void* ids, int wide, int64_t ignore, int v, float* sums, int* where, void* work, cudaStream_t stream) {
-  if (d % 8) return ncclInvalidArgument;
+static Backward sumsOf(int n, int d, const void* ids, int wide, int64_t ignore, int v, void* work) {
   Backward a = {};
-  a.tables = 1; a.n = n; a.d = d; a.stretch = stretchOf(n); a.stretches = (n + a.stretch - 1) / a.stretch; a.g = x;
+  a.tables = 1; a.n = n; a.d = d; a.stretch = stretchOf(n); a.stretches = (n + a.stretch - 1) / a.stretch;
   setKeys(&a.t[0], ids, wide, v, ignore, (uint8_t*)work, layoutOf(n, d));
-  a.t[0].compact = sums; a.t[0].where = where;
+  return a;
+}
+const uint2* tokenSortItems(int n, int d, int v, void* work) {
+  const Backward a = sumsOf(n, d, nullptr, 0, 0, v, work);
+  return a.t[0].buf[a.t[0].passes & 1];
+}
+ncclResult_t tokenSort(int n, int d, const void* ids, int wide, int64_t ignore, int v, void* work, cudaStream_t stream) {
+  CUDACHECK(launchBehind(sortTokensKernel, dim3(SORT_CTAS), SORT_THREADS, SORT_CTAS, stream, sumsOf(n, d, ids, wide, ignore, v, work)));
+  return ncclSuccess;
+}
+ncclResult_t tokenSums(const void* x, int n, int d, int v, const float* weights, const float* gout, int goutStride, float* sums, int* where, void* work, cudaStream_t stream) {
+  if (d % 8) return ncclInvalidArgument;
+  Backward a = sumsOf(n, d, nullptr, 0, 0, v, work);
+  a.g = x;
+  a.t[0].compact = sums; a.t[0].where = where; a.t[0].weights = weights; a.t[0].gout = gout; a.t[0].goutStride = goutStride;
   return backward<__nv_bfloat16, 8, true>(a, stream);
 }
 

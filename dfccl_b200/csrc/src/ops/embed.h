@@ -7,9 +7,13 @@
 
 namespace dfccl {
 
-// The fp32 sum of the rows of x [n, d] (bf16, d % 8 == 0) for every token of ids that is inside [0, v) and not `ignore`, in the order of the
-// rows: row where[token] of sums [n][d].  Entries of `where` [v] of other tokens are left as they are.  work: tokenSumsWork bytes.
+// Sorts the tokens of n rows that are inside [0, v) and not `ignore`, by token and row; the others are behind them as v.  work: tokenSumsWork bytes.
 size_t tokenSumsWork(int n, int d);
-ncclResult_t tokenSums(const void* x, int n, int d, const void* ids, int wide, int64_t ignore, int v, float* sums, int* where, void* work, cudaStream_t stream);
+ncclResult_t tokenSort(int n, int d, const void* ids, int wide, int64_t ignore, int v, void* work, cudaStream_t stream);
+// The sorted (token, row) [n], once it has run.
+const uint2* tokenSortItems(int n, int d, int v, void* work);
+// Behind it, with the same work: for every token the fp32 sum of weights_n gout_n x_n over its rows (x [n, d] bf16, d % 8 == 0; gout may be null), in
+// their order, -> row where[token] of sums [n][d], the place of one of the token's items.  Entries of `where` [v] of other tokens are left as they are.
+ncclResult_t tokenSums(const void* x, int n, int d, int v, const float* weights, const float* gout, int goutStride, float* sums, int* where, void* work, cudaStream_t stream);
 
 }  // namespace dfccl

@@ -133,6 +133,7 @@ struct JoinArgs {
   float t2;
   float* lse;
   float* loss;
+  float* rest;                  // [n][k] what is left of an entry's weight without its probability; of entries of one token all of it in the first
   // behind vocabPowers: the powers' bases and, to be written, the powers' share of a probability, 2^base / sum; rows whose sums say that
   // their base was no good raise `again`
   float* base;
@@ -190,30 +191,53 @@ __global__ void __launch_bounds__(1024) joinRowsKernel(const JoinArgs a) {
         if (st == ROW_LIST) share = 1.f / (1.f + acc.y);
         if (lane == 0) {
           a.share[row] = st == ROW_NONE ? 0.f : share;
+          a.rest[row] = acc.y * share;
           if (st == ROW_LIST && !(acc.x <= MOST_POWER && acc.y < INFINITY && fabsf(a.base[row]) < INFINITY)) *a.again = 1;
         }
       } else {
-        if (st == ROW_LIST) {                           // the list's own powers, each entry once
+        const size_t list = (size_t)row * a.rows.k;
+        const float2 others = acc;                      // (of entries that no list has)
+        int distinct = 0;
+        if (st == ROW_LIST) {                           // the list's own powers, each token once
           float2 own = make_float2(-INFINITY, 0.f);
           for (int i = lane; i < a.rows.k; i += 32) {
-            const size_t at = (size_t)row * a.rows.k + i;
-            if (!a.rows.targets && (a.rows.tokens[at] == VOCAB_NO_TOKEN || (i && a.rows.tokens[at] == a.rows.tokens[at - 1]))) continue;
-            own = joined(own, make_float2(a.picked[at] * a.rows.scale, 1.f));
+            if (!a.rows.targets && (a.rows.tokens[list + i] == VOCAB_NO_TOKEN || (i && a.rows.tokens[list + i] == a.rows.tokens[list + i - 1]))) continue;
+            own = joined(own, make_float2(a.picked[list + i] * a.rows.scale, 1.f));
+            ++distinct;
           }
 #pragma unroll
-          for (int o = 16; o; o >>= 1) own = joined(own, make_float2(__shfl_xor_sync(0xffffffffu, own.x, o), __shfl_xor_sync(0xffffffffu, own.y, o)));
+          for (int o = 16; o; o >>= 1) {
+            own = joined(own, make_float2(__shfl_xor_sync(0xffffffffu, own.x, o), __shfl_xor_sync(0xffffffffu, own.y, o)));
+            distinct += __shfl_xor_sync(0xffffffffu, distinct, o);
+          }
           acc = joined(acc, own);
         }
         l = acc.x + log2f(acc.y);
-        if (st == ROW_LIST)
+        if (distinct == 1) {                            // all on one token: from the others' powers, however small they are beside its own
+          const float u = a.picked[list] * a.rows.scale, ratio = others.y * exp2f(others.x - u);
           for (int i = lane; i < a.rows.k; i += 32) {
-            const size_t at = (size_t)row * a.rows.k + i;
-            if (!a.rows.targets && a.rows.tokens[at] == VOCAB_NO_TOKEN) continue;
-            const float q = a.rows.targets ? 1.f : a.rows.weights[at];
-            if (q == 0.f) continue;                     // 0 ln 0
-            sum += q * (logf(q) - (a.picked[at] * a.rows.scale - l) * LN2);
+            const float q = a.rows.targets || a.rows.tokens[list + i] == VOCAB_NO_TOKEN ? 1.f : a.rows.weights[list + i];
+            if (q != 0.f) sum += q * logf(q);           // (of entries that share the token)
+            a.rest[list + i] = i ? 0.f : others.y * exp2f(others.x - l);
           }
-        sum = warpSum(sum);
+          sum = warpSum(sum) + (ratio < 1e30f ? log1pf(ratio) : (l - u) * LN2);
+        } else {
+          for (int i = lane; i < a.rows.k; i += 32) {
+            float rest = 0.f;
+            if (st == ROW_LIST && a.rows.tokens[list + i] != VOCAB_NO_TOKEN) {
+              const int t = a.rows.tokens[list + i];
+              float q = a.rows.weights[list + i];
+              const float u = a.picked[list + i] * a.rows.scale - l;
+              if (q != 0.f) sum += q * (logf(q) - u * LN2);       // (0 ln 0)
+              if (i == 0 || a.rows.tokens[list + i - 1] != t) {
+                for (int j = i + 1; j < a.rows.k && a.rows.tokens[list + j] == t; ++j) q += a.rows.weights[list + j];
+                rest = q - exp2f(u);
+              }
+            }
+            a.rest[list + i] = rest;
+          }
+          sum = warpSum(sum);
+        }
         if (a.base && lane == 0) { a.base[row] = l; if (st == ROW_LIST) a.share[row] = 1.f; }
       }
       // x times the row's share, rounded to bf16: the right operand of the powers' product.  A row without a target is zeros whatever it holds.
@@ -252,7 +276,6 @@ struct PickArgs {
   float* picked;
   float* base;
   int* count;                    // or null
-  int* where; int v;             // [v] to be -1, or null
   int* words; int nWords;        // to be 0
 };
 __global__ void __launch_bounds__(256) pickLogitsKernel(const PickArgs a) {
@@ -272,7 +295,6 @@ __global__ void __launch_bounds__(256) pickLogitsKernel(const PickArgs a) {
     }
     for (int i = threadIdx.x; i < a.nWords; i += 256) a.words[i] = 0;
   }
-  if (a.where) for (int i = blockIdx.x * 256 + threadIdx.x; i < a.v; i += gridDim.x * 256) a.where[i] = -1;
   const int k = a.rows.k, fours = (k + 3) / 4;
   for (long long item = (long long)blockIdx.x * 8 + warp; item < (long long)a.n * fours; item += (long long)gridDim.x * 8) {
     const int row = (int)(item / fours), first = (int)(item - (long long)row * fours) * 4;
@@ -333,6 +355,68 @@ __global__ void __launch_bounds__(256) scaleResultsKernel(uint4* a, size_t na, u
   }
 }
 
+// What the entries of few rows' lists add to the weights' gradient (VocabExact), a block per entry: the first entry of a token adds up
+// g rest x over all entries of its token.  Groups of threads that share a row's packs take a part of the entries each, in their order.  On the
+// way, what keepRowsKernel does.  (Every entry is compared with every other: the limit keeps that, and a token that all of them share,
+// beside the gradient of the logits, which runs at the same time.)
+constexpr int FEW_ENTRIES = 4096, OWN_THREADS = 256, OWN_WARPS = OWN_THREADS / 32;
+__global__ void __launch_bounds__(OWN_THREADS) ownSumsKernel(const uint4* x, const VocabRows rows, int n, int packs, int lanes, const float* rest, const float* gout,
+                                                             int goutStride, float* sums, int* where, uint4* kept) {
+  __shared__ int list[FEW_ENTRIES];
+  __shared__ int counts[OWN_WARPS];
+  __shared__ float part[OWN_THREADS][9];
+  tc::grid_dependency_wait();
+  tc::grid_launch_dependents();
+  const int k = rows.k, entries = n * k, own = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (own % k == 0) {
+    const int row = own / k;
+    const bool keep = rowState(rows, row) != ROW_NONE;
+    for (int i = threadIdx.x; i < packs; i += OWN_THREADS) kept[(size_t)row * packs + i] = keep ? x[(size_t)row * packs + i] : make_uint4(0u, 0u, 0u, 0u);
+  }
+  auto tokenOf = [&](int e) { int t; if (rows.targets) rowState(rows, e, t); else t = rows.tokens[e]; return t; };
+  const int token = tokenOf(own);
+  if (token == VOCAB_NO_TOKEN) return;
+  int count = 0;
+  for (int base = 0; base < entries; base += OWN_THREADS) {
+    const int e = base + threadIdx.x;
+    const bool same = e < entries && tokenOf(e) == token;
+    if (__syncthreads_or(same && e < own)) return;       // not the first
+    const uint32_t votes = __ballot_sync(0xffffffffu, same);
+    if (lane == 0) counts[warp] = __popc(votes);
+    __syncthreads();
+    int at = count + __popc(votes & ((1u << lane) - 1));
+#pragma unroll
+    for (int w = 0; w < OWN_WARPS; ++w) { at += w < warp ? counts[w] : 0; count += counts[w]; }
+    if (same) list[at] = e;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) where[token] = own;
+  const int groups = OWN_THREADS / lanes, group = threadIdx.x / lanes, per = (count + groups - 1) / groups;
+  const int from = min(count, group * per), to = min(count, from + per);
+  for (int base = 0; base < packs; base += lanes) {
+    const int i = base + (threadIdx.x & (lanes - 1));
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (i < packs) {
+#pragma unroll 8
+      for (int m = from; m < to; ++m) {
+        const int e = list[m], row = e / k;
+        vocabMinus(f, -(rest[e] * (gout ? gout[(size_t)row * goutStride] : 1.f)), x[(size_t)row * packs + i]);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[threadIdx.x][e] = f[e];
+    __syncthreads();
+    if (group == 0 && i < packs) {
+      for (int g = 1; g < groups; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] += part[g * lanes + threadIdx.x][e];
+      float4* out = (float4*)sums + ((size_t)own * packs + i) * 2;
+      out[0] = make_float4(f[0], f[1], f[2], f[3]); out[1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
+  }
+}
+
 // x with zeros in the rows without a list: in the product of the weights' gradient they meet the zeros of the logits' gradient, and nothing
 // that x holds there (infinities, NaN) may come through.  n d 4 bytes: 8192 x 1024 takes 6 us beside 2300.
 __global__ void __launch_bounds__(256) keepRowsKernel(const uint4* x, const VocabRows rows, int n, int packs, uint4* out) {
@@ -361,12 +445,10 @@ __global__ void __launch_bounds__(256) joinSlicesKernel(const float* part, int s
     if (which) {
       const int row = (int)(i / rowPacks), c = (int)(i - (size_t)row * rowPacks);
       if (which == 1) {
-        int token;
-        const int st = rowState(exact.rows, row, token);
-        vocabExactX(f, st, exact.scale[row], (const uint4*)exact.w + (size_t)(st == ROW_LIST ? token : 0) * rowPacks + c);
-      } else {
-        const int at = exact.where[row];
-        if (at >= 0) vocabMinus(f, (const float4*)exact.sums + ((size_t)at * rowPacks + c) * 2);
+        vocabExactX<1>(f, exact, row, rowPacks * 8, c * 8, 1);
+      } else if (const float* sums = vocabSumsOf(exact, exact.first + row, rowPacks * 8)) {
+        const float4 p = ((const float4*)sums)[2 * c], q = ((const float4*)sums)[2 * c + 1];
+        f[0] -= p.x; f[1] -= p.y; f[2] -= p.z; f[3] -= p.w; f[4] -= q.x; f[5] -= q.y; f[6] -= q.z; f[7] -= q.w;
       }
     }
     ((uint4*)out)[i] = make_uint4(tc::pack_bf16x2(f[0] * scale, f[1] * scale), tc::pack_bf16x2(f[2] * scale, f[3] * scale), tc::pack_bf16x2(f[4] * scale, f[5] * scale),
@@ -389,10 +471,12 @@ struct BackwardPlan {
   VocabPlan cut;
   int slicesX, slicesW;           // of dx those of a whole piece: a shorter last one has fewer and adds to the first of them
   bool sumX, sumW;                // fp32 sums in memory: of dx because there are pieces or slices, of dw because there are slices
-  size_t dz, partX, partW, kept;  // bytes
-  size_t all() const { return dz + partX + partW + kept; }
+  int exact;                      // what the entries add to the results: 0 through dz, 1 by ownSumsKernel, 2 by sorted tokens
+  size_t dz, partX, partW, kept, sums, where, tokens;     // bytes
+  size_t all() const { return dz + partX + partW + kept + sums + where + tokens; }
 };
-BackwardPlan backwardPlan(int n, int v, int d, bool wantX, bool wantW) {
+// k = 0: targets.  Lists of more rows go through dz: their entries' roundings are many, and less than that of the results together.
+BackwardPlan backwardPlan(int n, int v, int d, int k, bool wantX, bool wantW) {
   BackwardPlan p;
   const int64_t limit = std::max<int64_t>(1 << 20, paramI64("LOSS_WORKSPACE_BYTES", 1ll << 30));
   const int64_t most = std::max<int64_t>(1, limit / (2ll * n) / VOCAB_TILE) * VOCAB_TILE;
@@ -407,6 +491,11 @@ BackwardPlan backwardPlan(int n, int v, int d, bool wantX, bool wantW) {
   p.partX = p.sumX ? up256((size_t)p.slicesX * n * d * 4) : 0;
   p.partW = p.sumW ? up256((size_t)p.slicesW * p.cols * d * 4) : 0;
   p.kept = wantW ? up256((size_t)n * d * 2) : 0;
+  const int64_t entries = (int64_t)n * std::max(1, k);
+  p.exact = entries <= FEW_ENTRIES ? 1 : k == 0 ? 2 : 0;
+  p.sums = p.exact && wantW ? up256((size_t)entries * d * 4) : 0;
+  p.where = p.exact && wantW ? up256((size_t)v * 4) : 0;
+  p.tokens = p.exact == 2 && wantW ? tokenSumsWork(n, d) : 0;
   return p;
 }
 
@@ -452,9 +541,9 @@ DF_API size_t dfcclLinearLossForwardWork(int n, int v, int k) {
 }
 
 DF_API ncclResult_t dfcclLinearLossForward(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, const void* tokens,
-                                           const void* weights, const void* state, int k, float temperature, int reduction, void* work, void* lse, void* rowLoss,
-                                           void* loss, void* count, cudaStream_t stream) {
-  if (!sizesOk(n, v, d, k) || !x || !w || !rowsOk(targets, tokens, weights, state, k, temperature) || !work || !lse || reduction < 0 || reduction > 2) return ncclInvalidArgument;
+                                           const void* weights, const void* state, int k, float temperature, int reduction, void* work, void* lse, void* rest,
+                                           void* rowLoss, void* loss, void* count, cudaStream_t stream) {
+  if (!sizesOk(n, v, d, k) || !x || !w || !rowsOk(targets, tokens, weights, state, k, temperature) || !work || !lse || !rest || reduction < 0 || reduction > 2) return ncclInvalidArgument;
   if ((((uintptr_t)x | (uintptr_t)w) & 15) || (reduction ? !loss || !count : !rowLoss)) return ncclInvalidArgument;
   const ForwardLayout l = forwardLayout(n, v, k);
   JoinArgs j = {};
@@ -466,13 +555,13 @@ DF_API ncclResult_t dfcclLinearLossForward(const void* x, const void* w, int n, 
   j.allLoss = losses; j.all = n; j.mean = reduction == 1;
   j.ticket = reduction ? (int*)((uint8_t*)work + l.parts + l.picked + l.loss) : nullptr;
   j.out = (float*)loss; j.count = (int*)count;
-  DFCHECK(pickLogits(PickArgs{(const uint4*)x, (const uint4*)w, j.allRows, n, d / 8, picked, nullptr, nullptr, nullptr, 0, j.ticket, j.ticket ? 1 : 0}, stream));
+  DFCHECK(pickLogits(PickArgs{(const uint4*)x, (const uint4*)w, j.allRows, n, d / 8, picked, nullptr, nullptr, j.ticket, j.ticket ? 1 : 0}, stream));
   for (int r = 0; r < n; r += ROWS) j.blocks += (std::min(ROWS, n - r) + 31) / 32;
   for (int r = 0; r < n; r += ROWS) {
     j.n = std::min(ROWS, n - r);
     j.picked = picked + (size_t)r * k;
     j.rows = rowsOf(targets, wide, v, ignore, tokens, weights, state, k, temperature, r);
-    j.lse = (float*)lse + r; j.loss = losses + r;
+    j.lse = (float*)lse + r; j.loss = losses + r; j.rest = (float*)rest + (size_t)r * k;
     // (the first beside pickLogitsKernel)
     DFCHECK(vocabStats((const __nv_bfloat16*)x + (size_t)r * d, w, j.n, v, d, j.rows, (float2*)j.parts, nullptr, r == 0, stream));
     CUDACHECK(launchBehind(joinRowsKernel<false>, (j.n + 31) / 32, 1024, stream, j));
@@ -480,36 +569,56 @@ DF_API ncclResult_t dfcclLinearLossForward(const void* x, const void* w, int n, 
   return ncclSuccess;
 }
 
-DF_API size_t dfcclLinearLossBackwardWork(int n, int v, int d, int wantX, int wantW) {
-  if (!sizesOk(n, v, d, 1) || !(wantX || wantW)) return 0;
-  const BackwardPlan p = backwardPlan(n, v, d, wantX != 0, wantW != 0);
+DF_API size_t dfcclLinearLossBackwardWork(int n, int v, int d, int k, int wantX, int wantW) {
+  if (!sizesOk(n, v, d, std::max(1, k)) || k < 0 || !(wantX || wantW)) return 0;
+  const BackwardPlan p = backwardPlan(n, v, d, k, wantX != 0, wantW != 0);
   return p.all();
 }
 
 DF_API ncclResult_t dfcclLinearLossBackward(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, const void* tokens,
-                                            const void* weights, const void* state, int k, float temperature, const void* lse, const void* gout, int goutStride,
-                                            const void* count, void* dx, void* dw, void* work, size_t workBytes, cudaStream_t stream) {
-  if (!sizesOk(n, v, d, k) || !x || !w || !rowsOk(targets, tokens, weights, state, k, temperature) || !lse || !gout || !work || !(dx || dw) || goutStride < 0) return ncclInvalidArgument;
+                                            const void* weights, const void* state, int k, float temperature, const void* lse, const void* rest,
+                                            const void* gout, int goutStride, const void* count, void* dx, void* dw, void* work, size_t workBytes, cudaStream_t stream) {
+  if (!sizesOk(n, v, d, k) || !x || !w || !rowsOk(targets, tokens, weights, state, k, temperature) || !lse || !rest || !gout || !work || !(dx || dw) || goutStride < 0) return ncclInvalidArgument;
   if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw) & 15) return ncclInvalidArgument;
-  const BackwardPlan p = backwardPlan(n, v, d, dx != nullptr, dw != nullptr);
+  const BackwardPlan p = backwardPlan(n, v, d, targets ? 0 : k, dx != nullptr, dw != nullptr);
   if (p.all() > workBytes) return ncclInvalidArgument;          // (the setting has changed since the size was asked for)
   void* dz = work;
   float* partX = p.sumX ? (float*)((uint8_t*)work + p.dz) : nullptr;
   float* partW = p.sumW ? (float*)((uint8_t*)work + p.dz + p.partX) : nullptr;
-  void* kept = (uint8_t*)work + p.dz + p.partX + p.partW;
+  uint8_t* at = (uint8_t*)work + p.dz + p.partX + p.partW;
+  void* kept = at;
+  float* sums = (float*)(at + p.kept);
+  int* where = (int*)(at + p.kept + p.sums);
+  void* sorted = at + p.kept + p.sums + p.where;
   const VocabRows rows = rowsOf(targets, wide, v, ignore, tokens, weights, state, k, temperature, 0);
-  if (dw) CUDACHECK(launchBehind(keepRowsKernel, std::min(n, 148 * 8), 256, stream, (const uint4*)x, rows, n, d / 8, (uint4*)kept));
-  const VocabGrad grad{(const float*)lse, goutStride ? (const float*)gout : nullptr, goutStride};
+  const float* rowGout = goutStride ? (const float*)gout : nullptr;
+  if (dw && p.exact == 1) {
+    int lanes = 8;
+    while (lanes < OWN_THREADS && lanes < d / 8) lanes *= 2;
+    CUDACHECK(launchBehind(ownSumsKernel, n * k, OWN_THREADS, stream, (const uint4*)x, rows, n, d / 8, lanes, (const float*)rest, rowGout, goutStride, sums, where,
+                           (uint4*)kept));
+  } else if (dw) {
+    if (p.exact) {
+      DFCHECK(tokenSort(n, d, targets, wide, ignore, v, sorted, stream));
+      DFCHECK(tokenSums(x, n, d, v, (const float*)rest, rowGout, goutStride, sums, where, sorted, stream));
+    }
+    CUDACHECK(launchBehind(keepRowsKernel, std::min(n, 148 * 8), 256, stream, (const uint4*)x, rows, n, d / 8, (uint4*)kept));
+  }
+  const VocabGrad grad{(const float*)lse, rowGout, goutStride, p.exact ? nullptr : (const float*)rest};
+  VocabExact exact{rows, nullptr, (const float*)rest, rowGout, goutStride, (const __nv_bfloat16*)w, sums, where,
+                   p.exact == 2 && dw ? tokenSortItems(n, d, v, sorted) : nullptr, p.exact == 1 ? n * k : n, 0};
+  const VocabExact* add = p.exact ? &exact : nullptr;
   const VocabFactor factor{goutStride ? nullptr : (const float*)gout, (const int*)count, temperature};
   for (int c = 0; c < v; c += p.cols) {
     const int cols = std::min(p.cols, v - c);
     const __nv_bfloat16* wc = (const __nv_bfloat16*)w + (size_t)c * d;
     __nv_bfloat16* dwc = dw ? (__nv_bfloat16*)dw + (size_t)c * d : nullptr;
-    DFCHECK(vocabGrad(x, wc, n, cols, c, d, rows, grad, dz, dw && c == 0, stream));      // (beside keepRowsKernel)
-    DFCHECK(vocabProducts(dz, kept, wc, n, cols, d, p.cut, factor, nullptr, VocabResult{p.sumX ? nullptr : dx, partX, c != 0}, VocabResult{p.sumW ? nullptr : dwc, partW, false}, stream));
-    if (p.sumW) DFCHECK(joinSlices(partW, p.slicesW, cols, d, factor, nullptr, 0, dwc, stream));
+    DFCHECK(vocabGrad(x, wc, n, cols, c, d, rows, grad, dz, dw && c == 0, stream));      // (beside the launch in front)
+    exact.first = c;
+    DFCHECK(vocabProducts(dz, kept, wc, n, cols, d, p.cut, factor, add, VocabResult{p.sumX ? nullptr : dx, partX, c != 0}, VocabResult{p.sumW ? nullptr : dwc, partW, false}, stream));
+    if (p.sumW) DFCHECK(joinSlices(partW, p.slicesW, cols, d, factor, add, 2, dwc, stream));
   }
-  if (p.sumX) DFCHECK(joinSlices(partX, p.slicesX, n, d, factor, nullptr, 0, dx, stream));
+  if (p.sumX) DFCHECK(joinSlices(partX, p.slicesX, n, d, factor, add, 1, dx, stream));
   return ncclSuccess;
 }
 
@@ -554,12 +663,13 @@ DF_API size_t dfcclCrossEntropyWithGradientsWork(int n, int v, int d, int wantX,
 }
 
 // Per piece of rows: powers of the logits relative to the targets' (vocabPowers), their sums, x times the rows' shares, the two products.  What the
-// targets themselves add to the gradients is most of their size and does not go through bf16 (VocabExact).  Rows with a power that is too
+// targets themselves add to the gradients does not go through bf16 (VocabExact).  Rows with a power that is too
 // large send their piece through statistics and powers once more, with the logarithms of the sums as bases: launches that find nothing
 // to do otherwise (2 us each).
 DF_API ncclResult_t dfcclCrossEntropyWithGradients(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, int reduction,
-                                                   void* work, size_t workBytes, void* lse, void* loss, void* count, void* dx, void* dw, cudaStream_t stream) {
-  if (!sizesOk(n, v, d, 1) || !x || !w || !targets || !work || !lse || !loss || !count || !(dx || dw) || reduction < 1 || reduction > 2) return ncclInvalidArgument;
+                                                   void* work, size_t workBytes, void* lse, void* rest, void* loss, void* count, void* dx, void* dw,
+                                                   cudaStream_t stream) {
+  if (!sizesOk(n, v, d, 1) || !x || !w || !targets || !work || !lse || !rest || !loss || !count || !(dx || dw) || reduction < 1 || reduction > 2) return ncclInvalidArgument;
   if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw) & 15) return ncclInvalidArgument;
   const OneGoPlan p = oneGoPlan(n, v, d, dx != nullptr, dw != nullptr);
   if (p.bytes > workBytes) return ncclInvalidArgument;           // (the setting has changed since the size was asked for)
@@ -573,8 +683,8 @@ DF_API ncclResult_t dfcclCrossEntropyWithGradients(const void* x, const void* w,
   const VocabRows all = rowsOf(targets, wide, v, ignore, nullptr, nullptr, nullptr, 1, 1.f, 0);
   const int pieces = (n + p.rows - 1) / p.rows, packs = d / 8;
   float* picked = (float*)(at + p.picked);
-  DFCHECK(pickLogits(PickArgs{(const uint4*)x, (const uint4*)w, all, n, packs, picked, base, (int*)count, dw ? where : nullptr, v, words, pieces + 1}, stream));
-  if (dw) DFCHECK(tokenSums(x, n, d, targets, wide, ignore, v, (float*)(at + p.sums), where, at + p.tokens, stream));
+  DFCHECK(pickLogits(PickArgs{(const uint4*)x, (const uint4*)w, all, n, packs, picked, base, (int*)count, words, pieces + 1}, stream));
+  if (dw) DFCHECK(tokenSort(n, d, targets, wide, ignore, v, at + p.tokens, stream));
   const VocabFactor factor{nullptr, reduction == 1 ? (const int*)count : nullptr, 1.f};
   JoinArgs j = {};
   j.parts = parts; j.stretches = vocabParts(v); j.t2 = 1.f;
@@ -585,7 +695,7 @@ DF_API ncclResult_t dfcclCrossEntropyWithGradients(const void* x, const void* w,
     const int r = i * p.rows, m = std::min(p.rows, n - r);
     const __nv_bfloat16* xr = (const __nv_bfloat16*)x + (size_t)r * d;
     j.rows = rowsOf(targets, wide, v, ignore, nullptr, nullptr, nullptr, 1, 1.f, r);
-    j.n = m; j.lse = (float*)lse + r; j.loss = losses + r; j.base = base + r; j.share = share + r; j.picked = picked + r;
+    j.n = m; j.lse = (float*)lse + r; j.loss = losses + r; j.base = base + r; j.share = share + r; j.picked = picked + r; j.rest = (float*)rest + r;
     j.x = (const uint4*)xr; j.shared = dw ? (uint4*)(at + p.shared) : nullptr; j.packs = packs;
     DFCHECK(vocabPowers(xr, w, m, v, d, j.rows, base + r, parts, powers, nullptr, stream));
     j.again = words + 1 + i; j.only = nullptr; j.ticket = nullptr;
@@ -594,7 +704,9 @@ DF_API ncclResult_t dfcclCrossEntropyWithGradients(const void* x, const void* w,
     j.only = j.again; j.ticket = words;
     CUDACHECK(launchBehind(joinRowsKernel<false>, (m + 31) / 32, 1024, stream, j));
     DFCHECK(vocabPowers(xr, w, m, v, d, j.rows, base + r, parts, powers, j.again, stream));
-    const VocabExact exact{j.rows, share + r, (const __nv_bfloat16*)w, (const float*)(at + p.sums), where};
+    if (dw && i == pieces - 1) DFCHECK(tokenSums(x, n, d, v, (const float*)rest, nullptr, 0, (float*)(at + p.sums), where, at + p.tokens, stream));
+    const VocabExact exact{j.rows, share + r, (const float*)rest + r, nullptr, 0, (const __nv_bfloat16*)w, (const float*)(at + p.sums), where,
+                           dw ? tokenSortItems(n, d, v, at + p.tokens) : nullptr, n, 0};
     __nv_bfloat16* dxr = dx ? (__nv_bfloat16*)dx + (size_t)r * d : nullptr;
     // (a shorter last piece has fewer slices of dw: it adds to the first of them)
     DFCHECK(vocabProducts(powers, at + p.shared, w, m, v, d, p.cut, factor, &exact, VocabResult{p.sumX ? nullptr : dxr, partX, false},

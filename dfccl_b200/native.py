@@ -195,10 +195,10 @@ def lib() -> C.CDLL:
             "dfcclEmbeddingForward": [vp, i, i, vp, i64, i64, vp, i, vp, i64, i64, vp, i, i, C.c_float, vp],
             "dfcclEmbeddingBackward": [vp, i, i, i, vp, i, i64, C.c_float, vp, i64, vp, i, vp, i64, vp, vp], "dfcclEmbeddingBackwardWork": [i, i, i],
             "dfcclTeacherRows": [vp, i, vp, i, i, i, i, C.c_float, vp, vp, vp, vp],
-            "dfcclLinearLossForward": [vp, vp, i, i, i, vp, i, i64, vp, vp, vp, i, C.c_float, i, vp, vp, vp, vp, vp, vp], "dfcclLinearLossForwardWork": [i, i, i],
-            "dfcclLinearLossBackward": [vp, vp, i, i, i, vp, i, i64, vp, vp, vp, i, C.c_float, vp, vp, i, vp, vp, vp, vp, sz, vp],
-            "dfcclCrossEntropyWithGradients": [vp, vp, i, i, i, vp, i, i64, i, vp, sz, vp, vp, vp, vp, vp, vp], "dfcclCrossEntropyWithGradientsWork": [i, i, i, i, i],
-            "dfcclScaleResults": [vp, sz, vp, sz, vp, vp], "dfcclLinearLossBackwardWork": [i, i, i, i, i], "dfcclLinearLossMaxList": [],
+            "dfcclLinearLossForward": [vp, vp, i, i, i, vp, i, i64, vp, vp, vp, i, C.c_float, i, vp, vp, vp, vp, vp, vp, vp], "dfcclLinearLossForwardWork": [i, i, i],
+            "dfcclLinearLossBackward": [vp, vp, i, i, i, vp, i, i64, vp, vp, vp, i, C.c_float, vp, vp, vp, i, vp, vp, vp, vp, sz, vp],
+            "dfcclCrossEntropyWithGradients": [vp, vp, i, i, i, vp, i, i64, i, vp, sz, vp, vp, vp, vp, vp, vp, vp], "dfcclCrossEntropyWithGradientsWork": [i, i, i, i, i],
+            "dfcclScaleResults": [vp, sz, vp, sz, vp, vp], "dfcclLinearLossBackwardWork": [i, i, i, i, i, i], "dfcclLinearLossMaxList": [],
             "dfcclGemmCheck": [C.POINTER(i)],
             "dfcclGemmPairResident": [C.POINTER(i)], "dfcclGemmPlan": [i, i, i, i, i, i, C.POINTER(i)],
             "dfcclGemmFused": [vp, vp, vp, i, i, i, vp, sz, vp],

@@ -71,14 +71,13 @@ def _forward(x, weight, rows, reduction):
     v, d = weight.shape
     n, device = x.numel() // d, x.device
     xp, wp = packed(x), packed(weight)
-    # log2 of the sums, the number of rows that count
-    kept = torch.empty(n + 1, dtype=torch.float32, device=device)
+    kept = torch.empty(n + 1 + n * rows.k, dtype=torch.float32, device=device)      # log2 of the sums, the number of rows that count, what is left of the weights
     loss = torch.empty(() if reduction else x.shape[:-1], dtype=torch.float32, device=device)
     if n:
         at, out = kept.data_ptr(), loss.data_ptr()
         with on_device(device):
             work = torch.empty(_forward_work(n, v, rows.k), dtype=torch.uint8, device=device)
-            nv.check(nv.long_entry("dfcclLinearLossForward")(xp.data_ptr(), wp.data_ptr(), n, v, d, *rows.args(), reduction, work.data_ptr(), at,
+            nv.check(nv.long_entry("dfcclLinearLossForward")(xp.data_ptr(), wp.data_ptr(), n, v, d, *rows.args(), reduction, work.data_ptr(), at, at + 4 * (n + 1),
                                                              None if reduction else out, out if reduction else None, at + 4 * n if reduction else None,
                                                              stream_of(x)), "dfcclLinearLossForward")
     elif reduction:
@@ -91,7 +90,7 @@ def _forward_with_gradients(x, weight, rows, reduction, want_x, want_w):
     v, d = weight.shape
     n, device = x.numel() // d, x.device
     xp, wp = packed(x), packed(weight)
-    kept = torch.empty(n + 1, dtype=torch.float32, device=device)
+    kept = torch.empty(2 * n + 1, dtype=torch.float32, device=device)
     loss = torch.empty((), dtype=torch.float32, device=device)
     dx = torch.empty(x.shape, dtype=x.dtype, device=device) if want_x else None
     dw = torch.empty(v, d, dtype=x.dtype, device=device) if want_w else None
@@ -100,7 +99,7 @@ def _forward_with_gradients(x, weight, rows, reduction, want_x, want_w):
         size = nv.lib().dfcclCrossEntropyWithGradientsWork(n, v, d, want_x, want_w)
         work = torch.empty(size, dtype=torch.uint8, device=device)
         nv.check(nv.long_entry("dfcclCrossEntropyWithGradients")(xp.data_ptr(), wp.data_ptr(), n, v, d, targets.data_ptr(), int(targets.dtype == torch.int64), rows.ignore,
-                                                                 reduction, work.data_ptr(), size, at, loss.data_ptr(), at + 4 * n,
+                                                                 reduction, work.data_ptr(), size, at, at + 4 * (n + 1), loss.data_ptr(), at + 4 * n,
                                                                  dx.data_ptr() if want_x else None, dw.data_ptr() if want_w else None, stream_of(x)),
                  "dfcclCrossEntropyWithGradients")
     return loss, xp, wp, kept, (dx, dw)
@@ -142,18 +141,19 @@ class _LinearLossFn(torch.autograd.Function):
         grads, ctx.grads = ctx.grads, None
         if grads is not None:
             return _scaled(grads, g)
-        (v, d), n, device = w.shape, kept.shape[0] - 1, x.device
+        (v, d), device = w.shape, x.device
+        n = x.numel() // d
         if n == 0:
             return torch.zeros_like(x) if want_x else None, torch.zeros_like(w) if want_w else None, None, None
         g = g.reshape(-1) if g.dim() else g
         dx = torch.empty(ctx.shape, dtype=x.dtype, device=device) if want_x else None
         dw = torch.empty(v, d, dtype=x.dtype, device=device) if want_w else None
         with on_device(device):
-            size = nv.lib().dfcclLinearLossBackwardWork(n, v, d, want_x, want_w)
+            size = nv.lib().dfcclLinearLossBackwardWork(n, v, d, 0 if ctx.rows.lists is None else ctx.rows.k, want_x, want_w)
             work = torch.empty(size, dtype=torch.uint8, device=device)
             at = kept.data_ptr()
-            nv.check(nv.long_entry("dfcclLinearLossBackward")(x.data_ptr(), w.data_ptr(), n, v, d, *ctx.rows.args(), at, g.data_ptr(), g.stride(0) if g.dim() else 0,
-                                                              at + 4 * n if ctx.mean else None, dx.data_ptr() if want_x else None,
+            nv.check(nv.long_entry("dfcclLinearLossBackward")(x.data_ptr(), w.data_ptr(), n, v, d, *ctx.rows.args(), at, at + 4 * (n + 1), g.data_ptr(),
+                                                              g.stride(0) if g.dim() else 0, at + 4 * n if ctx.mean else None, dx.data_ptr() if want_x else None,
                                                               dw.data_ptr() if want_w else None, work.data_ptr(), size, stream_of(x)), "dfcclLinearLossBackward")
         return dx, dw, None, None
 

@@ -77,8 +77,8 @@ def test_entries_refuse(native):
     """The C entry points answer with a status: no null pointers, no odd widths, no lists beyond the limit, no misaligned operands."""
     L, bad, p, q = native.lib(), native.INVALID_ARGUMENT, 4096, 4100
     assert L.dfcclLinearLossMaxList() == 256
-    ok = [p, p, 4, 9, 16, p, 1, -100, None, None, None, 1, 1.0, 0, p, p, p, None, None, None]
-    for at, value in ((0, None), (1, q), (2, 0), (3, 0), (4, 12), (5, None), (11, 0), (11, 2), (12, 0.0), (13, 3), (13, 1), (14, None), (15, None), (16, None)):
+    ok = [p, p, 4, 9, 16, p, 1, -100, None, None, None, 1, 1.0, 0, p, p, p, p, None, None, None]
+    for at, value in ((0, None), (1, q), (2, 0), (3, 0), (4, 12), (5, None), (11, 0), (11, 2), (12, 0.0), (13, 3), (13, 1), (14, None), (15, None), (16, None), (17, None)):
         args = list(ok)
         args[at] = value
         assert L.dfcclLinearLossForward(*args) == bad, (at, value)
@@ -87,15 +87,23 @@ def test_entries_refuse(native):
         args = list(lists)
         args[at] = value
         assert L.dfcclLinearLossForward(*args) == bad, (at, value)
-    ok = [p, p, 4, 9, 16, p, 1, -100, None, None, None, 1, 1.0, p, p, 0, None, p, p, p, 1 << 30, None]
-    for at, value in ((0, None), (1, q), (2, -1), (4, 4), (5, None), (11, 300), (12, -1.0), (13, None), (14, None), (15, -1), (17, q), (18, q), (19, None), (20, 16)):
+    ok = [p, p, 4, 9, 16, p, 1, -100, None, None, None, 1, 1.0, p, p, p, 0, None, p, p, p, 1 << 30, None]
+    for at, value in ((0, None), (1, q), (2, -1), (4, 4), (5, None), (11, 300), (12, -1.0), (13, None), (14, None), (15, None), (16, -1), (18, q), (19, q), (20, None), (21, 16)):
         args = list(ok)
         args[at] = value
         assert L.dfcclLinearLossBackward(*args) == bad, (at, value)
     args = list(ok)
-    args[17] = args[18] = None
+    args[18] = args[19] = None
     assert L.dfcclLinearLossBackward(*args) == bad
-    assert L.dfcclLinearLossForwardWork(4, 9, 0) == 0 and L.dfcclLinearLossBackwardWork(4, 9, 16, 0, 0) == 0
+    assert L.dfcclLinearLossForwardWork(4, 9, 0) == 0 and L.dfcclLinearLossBackwardWork(4, 9, 16, 0, 0, 0) == 0 and L.dfcclLinearLossBackwardWork(4, 9, 16, 257, 1, 1) == 0
+    ok = [p, p, 4, 9, 16, p, 1, -100, 1, p, 1 << 30, p, p, p, p, p, p, None]
+    for at, value in ((0, None), (1, q), (2, 0), (4, 12), (5, None), (8, 0), (8, 3), (9, None), (10, 16), (11, None), (12, None), (13, None), (14, None), (15, q), (16, q)):
+        args = list(ok)
+        args[at] = value
+        assert L.dfcclCrossEntropyWithGradients(*args) == bad, (at, value)
+    assert L.dfcclCrossEntropyWithGradientsWork(4, 9, 16, 0, 0) == 0 and L.dfcclCrossEntropyWithGradientsWork(4, 9, 16, 1, 0) > 0
+    for args in ((p, 12, None, 0, p, None), (q, 16, None, 0, p, None), (None, 16, None, 0, p, None), (None, 0, None, 0, p, None), (p, 16, p, 16, None, None)):
+        assert L.dfcclScaleResults(*args) == bad
     assert L.dfcclTeacherRows(p, native.INT32, p, 1, 4, 2, 9, 1.0, p, p, p, None) == bad and L.dfcclTeacherRows(p, native.FLOAT32, p, 1, 4, 257, 9, 1.0, p, p, p, None) == bad
     ok = [p, 1, 4, p, 9, 16, None, 0, None, 0, 0, p, 16, native.BFLOAT16, 1.0, None]
     for at, value in ((0, None), (2, 0), (3, None), (4, 0), (5, 8), (6, p), (11, None), (12, 0), (13, native.FLOAT64)):
@@ -108,7 +116,7 @@ def test_entries_refuse(native):
         args[at] = value
         assert L.dfcclEmbeddingBackward(*args) == bad, (at, value)
     assert L.dfcclEmbeddingBackwardWork(4, 16, 3) == 0 and L.dfcclEmbeddingBackwardWork(4, 16, 2) > 0
-    assert isinstance(L.dfcclLinearLossBackwardWork(1000, 50257, 1024, 1, 1), int) and C.sizeof(C.c_size_t) == 8
+    assert isinstance(L.dfcclLinearLossBackwardWork(1000, 50257, 1024, 0, 1, 1), int) and C.sizeof(C.c_size_t) == 8
 
 
 def test_long_entries(native):
