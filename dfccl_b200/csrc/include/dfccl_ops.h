@@ -91,13 +91,13 @@ ncclResult_t dfcclLinearLossBackward(const void* x, const void* w, int n, int v,
                                      const void* gout, int goutStride, const void* count, void* dx, void* dw, void* work, size_t workBytes, cudaStream_t stream);
 size_t dfcclLinearLossBackwardWork(int n, int v, int d, int k /* 0: targets */, int wantX, int wantW);
 int dfcclLinearLossMaxList(void);
-/* The cross entropy (reduction 1 or 2) and its gradients for a gradient of 1 in one go: the product of the logits is computed once instead of
+/* The loss (reduction 1 or 2) and its gradients for a gradient of 1 in one go: the product of the logits is computed once instead of
  * twice.  dx or dw may be null.  lse, rest, loss and count as above.  The powers of the logits exist for as many rows at a time as
  * DFCCL_LOSS_WORKSPACE_BYTES hold. */
-ncclResult_t dfcclCrossEntropyWithGradients(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, int reduction,
-                                            void* work, size_t workBytes, void* lse, void* rest, void* loss, void* count, void* dx, void* dw,
-                                            cudaStream_t stream);
-size_t dfcclCrossEntropyWithGradientsWork(int n, int v, int d, int wantX, int wantW);
+ncclResult_t dfcclLinearLossWithGradients(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, const void* tokens,
+                                          const void* weights, const void* state, int k, float temperature, int reduction, void* work, size_t workBytes,
+                                          void* lse, void* rest, void* loss, void* count, void* dx, void* dw, cudaStream_t stream);
+size_t dfcclLinearLossWithGradientsWork(int n, int v, int d, int k, int wantX, int wantW);
 /* Two bf16 arrays (na and nb elements, multiples of 8; either may be empty) times *scale (fp32), in place; left alone where it is 1. */
 ncclResult_t dfcclScaleResults(void* a, size_t na, void* b, size_t nb, const void* scale, cudaStream_t stream);
 

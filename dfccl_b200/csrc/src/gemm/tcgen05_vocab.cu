@@ -2,8 +2,8 @@
 // accumulators in tensor memory.  With z = x w^T, x [n, d] and the head w [v, d]:
 //   VOCAB_STATS     of every row the maximum and the sum of powers of each stretch of its logits, and the logits of its targets
 //   VOCAB_GRAD      dz = g (softmax(z) - target): the logits are computed again, what is stored is their gradient, rounded once
-//   VOCAB_POWERS    powers of the logits relative to a number known in front of the product (a target's logit), and their sums: the
-//                   logits are not computed again, for rows whose gradients are wanted with the loss
+//   VOCAB_POWERS    powers of the logits relative to a number known in front of the product (the largest logit of the row's list), and their
+//                   sums: the logits are not computed again, for rows whose gradients are wanted with the loss
 //   VOCAB_PRODUCTS  dx = dz w and dw = dz^T x, in one launch
 // A logit exists in tensor memory and registers only.
 //
@@ -295,12 +295,12 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
           __syncwarp();
           tmem_ld32(acc + i * 32, r);
           tmem_ld_wait();
-          if (MODE == VOCAB_STATS) {
+          if (MODE != VOCAB_GRAD) {
             if (c + 32 > p.N) {
 #pragma unroll
               for (int e = 0; e < 32; ++e) if (c + e >= p.N) r[e] = 0xff800000u;          // -inf
             }
-            while (list.next < c + 32) {
+            while (list.next < c + 32) {                 // the list's entries: no power
               if (list.next >= c) {
                 const int at = list.next - c;
 #pragma unroll
@@ -308,6 +308,8 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
               }
               list.step();
             }
+          }
+          if (MODE == VOCAB_STATS) {
             // running maximum and sum over the row's columns
             float m0 = __uint_as_float(r[0]), m1 = __uint_as_float(r[1]);
 #pragma unroll
@@ -319,15 +321,6 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
             sum = (s[0] + s[1]) + (s[2] + s[3]);
             top = now;
           } else if (MODE == VOCAB_POWERS) {
-            if (c + 32 > p.N) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) if (c + e >= p.N) r[e] = 0xff800000u;          // -inf
-            }
-            const int own = list.next - c;               // the target: no power
-            if (own >= 0 && own < 32) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) if (e == own) r[e] = 0xff800000u;
-            }
             float m0 = __uint_as_float(r[0]), m1 = __uint_as_float(r[1]);
 #pragma unroll
             for (int e = 2; e < 32; e += 2) { m0 = fmaxf(m0, __uint_as_float(r[e])); m1 = fmaxf(m1, __uint_as_float(r[e + 1])); }

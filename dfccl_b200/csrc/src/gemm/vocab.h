@@ -46,8 +46,8 @@ inline int vocabParts(int v) { return (v + VOCAB_TILE - 1) / VOCAB_TILE; }
 // has ended; the two run side by side.
 ncclResult_t vocabStats(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, float2* parts, const int* only, bool early, cudaStream_t stream);
 
-// powers = 2^(z scale - base) of every row with a target, 0 elsewhere: bf16, [n][ld], ld = v rounded up to 64 (zeros behind v).  Of each stretch
-// of a row's columns, without its target: {largest exponent, sum of the powers in fp32} -> parts [stretch][n].
+// powers = 2^(z scale - base) of every row with a list, 0 in the places of its entries and elsewhere: bf16, [n][ld], ld = v rounded up to 64 (zeros
+// behind v).  Of each stretch of a row's columns, without the list's: {largest exponent, sum of the powers in fp32} -> parts [stretch][n].
 ncclResult_t vocabPowers(const void* x, const void* w, int n, int v, int d, const VocabRows& rows, const float* base, float2* parts, void* powers, const int* only,
                          cudaStream_t stream);
 
@@ -99,6 +99,7 @@ struct VocabExact {
   const uint2* items;           // it counts where items[that].x is the token, or where, with items null, the rows' entry of that number is
   int entries;                  // of items or of the rows
   int first;                    // token of dw's first row
+  bool dense;                   // sums has a row for every token, at its number
 };
 
 // dx [n, d] = factor dz w and dw [v, d] = factor dz^T x in one launch.  A result is bf16 where `out` is given; otherwise `part` gets an fp32
@@ -121,7 +122,7 @@ __device__ __forceinline__ const float* vocabSumsOf(const VocabExact& x, int tok
   if (x.items) own = (int)x.items[at].x;
   else if (x.rows.targets) rowState(x.rows, at, own);
   else own = x.rows.tokens[at];
-  return own == token ? x.sums + (size_t)at * d : nullptr;
+  return own == token ? x.sums + (size_t)(x.dense ? token : at) * d : nullptr;
 }
 __device__ __forceinline__ void vocabMinus(float* f, float weight, const uint4& w) {
   const uint32_t p[4] = {w.x, w.y, w.z, w.w};

@@ -168,9 +168,10 @@ struct Table {
   // sums by themselves instead of a gradient: fp32 rows [n][d], used where `where` [rows] says
   float* compact;
   int* where;
-  const float* weights;           // [n] of the tokens there, times gout[n] where given
+  const float* weights;           // [n] of the tokens there, times gout of their row of g where given
   const float* gout;
-  int goutStride;
+  int goutStride, perRow;         // tokens that share a row of g
+  bool dense;                     // sums at the number of their token
 };
 struct Backward {
   Table t[MAX_TABLES];
@@ -306,7 +307,7 @@ __device__ __forceinline__ void storeRow(const Table& t, uint32_t row, int at, i
     Pack<float, E> o;
 #pragma unroll
     for (int e = 0; e < E; ++e) o.v[e] = acc[e];
-    *(Pack<float, E>*)(t.compact + (size_t)at * d + col) = o;
+    *(Pack<float, E>*)(t.compact + (size_t)(t.dense ? (int)row : at) * d + col) = o;
     if (col == 0) t.where[row] = at;
   } else {
     Pack<T, E> o;
@@ -332,8 +333,8 @@ __global__ void __launch_bounds__(128) sumStretchKernel(const Backward a) {
     const uint2 item = at >= 0 && at < a.n ? __ldcg(&items[at]) : make_uint2(0xffffffffu, 0u);
     keys[i + 1] = item.x;
     if (i >= 0 && i < count) {
-      tokens[i] = item.y;
-      if (COMPACT) weights[i] = item.x < (uint32_t)t.rows ? t.weights[item.y] * (t.gout ? t.gout[(size_t)item.y * t.goutStride] : 1.f) : 0.f;
+      tokens[i] = COMPACT ? item.y / t.perRow : item.y;
+      if (COMPACT) weights[i] = item.x < (uint32_t)t.rows ? t.weights[item.y] * (t.gout ? t.gout[(size_t)tokens[i] * t.goutStride] : 1.f) : 0.f;
     }
   }
   __syncthreads();
@@ -513,11 +514,13 @@ ncclResult_t tokenSort(int n, int d, const void* ids, int wide, int64_t ignore, 
   CUDACHECK(launchBehind(sortTokensKernel, dim3(SORT_CTAS), SORT_THREADS, SORT_CTAS, stream, sumsOf(n, d, ids, wide, ignore, v, work)));
   return ncclSuccess;
 }
-ncclResult_t tokenSums(const void* x, int n, int d, int v, const float* weights, const float* gout, int goutStride, float* sums, int* where, void* work, cudaStream_t stream) {
+ncclResult_t tokenSums(const void* x, int n, int d, int perRow, int v, const float* weights, const float* gout, int goutStride, float* sums, bool dense, int* where,
+                       void* work, cudaStream_t stream) {
   if (d % 8) return ncclInvalidArgument;
   Backward a = sumsOf(n, d, nullptr, 0, 0, v, work);
   a.g = x;
   a.t[0].compact = sums; a.t[0].where = where; a.t[0].weights = weights; a.t[0].gout = gout; a.t[0].goutStride = goutStride;
+  a.t[0].perRow = perRow; a.t[0].dense = dense;
   return backward<__nv_bfloat16, 8, true>(a, stream);
 }
 

@@ -184,61 +184,60 @@ __global__ void __launch_bounds__(1024) joinRowsKernel(const JoinArgs a) {
 #pragma unroll
       for (int o = 16; o; o >>= 1) acc = join(acc, make_float2(__shfl_xor_sync(0xffffffffu, acc.x, o), __shfl_xor_sync(0xffffffffu, acc.y, o)));
       const int st = rowState(a.rows, row);
-      float l, sum = 0.f, share = st == ROW_BAD ? __int_as_float(0x7fffffff) : 1.f;
+      float sum = 0.f, share = st == ROW_BAD ? __int_as_float(0x7fffffff) : 1.f;
+      const size_t list = (size_t)row * a.rows.k;
+      const float2 others = POWERS ? make_float2(a.base[row], acc.y) : acc;             // of entries that the list has not
+      float2 every = others;
+      int distinct = 0;
+      if (st == ROW_LIST) {                             // the list's own powers, each token once
+        float2 own = make_float2(-INFINITY, 0.f);
+        for (int i = lane; i < a.rows.k; i += 32) {
+          if (!a.rows.targets && (a.rows.tokens[list + i] == VOCAB_NO_TOKEN || (i && a.rows.tokens[list + i] == a.rows.tokens[list + i - 1]))) continue;
+          own = joined(own, make_float2(a.picked[list + i] * a.rows.scale, 1.f));
+          ++distinct;
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+          own = joined(own, make_float2(__shfl_xor_sync(0xffffffffu, own.x, o), __shfl_xor_sync(0xffffffffu, own.y, o)));
+          distinct += __shfl_xor_sync(0xffffffffu, distinct, o);
+        }
+        every = joined(others, own);
+      }
+      const float l = every.x + log2f(every.y);
+      if (distinct == 1) {                              // all on one token: from the others' powers, however small they are beside its own
+        const float u = a.picked[list] * a.rows.scale, ratio = others.y * exp2f(others.x - u);
+        for (int i = lane; i < a.rows.k; i += 32) {
+          const float q = a.rows.targets || a.rows.tokens[list + i] == VOCAB_NO_TOKEN ? 1.f : a.rows.weights[list + i];
+          if (q != 0.f) sum += q * logf(q);             // (of entries that share the token)
+          a.rest[list + i] = i ? 0.f : others.y * exp2f(others.x - l);
+        }
+        sum = warpSum(sum) + (ratio < 1e30f ? log1pf(ratio) : (l - u) * LN2);
+      } else {
+        for (int i = lane; i < a.rows.k; i += 32) {
+          float rest = 0.f;
+          if (st == ROW_LIST && a.rows.tokens[list + i] != VOCAB_NO_TOKEN) {
+            const int t = a.rows.tokens[list + i];
+            float q = a.rows.weights[list + i];
+            const float u = a.picked[list + i] * a.rows.scale - l;
+            if (q != 0.f) sum += q * (logf(q) - u * LN2);         // (0 ln 0)
+            if (i == 0 || a.rows.tokens[list + i - 1] != t) {
+              for (int j = i + 1; j < a.rows.k && a.rows.tokens[list + j] == t; ++j) q += a.rows.weights[list + j];
+              rest = q - exp2f(u);
+            }
+          }
+          a.rest[list + i] = rest;
+        }
+        sum = warpSum(sum);
+      }
       if (POWERS) {
-        l = a.base[row] + log2f(1.f + acc.y);           // the target's own power is 1
-        sum = log1pf(acc.y);
-        if (st == ROW_LIST) share = 1.f / (1.f + acc.y);
+        if (st == ROW_LIST) share = exp2f(others.x - l);
         if (lane == 0) {
           a.share[row] = st == ROW_NONE ? 0.f : share;
-          a.rest[row] = acc.y * share;
-          if (st == ROW_LIST && !(acc.x <= MOST_POWER && acc.y < INFINITY && fabsf(a.base[row]) < INFINITY)) *a.again = 1;
+          if (st == ROW_LIST && !(acc.x <= MOST_POWER && acc.y < INFINITY && fabsf(others.x) < INFINITY)) *a.again = 1;
         }
-      } else {
-        const size_t list = (size_t)row * a.rows.k;
-        const float2 others = acc;                      // (of entries that no list has)
-        int distinct = 0;
-        if (st == ROW_LIST) {                           // the list's own powers, each token once
-          float2 own = make_float2(-INFINITY, 0.f);
-          for (int i = lane; i < a.rows.k; i += 32) {
-            if (!a.rows.targets && (a.rows.tokens[list + i] == VOCAB_NO_TOKEN || (i && a.rows.tokens[list + i] == a.rows.tokens[list + i - 1]))) continue;
-            own = joined(own, make_float2(a.picked[list + i] * a.rows.scale, 1.f));
-            ++distinct;
-          }
-#pragma unroll
-          for (int o = 16; o; o >>= 1) {
-            own = joined(own, make_float2(__shfl_xor_sync(0xffffffffu, own.x, o), __shfl_xor_sync(0xffffffffu, own.y, o)));
-            distinct += __shfl_xor_sync(0xffffffffu, distinct, o);
-          }
-          acc = joined(acc, own);
-        }
-        l = acc.x + log2f(acc.y);
-        if (distinct == 1) {                            // all on one token: from the others' powers, however small they are beside its own
-          const float u = a.picked[list] * a.rows.scale, ratio = others.y * exp2f(others.x - u);
-          for (int i = lane; i < a.rows.k; i += 32) {
-            const float q = a.rows.targets || a.rows.tokens[list + i] == VOCAB_NO_TOKEN ? 1.f : a.rows.weights[list + i];
-            if (q != 0.f) sum += q * logf(q);           // (of entries that share the token)
-            a.rest[list + i] = i ? 0.f : others.y * exp2f(others.x - l);
-          }
-          sum = warpSum(sum) + (ratio < 1e30f ? log1pf(ratio) : (l - u) * LN2);
-        } else {
-          for (int i = lane; i < a.rows.k; i += 32) {
-            float rest = 0.f;
-            if (st == ROW_LIST && a.rows.tokens[list + i] != VOCAB_NO_TOKEN) {
-              const int t = a.rows.tokens[list + i];
-              float q = a.rows.weights[list + i];
-              const float u = a.picked[list + i] * a.rows.scale - l;
-              if (q != 0.f) sum += q * (logf(q) - u * LN2);       // (0 ln 0)
-              if (i == 0 || a.rows.tokens[list + i - 1] != t) {
-                for (int j = i + 1; j < a.rows.k && a.rows.tokens[list + j] == t; ++j) q += a.rows.weights[list + j];
-                rest = q - exp2f(u);
-              }
-            }
-            a.rest[list + i] = rest;
-          }
-          sum = warpSum(sum);
-        }
-        if (a.base && lane == 0) { a.base[row] = l; if (st == ROW_LIST) a.share[row] = 1.f; }
+      } else if (a.base && lane == 0) {
+        a.base[row] = l;
+        if (st == ROW_LIST) a.share[row] = 1.f;
       }
       // x times the row's share, rounded to bf16: the right operand of the powers' product.  A row without a target is zeros whatever it holds.
       if (a.shared)
@@ -267,8 +266,8 @@ __global__ void __launch_bounds__(1024) joinRowsKernel(const JoinArgs a) {
   reduceLoss(a.allLoss, a.allRows, a.all, a.mean, a.out, a.count);
 }
 
-// In front of the products: the logits of the rows' lists by fp32 sums, a warp for four entries of a row, -> picked [n][k] (and times `scale`, as
-// the bases of powers, where `base` is given; k = 1 there).  On the way, words set to their start and the number of rows that count.
+// In front of the products: the logits of the rows' lists by fp32 sums, a warp for four entries of a row, -> picked [n][k].  Where `base` is
+// given, a warp for a row, and the largest of its entries times `scale` is the base of its powers.  On the way, words set to their start and the number of rows that count.
 struct PickArgs {
   const uint4* x; const uint4* w;
   VocabRows rows;
@@ -295,48 +294,52 @@ __global__ void __launch_bounds__(256) pickLogitsKernel(const PickArgs a) {
     }
     for (int i = threadIdx.x; i < a.nWords; i += 256) a.words[i] = 0;
   }
-  const int k = a.rows.k, fours = (k + 3) / 4;
+  const int k = a.rows.k, fours = a.base ? 1 : (k + 3) / 4;
   for (long long item = (long long)blockIdx.x * 8 + warp; item < (long long)a.n * fours; item += (long long)gridDim.x * 8) {
-    const int row = (int)(item / fours), first = (int)(item - (long long)row * fours) * 4;
-    int token;
+    const int row = (int)(item / fours);
+    int first = (int)(item - (long long)row * fours) * 4, token;
+    const int end = a.base ? k : min(k, first + 4);
     const bool list = rowState(a.rows, row, token) == ROW_LIST;
-    const uint4* w[4];
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    bool some = false;
+    float most = -INFINITY;
+    bool odd = false;                                   // (a maximum passes over what is not a number)
+    for (; first < end; first += 4) {
+      const uint4* w[4];
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      bool some = false;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      int t = VOCAB_NO_TOKEN;
-      if (list) t = a.rows.targets ? e ? VOCAB_NO_TOKEN : token : first + e < k ? a.rows.tokens[(size_t)row * k + first + e] : VOCAB_NO_TOKEN;
-      w[e] = t == VOCAB_NO_TOKEN ? nullptr : a.w + (size_t)t * a.packs;
-      some = some || w[e];
-    }
-    if (some)
-      for (int i = lane; i < a.packs; i += 32) {
-        const uint4 x = a.x[(size_t)row * a.packs + i];
-        const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
-        uint4 y[4];
+      for (int e = 0; e < 4; ++e) {
+        int t = VOCAB_NO_TOKEN;
+        if (list) t = a.rows.targets ? e ? VOCAB_NO_TOKEN : token : first + e < k ? a.rows.tokens[(size_t)row * k + first + e] : VOCAB_NO_TOKEN;
+        w[e] = t == VOCAB_NO_TOKEN ? nullptr : a.w + (size_t)t * a.packs;
+        some = some || w[e];
+      }
+      if (some)
+        for (int i = lane; i < a.packs; i += 32) {
+          const uint4 x = a.x[(size_t)row * a.packs + i];
+          const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
+          uint4 y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = w[e] ? w[e][i] : make_uint4(0u, 0u, 0u, 0u);
+          for (int e = 0; e < 4; ++e) y[e] = w[e] ? w[e][i] : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t yw[4] = {y[e].x, y[e].y, y[e].z, y[e].w};
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t yw[4] = {y[e].x, y[e].y, y[e].z, y[e].w};
 #pragma unroll
-          for (int q = 0; q < 4; ++q) sum[e] = fmaf(bf16Lo(xw[q]), bf16Lo(yw[q]), fmaf(bf16Hi(xw[q]), bf16Hi(yw[q]), sum[e]));
+            for (int q = 0; q < 4; ++q) sum[e] = fmaf(bf16Lo(xw[q]), bf16Lo(yw[q]), fmaf(bf16Hi(xw[q]), bf16Hi(yw[q]), sum[e]));
+          }
         }
-      }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (first + e >= k) break;
-      const float z = warpSum(sum[e]);
-      if (lane == 0) {
-        a.picked[(size_t)row * k + first + e] = z;
-        if (a.base) a.base[row] = z * a.rows.scale;
+      for (int e = 0; e < 4; ++e) {
+        if (first + e >= k) break;
+        const float z = warpSum(sum[e]);
+        if (lane == 0) a.picked[(size_t)row * k + first + e] = z;
+        if (w[e]) { most = fmaxf(most, z); odd = odd || z != z; }
       }
     }
+    if (a.base && lane == 0) a.base[row] = !list ? 0.f : odd ? __int_as_float(0x7fffffff) : most * a.rows.scale;
   }
 }
 ncclResult_t pickLogits(const PickArgs& a, cudaStream_t stream) {
-  const long long items = (long long)a.n * ((a.rows.k + 3) / 4);
+  const long long items = (long long)a.n * (a.base ? 1 : (a.rows.k + 3) / 4);
   CUDACHECK(launchBehind(pickLogitsKernel, dim3((unsigned)std::min<long long>((items + 7) / 8, 148 * 8)), 256, stream, a));
   return ncclSuccess;
 }
@@ -600,13 +603,13 @@ DF_API ncclResult_t dfcclLinearLossBackward(const void* x, const void* w, int n,
   } else if (dw) {
     if (p.exact) {
       DFCHECK(tokenSort(n, d, targets, wide, ignore, v, sorted, stream));
-      DFCHECK(tokenSums(x, n, d, v, (const float*)rest, rowGout, goutStride, sums, where, sorted, stream));
+      DFCHECK(tokenSums(x, n, d, 1, v, (const float*)rest, rowGout, goutStride, sums, false, where, sorted, stream));
     }
     CUDACHECK(launchBehind(keepRowsKernel, std::min(n, 148 * 8), 256, stream, (const uint4*)x, rows, n, d / 8, (uint4*)kept));
   }
   const VocabGrad grad{(const float*)lse, rowGout, goutStride, p.exact ? nullptr : (const float*)rest};
   VocabExact exact{rows, nullptr, (const float*)rest, rowGout, goutStride, (const __nv_bfloat16*)w, sums, where,
-                   p.exact == 2 && dw ? tokenSortItems(n, d, v, sorted) : nullptr, p.exact == 1 ? n * k : n, 0};
+                   p.exact == 2 && dw ? tokenSortItems(n, d, v, sorted) : nullptr, p.exact == 1 ? n * k : n, 0, false};
   const VocabExact* add = p.exact ? &exact : nullptr;
   const VocabFactor factor{goutStride ? nullptr : (const float*)gout, (const int*)count, temperature};
   for (int c = 0; c < v; c += p.cols) {
@@ -628,10 +631,10 @@ struct OneGoPlan {
   int rows;                       // of a piece (all of them, or a multiple of the tile)
   VocabPlan cut;
   int slicesX, slicesW;
-  bool sumX, sumW;
+  bool sumX, sumW, dense;         // dense: of the entries' sums there is a row for every token of the vocabulary
   size_t powers, parts, partX, partW, shared, base, share, losses, words, where, sums, tokens, picked, bytes;
 };
-OneGoPlan oneGoPlan(int n, int v, int d, bool wantX, bool wantW) {
+OneGoPlan oneGoPlan(int n, int v, int d, int k, bool wantX, bool wantW) {
   OneGoPlan p = {};
   const size_t ld = (size_t)(v + 63) / 64 * 64;
   const int64_t limit = std::max<int64_t>(1 << 20, paramI64("LOSS_WORKSPACE_BYTES", 1ll << 30));
@@ -649,29 +652,30 @@ OneGoPlan oneGoPlan(int n, int v, int d, bool wantX, bool wantW) {
   p.partX = take(p.sumX ? (size_t)p.slicesX * p.rows * d * 4 : 0);
   p.partW = take(p.sumW ? (size_t)p.slicesW * v * d * 4 : 0);
   p.shared = take(wantW ? (size_t)p.rows * d * 2 : 0);
-  p.base = take((size_t)n * 4); p.share = take((size_t)n * 4); p.losses = take((size_t)n * 4); p.picked = take((size_t)n * 4);
+  p.base = take((size_t)n * 4); p.share = take((size_t)n * 4); p.losses = take((size_t)n * 4); p.picked = take((size_t)n * k * 4);
   p.words = take((size_t)(pieces + 1) * 4);
   p.where = take(wantW ? (size_t)v * 4 : 0);
-  p.sums = take(wantW ? (size_t)n * d * 4 : 0);
-  p.tokens = take(wantW ? tokenSumsWork(n, d) : 0);
+  p.dense = (int64_t)n * k > v;
+  p.sums = take(wantW ? (p.dense ? (size_t)v : (size_t)n * k) * d * 4 : 0);
+  p.tokens = take(wantW ? tokenSumsWork(n * k, d) : 0);
   return p;
 }
 }  // namespace
 
-DF_API size_t dfcclCrossEntropyWithGradientsWork(int n, int v, int d, int wantX, int wantW) {
-  return sizesOk(n, v, d, 1) && (wantX || wantW) ? oneGoPlan(n, v, d, wantX != 0, wantW != 0).bytes : 0;
+DF_API size_t dfcclLinearLossWithGradientsWork(int n, int v, int d, int k, int wantX, int wantW) {
+  return sizesOk(n, v, d, k) && (int64_t)n * k <= 0x7fffffff - 4096 && (wantX || wantW) ? oneGoPlan(n, v, d, k, wantX != 0, wantW != 0).bytes : 0;
 }
 
-// Per piece of rows: powers of the logits relative to the targets' (vocabPowers), their sums, x times the rows' shares, the two products.  What the
-// targets themselves add to the gradients does not go through bf16 (VocabExact).  Rows with a power that is too
+// Per piece of rows: powers of the logits relative to the largest of the row's list (vocabPowers), their sums, x times the rows' shares, the two
+// products.  What the lists themselves add to the gradients does not go through bf16 (VocabExact).  Rows with a power that is too
 // large send their piece through statistics and powers once more, with the logarithms of the sums as bases: launches that find nothing
 // to do otherwise (2 us each).
-DF_API ncclResult_t dfcclCrossEntropyWithGradients(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, int reduction,
-                                                   void* work, size_t workBytes, void* lse, void* rest, void* loss, void* count, void* dx, void* dw,
-                                                   cudaStream_t stream) {
-  if (!sizesOk(n, v, d, 1) || !x || !w || !targets || !work || !lse || !rest || !loss || !count || !(dx || dw) || reduction < 1 || reduction > 2) return ncclInvalidArgument;
+DF_API ncclResult_t dfcclLinearLossWithGradients(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, const void* tokens,
+                                                 const void* weights, const void* state, int k, float temperature, int reduction, void* work, size_t workBytes,
+                                                 void* lse, void* rest, void* loss, void* count, void* dx, void* dw, cudaStream_t stream) {
+  if (!sizesOk(n, v, d, k) || (int64_t)n * k > 0x7fffffff - 4096 || !x || !w || !rowsOk(targets, tokens, weights, state, k, temperature) || !work || !lse || !rest || !loss || !count || !(dx || dw) || reduction < 1 || reduction > 2) return ncclInvalidArgument;
   if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw) & 15) return ncclInvalidArgument;
-  const OneGoPlan p = oneGoPlan(n, v, d, dx != nullptr, dw != nullptr);
+  const OneGoPlan p = oneGoPlan(n, v, d, k, dx != nullptr, dw != nullptr);
   if (p.bytes > workBytes) return ncclInvalidArgument;           // (the setting has changed since the size was asked for)
   uint8_t* at = (uint8_t*)work;
   void* powers = at + p.powers;
@@ -680,22 +684,23 @@ DF_API ncclResult_t dfcclCrossEntropyWithGradients(const void* x, const void* w,
   float* partW = p.sumW ? (float*)(at + p.partW) : nullptr;
   float *base = (float*)(at + p.base), *share = (float*)(at + p.share), *losses = (float*)(at + p.losses);
   int *words = (int*)(at + p.words), *where = (int*)(at + p.where);
-  const VocabRows all = rowsOf(targets, wide, v, ignore, nullptr, nullptr, nullptr, 1, 1.f, 0);
+  const VocabRows all = rowsOf(targets, wide, v, ignore, tokens, weights, state, k, temperature, 0);
   const int pieces = (n + p.rows - 1) / p.rows, packs = d / 8;
   float* picked = (float*)(at + p.picked);
   DFCHECK(pickLogits(PickArgs{(const uint4*)x, (const uint4*)w, all, n, packs, picked, base, (int*)count, words, pieces + 1}, stream));
-  if (dw) DFCHECK(tokenSort(n, d, targets, wide, ignore, v, at + p.tokens, stream));
-  const VocabFactor factor{nullptr, reduction == 1 ? (const int*)count : nullptr, 1.f};
+  if (dw) DFCHECK(targets ? tokenSort(n, d, targets, wide, ignore, v, at + p.tokens, stream) : tokenSort(n * k, d, tokens, 0, -1, v, at + p.tokens, stream));
+  const VocabFactor factor{nullptr, reduction == 1 ? (const int*)count : nullptr, temperature};
   JoinArgs j = {};
-  j.parts = parts; j.stretches = vocabParts(v); j.t2 = 1.f;
+  j.parts = parts; j.stretches = vocabParts(v); j.t2 = temperature * temperature;
   j.allRows = all; j.allLoss = losses; j.all = n; j.mean = reduction == 1;
   j.out = (float*)loss; j.count = (int*)count;
   for (int r = 0; r < n; r += p.rows) j.blocks += (std::min(p.rows, n - r) + 31) / 32;
   for (int i = 0; i < pieces; ++i) {
     const int r = i * p.rows, m = std::min(p.rows, n - r);
     const __nv_bfloat16* xr = (const __nv_bfloat16*)x + (size_t)r * d;
-    j.rows = rowsOf(targets, wide, v, ignore, nullptr, nullptr, nullptr, 1, 1.f, r);
-    j.n = m; j.lse = (float*)lse + r; j.loss = losses + r; j.base = base + r; j.share = share + r; j.picked = picked + r; j.rest = (float*)rest + r;
+    j.rows = rowsOf(targets, wide, v, ignore, tokens, weights, state, k, temperature, r);
+    j.n = m; j.lse = (float*)lse + r; j.loss = losses + r; j.base = base + r; j.share = share + r;
+    j.picked = picked + (size_t)r * k; j.rest = (float*)rest + (size_t)r * k;
     j.x = (const uint4*)xr; j.shared = dw ? (uint4*)(at + p.shared) : nullptr; j.packs = packs;
     DFCHECK(vocabPowers(xr, w, m, v, d, j.rows, base + r, parts, powers, nullptr, stream));
     j.again = words + 1 + i; j.only = nullptr; j.ticket = nullptr;
@@ -704,9 +709,9 @@ DF_API ncclResult_t dfcclCrossEntropyWithGradients(const void* x, const void* w,
     j.only = j.again; j.ticket = words;
     CUDACHECK(launchBehind(joinRowsKernel<false>, (m + 31) / 32, 1024, stream, j));
     DFCHECK(vocabPowers(xr, w, m, v, d, j.rows, base + r, parts, powers, j.again, stream));
-    if (dw && i == pieces - 1) DFCHECK(tokenSums(x, n, d, v, (const float*)rest, nullptr, 0, (float*)(at + p.sums), where, at + p.tokens, stream));
-    const VocabExact exact{j.rows, share + r, (const float*)rest + r, nullptr, 0, (const __nv_bfloat16*)w, (const float*)(at + p.sums), where,
-                           dw ? tokenSortItems(n, d, v, at + p.tokens) : nullptr, n, 0};
+    if (dw && i == pieces - 1) DFCHECK(tokenSums(x, n * k, d, k, v, (const float*)rest, nullptr, 0, (float*)(at + p.sums), p.dense, where, at + p.tokens, stream));
+    const VocabExact exact{j.rows, share + r, (const float*)rest + (size_t)r * k, nullptr, 0, (const __nv_bfloat16*)w, (const float*)(at + p.sums), where,
+                           dw ? tokenSortItems(n * k, d, v, at + p.tokens) : nullptr, n * k, 0, p.dense};
     __nv_bfloat16* dxr = dx ? (__nv_bfloat16*)dx + (size_t)r * d : nullptr;
     // (a shorter last piece has fewer slices of dw: it adds to the first of them)
     DFCHECK(vocabProducts(powers, at + p.shared, w, m, v, d, p.cut, factor, &exact, VocabResult{p.sumX ? nullptr : dxr, partX, false},

@@ -13,8 +13,9 @@ from .block import packed
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 MAX_LIST = 256                       # entries of a teacher's list
-# Rows x vocabulary x width from which a reduced cross entropy makes its gradients with the loss.
+# Rows x vocabulary x width from which a reduced loss makes its gradients with the loss; lists of at most a share of the vocabulary.
 ONE_GO_FROM = 2 ** 35
+LIST_SHARE = 1024
 
 
 def linear_loss_supported(x: torch.Tensor, weight: torch.Tensor) -> bool:
@@ -90,18 +91,17 @@ def _forward_with_gradients(x, weight, rows, reduction, want_x, want_w):
     v, d = weight.shape
     n, device = x.numel() // d, x.device
     xp, wp = packed(x), packed(weight)
-    kept = torch.empty(2 * n + 1, dtype=torch.float32, device=device)
+    kept = torch.empty(n + 1 + n * rows.k, dtype=torch.float32, device=device)
     loss = torch.empty((), dtype=torch.float32, device=device)
     dx = torch.empty(x.shape, dtype=x.dtype, device=device) if want_x else None
     dw = torch.empty(v, d, dtype=x.dtype, device=device) if want_w else None
-    targets, at = rows.targets, kept.data_ptr()
+    at = kept.data_ptr()
     with on_device(device):
-        size = nv.lib().dfcclCrossEntropyWithGradientsWork(n, v, d, want_x, want_w)
+        size = nv.lib().dfcclLinearLossWithGradientsWork(n, v, d, rows.k, want_x, want_w)
         work = torch.empty(size, dtype=torch.uint8, device=device)
-        nv.check(nv.long_entry("dfcclCrossEntropyWithGradients")(xp.data_ptr(), wp.data_ptr(), n, v, d, targets.data_ptr(), int(targets.dtype == torch.int64), rows.ignore,
-                                                                 reduction, work.data_ptr(), size, at, at + 4 * (n + 1), loss.data_ptr(), at + 4 * n,
-                                                                 dx.data_ptr() if want_x else None, dw.data_ptr() if want_w else None, stream_of(x)),
-                 "dfcclCrossEntropyWithGradients")
+        nv.check(nv.long_entry("dfcclLinearLossWithGradients")(xp.data_ptr(), wp.data_ptr(), n, v, d, *rows.args(), reduction, work.data_ptr(), size, at, at + 4 * (n + 1),
+                                                               loss.data_ptr(), at + 4 * n, dx.data_ptr() if want_x else None,
+                                                               dw.data_ptr() if want_w else None, stream_of(x)), "dfcclLinearLossWithGradients")
     return loss, xp, wp, kept, (dx, dw)
 
 
@@ -115,14 +115,14 @@ def _scaled(grads, g):
 
 
 class _LinearLossFn(torch.autograd.Function):
-    """A reduced cross entropy of some size makes its gradients with the loss, which saves computing the logits a second time: the
-    first backward pass scales them.  Another pass over the same graph, and every other loss, computes the logits again."""
+    """A reduced loss of some size makes its gradients with the loss, which saves computing the logits a second time: the first
+    backward pass scales them.  Another pass over the same graph, and every other loss, computes the logits again."""
 
     @staticmethod
     def forward(ctx, x, weight, rows, reduction):
         want_x, want_w = ctx.needs_input_grad[:2]
         ctx.grads = None
-        if reduction and rows.lists is None and x.numel() * weight.shape[0] >= ONE_GO_FROM and (want_x or want_w):
+        if reduction and (want_x or want_w) and x.numel() * weight.shape[0] >= ONE_GO_FROM and (rows.lists is None or rows.k * LIST_SHARE <= weight.shape[0]):
             loss, xp, wp, kept, ctx.grads = _forward_with_gradients(x, weight, rows, reduction, want_x, want_w)
         else:
             loss, xp, wp, kept = _forward(x, weight, rows, reduction)

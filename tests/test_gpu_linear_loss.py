@@ -91,10 +91,16 @@ def test_cross_entropy(n, v, d):
     assert check_kernels()
 
 
+@pytest.mark.parametrize("form", ["two", "one go", "one go in pieces"])
 @pytest.mark.parametrize("n,v,d,k,temp", [(1, 1, 8, 1, 1.0), (1, 300, 16, 5, 2.0), (77, 1000, 64, 1, 0.5), (130, 515, 72, 32, 1.0), (257, 2049, 264, 33, 3.0),
                                           (300, 256, 128, 256, 2.0), (500, 5001, 320, 100, 1.5), (33, 50257, 64, 64, 1.0)])
-def test_distillation(n, v, d, k, temp):
+def test_distillation(n, v, d, k, temp, form, monkeypatch):
+    from dfccl_b200.ops import loss as module
     from dfccl_b200.ops.loss import linear_distillation
+    monkeypatch.setattr(module, "ONE_GO_FROM", 1 << 60 if form == "two" else 0)
+    monkeypatch.setattr(module, "LIST_SHARE", 0)
+    if form == "one go in pieces":
+        monkeypatch.setenv("DFCCL_LOSS_WORKSPACE_BYTES", str(1 << 20))
     x, w, gen = problem(n, v, d, n + 3 * v + 5 * d + k)
     tokens = torch.randint(0, v, (n, k), generator=gen, device="cuda")           # in any order, some twice
     logits = torch.randn(n, k, generator=gen, device="cuda") * 3
@@ -112,8 +118,10 @@ def test_distillation(n, v, d, k, temp):
     gout = torch.randn(n, generator=gen, device="cuda")
     check_gradients(torch.autograd.grad(rows, [x, w], gout), x.detach(), w.detach(), dz, gout.double(), temp)
     total = linear_distillation(x, w, logits.to(torch.float32), tokens.int(), temperature=temp)
+    mean = loss.sum().item() / max(1, int(valid.sum()))
+    assert abs(total.item() - mean) <= 2 * temp * logit_error(x.detach(), w.detach()).max().item() + 2 * LN * (temp * temp + loss.abs().max().item())
     got = torch.autograd.grad(total, [x, w])
-    check_gradients(got, x.detach(), w.detach(), dz, torch.ones(n, device="cuda").double() / max(1, int(valid.sum())), temp)
+    check_gradients(got, x.detach(), w.detach(), dz, torch.ones(n, device="cuda").double() / max(1, int(valid.sum())), temp, more=0.0 if form == "two" else 2.0 ** -8 * (1 + 2.0 ** -8))
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -213,6 +221,18 @@ def test_gradients_with_the_loss_of_odd_rows(monkeypatch):
         a.grad[hole] += 0                                # (zeros stay)
         check_gradients((a.grad, b.grad), x, w, dz, torch.ones(n, device="cuda").double(), 1.0, more=2.0 ** -8)
         assert bool((a.grad[hole] == 0).all())
+        # lists: the student nearly certain of an entry, or of none
+        lists = torch.stack([t, (t + 1) % v, t], dim=1)
+        teacher = torch.tensor([2.0, 1.0, 0.5], device="cuda").expand(n, 3)
+        q = torch.softmax(teacher.double(), dim=1) * (~hole).double()[:, None]
+        loss, dz = reference(x, w, lists, q, 1.0)
+        a, b = dirty.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        monkeypatch.setattr(module, "LIST_SHARE", 0)
+        value = module.linear_distillation(a, b, teacher, torch.where(hole[:, None], -1, lists), reduction="sum")
+        assert abs(value.item() - loss.sum().item()) <= n * 2 * logit_error(x, w).max().item() + 2 * LN * (n + loss.sum().item())
+        value.backward()
+        check_gradients((a.grad, b.grad), x, w, dz, torch.ones(n, device="cuda").double(), 1.0, more=2.0 ** -8)
+        assert bool((a.grad[hole] == 0).all())
     zero, b = dirty.clone().requires_grad_(True), w.clone().requires_grad_(True)
     value = module.linear_cross_entropy(zero, b, torch.full_like(t, -100))
     value.backward()
@@ -230,6 +250,32 @@ def test_gradients_with_the_loss_of_odd_rows(monkeypatch):
         odd = [module.linear_cross_entropy(ones.clone().requires_grad_(True), w2, torch.full_like(t, c), reduction="sum") for c in (k, 20)]
         for p, q in zip(plain, odd):
             assert torch.equal(p.isnan(), q.isnan()) and (p.isnan().item() or abs(p.item() - q.item()) <= 1e-5 * abs(p.item()) or p.item() == q.item())
+
+
+@pytest.mark.parametrize("one_go", [False, True])
+@pytest.mark.parametrize("n", [3, 5000])
+def test_gradients_of_nearly_certain_rows(n, one_go, monkeypatch):
+    """Rows whose target has all but 1e-4 of the probability: their gradients are that small, and as exact as any other."""
+    from dfccl_b200.ops import loss as module
+    monkeypatch.setattr(module, "ONE_GO_FROM", 0 if one_go else 1 << 60)
+    monkeypatch.setattr(module, "LIST_SHARE", 0)
+    v, d = 300, 64
+    gen = torch.Generator(device="cuda").manual_seed(61)
+    w = (torch.randn(v, d, generator=gen, device="cuda") * 0.05).to(torch.bfloat16)
+    t = torch.randint(0, v, (n,), generator=gen, device="cuda")
+    wt = w[t].float()
+    x = (torch.randn(n, d, generator=gen, device="cuda") * 0.2 + wt * (14.5 / wt.square().sum(dim=1, keepdim=True))).to(torch.bfloat16)
+    loss, dz = reference(x, w, t[:, None], torch.ones(n, 1, dtype=torch.float64, device="cuda"), 1.0)
+    assert 2e-6 < loss.median().item() < 1e-2
+    for call in (lambda a, b: module.linear_cross_entropy(a, b, t), lambda a, b: module.linear_distillation(a, b, torch.zeros(n, 1, device="cuda"), t[:, None])):
+        a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        value = call(a, b)
+        # logits of 15 and less, off by 2**-20: of the others' powers, and so of the loss and all gradients, that share
+        assert abs(value.item() - loss.mean().item()) <= 2.0 ** -18 * loss.mean().item()
+        ga, gb = torch.autograd.grad(value, [a, b])
+        for got, want in ((ga, dz @ w.double() / n), (gb, dz.t() @ x.double() / n)):
+            # a rounding of the result, and of x times a row's share beside the others' powers: below 2**-9 and 2**-8 in the 2-norm
+            assert (got.double() - want).norm().item() <= 2.0 ** -8 * 1.5 * want.norm().item()
 
 
 def test_small_losses_and_large_logits():
@@ -365,6 +411,7 @@ def test_other_stream_and_graphs(one_go, monkeypatch):
     from dfccl_b200.ops.gemm import check_kernels
     from dfccl_b200.ops.loss import linear_cross_entropy, linear_distillation
     monkeypatch.setattr(module, "ONE_GO_FROM", 0 if one_go else 1 << 60)
+    monkeypatch.setattr(module, "LIST_SHARE", 0)
     x, w, gen = problem(300, 3001, 128, 41)
     w.requires_grad_(True)
     xs = [torch.randn(300, 128, generator=gen, device="cuda").to(torch.bfloat16) for _ in range(3)]

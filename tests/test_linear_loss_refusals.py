@@ -96,12 +96,14 @@ def test_entries_refuse(native):
     args[18] = args[19] = None
     assert L.dfcclLinearLossBackward(*args) == bad
     assert L.dfcclLinearLossForwardWork(4, 9, 0) == 0 and L.dfcclLinearLossBackwardWork(4, 9, 16, 0, 0, 0) == 0 and L.dfcclLinearLossBackwardWork(4, 9, 16, 257, 1, 1) == 0
-    ok = [p, p, 4, 9, 16, p, 1, -100, 1, p, 1 << 30, p, p, p, p, p, p, None]
-    for at, value in ((0, None), (1, q), (2, 0), (4, 12), (5, None), (8, 0), (8, 3), (9, None), (10, 16), (11, None), (12, None), (13, None), (14, None), (15, q), (16, q)):
+    ok = [p, p, 4, 9, 16, p, 1, -100, None, None, None, 1, 1.0, 1, p, 1 << 30, p, p, p, p, p, p, None]
+    for at, value in ((0, None), (1, q), (2, 0), (4, 12), (5, None), (11, 2), (12, 0.0), (13, 0), (13, 3), (14, None), (15, 16), (16, None), (17, None), (18, None), (19, None),
+                      (20, q), (21, q)):
         args = list(ok)
         args[at] = value
-        assert L.dfcclCrossEntropyWithGradients(*args) == bad, (at, value)
-    assert L.dfcclCrossEntropyWithGradientsWork(4, 9, 16, 0, 0) == 0 and L.dfcclCrossEntropyWithGradientsWork(4, 9, 16, 1, 0) > 0
+        assert L.dfcclLinearLossWithGradients(*args) == bad, (at, value)
+    assert L.dfcclLinearLossWithGradientsWork(4, 9, 16, 1, 0, 0) == 0 and L.dfcclLinearLossWithGradientsWork(4, 9, 16, 1, 1, 0) > 0
+    assert L.dfcclLinearLossWithGradientsWork(2 ** 24, 9, 16, 256, 1, 1) == 0
     for args in ((p, 12, None, 0, p, None), (q, 16, None, 0, p, None), (None, 16, None, 0, p, None), (None, 0, None, 0, p, None), (p, 16, p, 16, None, None)):
         assert L.dfcclScaleResults(*args) == bad
     assert L.dfcclTeacherRows(p, native.INT32, p, 1, 4, 2, 9, 1.0, p, p, p, None) == bad and L.dfcclTeacherRows(p, native.FLOAT32, p, 1, 4, 257, 9, 1.0, p, p, p, None) == bad
