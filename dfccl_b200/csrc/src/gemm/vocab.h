@@ -100,6 +100,7 @@ struct VocabExact {
   int entries;                  // of items or of the rows
   int first;                    // token of dw's first row
   bool dense;                   // sums has a row for every token, at its number
+  const float* listed;          // [n][d] sum_k rest_nk w_token(n,k), or null: from w on the way
 };
 
 // dx [n, d] = factor dz w and dw [v, d] = factor dz^T x in one launch.  A result is bf16 where `out` is given; otherwise `part` gets an fp32
@@ -149,6 +150,17 @@ __device__ __forceinline__ void vocabExactX(float (&f)[8 * P], const VocabExact&
     for (int e = 0; e < 8 * P; ++e) f[e] *= s;
   }
   const float g = x.gout ? x.gout[(size_t)row * x.goutStride] : 1.f;
+  if (x.listed) {
+    const float4* src = (const float4*)(x.listed + (size_t)row * d + c);
+#pragma unroll
+    for (int v = 0; v < 2 * P; ++v) {
+      if (v / 2 >= packs) break;
+      const float4 q = src[v];
+      f[4 * v] = fmaf(-g, q.x, f[4 * v]); f[4 * v + 1] = fmaf(-g, q.y, f[4 * v + 1]);
+      f[4 * v + 2] = fmaf(-g, q.z, f[4 * v + 2]); f[4 * v + 3] = fmaf(-g, q.w, f[4 * v + 3]);
+    }
+    return;
+  }
   const size_t at = (size_t)row * x.rows.k;
   for (int i = 0; i < x.rows.k; i += 2) {
     const uint4* src[2];

@@ -276,10 +276,11 @@ struct PickArgs {
   float* base;
   int* count;                    // or null
   int* words; int nWords;        // to be 0
+  int beside;                    // the sort in front runs beside this kernel, which ends behind it
 };
 __global__ void __launch_bounds__(256) pickLogitsKernel(const PickArgs a) {
   __shared__ int counts[8];
-  tc::grid_dependency_wait();
+  if (!a.beside) tc::grid_dependency_wait();
   tc::grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (blockIdx.x == 0) {
@@ -337,11 +338,43 @@ __global__ void __launch_bounds__(256) pickLogitsKernel(const PickArgs a) {
     }
     if (a.base && lane == 0) a.base[row] = !list ? 0.f : odd ? __int_as_float(0x7fffffff) : most * a.rows.scale;
   }
+  // (one block waits for the sort, and with it the kernel: blocks that waited would keep those behind them from starting)
+  if (a.beside && blockIdx.x == gridDim.x - 1) tc::grid_dependency_wait();
 }
 ncclResult_t pickLogits(const PickArgs& a, cudaStream_t stream) {
   const long long items = (long long)a.n * (a.base ? 1 : (a.rows.k + 3) / 4);
   CUDACHECK(launchBehind(pickLogitsKernel, dim3((unsigned)std::min<long long>((items + 7) / 8, 148 * 8)), 256, stream, a));
   return ncclSuccess;
+}
+
+// The sum over each row's list of rest w: a block per row, a thread per pack of columns.  As many bytes of w from L2 as the list has rows, as in
+// pickLogitsKernel; 8192 lists of 32 and 1024 columns take TODO us, and 128 us within the product's own epilogue.
+__global__ void __launch_bounds__(128) listSumsKernel(const uint4* w, const VocabRows rows, const float* rest, int n, int packs, float4* out) {
+  __shared__ int tokens[MAX_LIST];
+  __shared__ float weights[MAX_LIST];
+  tc::grid_dependency_wait();
+  tc::grid_launch_dependents();
+  for (int row = blockIdx.x; row < n; row += gridDim.x) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows.k; i += 128) {
+      const int t = rows.tokens[(size_t)row * rows.k + i];
+      const float q = rest[(size_t)row * rows.k + i];
+      tokens[i] = t == VOCAB_NO_TOKEN ? 0 : t;
+      weights[i] = t == VOCAB_NO_TOKEN ? 0.f : q;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < packs; i += 128) {
+      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+      for (int k = 0; k < rows.k; ++k) {
+        const float q = weights[k];
+        const uint4 p = q != 0.f ? w[(size_t)tokens[k] * packs + i] : make_uint4(0u, 0u, 0u, 0u);
+        vocabMinus(f, -q, p);
+      }
+      float4* dst = out + ((size_t)row * packs + i) * 2;
+      dst[0] = make_float4(f[0], f[1], f[2], f[3]); dst[1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
+  }
 }
 
 // Two results times one number on the device, in place; nothing is read or written where it is 1.
@@ -558,7 +591,7 @@ DF_API ncclResult_t dfcclLinearLossForward(const void* x, const void* w, int n, 
   j.allLoss = losses; j.all = n; j.mean = reduction == 1;
   j.ticket = reduction ? (int*)((uint8_t*)work + l.parts + l.picked + l.loss) : nullptr;
   j.out = (float*)loss; j.count = (int*)count;
-  DFCHECK(pickLogits(PickArgs{(const uint4*)x, (const uint4*)w, j.allRows, n, d / 8, picked, nullptr, nullptr, j.ticket, j.ticket ? 1 : 0}, stream));
+  DFCHECK(pickLogits(PickArgs{(const uint4*)x, (const uint4*)w, j.allRows, n, d / 8, picked, nullptr, nullptr, j.ticket, j.ticket ? 1 : 0, 0}, stream));
   for (int r = 0; r < n; r += ROWS) j.blocks += (std::min(ROWS, n - r) + 31) / 32;
   for (int r = 0; r < n; r += ROWS) {
     j.n = std::min(ROWS, n - r);
@@ -609,7 +642,7 @@ DF_API ncclResult_t dfcclLinearLossBackward(const void* x, const void* w, int n,
   }
   const VocabGrad grad{(const float*)lse, rowGout, goutStride, p.exact ? nullptr : (const float*)rest};
   VocabExact exact{rows, nullptr, (const float*)rest, rowGout, goutStride, (const __nv_bfloat16*)w, sums, where,
-                   p.exact == 2 && dw ? tokenSortItems(n, d, v, sorted) : nullptr, p.exact == 1 ? n * k : n, 0, false};
+                   p.exact == 2 && dw ? tokenSortItems(n, d, v, sorted) : nullptr, p.exact == 1 ? n * k : n, 0, false, nullptr};
   const VocabExact* add = p.exact ? &exact : nullptr;
   const VocabFactor factor{goutStride ? nullptr : (const float*)gout, (const int*)count, temperature};
   for (int c = 0; c < v; c += p.cols) {
@@ -632,7 +665,7 @@ struct OneGoPlan {
   VocabPlan cut;
   int slicesX, slicesW;
   bool sumX, sumW, dense;         // dense: of the entries' sums there is a row for every token of the vocabulary
-  size_t powers, parts, partX, partW, shared, base, share, losses, words, where, sums, tokens, picked, bytes;
+  size_t listedBytes, listed, powers, parts, partX, partW, shared, base, share, losses, words, where, sums, tokens, picked, bytes;
 };
 OneGoPlan oneGoPlan(int n, int v, int d, int k, bool wantX, bool wantW) {
   OneGoPlan p = {};
@@ -658,6 +691,8 @@ OneGoPlan oneGoPlan(int n, int v, int d, int k, bool wantX, bool wantW) {
   p.dense = (int64_t)n * k > v;
   p.sums = take(wantW ? (p.dense ? (size_t)v : (size_t)n * k) * d * 4 : 0);
   p.tokens = take(wantW ? tokenSumsWork(n * k, d) : 0);
+  p.listedBytes = wantX && k > 4 ? (size_t)p.rows * d * 4 : 0;
+  p.listed = take(p.listedBytes);
   return p;
 }
 }  // namespace
@@ -687,8 +722,9 @@ DF_API ncclResult_t dfcclLinearLossWithGradients(const void* x, const void* w, i
   const VocabRows all = rowsOf(targets, wide, v, ignore, tokens, weights, state, k, temperature, 0);
   const int pieces = (n + p.rows - 1) / p.rows, packs = d / 8;
   float* picked = (float*)(at + p.picked);
-  DFCHECK(pickLogits(PickArgs{(const uint4*)x, (const uint4*)w, all, n, packs, picked, base, (int*)count, words, pieces + 1}, stream));
+  float* listed = p.listedBytes ? (float*)(at + p.listed) : nullptr;
   if (dw) DFCHECK(targets ? tokenSort(n, d, targets, wide, ignore, v, at + p.tokens, stream) : tokenSort(n * k, d, tokens, 0, -1, v, at + p.tokens, stream));
+  DFCHECK(pickLogits(PickArgs{(const uint4*)x, (const uint4*)w, all, n, packs, picked, base, (int*)count, words, pieces + 1, dw ? 1 : 0}, stream));
   const VocabFactor factor{nullptr, reduction == 1 ? (const int*)count : nullptr, temperature};
   JoinArgs j = {};
   j.parts = parts; j.stretches = vocabParts(v); j.t2 = temperature * temperature;
@@ -710,8 +746,9 @@ DF_API ncclResult_t dfcclLinearLossWithGradients(const void* x, const void* w, i
     CUDACHECK(launchBehind(joinRowsKernel<false>, (m + 31) / 32, 1024, stream, j));
     DFCHECK(vocabPowers(xr, w, m, v, d, j.rows, base + r, parts, powers, j.again, stream));
     if (dw && i == pieces - 1) DFCHECK(tokenSums(x, n * k, d, k, v, (const float*)rest, nullptr, 0, (float*)(at + p.sums), p.dense, where, at + p.tokens, stream));
+    if (listed) CUDACHECK(launchBehind(listSumsKernel, std::min(m, 148 * 16), 128, stream, (const uint4*)w, j.rows, (const float*)rest + (size_t)r * k, m, packs, (float4*)listed));
     const VocabExact exact{j.rows, share + r, (const float*)rest + (size_t)r * k, nullptr, 0, (const __nv_bfloat16*)w, (const float*)(at + p.sums), where,
-                           dw ? tokenSortItems(n * k, d, v, at + p.tokens) : nullptr, n * k, 0, p.dense};
+                           dw ? tokenSortItems(n * k, d, v, at + p.tokens) : nullptr, n * k, 0, p.dense, listed};
     __nv_bfloat16* dxr = dx ? (__nv_bfloat16*)dx + (size_t)r * d : nullptr;
     // (a shorter last piece has fewer slices of dw: it adds to the first of them)
     DFCHECK(vocabProducts(powers, at + p.shared, w, m, v, d, p.cut, factor, &exact, VocabResult{p.sumX ? nullptr : dxr, partX, false},
