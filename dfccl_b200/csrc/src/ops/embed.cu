@@ -1,13 +1,15 @@
 // Embedding of tokens: y = scale w[id] + p[position] per token, and the gradients of both tables by sorted tokens.
 // The reference has no counterpart (it is a collective library); the GPT-2 workload's first stage uses these.
 //
-// Forward: a gather, bound by memory (or by its launch, for few tokens): 16 bytes per thread and access where rows allow it.
+// Forward: a gather, bound by memory (or by its launch, for few tokens): 16 bytes per thread and access where rows allow it.  131072 tokens of
+// 1024 bf16 with positions: 60 us, 537 MB to and from L2 and 300 of DRAM; 8192: 6.7; one: 2.
 // Backward: dw[v] = scale sum over tokens with id v of g, in fp32, in the order of the tokens, rounded once.  Three launches:
 //   1. one cluster of eight blocks per table sorts (id, token) by id - a stable radix sort, eight bits a pass, whose counts meet in
-//      distributed shared memory - while the other blocks clear the gradients, which is what the time goes into: most rows of a
-//      large table have no token;
-//   2. the sorted tokens in stretches: rows whose tokens lie inside one are summed and stored, others leave one or two sums;
-//   3. those are added up, stretch by stretch.
+//      distributed shared memory - while another launch clears the gradients, which is what the time goes into: most rows of a
+//      large table have no token (50257 x 1024 bf16: 17 us; the sort of 8192 tokens 15, of 131072 49);
+//   2. the sorted tokens in stretches: rows whose tokens lie inside one are summed and stored, others leave one or two sums (8192 x 1024 and
+//      positions: 9 us; 131072: 90, 600 MB at 6.7 TB/s: g is read once per table);
+//   3. those are added up, stretch by stretch (8 us; 16).
 // No result is added to by atomics, so a call repeats itself bit by bit.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>

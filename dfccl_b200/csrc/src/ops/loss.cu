@@ -348,7 +348,7 @@ ncclResult_t pickLogits(const PickArgs& a, cudaStream_t stream) {
 }
 
 // The sum over each row's list of rest w: a block per row, a thread per pack of columns.  As many bytes of w from L2 as the list has rows, as in
-// pickLogitsKernel; 8192 lists of 32 and 1024 columns take TODO us, and 128 us within the product's own epilogue.
+// pickLogitsKernel; 8192 lists of 32 and 1024 columns take 55 us; on the way, in the product's epilogue, 128.
 __global__ void __launch_bounds__(128) listSumsKernel(const uint4* w, const VocabRows rows, const float* rest, int n, int packs, float4* out) {
   __shared__ int tokens[MAX_LIST];
   __shared__ float weights[MAX_LIST];

@@ -13,8 +13,12 @@ from .block import packed
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 MAX_LIST = 256                       # entries of a teacher's list
-# Rows x vocabulary x width from which a reduced loss makes its gradients with the loss; lists of at most a share of the vocabulary.
-ONE_GO_FROM = 2 ** 35
+# Rows x vocabulary x width from which a reduced loss makes its gradients with the loss, and how many times that for lists, of at most a share
+# of the vocabulary.  GPU time in us, logits computed twice / once, 50257 entries: targets 256 x 768 144 / 146, 512 x 768 174 / 168, 1024 x 768 258 / 221,
+# 2048 x 1024 587 / 461; lists of 8 1024 x 768 248 / 250, 2048 x 768 444 / 390, of 32 1024 x 768 262 / 322, 2048 x 768 483 / 457, of 48 4096 x 1024 1216 / 1130,
+# of 256 1814 / 1919 (the sorting of the entries); 16384 x 2000 x 1024 278 / 237.
+ONE_GO_FROM = 2 ** 34
+LISTS_TIMES = 4
 LIST_SHARE = 1024
 
 
@@ -122,7 +126,8 @@ class _LinearLossFn(torch.autograd.Function):
     def forward(ctx, x, weight, rows, reduction):
         want_x, want_w = ctx.needs_input_grad[:2]
         ctx.grads = None
-        if reduction and (want_x or want_w) and x.numel() * weight.shape[0] >= ONE_GO_FROM and (rows.lists is None or rows.k * LIST_SHARE <= weight.shape[0]):
+        from_size = ONE_GO_FROM if rows.lists is None else ONE_GO_FROM * LISTS_TIMES
+        if reduction and (want_x or want_w) and x.numel() * weight.shape[0] >= from_size and (rows.lists is None or rows.k * LIST_SHARE <= weight.shape[0]):
             loss, xp, wp, kept, ctx.grads = _forward_with_gradients(x, weight, rows, reduction, want_x, want_w)
         else:
             loss, xp, wp, kept = _forward(x, weight, rows, reduction)
@@ -169,9 +174,10 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
 
     ``x`` [..., d] and ``weight`` [vocabulary, d] are bf16, d a multiple of 8; ``targets`` [...] int64 or int32.  Rows of target
     ``ignore_index`` have no loss and give no gradient, whatever ``x`` holds there; ``"mean"`` is over the other rows, and 0 where
-    there is none.  Logits and sums are fp32; the gradient of a logit is rounded once, to bf16, on its way into the products that
-    make the gradients of ``x`` and ``weight``.  It exists for as many columns at a time as ``DFCCL_LOSS_WORKSPACE_BYTES`` (1 GiB)
-    hold.  There is no check of the targets' values on the host: one outside the vocabulary makes its row's loss and gradients NaN."""
+    there is none.  Logits and sums are fp32; the probabilities are rounded to bf16 on their way into the products that make the
+    gradients of ``x`` and ``weight``, what the targets add to them is not.  They exist for as many columns or rows at a time as
+    ``DFCCL_LOSS_WORKSPACE_BYTES`` (1 GiB) hold.  Large reduced losses make their gradients with the loss and keep them until the
+    first backward pass.  There is no check of the targets' values on the host: one outside the vocabulary makes its row's loss and gradients NaN."""
     _check(x, weight, targets, "targets", reduction)
     if targets.shape != x.shape[:-1]:
         raise ValueError(f"targets of {tuple(targets.shape)} for x of {tuple(x.shape)}")
