@@ -32,6 +32,11 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
 
 
+def _pitch(t: torch.Tensor) -> int:
+    """Elements from row to row; of a single row the stride may be anything."""
+    return max(t.stride(0), t.shape[1])
+
+
 def _forward(ids, weight, positions, position_weight, scale):
     n, d = ids.numel(), weight.shape[1]
     out = torch.empty(*ids.shape, d, dtype=weight.dtype, device=weight.device)
@@ -42,9 +47,9 @@ def _forward(ids, weight, positions, position_weight, scale):
         second = (None, 0, None, 0, 0)
     else:
         p = _rows(position_weight)
-        second = (positions.data_ptr(), int(positions.dtype == torch.int64), p.data_ptr(), p.shape[0], p.stride(0))
+        second = (positions.data_ptr(), int(positions.dtype == torch.int64), p.data_ptr(), p.shape[0], _pitch(p))
     with on_device(w.device):
-        nv.check(nv.long_entry("dfcclEmbeddingForward")(ids.data_ptr(), int(ids.dtype == torch.int64), n, w.data_ptr(), w.shape[0], w.stride(0), *second, out.data_ptr(),
+        nv.check(nv.long_entry("dfcclEmbeddingForward")(ids.data_ptr(), int(ids.dtype == torch.int64), n, w.data_ptr(), w.shape[0], _pitch(w), *second, out.data_ptr(),
                                                         d, nccl_dtype(w.dtype), scale, stream_of(w)), "dfcclEmbeddingForward")
     return out
 

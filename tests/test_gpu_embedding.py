@@ -125,6 +125,13 @@ def test_strides_and_shapes():
     assert bool((w.grad == 0).all())
 
 
+def test_a_table_of_one_row_with_any_stride():
+    from dfccl_b200.ops.embedding import embedding
+    one = torch.arange(40.0, device="cuda").as_strided((1, 40), (0, 1))
+    ids = torch.zeros(3, dtype=torch.int64, device="cuda")
+    assert torch.equal(embedding(ids, one, positions=ids, position_weight=one), 2 * one.expand(3, 40))
+
+
 def test_other_stream_and_graph():
     """On a stream of its own; forward and backward captured and replayed for other tokens, beside a second graph."""
     from dfccl_b200.ops.embedding import embedding
