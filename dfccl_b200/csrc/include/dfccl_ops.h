@@ -78,8 +78,9 @@ size_t dfcclEmbeddingBackwardWork(int n, int d, int tables);
  * gradient), 1 a row with some, 2 a row with a token outside the vocabulary (NaN). */
 ncclResult_t dfcclTeacherRows(const void* logits, int logitType, const void* tokens, int wide, int n, int k, int v, float temperature,
                               void* outTokens /* int32 [n, k] */, void* outWeights /* fp32 [n, k] */, void* state /* int32 [n] */, cudaStream_t stream);
-/* lse [n]: log2 of the sum of 2^(z log2(e) / T); rest [n, k]: what of the entries' weights their probabilities leave; both are kept for the backward pass.  reduction 0: rowLoss [n]; 1 (mean over the rows with a target
- * or list; 0 where there is none) or 2 (sum): loss and count (int32), one each.  All fp32. */
+/* lse [n]: log2 of the sum of 2^(z log2(e) / T); rest [n, k]: what of the entries' weights their probabilities leave; both are kept for the
+ * backward pass.  reduction 0: rowLoss [n]; 1 (mean over the rows with a target or list; 0 where there is none) or 2 (sum): loss and
+ * count (int32), one each.  All fp32. */
 ncclResult_t dfcclLinearLossForward(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, const void* tokens,
                                     const void* weights, const void* state, int k, float temperature, int reduction, void* work, void* lse, void* rest,
                                     void* rowLoss, void* loss, void* count, cudaStream_t stream);
@@ -100,6 +101,8 @@ ncclResult_t dfcclLinearLossWithGradients(const void* x, const void* w, int n, i
 size_t dfcclLinearLossWithGradientsWork(int n, int v, int d, int k, int wantX, int wantW);
 /* Two bf16 arrays (na and nb elements, multiples of 8; either may be empty) times *scale (fp32), in place; left alone where it is 1. */
 ncclResult_t dfcclScaleResults(void* a, size_t na, void* b, size_t nb, const void* scale, cudaStream_t stream);
+/* A number of the graph that the stream is captured into, 0 where there is none. */
+uint64_t dfcclCaptureId(cudaStream_t stream);
 
 /* ---- fabric probes (roofline inputs): mean device time in microseconds */
 /* direction 0 = read the peer's heap, 1 = write it; loadKind selects the load instruction form; `unroll` independent

@@ -8,7 +8,7 @@
 // A logit exists in tensor memory and registers only.  What bounds them is the tensor cores: busy 91 % of the cycles in the tiles of z, 93 - 95 % in
 // the gradients' products (2048 x 50257 x 1024); 8192 x 50257 x 1024 takes 527 us (statistics), 566 (powers) and 1130 (products), 1.60, 1.49 and 1.49
 // PFLOP/s of the 1.64 that a library product of 8192^3 reaches, and less where such kernels run for long, by the power limit.  Widths below
-// 640 are bound by the epilogue (d = 64: 92 us for statistics of 4096 x 50257, 29 of them a power's share of the special function units).
+// 640 are bound by the epilogue (d = 64: 92 us for statistics of 4096 x 50257, 46 of them the powers in the special function units).
 //
 // Tiles of 256 x 256, stages of 64 of the contraction, roles as in tcgen05_gemm_pair.cu (TMA producer, MMA issuer, eight epilogue warps,
 // two accumulators).  All of n, v are any number, d a multiple of 8: the tensor maps give zeros outside, the epilogues store inside.

@@ -267,7 +267,8 @@ __global__ void __launch_bounds__(1024) joinRowsKernel(const JoinArgs a) {
 }
 
 // In front of the products: the logits of the rows' lists by fp32 sums, a warp for four entries of a row, -> picked [n][k].  Where `base` is
-// given, a warp for a row, and the largest of its entries times `scale` is the base of its powers.  On the way, words set to their start and the number of rows that count.
+// given, a warp for a row, and the largest of its entries times `scale` is the base of its powers.  On the way, words set to their start and
+// the number of rows that count.
 struct PickArgs {
   const uint4* x; const uint4* w;
   VocabRows rows;
@@ -377,7 +378,8 @@ __global__ void __launch_bounds__(128) listSumsKernel(const uint4* w, const Voca
   }
 }
 
-// Two results times one number on the device, in place; nothing is read or written where it is 1.
+// Two results times one number on the device, in place; nothing is read or written where it is 1.  (What is not a power of two rounds them to
+// bf16 a second time: the number is not known when they are made, and as fp32 they would take twice the memory until then.)
 __global__ void __launch_bounds__(256) scaleResultsKernel(uint4* a, size_t na, uint4* b, size_t nb, const float* scale) {
   tc::grid_dependency_wait();
   tc::grid_launch_dependents();
@@ -454,7 +456,7 @@ __global__ void __launch_bounds__(OWN_THREADS) ownSumsKernel(const uint4* x, con
 }
 
 // x with zeros in the rows without a list: in the product of the weights' gradient they meet the zeros of the logits' gradient, and nothing
-// that x holds there (infinities, NaN) may come through.  n d 4 bytes: 8192 x 1024 takes 6 us beside 2300.
+// that x holds there (infinities, NaN) may come through.  n d 4 bytes: 8192 x 1024 takes 15 us (cold) beside the 1700 of the losses and gradients.
 __global__ void __launch_bounds__(256) keepRowsKernel(const uint4* x, const VocabRows rows, int n, int packs, uint4* out) {
   tc::grid_dependency_wait();
   tc::grid_launch_dependents();
@@ -708,7 +710,9 @@ DF_API size_t dfcclLinearLossWithGradientsWork(int n, int v, int d, int k, int w
 DF_API ncclResult_t dfcclLinearLossWithGradients(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, const void* tokens,
                                                  const void* weights, const void* state, int k, float temperature, int reduction, void* work, size_t workBytes,
                                                  void* lse, void* rest, void* loss, void* count, void* dx, void* dw, cudaStream_t stream) {
-  if (!sizesOk(n, v, d, k) || (int64_t)n * k > 0x7fffffff - 4096 || !x || !w || !rowsOk(targets, tokens, weights, state, k, temperature) || !work || !lse || !rest || !loss || !count || !(dx || dw) || reduction < 1 || reduction > 2) return ncclInvalidArgument;
+  if (!sizesOk(n, v, d, k) || (int64_t)n * k > 0x7fffffff - 4096 || !x || !w || !rowsOk(targets, tokens, weights, state, k, temperature) || !work || !lse ||
+      !rest || !loss || !count || !(dx || dw) || reduction < 1 || reduction > 2)
+    return ncclInvalidArgument;
   if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw) & 15) return ncclInvalidArgument;
   const OneGoPlan p = oneGoPlan(n, v, d, k, dx != nullptr, dw != nullptr);
   if (p.bytes > workBytes) return ncclInvalidArgument;           // (the setting has changed since the size was asked for)
@@ -746,7 +750,8 @@ DF_API ncclResult_t dfcclLinearLossWithGradients(const void* x, const void* w, i
     CUDACHECK(launchBehind(joinRowsKernel<false>, (m + 31) / 32, 1024, stream, j));
     DFCHECK(vocabPowers(xr, w, m, v, d, j.rows, base + r, parts, powers, j.again, stream));
     if (dw && i == pieces - 1) DFCHECK(tokenSums(x, n * k, d, k, v, (const float*)rest, nullptr, 0, (float*)(at + p.sums), p.dense, where, at + p.tokens, stream));
-    if (listed) CUDACHECK(launchBehind(listSumsKernel, std::min(m, 148 * 16), 128, stream, (const uint4*)w, j.rows, (const float*)rest + (size_t)r * k, m, packs, (float4*)listed));
+    if (listed)
+      CUDACHECK(launchBehind(listSumsKernel, std::min(m, 148 * 16), 128, stream, (const uint4*)w, j.rows, (const float*)rest + (size_t)r * k, m, packs, (float4*)listed));
     const VocabExact exact{j.rows, share + r, (const float*)rest + (size_t)r * k, nullptr, 0, (const __nv_bfloat16*)w, (const float*)(at + p.sums), where,
                            dw ? tokenSortItems(n * k, d, v, at + p.tokens) : nullptr, n * k, 0, p.dense, listed};
     __nv_bfloat16* dxr = dx ? (__nv_bfloat16*)dx + (size_t)r * d : nullptr;
@@ -757,6 +762,13 @@ DF_API ncclResult_t dfcclLinearLossWithGradients(const void* x, const void* w, i
     if (p.sumW && i == pieces - 1) DFCHECK(joinSlices(partW, p.slicesW, v, d, factor, &exact, 2, dw, stream));
   }
   return ncclSuccess;
+}
+
+DF_API uint64_t dfcclCaptureId(cudaStream_t stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(stream, &status, &id) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
+  return status == cudaStreamCaptureStatusNone ? 0 : id;
 }
 
 DF_API ncclResult_t dfcclScaleResults(void* a, size_t na, void* b, size_t nb, const void* scale, cudaStream_t stream) {

@@ -60,6 +60,8 @@ static PyObject* call_long(PyObject* self, PyObject* const* args, Py_ssize_t n) 
   return PyLong_FromLong(r);
 }
 
-static PyMethodDef methods[] = {{"call_long", (PyCFunction)(void (*)(void))call_long, METH_FASTCALL, "call_long(address, arguments...) -> int"}, {"call", (PyCFunction)(void (*)(void))call, METH_FASTCALL, "call(address, arguments...) -> int"}, {NULL, NULL, 0, NULL}};
+static PyMethodDef methods[] = {{"call", (PyCFunction)(void (*)(void))call, METH_FASTCALL, "call(address, arguments...) -> int"},
+                                {"call_long", (PyCFunction)(void (*)(void))call_long, METH_FASTCALL, "call_long(address, arguments...) -> int"},
+                                {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "dfccl_hostcall", NULL, -1, methods, NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit_dfccl_hostcall(void) { return PyModule_Create(&module); }

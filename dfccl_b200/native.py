@@ -198,7 +198,7 @@ def lib() -> C.CDLL:
             "dfcclLinearLossForward": [vp, vp, i, i, i, vp, i, i64, vp, vp, vp, i, C.c_float, i, vp, vp, vp, vp, vp, vp, vp], "dfcclLinearLossForwardWork": [i, i, i],
             "dfcclLinearLossBackward": [vp, vp, i, i, i, vp, i, i64, vp, vp, vp, i, C.c_float, vp, vp, vp, i, vp, vp, vp, vp, sz, vp],
             "dfcclLinearLossWithGradients": [vp, vp, i, i, i, vp, i, i64, vp, vp, vp, i, C.c_float, i, vp, sz, vp, vp, vp, vp, vp, vp, vp], "dfcclLinearLossWithGradientsWork": [i, i, i, i, i, i],
-            "dfcclScaleResults": [vp, sz, vp, sz, vp, vp], "dfcclLinearLossBackwardWork": [i, i, i, i, i, i], "dfcclLinearLossMaxList": [],
+            "dfcclScaleResults": [vp, sz, vp, sz, vp, vp], "dfcclCaptureId": [vp], "dfcclLinearLossBackwardWork": [i, i, i, i, i, i], "dfcclLinearLossMaxList": [],
             "dfcclGemmCheck": [C.POINTER(i)],
             "dfcclGemmPairResident": [C.POINTER(i)], "dfcclGemmPlan": [i, i, i, i, i, i, C.POINTER(i)],
             "dfcclGemmFused": [vp, vp, vp, i, i, i, vp, sz, vp],
@@ -227,6 +227,7 @@ def lib() -> C.CDLL:
         L.dfcclLayerNormWork.restype = L.dfcclColumnSumWork.restype = sz
         L.dfcclEmbeddingBackwardWork.restype = L.dfcclLinearLossForwardWork.restype = L.dfcclLinearLossBackwardWork.restype = sz
         L.dfcclLinearLossWithGradientsWork.restype = sz
+        L.dfcclCaptureId.restype = C.c_uint64
         L.dfcclParam.argtypes = [C.c_char_p, C.c_longlong]
         L.dfcclParam.restype = C.c_longlong
         L.dfcclLogReset.argtypes = []

@@ -20,6 +20,7 @@ MAX_LIST = 256                       # entries of a teacher's list
 ONE_GO_FROM = 2 ** 34
 LISTS_TIMES = 4
 LIST_SHARE = 1024
+MOST_ENTRIES = 2 ** 31 - 4096        # of all lists together, as their sorting counts them
 
 
 def linear_loss_supported(x: torch.Tensor, weight: torch.Tensor) -> bool:
@@ -110,7 +111,7 @@ def _forward_with_gradients(x, weight, rows, reduction, want_x, want_w):
 
 
 def _scaled(grads, g):
-    """The gradients times that of the loss, in place: nothing else holds them."""
+    """The gradients times that of the loss, in place: nothing else holds them, and whatever runs this again makes them anew."""
     dx, dw = grads
     with on_device(g.device):
         nv.check(nv.entry("dfcclScaleResults")(None if dx is None else dx.data_ptr(), 0 if dx is None else dx.numel(), None if dw is None else dw.data_ptr(),
@@ -120,15 +121,18 @@ def _scaled(grads, g):
 
 class _LinearLossFn(torch.autograd.Function):
     """A reduced loss of some size makes its gradients with the loss, which saves computing the logits a second time: the first
-    backward pass scales them.  Another pass over the same graph, and every other loss, computes the logits again."""
+    backward pass scales them.  Another pass over the same graph, one captured into a CUDA graph that has not captured the loss
+    (its replays would scale what they have scaled before), and every other loss, computes the logits again."""
 
     @staticmethod
     def forward(ctx, x, weight, rows, reduction):
         want_x, want_w = ctx.needs_input_grad[:2]
         ctx.grads = None
         from_size = ONE_GO_FROM if rows.lists is None else ONE_GO_FROM * LISTS_TIMES
-        if reduction and (want_x or want_w) and x.numel() * weight.shape[0] >= from_size and (rows.lists is None or rows.k * LIST_SHARE <= weight.shape[0]):
+        few = rows.lists is None or (rows.k * LIST_SHARE <= weight.shape[0] and rows.lists[0].numel() <= MOST_ENTRIES)
+        if reduction and (want_x or want_w) and x.numel() * weight.shape[0] >= from_size and few:
             loss, xp, wp, kept, ctx.grads = _forward_with_gradients(x, weight, rows, reduction, want_x, want_w)
+            ctx.capture = nv.lib().dfcclCaptureId(stream_of(x))
         else:
             loss, xp, wp, kept = _forward(x, weight, rows, reduction)
         ctx.save_for_backward(xp, wp, kept, *rows.tensors())
@@ -144,7 +148,7 @@ class _LinearLossFn(torch.autograd.Function):
             return None, None, None, None
         x, w, kept = ctx.saved_tensors[:3]                  # (asking for them notices a change in place, of the targets too)
         grads, ctx.grads = ctx.grads, None
-        if grads is not None:
+        if grads is not None and ctx.capture == nv.lib().dfcclCaptureId(stream_of(x)):
             return _scaled(grads, g)
         (v, d), device = w.shape, x.device
         n = x.numel() // d

@@ -446,6 +446,49 @@ def test_other_stream_and_graphs(one_go, monkeypatch):
     assert check_kernels()
 
 
+@pytest.mark.parametrize("loss_captured", [False, True])
+@pytest.mark.parametrize("lists", [False, True])
+def test_backward_pass_captured_apart_from_the_loss(lists, loss_captured, monkeypatch):
+    """Each replay of the pass gives the gradients of the loss, however often the same loss's pass is replayed."""
+    from dfccl_b200.ops import loss as module
+    from dfccl_b200.ops.gemm import check_kernels
+    from dfccl_b200.ops.loss import linear_cross_entropy, linear_distillation
+    monkeypatch.setattr(module, "ONE_GO_FROM", 0)
+    monkeypatch.setattr(module, "LIST_SHARE", 0)
+    x, w, gen = problem(300, 3001, 128, 51)
+    x.requires_grad_(True), w.requires_grad_(True)
+    t = torch.randint(0, 3001, (300, 4), generator=gen, device="cuda")
+    teacher = torch.randn(300, 4, generator=gen, device="cuda")
+    g = torch.full((), 3.0, device="cuda")
+
+    def loss_of():
+        return linear_distillation(x, w, teacher, t, temperature=2.0) if lists else linear_cross_entropy(x, w, t[:, 0])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        loss = loss_of()
+        first = torch.autograd.grad(loss, [x, w], g, retain_graph=True)
+        want = torch.autograd.grad(loss, [x, w], g)            # the logits computed again, as in the captured pass
+        loss = None if loss_captured else loss_of()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(first, want):                              # (each: probabilities, and the result up to twice, rounded)
+        assert (a.double() - b.double()).norm().item() <= 3 * 2.0 ** -8 * b.double().norm().item()
+    graphs = []
+    if loss_captured:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[0], stream=side):
+            loss = loss_of()
+    graphs.append(torch.cuda.CUDAGraph())
+    with torch.cuda.graph(graphs[-1], stream=side, pool=graphs[0].pool() if loss_captured else None):
+        got = torch.autograd.grad(loss, [x, w], g, retain_graph=True)
+    graphs[0].replay()
+    for _ in range(3):
+        graphs[-1].replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert check_kernels()
+
+
 def test_many_rows_and_wide_ones():
     """More rows than the statistics take at a time, a width of many stages, row numbers beyond 16 bits."""
     from dfccl_b200.ops.gemm import check_kernels
