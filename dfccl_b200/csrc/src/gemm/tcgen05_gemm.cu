@@ -446,8 +446,17 @@ ncclResult_t encodeMap(CUtensorMap* m, const MapKey& k) {
   cuuint64_t strides[2] = {k.s1, 128};
   cuuint32_t box[3] = {k.b0, k.b1, k.b2};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, k.b2 ? 3 : 2, (void*)k.base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  k.b0 == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, k.b2 ? 3 : 2, (void*)k.base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              k.b0 == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {      // a thread without a call of the runtime so far (a backward pass's): this binds it to its device
+    int dev = 0;
+    CUDACHECK(cudaGetDevice(&dev));
+    CUDACHECK(cudaSetDevice(dev));
+    r = encode();
+  }
   if (r != CUDA_SUCCESS) {
     DF_WARN("cuTensorMapEncodeTiled failed (%d) for %llu x %llu at %p", (int)r, (unsigned long long)k.d1, (unsigned long long)(k.d2 ? k.d2 * 64 : k.d0), k.base);
     return ncclInvalidArgument;

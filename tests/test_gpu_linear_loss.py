@@ -3,6 +3,9 @@
 What may be off, by arithmetic: a logit of d terms is added up in fp32 in steps of 16, each at most one step of its type (2**-23 of the
 magnitudes' sum) off; a power of two or logarithm is a few of those; a gradient of a logit is rounded once to bf16 (2**-8 at most, less
 than 2**-9 in the 2-norm over many), the gradients of x and weight once more."""
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -444,6 +447,46 @@ def test_other_stream_and_graphs(one_go, monkeypatch):
         for k, (_, _, _, out) in enumerate(graphs):
             assert all(torch.equal(p, q) for p, q in zip(out, want[(turn + k) % 3]))
     assert check_kernels()
+
+
+@pytest.mark.parametrize("one_go", [False, True])
+@pytest.mark.parametrize("lists", [False, True])
+def test_one_gradient_of_two(lists, one_go, monkeypatch):
+    """A frozen head, or inputs that want no gradient: the other gradient is the same."""
+    from dfccl_b200.ops import loss as module
+    from dfccl_b200.ops.loss import linear_cross_entropy, linear_distillation
+    monkeypatch.setattr(module, "ONE_GO_FROM", 0 if one_go else 1 << 60)
+    monkeypatch.setattr(module, "LIST_SHARE", 0)
+    for n, v, d, k in ((3, 700, 64, 2), (300, 3001, 136, 20)):
+        x, w, gen = problem(n, v, d, 61)
+        t = torch.randint(0, v, (n, k), generator=gen, device="cuda")
+        teacher = torch.randn(n, k, generator=gen, device="cuda")
+
+        def gradients(want_x, want_w):
+            a, b = x.clone().requires_grad_(want_x), w.clone().requires_grad_(want_w)
+            loss = linear_distillation(a, b, teacher, t) if lists else linear_cross_entropy(a, b, t[:, 0])
+            loss.backward()
+            return a.grad, b.grad
+
+        both, left, right = gradients(True, True), gradients(True, False), gradients(False, True)
+        assert left[1] is None and right[0] is None
+        for a, b in ((left[0], both[0]), (right[1], both[1])):     # (slices of the contraction may be cut elsewhere: results a rounding apart)
+            assert bool(((a.double() - b.double()).abs() <= 2.0 ** -7 * b.double().abs() + 1e-6 * b.double().abs().max()).all())
+
+
+def test_first_backward_pass_of_a_process_with_a_frozen_head():
+    """The thread of backward passes has made no call of the CUDA runtime yet."""
+    code = """
+import torch
+from dfccl_b200.ops.loss import linear_cross_entropy
+x = torch.randn(5, 64, device="cuda").to(torch.bfloat16).requires_grad_(True)
+w = torch.randn(300, 64, device="cuda").to(torch.bfloat16)
+torch.empty(1 << 24, device="cuda")
+linear_cross_entropy(x, w, torch.arange(5, device="cuda")).backward()
+assert x.grad.isfinite().all() and (x.grad != 0).any()
+"""
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
 
 
 @pytest.mark.parametrize("loss_captured", [False, True])
