@@ -33,8 +33,11 @@ enum VocabMode { VOCAB_STATS, VOCAB_GRAD, VOCAB_POWERS, VOCAB_PRODUCTS };
 // one for each accumulator: the waits of one tile (for its rows' targets, tensor memory, powers) lie beside the other's.
 constexpr int PARTS = 2, EPI_WARPS = 4 * PARTS;
 __host__ __device__ constexpr int groupsOf(int mode) { return mode == VOCAB_PRODUCTS ? 1 : 2; }
+// Columns at a time.  (Powers that are stored and summed: with 32 the registers of 576 threads do not do; 4096 x 50257 x 256 with both gradients 386 us
+// instead of 350.  Statistics with 16 are 2 - 6 % slower.  Loading the next columns ahead, the registers allowing it, gains nothing: the other warps do.)
+__host__ __device__ constexpr int unitOf(int mode) { return mode == VOCAB_POWERS ? 16 : 32; }
 __host__ __device__ constexpr int threadsOf(int mode) { return 64 + 32 * EPI_WARPS * groupsOf(mode); }
-constexpr int JOIN_BYTES = 2 * HALF * 8;                                          // what one part of a tile's rows leaves for the other, of either group
+constexpr int JOIN_BYTES = 4 * HALF * 8;                                          // what one part of a tile's rows leaves for the other, of four tiles in turn
 constexpr uint64_t WAIT_NS = 4000000000ull;                                       // nothing here waits on another GPU
 static_assert(STAGES * STAGE_BYTES + JOIN_BYTES + 1024 + 512 <= SMEM_BYTES, "stages");
 
@@ -128,20 +131,23 @@ struct List {
   __device__ __forceinline__ void step() { next = next2; q = q2; load(behind++, next2, q2); }
 };
 
+__device__ __forceinline__ void tmemLoad(uint32_t at, uint32_t (&r)[16]) { tmem_ld16(at, r); }
+__device__ __forceinline__ void tmemLoad(uint32_t at, uint32_t (&r)[32]) { tmem_ld32(at, r); }
+
 template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threadsOf(MODE), 1)
 dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtensorMap mapB0, const __grid_constant__ CUtensorMap mapA1,
                  const __grid_constant__ CUtensorMap mapB1, const __grid_constant__ VocabArgs g) {
   extern __shared__ uint8_t smemRaw[];
-  constexpr int GROUPS = groupsOf(MODE);
+  constexpr int GROUPS = groupsOf(MODE), UNIT = unitOf(MODE);
   uint8_t* smem = (uint8_t*)(((uintptr_t)smemRaw + 1023) & ~(uintptr_t)1023);       // the same offset in both CTAs
-  float2* joinBuf = (float2*)(smem + STAGES * STAGE_BYTES);          // [2 groups][HALF rows]
+  float2* joinBuf = (float2*)(smem + STAGES * STAGE_BYTES);          // [4 tiles][HALF rows]
   uint64_t* fullBar = (uint64_t*)(smem + STAGES * STAGE_BYTES + JOIN_BYTES);      // used in the leader only
   uint64_t* emptyBar = fullBar + STAGES;                             // in both CTAs (commit to both)
   uint64_t* accFull = emptyBar + STAGES;                             // [2] in both CTAs
   uint64_t* accEmpty = accFull + 2;                                  // [2] used in the leader only
-  uint64_t* joinBar = accEmpty + 2;                                  // [4 quarters][2 groups] the other part of 32 rows is in place
-  uint32_t* tmemBaseSlot = (uint32_t*)(joinBar + 8);
+  uint64_t* joinBar = accEmpty + 2;                                  // [4 quarters][4 tiles] the other part of 32 rows is in place
+  uint32_t* tmemBaseSlot = (uint32_t*)(joinBar + 16);
   volatile uint32_t* giveUp = tmemBaseSlot + 1;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -154,7 +160,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&fullBar[s], 1); mbar_init(&emptyBar[s], 1); }
     for (int a = 0; a < 2; ++a) { mbar_init(&accFull[a], 1); mbar_init(&accEmpty[a], 2 * EPI_WARPS); }
-    for (int a = 0; a < 8; ++a) mbar_init(&joinBar[a], 1);
+    for (int a = 0; a < 16; ++a) mbar_init(&joinBar[a], 1);
     *giveUp = 0;
     mbar_fence_init();
     tma_prefetch_desc(&mapA0);
@@ -257,6 +263,13 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
     const int quarter = warp & 3, part = (warp - 2) >> 2 & 1, group = (warp - 2) >> 3;
     const uint32_t accEmptyLeader0 = mapa_u32(smem_u32(&accEmpty[0]), 0), accEmptyLeader1 = mapa_u32(smem_u32(&accEmpty[1]), 0);
     const float factor = MODE == VOCAB_PRODUCTS ? vocabFactor(g.factor) : 1.f;
+    // an accumulator goes back to the item after the next: every arrival is waited for
+    auto release = [&](int j) {
+      if (j + 2 >= count) return;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster_relaxed(j & 1 ? accEmptyLeader1 : accEmptyLeader0);
+    };
     for (int j = group; j < count; j += GROUPS) {
       int item;
       const int which = MODE == VOCAB_PRODUCTS ? items.at(j, item) : (items.at(j, item), 0);
@@ -266,8 +279,6 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
       const int row0 = t.mt * T + (int)cr * HALF + quarter * 32, row = row0 + lane, tn = MODE == VOCAB_PRODUCTS ? p.tn : T, col0 = t.nt * tn;
       const bool mine = row0 < p.M, here = row < p.M;
       const uint32_t acc = tmemBase + ((uint32_t)(quarter * 32) << 16) + ab * T;
-      uint32_t r[32];
-
       if (MODE != VOCAB_PRODUCTS) {
         List list;
         list.none();
@@ -290,102 +301,102 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
         if (!mbar_wait(&accFull[ab], (j >> 1) & 1, giveUp, WAIT_NS)) break;
         tc_fence_after();
         float top = -INFINITY, sum = 0.f;
-        const int cols = MODE == VOCAB_STATS ? p.N : g.ld, steps = (min(T, cols - col0) + 31) / 32;
+        const int cols = MODE == VOCAB_STATS ? p.N : g.ld, units = (min(T, cols - col0) + UNIT - 1) / UNIT;
+        uint32_t r[UNIT];
 #pragma unroll 1
-        for (int i = part; i < steps; i += PARTS) {
+        for (int i = part; i < units; i += PARTS) {
           if (!mine) break;
-          const int c = col0 + i * 32;
+          const int c = col0 + i * UNIT;
           __syncwarp();
-          tmem_ld32(acc + i * 32, r);
+          tmemLoad(acc + i * UNIT, r);
           tmem_ld_wait();
           if (MODE != VOCAB_GRAD) {
-            if (c + 32 > p.N) {
+            if (c + UNIT > p.N) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) if (c + e >= p.N) r[e] = 0xff800000u;          // -inf
+              for (int e = 0; e < UNIT; ++e) if (c + e >= p.N) r[e] = 0xff800000u;          // -inf
             }
-            while (list.next < c + 32) {                 // the list's entries: no power
+            while (list.next < c + UNIT) {               // the list's entries: no power
               if (list.next >= c) {
                 const int at = list.next - c;
 #pragma unroll
-                for (int e = 0; e < 32; ++e) if (e == at) r[e] = 0xff800000u;
+                for (int e = 0; e < UNIT; ++e) if (e == at) r[e] = 0xff800000u;
               }
               list.step();
             }
-          }
-          if (MODE == VOCAB_STATS) {
-            // running maximum and sum over the row's columns
-            float m0 = __uint_as_float(r[0]), m1 = __uint_as_float(r[1]);
+            float m[4];
 #pragma unroll
-            for (int e = 2; e < 32; e += 2) { m0 = fmaxf(m0, __uint_as_float(r[e])); m1 = fmaxf(m1, __uint_as_float(r[e + 1])); }
-            const float now = fmaxf(top, fmaxf(m0, m1) * scale), base = now == -INFINITY ? 0.f : now;
-            float s[4] = {sum * exp2Approx(top - base), 0.f, 0.f, 0.f};
+            for (int e = 0; e < 4; ++e) m[e] = __uint_as_float(r[e]);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) s[e & 3] += exp2Approx(fmaf(__uint_as_float(r[e]), scale, -base));
-            sum = (s[0] + s[1]) + (s[2] + s[3]);
-            top = now;
-          } else if (MODE == VOCAB_POWERS) {
-            float m0 = __uint_as_float(r[0]), m1 = __uint_as_float(r[1]);
-#pragma unroll
-            for (int e = 2; e < 32; e += 2) { m0 = fmaxf(m0, __uint_as_float(r[e])); m1 = fmaxf(m1, __uint_as_float(r[e + 1])); }
-            top = fmaxf(top, fmaf(fmaxf(m0, m1), scale, -lse));
+            for (int e = 4; e < UNIT; ++e) m[e & 3] = fmaxf(m[e & 3], __uint_as_float(r[e]));
+            const float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+            float base = lse;
+            if (MODE == VOCAB_STATS) {
+              // running maximum and sum over the row's columns
+              const float now = fmaxf(top, most * scale);
+              base = now == -INFINITY ? 0.f : now;
+              sum *= exp2Approx(top - base);
+              top = now;
+            } else {
+              top = fmaxf(top, fmaf(most, scale, -base));
+            }
             float s[4] = {sum, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float v = exp2Approx(fmaf(__uint_as_float(r[e]), scale, -lse));
+            for (int e = 0; e < UNIT; ++e) {
+              const float v = exp2Approx(fmaf(__uint_as_float(r[e]), scale, -base));
               s[e & 3] += v;
-              r[e] = __float_as_uint(v);
+              if (MODE == VOCAB_POWERS) r[e] = __float_as_uint(v);
             }
             sum = (s[0] + s[1]) + (s[2] + s[3]);
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(exp2Approx(fmaf(__uint_as_float(r[e]), scale, -lse)));
+            for (int e = 0; e < UNIT; ++e) r[e] = __float_as_uint(exp2Approx(fmaf(__uint_as_float(r[e]), scale, -lse)));
             int before = -1;
-            while (list.next < g.first + c + 32) {
+            while (list.next < g.first + c + UNIT) {
               if (list.next >= g.first + c) {
                 const int at = list.next - g.first - c;
                 if (at != before) {                      // (the first entry of a token has all of it)
 #pragma unroll
-                  for (int e = 0; e < 32; ++e) if (e == at) r[e] = __float_as_uint(-list.q);
+                  for (int e = 0; e < UNIT; ++e) if (e == at) r[e] = __float_as_uint(-list.q);
                 }
                 before = at;
               }
               list.step();
             }
-            if (c + 32 > p.N) {
+            if (c + UNIT > p.N) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) if (c + e >= p.N) r[e] = 0u;
+              for (int e = 0; e < UNIT; ++e) if (c + e >= p.N) r[e] = 0u;
             }
           }
           // (a row without a gradient may hold anything, infinities and NaN among it)
-          if (MODE != VOCAB_STATS) {
-            if (here) {
-              uint4 o[4];
+          if (MODE != VOCAB_STATS && here) {
+            uint4 o[UNIT / 8];
 #pragma unroll
-              for (int v = 0; v < 4; ++v) {
-                uint32_t* ow = (uint32_t*)&o[v];
+            for (int v = 0; v < UNIT / 8; ++v) {
+              uint32_t* ow = (uint32_t*)&o[v];
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                  float lo = __uint_as_float(r[8 * v + 2 * w]), hi = __uint_as_float(r[8 * v + 2 * w + 1]);
-                  if (MODE == VOCAB_GRAD) { lo *= coef; hi *= coef; }
-                  ow[w] = coef == 0.f ? 0u : pack_bf16x2(lo, hi);
-                }
+              for (int w = 0; w < 4; ++w) {
+                float lo = __uint_as_float(r[8 * v + 2 * w]), hi = __uint_as_float(r[8 * v + 2 * w + 1]);
+                if (MODE == VOCAB_GRAD) { lo *= coef; hi *= coef; }
+                ow[w] = coef == 0.f ? 0u : pack_bf16x2(lo, hi);
               }
-              __nv_bfloat16* dst = g.dz + (size_t)row * g.ld + c;
-              st_global32(dst, o, true);
-              st_global32(dst + 16, o + 2, true);
             }
+            __nv_bfloat16* dst = g.dz + (size_t)row * g.ld + c;
+#pragma unroll
+            for (int v = 0; v < UNIT / 8; v += 2) st_global32(dst + 8 * v, o + v, true);
           }
         }
+        release(j);
         if (MODE != VOCAB_GRAD) {
-          // The parts of a row meet in the first one's warp.  (Its arrival on accEmpty, behind this, keeps the other from the group's next tile.)
-          uint64_t* bar = joinBar + quarter * 2 + ab;
-          float2* at = joinBuf + ab * HALF + quarter * 32 + lane;
+          // The parts of a row meet in the first one's warp.  (The other comes back to this place four tiles on, when the first has released
+          // the tile in between.)
+          uint64_t* bar = joinBar + quarter * 4 + (j & 3);
+          float2* at = joinBuf + (j & 3) * HALF + quarter * 32 + lane;
           if (part) {
             *at = make_float2(top, sum);
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
           } else {
-            if (!mbar_wait(bar, (j >> 1) & 1, giveUp, WAIT_NS)) break;
+            if (!mbar_wait(bar, (j >> 2) & 1, giveUp, WAIT_NS)) break;
             const float2 q = *at;
             const float m = fmaxf(top, q.x), base = m == -INFINITY ? 0.f : m;
             sum = MODE == VOCAB_POWERS ? sum + q.y : sum * exp2Approx(top - base) + q.y * exp2Approx(q.x - base);
@@ -401,6 +412,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
         for (int i = part; i < steps; i += PARTS) {
           if (!mine) break;
           const int c = col0 + i * 32, packs = min(4, (p.N - c) / 8);
+          uint32_t r[32];
           __syncwarp();
           tmem_ld32(acc + i * 32, r);
           tmem_ld_wait();
@@ -443,11 +455,7 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
           }
         }
       }
-      if (j + 2 < count) {                             // released to the item after the next: every arrival is waited for
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_relaxed(ab ? accEmptyLeader1 : accEmptyLeader0);
-      }
+      if (MODE == VOCAB_PRODUCTS) release(j);
     }
   }
 
