@@ -469,6 +469,10 @@ dfcclVocabKernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constan
   if (threadIdx.x == 0 && *giveUp) { atomicExch(g.err, 1u); *(volatile uint32_t*)g.errHost = 1u; __threadfence_system(); }
 }
 
+// A tile's way out of tensor memory, in blocks of the contraction: no item takes less (3950 clocks and 512).  With items of one block counted as
+// that, few pairs got nearly all of dw of 32 rows: 50257 x 1024 with both gradients took 257 us instead of 120.
+constexpr int STORE = 8;
+
 template <int MODE>
 ncclResult_t launchVocab(const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1, const CUtensorMap& b1, VocabArgs& g, cudaStream_t stream) {
   CUDACHECK(oncePerDevice([] { return allowSharedMemory(dfcclVocabKernel<MODE>, SMEM_BYTES); }));
@@ -480,7 +484,7 @@ ncclResult_t launchVocab(const CUtensorMap& a0, const CUtensorMap& b0, const CUt
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization; at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at; cfg.numAttrs = 1;
   // the head start of pairs with one item less of the first product: as many items of the second as that one takes
-  const int64_t c1 = g.p[0].items ? g.p[0].perSlice : 0, c2 = g.p[1].items ? std::max(1, g.p[1].perSlice) : 1;
+  const int64_t c1 = std::max(g.p[0].perSlice, STORE), c2 = std::max(g.p[1].perSlice, STORE);
   g.headStart = g.p[1].items ? (int)((c1 + c2 / 2) / c2) : 0;
   CUDACHECK(cudaLaunchKernelEx(&cfg, dfcclVocabKernel<MODE>, a0, b0, a1, b1, g));
   return ncclSuccess;
@@ -543,18 +547,47 @@ static int productWidth(int d) {
   return std::max(128, ((d + tiles - 1) / tiles + 31) / 32 * 32);
 }
 
-// A product is cut into slices of its contraction where its tiles alone would keep pairs waiting: until the longest item is no more
-// than a pair's share of all the work.
+// How long the pair with most to do is busy with `i1` items of `c1` blocks and `i2` of `c2`, handed out as Items does.
+static int64_t longest(int64_t i1, int64_t c1, int64_t i2, int64_t c2, int64_t pairs) {
+  const int64_t whole = i1 / pairs, r = i1 % pairs, e = pairs - r;
+  if (!i2) return (whole + (r != 0)) * c1;
+  const int64_t ahead = r ? (c1 + c2 / 2) / c2 : 0, left = std::max<int64_t>(0, i2 - ahead * e), each = (left + pairs - 1) / pairs;
+  const int64_t alone = whole * c1 + (std::min(ahead, (i2 + e - 1) / e) + each) * c2;
+  return r ? std::max(alone, (whole + 1) * c1 + each * c2) : alone;
+}
+
+// A product is cut into slices of its contraction where its tiles alone would keep pairs waiting: of some numbers of slices - none, as many as
+// fill the pairs once, twice ..., or as give each item no more than a pair's share of all the work - those that by this estimate are
+// through first.  A slice costs its sums a way to memory and back and the launch that joins them 3 us; none is cut below 16 blocks.
+// 512 x 50257 x 1024, dx alone: 9 slices of 8 tiles on 74 pairs instead of 10.
 VocabPlan vocabProductPlan(int n, int v, int d, bool wantX, bool wantW, int pairs) {
-  const int64_t tn = (n + T - 1) / T, tv = (v + T - 1) / T, td = (d + productWidth(d) - 1) / productWidth(d), kn = (n + BK - 1) / BK, kv = (v + BK - 1) / BK;
-  const int64_t all = (wantX ? tn * td * kv : 0) + (wantW ? tv * td * kn : 0), share = std::max<int64_t>(1, all / pairs);
-  // A slice costs its sums a way to memory and back: none is cut below 16 blocks.
-  auto cut = [&](int64_t tiles, int64_t k) -> int {
-    if (k <= share || tiles >= 4 * pairs) return (int)k;
-    const int64_t slices = std::max<int64_t>(1, std::min<int64_t>((k + share - 1) / share, k / 16));
-    return (int)((k + slices - 1) / slices);
-  };
-  return VocabPlan{cut(tn * td, kv), cut(tv * td, kn)};
+  constexpr double BLOCK_US = 0.27, BYTES_US = 6.5e6;              // a block under a tile of 256 columns; of memory
+  const int tn = productWidth(d);
+  const int64_t td = (d + tn - 1) / tn;
+  struct Side { int64_t tiles, k, area; int64_t slices[6]; };
+  Side x{(n + T - 1) / T * td, (v + BK - 1) / BK, (int64_t)n * d, {}}, w{(v + T - 1) / T * td, (n + BK - 1) / BK, (int64_t)v * d, {}};
+  if (!wantX) x.tiles = 0;
+  if (!wantW) w.tiles = 0;
+  const int64_t share = std::max<int64_t>(1, (x.tiles * std::max<int64_t>(x.k, STORE) + w.tiles * std::max<int64_t>(w.k, STORE)) / pairs);
+  for (Side* s : {&x, &w}) {
+    const int64_t most = std::max<int64_t>(1, s->k / 16);
+    for (int i = 0; i < 6; ++i)
+      s->slices[i] = std::min(most, i == 0 || !s->tiles || s->tiles >= 4 * pairs ? 1 : i == 5 ? (s->k + share - 1) / share : std::max<int64_t>(1, i * pairs / s->tiles));
+  }
+  VocabPlan best{(int)x.k, (int)w.k};
+  double least = 0.0;
+  for (int i = 0; i < 6; ++i)
+    for (int j = 0; j < 6; ++j) {
+      if ((i && x.slices[i] == x.slices[0]) || (j && w.slices[j] == w.slices[0])) continue;
+      const int64_t perX = (x.k + x.slices[i] - 1) / x.slices[i], perW = (w.k + w.slices[j] - 1) / w.slices[j];
+      const int64_t sx = (x.k + perX - 1) / perX, sw = (w.k + perW - 1) / perW;
+      const int64_t cx = std::max<int64_t>(perX, STORE), cw = std::max<int64_t>(perW, STORE);
+      const int64_t blocks = x.tiles ? longest(x.tiles * sx, cx, w.tiles * sw, cw, pairs) : longest(w.tiles * sw, cw, 0, 0, pairs);
+      auto join = [&](const Side& s, int64_t slices) { return s.tiles && slices > 1 ? 3.0 + (double)(slices * s.area * 8) / BYTES_US : 0.0; };
+      const double us = blocks * BLOCK_US * tn / T + join(x, sx) + join(w, sw);
+      if ((i | j) == 0 || us < least) { least = us; best = VocabPlan{(int)perX, (int)perW}; }
+    }
+  return best;
 }
 
 ncclResult_t vocabProducts(const void* dz, const void* x, const void* w, int n, int v, int d, const VocabPlan& plan, const VocabFactor& factor, const VocabExact* exact,

@@ -475,7 +475,8 @@ __global__ void __launch_bounds__(256) joinSlicesKernel(const float* part, int s
   const float scale = vocabFactor(factor);
   for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < packs; i += (size_t)gridDim.x * 256) {
     float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < slices; ++s) {
+#pragma unroll 8
+    for (int s = 0; s < slices; ++s) {                  // (eight on their way at a time: few rows leave few threads, and up to 49 slices)
       const float4* src = (const float4*)part + ((size_t)s * packs + i) * 2;
       const float4 x = src[0], y = src[1];
       f[0] += x.x; f[1] += x.y; f[2] += x.z; f[3] += x.w; f[4] += y.x; f[5] += y.y; f[6] += y.z; f[7] += y.w;
