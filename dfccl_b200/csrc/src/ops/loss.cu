@@ -397,11 +397,11 @@ __global__ void __launch_bounds__(256) scaleResultsKernel(uint4* a, size_t na, u
 // g rest x over all entries of its token.  Groups of threads that share a row's packs take a part of the entries each, in their order.  On the
 // way, what keepRowsKernel does.  (Every entry is compared with every other: the limit keeps that, and a token that all of them share,
 // beside the gradient of the logits, which runs at the same time.)
-constexpr int FEW_ENTRIES = 4096, OWN_THREADS = 256, OWN_WARPS = OWN_THREADS / 32;
+constexpr int FEW_ENTRIES = 2048, OWN_THREADS = 256, OWN_WARPS = OWN_THREADS / 32, AT_ONCE = 4;
 __global__ void __launch_bounds__(OWN_THREADS) ownSumsKernel(const uint4* x, const VocabRows rows, int n, int packs, int lanes, const float* rest, const float* gout,
                                                              int goutStride, float* sums, int* where, uint4* kept) {
   __shared__ int list[FEW_ENTRIES];
-  __shared__ int counts[OWN_WARPS];
+  __shared__ int counts[AT_ONCE][OWN_WARPS];
   __shared__ float part[OWN_THREADS][9];
   tc::grid_dependency_wait();
   tc::grid_launch_dependents();
@@ -415,17 +415,29 @@ __global__ void __launch_bounds__(OWN_THREADS) ownSumsKernel(const uint4* x, con
   const int token = tokenOf(own);
   if (token == VOCAB_NO_TOKEN) return;
   int count = 0;
-  for (int base = 0; base < entries; base += OWN_THREADS) {
-    const int e = base + threadIdx.x;
-    const bool same = e < entries && tokenOf(e) == token;
-    if (__syncthreads_or(same && e < own)) return;       // not the first
-    const uint32_t votes = __ballot_sync(0xffffffffu, same);
-    if (lane == 0) counts[warp] = __popc(votes);
-    __syncthreads();
-    int at = count + __popc(votes & ((1u << lane) - 1));
+  for (int base = 0; base < entries; base += OWN_THREADS * AT_ONCE) {
+    bool same[AT_ONCE], front = false;
 #pragma unroll
-    for (int w = 0; w < OWN_WARPS; ++w) { at += w < warp ? counts[w] : 0; count += counts[w]; }
-    if (same) list[at] = e;
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int e = base + u * OWN_THREADS + threadIdx.x;
+      same[u] = e < entries && tokenOf(e) == token;
+      front = front || (same[u] && e < own);
+    }
+    if (__syncthreads_or(front)) return;                 // not the first
+    uint32_t votes[AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      votes[u] = __ballot_sync(0xffffffffu, same[u]);
+      if (lane == 0) counts[u][warp] = __popc(votes[u]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      int at = count + __popc(votes[u] & ((1u << lane) - 1));
+#pragma unroll
+      for (int w = 0; w < OWN_WARPS; ++w) { at += w < warp ? counts[u][w] : 0; count += counts[u][w]; }
+      if (same[u]) list[at] = base + u * OWN_THREADS + threadIdx.x;
+    }
   }
   __syncthreads();
   if (threadIdx.x == 0) where[token] = own;
@@ -511,10 +523,12 @@ struct BackwardPlan {
   int slicesX, slicesW;           // of dx those of a whole piece: a shorter last one has fewer and adds to the first of them
   bool sumX, sumW;                // fp32 sums in memory: of dx because there are pieces or slices, of dw because there are slices
   int exact;                      // what the entries add to the results: 0 through dz, 1 by ownSumsKernel, 2 by sorted tokens
-  size_t dz, partX, partW, kept, sums, where, tokens;     // bytes
-  size_t all() const { return dz + partX + partW + kept + sums + where + tokens; }
+  size_t dz, partX, partW, kept, sums, where, tokens, listed;     // bytes
+  size_t all() const { return dz + partX + partW + kept + sums + where + tokens + listed; }
 };
-// k = 0: targets.  Lists of more rows go through dz: their entries' roundings are many, and less than that of the results together.
+// k = 0: targets.  More of them go by sorted tokens (us, GPU, both gradients by themselves / sorted: 2048 x 2000 x 64 44 / 51, 4096 68 / 61).  Longer
+// lists go through dz: their entries' roundings are many, and less than that of the results together (256 lists of 8, 2000 x 64: 58 / through dz 40,
+// 512: 75 / 40).
 BackwardPlan backwardPlan(int n, int v, int d, int k, bool wantX, bool wantW) {
   BackwardPlan p;
   const int64_t limit = std::max<int64_t>(1 << 20, paramI64("LOSS_WORKSPACE_BYTES", 1ll << 30));
@@ -535,6 +549,7 @@ BackwardPlan backwardPlan(int n, int v, int d, int k, bool wantX, bool wantW) {
   p.sums = p.exact && wantW ? up256((size_t)entries * d * 4) : 0;
   p.where = p.exact && wantW ? up256((size_t)v * 4) : 0;
   p.tokens = p.exact == 2 && wantW ? tokenSumsWork(n, d) : 0;
+  p.listed = p.exact && wantX && k > 4 ? up256((size_t)n * d * 4) : 0;
   return p;
 }
 
@@ -629,8 +644,10 @@ DF_API ncclResult_t dfcclLinearLossBackward(const void* x, const void* w, int n,
   float* sums = (float*)(at + p.kept);
   int* where = (int*)(at + p.kept + p.sums);
   void* sorted = at + p.kept + p.sums + p.where;
+  float* listed = p.listed ? (float*)(at + p.kept + p.sums + p.where + p.tokens) : nullptr;
   const VocabRows rows = rowsOf(targets, wide, v, ignore, tokens, weights, state, k, temperature, 0);
   const float* rowGout = goutStride ? (const float*)gout : nullptr;
+  if (listed) CUDACHECK(launchBehind(listSumsKernel, std::min(n, 148 * 16), 128, stream, (const uint4*)w, rows, (const float*)rest, n, d / 8, (float4*)listed));
   if (dw && p.exact == 1) {
     int lanes = 8;
     while (lanes < OWN_THREADS && lanes < d / 8) lanes *= 2;
@@ -645,7 +662,7 @@ DF_API ncclResult_t dfcclLinearLossBackward(const void* x, const void* w, int n,
   }
   const VocabGrad grad{(const float*)lse, rowGout, goutStride, p.exact ? nullptr : (const float*)rest};
   VocabExact exact{rows, nullptr, (const float*)rest, rowGout, goutStride, (const __nv_bfloat16*)w, sums, where,
-                   p.exact == 2 && dw ? tokenSortItems(n, d, v, sorted) : nullptr, p.exact == 1 ? n * k : n, 0, false, nullptr};
+                   p.exact == 2 && dw ? tokenSortItems(n, d, v, sorted) : nullptr, p.exact == 1 ? n * k : n, 0, false, listed};
   const VocabExact* add = p.exact ? &exact : nullptr;
   const VocabFactor factor{goutStride ? nullptr : (const float*)gout, (const int*)count, temperature};
   for (int c = 0; c < v; c += p.cols) {

@@ -13,12 +13,14 @@ from .block import packed
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 MAX_LIST = 256                       # entries of a teacher's list
-# Rows x vocabulary x width from which a reduced loss makes its gradients with the loss, and how many times that for lists, of at most a share
-# of the vocabulary.  GPU time in us, logits computed twice / once, 50257 entries: targets 256 x 768 144 / 146, 512 x 768 174 / 168, 1024 x 768 258 / 221,
-# 2048 x 1024 587 / 461; lists of 8 1024 x 768 248 / 250, 2048 x 768 444 / 390, of 32 1024 x 768 262 / 322, 2048 x 768 483 / 457, of 48 4096 x 1024 1216 / 1130,
-# of 256 1814 / 1919 (the sorting of the entries); 16384 x 2000 x 1024 278 / 237.
-ONE_GO_FROM = 2 ** 34
-LISTS_TIMES = 4
+# Rows x vocabulary (counted as SMALL_VOCABULARY at least) above which a reduced loss makes its gradients with the loss, and how many times that
+# for lists, of at most a share of the vocabulary.  GPU time in us, logits computed twice / once: targets 512 x 50257 x 64 75 / 79, 1024 x 50257 x 64
+# 115 / 108, x 256 140 / 132, 2048 x 2000 x 256 59 / 62, 3000 x 2000 x 256 75 / 68, 3000 x 500 x 64 62 / 54; 50257 entries x 256, lists of 8 1024 138 / 143,
+# 1500 179 / 175, 2048 230 / 220, of 32 1024 158 / 171, 1500 206 / 208, 2048 272 / 258; 8192 x 8000 x 256, lists of 8 185 / 197, of 32 269 / 305; 4096 x 50257
+# x 1024, lists of 48 1216 / 1130, of 256 1814 / 1919 (the sorting of the entries).
+ONE_GO_FROM = 2 ** 25
+SMALL_VOCABULARY = 14000            # of 2400 rows
+LISTS_TIMES = 2
 LIST_SHARE = 1024
 MOST_ENTRIES = 2 ** 31 - 4096        # of all lists together, as their sorting counts them
 
@@ -78,7 +80,7 @@ def _forward(x, weight, rows, reduction):
     n, device = x.numel() // d, x.device
     xp, wp = packed(x), packed(weight)
     kept = torch.empty(n + 1 + n * rows.k, dtype=torch.float32, device=device)      # log2 of the sums, the number of rows that count, what is left of the weights
-    loss = torch.empty(() if reduction else x.shape[:-1], dtype=torch.float32, device=device)
+    loss = kept.new_empty(() if reduction else x.shape[:-1])
     if n:
         at, out = kept.data_ptr(), loss.data_ptr()
         with on_device(device):
@@ -97,9 +99,9 @@ def _forward_with_gradients(x, weight, rows, reduction, want_x, want_w):
     n, device = x.numel() // d, x.device
     xp, wp = packed(x), packed(weight)
     kept = torch.empty(n + 1 + n * rows.k, dtype=torch.float32, device=device)
-    loss = torch.empty((), dtype=torch.float32, device=device)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=device) if want_x else None
-    dw = torch.empty(v, d, dtype=x.dtype, device=device) if want_w else None
+    loss = kept.new_empty(())
+    dx = torch.empty_like(xp) if want_x else None
+    dw = torch.empty_like(wp) if want_w else None
     at = kept.data_ptr()
     with on_device(device):
         size = nv.lib().dfcclLinearLossWithGradientsWork(n, v, d, rows.k, want_x, want_w)
@@ -128,15 +130,18 @@ class _LinearLossFn(torch.autograd.Function):
     def forward(ctx, x, weight, rows, reduction):
         want_x, want_w = ctx.needs_input_grad[:2]
         ctx.grads = None
-        from_size = ONE_GO_FROM if rows.lists is None else ONE_GO_FROM * LISTS_TIMES
-        few = rows.lists is None or (rows.k * LIST_SHARE <= weight.shape[0] and rows.lists[0].numel() <= MOST_ENTRIES)
-        if reduction and (want_x or want_w) and x.numel() * weight.shape[0] >= from_size and few:
+        n, v = x.numel() // weight.shape[1], weight.shape[0]
+        if rows.lists is None:
+            one_go = n * max(v, SMALL_VOCABULARY) > ONE_GO_FROM
+        else:
+            one_go = n * v > ONE_GO_FROM * LISTS_TIMES and rows.k * LIST_SHARE <= v and n * rows.k <= MOST_ENTRIES
+        if reduction and (want_x or want_w) and one_go:
             loss, xp, wp, kept, ctx.grads = _forward_with_gradients(x, weight, rows, reduction, want_x, want_w)
             ctx.capture = nv.lib().dfcclCaptureId(stream_of(x))
         else:
             loss, xp, wp, kept = _forward(x, weight, rows, reduction)
         ctx.save_for_backward(xp, wp, kept, *rows.tensors())
-        ctx.rows, ctx.mean, ctx.shape = rows, reduction == 1, x.shape
+        ctx.rows, ctx.mean = rows, reduction == 1
         ctx.set_materialize_grads(False)
         return loss
 
@@ -155,8 +160,8 @@ class _LinearLossFn(torch.autograd.Function):
         if n == 0:
             return torch.zeros_like(x) if want_x else None, torch.zeros_like(w) if want_w else None, None, None
         g = g.reshape(-1) if g.dim() else g
-        dx = torch.empty(ctx.shape, dtype=x.dtype, device=device) if want_x else None
-        dw = torch.empty(v, d, dtype=x.dtype, device=device) if want_w else None
+        dx = torch.empty_like(x) if want_x else None
+        dw = torch.empty_like(w) if want_w else None
         with on_device(device):
             size = nv.lib().dfcclLinearLossBackwardWork(n, v, d, 0 if ctx.rows.lists is None else ctx.rows.k, want_x, want_w)
             work = torch.empty(size, dtype=torch.uint8, device=device)
