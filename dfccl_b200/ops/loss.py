@@ -58,33 +58,36 @@ def _forward_work(n: int, v: int, k: int) -> int:
 
 
 class _Rows:
-    """What the rows are compared with, as the C interface takes it: a target each, or lists of ``k`` entries."""
-    __slots__ = ("targets", "ignore", "lists", "k", "temperature")
+    """What the rows are compared with, as the C interface takes it: a target each, or lists of ``k`` entries (of ``entries`` in
+    all: their tokens, behind them their weights, behind those the rows' states, 32 bits each)."""
+    __slots__ = ("targets", "ignore", "lists", "entries", "k", "temperature")
 
-    def __init__(self, targets, ignore, lists, k, temperature):
-        self.targets, self.ignore, self.lists, self.k, self.temperature = targets, ignore, lists, k, temperature
+    def __init__(self, targets, ignore, lists, entries, k, temperature):
+        self.targets, self.ignore, self.lists, self.entries, self.k, self.temperature = targets, ignore, lists, entries, k, temperature
 
-    def tensors(self):
-        return (self.targets,) if self.lists is None else self.lists
+    def tensor(self):
+        return self.targets if self.lists is None else self.lists
 
     def args(self):
         if self.lists is None:
             return self.targets.data_ptr(), int(self.targets.dtype == torch.int64), self.ignore, None, None, None, 1, 1.0
-        tokens, weights, state = self.lists
-        return None, 0, 0, tokens.data_ptr(), weights.data_ptr(), state.data_ptr(), self.k, self.temperature
+        at = self.lists.data_ptr()
+        return None, 0, 0, at, at + 4 * self.entries, at + 8 * self.entries, self.k, self.temperature
 
 
-def _forward(x, weight, rows, reduction):
-    """(loss, x and weight as the kernels read them, what the backward pass needs of the sums)."""
+def _forward(x, weight, rows, reduction, keep):
+    """(loss, x and weight as the kernels read them, what the backward pass needs of the sums where ``keep`` is set)."""
     v, d = weight.shape
     n, device = x.numel() // d, x.device
     xp, wp = packed(x), packed(weight)
-    kept = torch.empty(n + 1 + n * rows.k, dtype=torch.float32, device=device)      # log2 of the sums, the number of rows that count, what is left of the weights
+    # log2 of the sums, the number of rows that count, what is left of the weights; where nobody wants them, behind the workspace
+    words, behind = n + 1 + n * rows.k, 0 if keep or not n else _forward_work(n, v, rows.k) // 4
+    kept = torch.empty(behind + words, dtype=torch.float32, device=device)
     loss = kept.new_empty(() if reduction else x.shape[:-1])
     if n:
-        at, out = kept.data_ptr(), loss.data_ptr()
+        at, out = kept.data_ptr() + 4 * behind, loss.data_ptr()
         with on_device(device):
-            work = torch.empty(_forward_work(n, v, rows.k), dtype=torch.uint8, device=device)
+            work = kept if behind else torch.empty(_forward_work(n, v, rows.k), dtype=torch.uint8, device=device)
             nv.check(nv.long_entry("dfcclLinearLossForward")(xp.data_ptr(), wp.data_ptr(), n, v, d, *rows.args(), reduction, work.data_ptr(), at, at + 4 * (n + 1),
                                                              None if reduction else out, out if reduction else None, at + 4 * n if reduction else None,
                                                              stream_of(x)), "dfcclLinearLossForward")
@@ -134,13 +137,13 @@ class _LinearLossFn(torch.autograd.Function):
         if rows.lists is None:
             one_go = n * max(v, SMALL_VOCABULARY) > ONE_GO_FROM
         else:
-            one_go = n * v > ONE_GO_FROM * LISTS_TIMES and rows.k * LIST_SHARE <= v and n * rows.k <= MOST_ENTRIES
+            one_go = n * v > ONE_GO_FROM * LISTS_TIMES and rows.k * LIST_SHARE <= v and rows.entries <= MOST_ENTRIES
         if reduction and (want_x or want_w) and one_go:
             loss, xp, wp, kept, ctx.grads = _forward_with_gradients(x, weight, rows, reduction, want_x, want_w)
             ctx.capture = nv.lib().dfcclCaptureId(stream_of(x))
         else:
-            loss, xp, wp, kept = _forward(x, weight, rows, reduction)
-        ctx.save_for_backward(xp, wp, kept, *rows.tensors())
+            loss, xp, wp, kept = _forward(x, weight, rows, reduction, True)
+        ctx.save_for_backward(xp, wp, kept, rows.tensor())
         ctx.rows, ctx.mean = rows, reduction == 1
         ctx.set_materialize_grads(False)
         return loss
@@ -175,7 +178,7 @@ class _LinearLossFn(torch.autograd.Function):
 def _loss(x, weight, rows, reduction):
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _LinearLossFn.apply(x, weight, rows, REDUCTIONS[reduction])
-    return _forward(x, weight, rows, REDUCTIONS[reduction])[0]
+    return _forward(x, weight, rows, REDUCTIONS[reduction], False)[0]
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
@@ -191,7 +194,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     if targets.shape != x.shape[:-1]:
         raise ValueError(f"targets of {tuple(targets.shape)} for x of {tuple(x.shape)}")
     _on_one_gpu(x.device, weight, targets)
-    return _loss(x, weight, _Rows(targets.contiguous(), ignore_index, None, 1, 1.0), reduction)
+    return _loss(x, weight, _Rows(targets.contiguous(), ignore_index, None, targets.numel(), 1, 1.0), reduction)
 
 
 def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor, teacher_tokens: torch.Tensor, *, temperature: float = 1.0,
@@ -218,10 +221,10 @@ def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_logits: t
     _on_one_gpu(device, weight, teacher_logits, teacher_tokens)
     n, v = teacher_tokens.numel() // k, weight.shape[0]
     lists = torch.empty(2 * n * k + n, dtype=torch.int32, device=device)
-    tokens, weights, state = lists[:n * k], lists[n * k:2 * n * k].view(torch.float32), lists[2 * n * k:]
+    rows = _Rows(None, 0, lists, n * k, k, temperature)
     logits, listed = teacher_logits.detach().contiguous(), teacher_tokens.contiguous()
     if n:
         with on_device(device):
             nv.check(nv.long_entry("dfcclTeacherRows")(logits.data_ptr(), nccl_dtype(logits.dtype), listed.data_ptr(), int(listed.dtype == torch.int64), n, k, v,
-                                               temperature, tokens.data_ptr(), weights.data_ptr(), state.data_ptr(), stream_of(x)), "dfcclTeacherRows")
-    return _loss(x, weight, _Rows(None, 0, (tokens, weights, state), k, temperature), reduction)
+                                               temperature, *rows.args()[3:6], stream_of(x)), "dfcclTeacherRows")
+    return _loss(x, weight, rows, reduction)
