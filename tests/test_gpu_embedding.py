@@ -132,6 +132,26 @@ def test_a_table_of_one_row_with_any_stride():
     assert torch.equal(embedding(ids, one, positions=ids, position_weight=one), 2 * one.expand(3, 40))
 
 
+def test_tables_and_results_of_more_elements_than_31_bits_count():
+    from dfccl_b200.ops.embedding import embedding
+    rows, d = 530003, 4096
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    small = torch.randn(100, d, generator=gen, device="cuda").to(torch.bfloat16).requires_grad_(True)
+    ids = torch.randint(0, 100, (rows,), generator=gen, device="cuda")
+    out = embedding(ids, small)
+    assert torch.equal(out[-1000:], small[ids[-1000:]])
+    g = torch.zeros(rows, d, dtype=torch.bfloat16, device="cuda")
+    g[-1000:] = 1
+    assert torch.equal(torch.autograd.grad(out, [small], g)[0][:, 7].float(), torch.bincount(ids[-1000:], minlength=100).float())
+    del out
+    large = g.requires_grad_(True)                            # its last rows are ones, the others zeros
+    ids = torch.tensor([rows - 1, 0, rows - 2, rows - 1, rows - 1001], device="cuda")
+    out = embedding(ids, large)
+    assert out[:, -1].tolist() == [1.0, 0.0, 1.0, 1.0, 0.0]
+    grad = torch.autograd.grad(out, [large], torch.ones_like(out))[0]
+    assert grad[[0, 1, rows - 1001, rows - 2, rows - 1], -1].tolist() == [1.0, 0.0, 1.0, 1.0, 2.0] and grad.sum(dtype=torch.float64).item() == 5.0 * d
+
+
 def test_other_stream_and_graph():
     """On a stream of its own; forward and backward captured and replayed for other tokens, beside a second graph."""
     from dfccl_b200.ops.embedding import embedding

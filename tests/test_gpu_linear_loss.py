@@ -552,6 +552,32 @@ def test_many_rows_and_wide_ones():
     assert check_kernels()
 
 
+@pytest.mark.parametrize("one_go", [False, True])
+def test_a_head_of_more_elements_than_31_bits_count(one_go, monkeypatch):
+    """The last rows of the vocabulary, where the offsets of w and of its gradient need 64 bits, and dx, which sums over all of it."""
+    from dfccl_b200.ops import loss as module
+    from dfccl_b200.ops.loss import linear_cross_entropy
+    monkeypatch.setattr(module, "ONE_GO_FROM", 0 if one_go else 1 << 60)
+    n, v, d, last = 40, 530003, 4096, 64
+    gen = torch.Generator(device="cuda").manual_seed(71)
+    x = torch.randn(n, d, generator=gen, device="cuda").to(torch.bfloat16).requires_grad_(True)
+    w = (torch.randn(v, d, generator=gen, device="cuda", dtype=torch.bfloat16) * 0.03125).requires_grad_(True)
+    t = torch.randint(0, v, (n,), generator=gen, device="cuda")
+    t[::2] = v - 1 - torch.arange(n // 2, device="cuda")
+    loss = linear_cross_entropy(x, w, t)
+    dx, dw = torch.autograd.grad(loss, [x, w])
+    xd, cuts = x.detach().double(), range(0, v, 65536)
+    z = torch.cat([xd @ w.detach()[c:c + 65536].double().t() for c in cuts], dim=1)
+    assert abs(loss.item() - torch.nn.functional.cross_entropy(z, t).item()) <= 1e-5 * loss.item()
+    dz = torch.softmax(z, dim=1).scatter_add(1, t[:, None], torch.full((n, 1), -1.0, dtype=torch.float64, device="cuda")) / n
+    want = sum(dz[:, c:c + 65536] @ w.detach()[c:c + 65536].double() for c in cuts)
+    # (each result two roundings, as everywhere above)
+    assert (dx.double() - want).norm() <= 2.0 ** -8 * want.norm()
+    for rows in (slice(0, last), slice(v - last, v)):
+        want = dz[:, rows].t() @ xd
+        assert (dw[rows].double() - want).norm() <= 2.0 ** -8 * want.norm()
+
+
 def test_calls_on_two_streams_at_once():
     """Two losses and an embedding on streams of their own, in flight together, each as by itself."""
     from dfccl_b200.ops.embedding import embedding
