@@ -1,7 +1,8 @@
 // Products over a large vocabulary for the losses of a language model's head, on CTA pairs (tcgen05 cta_group::2), bf16 with fp32
 // accumulators in tensor memory.  With z = x w^T, x [n, d] and the head w [v, d]:
-//   VOCAB_STATS     of every row the maximum and the sum of powers of each stretch of its logits, and the logits of its targets
-//   VOCAB_GRAD      dz = g (softmax(z) - target): the logits are computed again, what is stored is their gradient, rounded once
+//   VOCAB_STATS     of every row the maximum and the sum of powers of each stretch of its logits, without those of its targets
+//   VOCAB_GRAD      dz = g (softmax(z) - target): the logits are computed again, what is stored is their gradient, rounded once (in the targets' places 0,
+//                   or theirs: vocab.h)
 //   VOCAB_POWERS    powers of the logits relative to a number known in front of the product (the largest logit of the row's list), and their
 //                   sums: the logits are not computed again, for rows whose gradients are wanted with the loss
 //   VOCAB_PRODUCTS  dx = dz w and dw = dz^T x, in one launch
