@@ -161,12 +161,29 @@ template <bool POWERS>
 __global__ void __launch_bounds__(1024) joinRowsKernel(const JoinArgs a) {
   __shared__ float2 part[32][33];
   __shared__ int last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row0 = blockIdx.x * 32, row = row0 + warp;
+  const size_t list = (size_t)row * a.rows.k;
+  // The rows' lists are older than the launches that run beside this one (those have waited for them): their way is over when the parts come.
+  int st = ROW_NONE, token = VOCAB_NO_TOKEN, tokenFront = VOCAB_NO_TOKEN;
+  float weight = 0.f;
+  if (row < a.n) {
+    st = rowState(a.rows, row, token);
+    if (!a.rows.targets && lane < a.rows.k) {
+      token = a.rows.tokens[list + lane];
+      tokenFront = lane ? a.rows.tokens[list + lane - 1] : VOCAB_NO_TOKEN;
+      weight = a.rows.weights[list + lane];
+    }
+  }
   tc::grid_dependency_wait();
   tc::grid_launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row0 = blockIdx.x * 32;
+  auto tokenAt = [&](int i) { return i == lane ? token : a.rows.tokens[list + i]; };
+  auto frontOf = [&](int i) { return i == lane ? tokenFront : a.rows.tokens[list + i - 1]; };
+  auto weightAt = [&](int i) { return i == lane ? weight : a.rows.weights[list + i]; };
   auto join = [](float2 x, float2 y) { return POWERS ? make_float2(fmaxf(x.x, y.x), x.y + y.y) : joined(x, y); };
   if (!a.only || *a.only) {
     float2 acc = make_float2(-INFINITY, 0.f);
+    const float mine = row < a.n && lane < a.rows.k ? a.picked[list + lane] : 0.f, base = POWERS && row < a.n ? a.base[row] : 0.f;
+    auto pickedAt = [&](int i) { return i == lane ? mine : a.picked[list + i]; };
     if (row0 + lane < a.n) {
       for (int i = warp; i < a.stretches; i += 32 * 8) {
         float2 p[8];
@@ -178,22 +195,19 @@ __global__ void __launch_bounds__(1024) joinRowsKernel(const JoinArgs a) {
     }
     part[warp][lane] = acc;
     __syncthreads();
-    const int row = row0 + warp;
     if (row < a.n) {
       acc = part[lane][warp];
 #pragma unroll
       for (int o = 16; o; o >>= 1) acc = join(acc, make_float2(__shfl_xor_sync(0xffffffffu, acc.x, o), __shfl_xor_sync(0xffffffffu, acc.y, o)));
-      const int st = rowState(a.rows, row);
       float sum = 0.f, share = st == ROW_BAD ? __int_as_float(0x7fffffff) : 1.f;
-      const size_t list = (size_t)row * a.rows.k;
-      const float2 others = POWERS ? make_float2(a.base[row], acc.y) : acc;             // of entries that the list has not
+      const float2 others = POWERS ? make_float2(base, acc.y) : acc;             // of entries that the list has not
       float2 every = others;
       int distinct = 0;
       if (st == ROW_LIST) {                             // the list's own powers, each token once
         float2 own = make_float2(-INFINITY, 0.f);
         for (int i = lane; i < a.rows.k; i += 32) {
-          if (!a.rows.targets && (a.rows.tokens[list + i] == VOCAB_NO_TOKEN || (i && a.rows.tokens[list + i] == a.rows.tokens[list + i - 1]))) continue;
-          own = joined(own, make_float2(a.picked[list + i] * a.rows.scale, 1.f));
+          if (!a.rows.targets && (tokenAt(i) == VOCAB_NO_TOKEN || (i && tokenAt(i) == frontOf(i)))) continue;
+          own = joined(own, make_float2(pickedAt(i) * a.rows.scale, 1.f));
           ++distinct;
         }
 #pragma unroll
@@ -205,9 +219,9 @@ __global__ void __launch_bounds__(1024) joinRowsKernel(const JoinArgs a) {
       }
       const float l = every.x + log2f(every.y);
       if (distinct == 1) {                              // all on one token: from the others' powers, however small they are beside its own
-        const float u = a.picked[list] * a.rows.scale, ratio = others.y * exp2f(others.x - u);
+        const float u = __shfl_sync(0xffffffffu, mine, 0) * a.rows.scale, ratio = others.y * exp2f(others.x - u);
         for (int i = lane; i < a.rows.k; i += 32) {
-          const float q = a.rows.targets || a.rows.tokens[list + i] == VOCAB_NO_TOKEN ? 1.f : a.rows.weights[list + i];
+          const float q = a.rows.targets || tokenAt(i) == VOCAB_NO_TOKEN ? 1.f : weightAt(i);
           if (q != 0.f) sum += q * logf(q);             // (of entries that share the token)
           a.rest[list + i] = i ? 0.f : others.y * exp2f(others.x - l);
         }
@@ -215,12 +229,12 @@ __global__ void __launch_bounds__(1024) joinRowsKernel(const JoinArgs a) {
       } else {
         for (int i = lane; i < a.rows.k; i += 32) {
           float rest = 0.f;
-          if (st == ROW_LIST && a.rows.tokens[list + i] != VOCAB_NO_TOKEN) {
-            const int t = a.rows.tokens[list + i];
-            float q = a.rows.weights[list + i];
-            const float u = a.picked[list + i] * a.rows.scale - l;
+          if (st == ROW_LIST && tokenAt(i) != VOCAB_NO_TOKEN) {
+            const int t = tokenAt(i);
+            float q = weightAt(i);
+            const float u = pickedAt(i) * a.rows.scale - l;
             if (q != 0.f) sum += q * (logf(q) - u * LN2);         // (0 ln 0)
-            if (i == 0 || a.rows.tokens[list + i - 1] != t) {
+            if (i == 0 || frontOf(i) != t) {
               for (int j = i + 1; j < a.rows.k && a.rows.tokens[list + j] == t; ++j) q += a.rows.weights[list + j];
               rest = q - exp2f(u);
             }
