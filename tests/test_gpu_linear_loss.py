@@ -3,6 +3,7 @@
 What may be off, by arithmetic: a logit of d terms is added up in fp32 in steps of 16, each at most one step of its type (2**-23 of the
 magnitudes' sum) off; a power of two or logarithm is a few of those; a gradient of a logit is rounded once to bf16 (2**-8 at most, less
 than 2**-9 in the 2-norm over many), the gradients of x and weight once more."""
+import pathlib
 import subprocess
 import sys
 
@@ -485,7 +486,7 @@ torch.empty(1 << 24, device="cuda")
 linear_cross_entropy(x, w, torch.arange(5, device="cuda")).backward()
 assert x.grad.isfinite().all() and (x.grad != 0).any()
 """
-    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=pathlib.Path(__file__).parents[1])
     assert run.returncode == 0, run.stderr[-2000:]
 
 
