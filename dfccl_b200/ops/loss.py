@@ -17,10 +17,12 @@ MAX_LIST = 256                       # entries of a teacher's list
 # for lists, of at most a share of the vocabulary.  GPU time in us, logits computed twice / once: targets 512 x 50257 x 64 75 / 79, 1024 x 50257 x 64
 # 115 / 108, x 256 140 / 132, 2048 x 2000 x 256 59 / 62, 3000 x 2000 x 256 75 / 68, 3000 x 500 x 64 62 / 54; 50257 entries x 256, lists of 8 1024 138 / 143,
 # 1500 179 / 175, 2048 230 / 220, of 32 1024 158 / 171, 1500 206 / 208, 2048 272 / 258; 8192 x 8000 x 256, lists of 8 185 / 197, of 32 269 / 305; 4096 x 50257
-# x 1024, lists of 48 1216 / 1130, of 256 1814 / 1919 (the sorting of the entries).
+# x 1024, lists of 48 1216 / 1130, of 256 1814 / 1919 (the sorting of the entries).  Targets over a head whose way from memory takes longer than what one go
+# has more to launch: 64 x 50257 x 512 97 / 102, x 768 110 / 108, x 1024 134 / 132; 512 x 50257 x 1024 220 / 203; 64 x 131072 x 1024 279 / 251, x 4096 996 / 840.
 ONE_GO_FROM = 2 ** 25
 SMALL_VOCABULARY = 14000            # of 2400 rows
 LISTS_TIMES = 2
+LARGE_HEAD = 0.8                     # of 2 ** 25 / 0.8 elements
 LIST_SHARE = 1024
 MOST_ENTRIES = 2 ** 31 - 4096        # of all lists together, as their sorting counts them
 
@@ -135,10 +137,10 @@ class _LinearLossFn(torch.autograd.Function):
         ctx.grads = None
         n, v = x.numel() // weight.shape[1], weight.shape[0]
         if rows.lists is None:
-            one_go = n * max(v, SMALL_VOCABULARY) > ONE_GO_FROM
+            one_go = n * max(v, SMALL_VOCABULARY) > ONE_GO_FROM or weight.numel() * LARGE_HEAD > ONE_GO_FROM
         else:
             one_go = n * v > ONE_GO_FROM * LISTS_TIMES and rows.k * LIST_SHARE <= v and rows.entries <= MOST_ENTRIES
-        if reduction and (want_x or want_w) and one_go:
+        if n and reduction and (want_x or want_w) and one_go:
             loss, xp, wp, kept, ctx.grads = _forward_with_gradients(x, weight, rows, reduction, want_x, want_w)
             ctx.capture = nv.lib().dfcclCaptureId(stream_of(x))
         else:

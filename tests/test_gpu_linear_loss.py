@@ -475,6 +475,22 @@ def test_one_gradient_of_two(lists, one_go, monkeypatch):
             assert bool(((a.double() - b.double()).abs() <= 2.0 ** -7 * b.double().abs() + 1e-6 * b.double().abs().max()).all())
 
 
+@pytest.mark.parametrize("one_go", [False, True])
+def test_no_rows(one_go, monkeypatch):
+    from dfccl_b200.ops import loss as module
+    from dfccl_b200.ops.loss import linear_cross_entropy, linear_distillation
+    monkeypatch.setattr(module, "ONE_GO_FROM", 0 if one_go else 1 << 60)
+    monkeypatch.setattr(module, "LIST_SHARE", 0)
+    x = torch.empty(0, 4, 64, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    w = torch.ones(300, 64, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    none = torch.empty(0, 4, 2, dtype=torch.int64, device="cuda")
+    for reduction in ("none", "sum", "mean"):
+        for loss in (linear_cross_entropy(x, w, none[..., 0], reduction=reduction), linear_distillation(x, w, none.float(), none, reduction=reduction)):
+            assert loss.shape == ((0, 4) if reduction == "none" else ()) and loss.sum().item() == 0.0
+            dx, dw = torch.autograd.grad(loss.sum(), [x, w])
+            assert dx.shape == x.shape and bool((dw == 0).all())
+
+
 def test_first_backward_pass_of_a_process_with_a_frozen_head():
     """The thread of backward passes has made no call of the CUDA runtime yet."""
     code = """
