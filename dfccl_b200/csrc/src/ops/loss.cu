@@ -23,6 +23,7 @@ namespace dfccl {
 namespace {
 
 constexpr int MAX_LIST = 256;          // entries of a teacher's list
+constexpr int MOST_SORTED = 0x7fffffff - 4096;      // entries of all lists together that are sorted, as 31 bits count them
 constexpr int ROWS = 16384;            // rows of a forward product at a time: bounds its partial sums (26 MB at 50257 columns)
 constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
 
@@ -537,12 +538,13 @@ struct BackwardPlan {
   int slicesX, slicesW;           // of dx those of a whole piece: a shorter last one has fewer and adds to the first of them
   bool sumX, sumW;                // fp32 sums in memory: of dx because there are pieces or slices, of dw because there are slices
   int exact;                      // what the entries add to the results: 0 through dz, 1 by ownSumsKernel, 2 by sorted tokens
+  bool dense;                     // of the sorted entries' sums there is a row for every token of the vocabulary
   size_t dz, partX, partW, kept, sums, where, tokens, listed;     // bytes
   size_t all() const { return dz + partX + partW + kept + sums + where + tokens + listed; }
 };
-// k = 0: targets.  More of them go by sorted tokens (us, GPU, both gradients by themselves / sorted: 2048 x 2000 x 64 44 / 51, 4096 68 / 61).  Longer
-// lists go through dz: their entries' roundings are many, and less than that of the results together (256 lists of 8, 2000 x 64: 58 / through dz 40,
-// 512: 75 / 40).
+// k = 0: targets.  More entries go by sorted tokens (us, GPU, both gradients by themselves / sorted: targets 2048 x 2000 x 64 44 / 51, 4096 68 / 61).
+// That costs lists up to as much as one product (1777 x 30011 x 640, lists of 17: 287 us; with the lists' shares rounded to bf16 in dz 238, and both
+// gradients 2.3e-3 off instead of 1.7e-3, which is what rounding the results costs).  Only entries that 31 bits do not count go through dz.
 BackwardPlan backwardPlan(int n, int v, int d, int k, bool wantX, bool wantW) {
   BackwardPlan p;
   const int64_t limit = std::max<int64_t>(1 << 20, paramI64("LOSS_WORKSPACE_BYTES", 1ll << 30));
@@ -559,10 +561,11 @@ BackwardPlan backwardPlan(int n, int v, int d, int k, bool wantX, bool wantW) {
   p.partW = p.sumW ? up256((size_t)p.slicesW * p.cols * d * 4) : 0;
   p.kept = wantW ? up256((size_t)n * d * 2) : 0;
   const int64_t entries = (int64_t)n * std::max(1, k);
-  p.exact = entries <= FEW_ENTRIES ? 1 : k == 0 ? 2 : 0;
-  p.sums = p.exact && wantW ? up256((size_t)entries * d * 4) : 0;
+  p.exact = entries <= FEW_ENTRIES ? 1 : entries <= MOST_SORTED ? 2 : 0;
+  p.dense = p.exact == 2 && entries > v;
+  p.sums = p.exact && wantW ? up256((p.dense ? (size_t)v : (size_t)entries) * d * 4) : 0;
   p.where = p.exact && wantW ? up256((size_t)v * 4) : 0;
-  p.tokens = p.exact == 2 && wantW ? tokenSumsWork(n, d) : 0;
+  p.tokens = p.exact == 2 && wantW ? tokenSumsWork((int)entries, d) : 0;
   p.listed = p.exact && wantX && k > 4 ? up256((size_t)n * d * 4) : 0;
   return p;
 }
@@ -669,14 +672,14 @@ DF_API ncclResult_t dfcclLinearLossBackward(const void* x, const void* w, int n,
                            (uint4*)kept));
   } else if (dw) {
     if (p.exact) {
-      DFCHECK(tokenSort(n, d, targets, wide, ignore, v, sorted, stream));
-      DFCHECK(tokenSums(x, n, d, 1, v, (const float*)rest, rowGout, goutStride, sums, false, where, sorted, stream));
+      DFCHECK(targets ? tokenSort(n, d, targets, wide, ignore, v, sorted, stream) : tokenSort(n * k, d, tokens, 0, -1, v, sorted, stream));
+      DFCHECK(tokenSums(x, n * k, d, k, v, (const float*)rest, rowGout, goutStride, sums, p.dense, where, sorted, stream));
     }
     CUDACHECK(launchBehind(keepRowsKernel, std::min(n, 148 * 8), 256, stream, (const uint4*)x, rows, n, d / 8, (uint4*)kept));
   }
   const VocabGrad grad{(const float*)lse, rowGout, goutStride, p.exact ? nullptr : (const float*)rest};
   VocabExact exact{rows, nullptr, (const float*)rest, rowGout, goutStride, (const __nv_bfloat16*)w, sums, where,
-                   p.exact == 2 && dw ? tokenSortItems(n, d, v, sorted) : nullptr, p.exact == 1 ? n * k : n, 0, false, listed};
+                   p.exact == 2 && dw ? tokenSortItems(n * k, d, v, sorted) : nullptr, p.exact ? n * k : 0, 0, p.dense, listed};
   const VocabExact* add = p.exact ? &exact : nullptr;
   const VocabFactor factor{goutStride ? nullptr : (const float*)gout, (const int*)count, temperature};
   for (int c = 0; c < v; c += p.cols) {
@@ -732,7 +735,7 @@ OneGoPlan oneGoPlan(int n, int v, int d, int k, bool wantX, bool wantW) {
 }  // namespace
 
 DF_API size_t dfcclLinearLossWithGradientsWork(int n, int v, int d, int k, int wantX, int wantW) {
-  return sizesOk(n, v, d, k) && (int64_t)n * k <= 0x7fffffff - 4096 && (wantX || wantW) ? oneGoPlan(n, v, d, k, wantX != 0, wantW != 0).bytes : 0;
+  return sizesOk(n, v, d, k) && (int64_t)n * k <= MOST_SORTED && (wantX || wantW) ? oneGoPlan(n, v, d, k, wantX != 0, wantW != 0).bytes : 0;
 }
 
 // Per piece of rows: powers of the logits relative to the largest of the row's list (vocabPowers), their sums, x times the rows' shares, the two
@@ -742,7 +745,7 @@ DF_API size_t dfcclLinearLossWithGradientsWork(int n, int v, int d, int k, int w
 DF_API ncclResult_t dfcclLinearLossWithGradients(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, const void* tokens,
                                                  const void* weights, const void* state, int k, float temperature, int reduction, void* work, size_t workBytes,
                                                  void* lse, void* rest, void* loss, void* count, void* dx, void* dw, cudaStream_t stream) {
-  if (!sizesOk(n, v, d, k) || (int64_t)n * k > 0x7fffffff - 4096 || !x || !w || !rowsOk(targets, tokens, weights, state, k, temperature) || !work || !lse ||
+  if (!sizesOk(n, v, d, k) || (int64_t)n * k > MOST_SORTED || !x || !w || !rowsOk(targets, tokens, weights, state, k, temperature) || !work || !lse ||
       !rest || !loss || !count || !(dx || dw) || reduction < 1 || reduction > 2)
     return ncclInvalidArgument;
   if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw) & 15) return ncclInvalidArgument;

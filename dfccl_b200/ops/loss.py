@@ -13,18 +13,18 @@ from .block import packed
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 MAX_LIST = 256                       # entries of a teacher's list
-# Rows x vocabulary (counted as SMALL_VOCABULARY at least) above which a reduced loss makes its gradients with the loss, and how many times that
-# for lists, of at most a share of the vocabulary.  GPU time in us, logits computed twice / once: targets 512 x 50257 x 64 75 / 79, 1024 x 50257 x 64
-# 115 / 108, x 256 140 / 132, 2048 x 2000 x 256 59 / 62, 3000 x 2000 x 256 75 / 68, 3000 x 500 x 64 62 / 54; 50257 entries x 256, lists of 8 1024 138 / 143,
-# 1500 179 / 175, 2048 230 / 220, of 32 1024 158 / 171, 1500 206 / 208, 2048 272 / 258; 8192 x 8000 x 256, lists of 8 185 / 197, of 32 269 / 305; 4096 x 50257
-# x 1024, lists of 48 1216 / 1130, of 256 1814 / 1919 (the sorting of the entries).  Targets over a head whose way from memory takes longer than what one go
-# has more to launch: 64 x 50257 x 512 97 / 102, x 768 110 / 108, x 1024 134 / 132; 512 x 50257 x 1024 220 / 203; 64 x 131072 x 1024 279 / 251, x 4096 996 / 840.
+# Rows x vocabulary (counted as SMALL_VOCABULARY at least beside targets) above which a reduced loss makes its gradients with the loss.  GPU time in us,
+# logits computed twice / once: targets 512 x 50257 x 64 75 / 79, 1024 x 50257 x 64 115 / 108, x 256 140 / 132, 2048 x 2000 x 256 59 / 62, 3000 x 2000 x 256
+# 75 / 68, 3000 x 500 x 64 62 / 54.  A head whose way from memory takes longer than what one go has more to launch: targets 64 x 50257 x 512 97 / 102, x 768
+# 110 / 108, x 1024 134 / 132; 512 x 50257 x 1024 220 / 203; 64 x 131072 x 1024 279 / 251, x 4096 996 / 840; lists of 8 64 x 50257 x 64 74 / 80, x 768
+# 137 / 133, x 1024 164 / 158, 64 x 32000 x 4096 408 / 383.  Lists of more than 2048 entries together, which both ways sort: lists of 8 256 x 2000 x 64 55 / 62,
+# 300 68 / 64, 2048 80 / 72; 256 x 8000 x 256 68 / 74, of 64 100 / 98; of 32 8192 x 8000 x 256 381 / 299, 256 x 32000 x 4096 502 / 512, 2048 1622 / 1294; of 17
+# 1777 x 30011 x 640 287 / 242, of 128 496 / 404; of 256 4096 x 50257 x 1024 2238 / 1755.
 ONE_GO_FROM = 2 ** 25
 SMALL_VOCABULARY = 14000            # of 2400 rows
-LISTS_TIMES = 2
 LARGE_HEAD = 0.8                     # of 2 ** 25 / 0.8 elements
-LIST_SHARE = 1024
-MOST_ENTRIES = 2 ** 31 - 4096        # of all lists together, as their sorting counts them
+LIST_SHARE = 2 ** 14                 # an entry of a list: of 2048 entries
+MOST_ENTRIES = 2 ** 31 - 4097        # of all lists together, as their sorting counts them
 
 
 def linear_loss_supported(x: torch.Tensor, weight: torch.Tensor) -> bool:
@@ -136,10 +136,8 @@ class _LinearLossFn(torch.autograd.Function):
         want_x, want_w = ctx.needs_input_grad[:2]
         ctx.grads = None
         n, v = x.numel() // weight.shape[1], weight.shape[0]
-        if rows.lists is None:
-            one_go = n * max(v, SMALL_VOCABULARY) > ONE_GO_FROM or weight.numel() * LARGE_HEAD > ONE_GO_FROM
-        else:
-            one_go = n * v > ONE_GO_FROM * LISTS_TIMES and rows.k * LIST_SHARE <= v and rows.entries <= MOST_ENTRIES
+        least = n * max(v, SMALL_VOCABULARY) if rows.lists is None else max(n * v, rows.entries * LIST_SHARE)
+        one_go = max(least, weight.numel() * LARGE_HEAD) > ONE_GO_FROM and rows.entries <= MOST_ENTRIES
         if n and reduction and (want_x or want_w) and one_go:
             loss, xp, wp, kept, ctx.grads = _forward_with_gradients(x, weight, rows, reduction, want_x, want_w)
             ctx.capture = nv.lib().dfcclCaptureId(stream_of(x))

@@ -645,3 +645,59 @@ def test_a_models_two_ends():
     for a, b in zip(*grads):
         assert (a - b).norm().item() <= 0.03 * a.norm().item()       # several roundings of 2**-9 on either side, through a block
     comm.destroy()
+
+
+def certain_lists(n, v, d, k, seed):
+    """Rows whose lists' tokens have all but some 1e-4 of the student's probability, and a teacher who weighs them differently: what the lists
+    add is nearly all of both gradients.  Returns x, w, tokens, teacher's logits."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    w = (torch.randn(v, d, generator=gen, device="cuda") * 0.05).to(torch.bfloat16)
+    tokens = torch.rand(n, v, generator=gen, device="cuda").topk(k, dim=1).indices
+    # the smallest x with a logit of 15 for each of the row's tokens
+    wt = w[tokens].double()
+    x = (wt.transpose(1, 2) @ torch.linalg.inv(wt @ wt.transpose(1, 2)) @ torch.full((n, k, 1), 15.0, dtype=torch.float64, device="cuda"))[..., 0]
+    return x.to(torch.bfloat16), w, tokens, torch.randn(n, k, generator=gen, device="cuda")
+
+
+def check_lists(got, x, w, tokens, q, share, temp=1.0):
+    """Against 64 bits, element by element: half a step of the result, half a step of bf16 (2**-8) for the probabilities of what stands in no list, and
+    fp32 for the lists' own, which are q less a probability."""
+    loss, dz = reference(x, w, tokens, q, temp)
+    dz = dz * share[:, None]
+    err = 3 * logit_error(x, w).max().item() / temp + 2.0 ** -18             # of a probability, relative
+    p = temp * share.abs()[:, None] * torch.softmax(x.double() @ w.double().t() / temp, dim=1)
+    listed = torch.zeros_like(dz).scatter_(1, tokens, 1.0)
+    off = p * err + torch.where(listed > 0, 2.0 ** -22 * temp * share.abs()[:, None], p * 2.0 ** -8 * (1 + 2.0 ** -8))
+    xd, wd = x.double(), w.double()
+    depth = (max(dz.shape) / 16 + 8) * 2.0 ** -23
+    for name, g, want, bound, size in (("dx", got[0], dz @ wd, off @ wd.abs(), dz.abs() @ wd.abs()),
+                                       ("dw", got[1], dz.t() @ xd, off.t() @ xd.abs(), dz.abs().t() @ xd.abs())):
+        if g is not None:
+            assert bool(((g.double() - want).abs() <= bound * (1 + 2.0 ** -8) + want.abs() * 2.0 ** -8 + size * depth + 1e-38).all()), name
+    return loss
+
+
+# entries below and above 2048, below and above the vocabulary, lists that fit the products' epilogue and longer ones
+@pytest.mark.parametrize("n,v,d,k", [(500, 300, 64, 3), (700, 300, 64, 3), (700, 300, 64, 7), (800, 4001, 128, 3), (300, 4001, 136, 9), (2500, 257, 264, 4)])
+@pytest.mark.parametrize("limit", [1 << 20, 1 << 30])
+def test_what_lists_add_keeps_its_digits(n, v, d, k, limit, monkeypatch):
+    """Whichever way the loss goes, however many entries there are, in one piece of the vocabulary or several."""
+    from dfccl_b200.ops import loss as module
+    from dfccl_b200.ops.gemm import check_kernels
+    monkeypatch.setenv("DFCCL_LOSS_WORKSPACE_BYTES", str(limit))
+    monkeypatch.setattr(module, "ONE_GO_FROM", 1 << 60)
+    x, w, tokens, teacher = certain_lists(n, v, d, k, n + v + d + k)
+    hole = torch.arange(n, device="cuda") % 9 == 4
+    q = torch.softmax(teacher.double(), dim=1) * (~hole).double()[:, None]
+    given = torch.where(hole[:, None], -1, tokens)
+    gout = torch.randn(n, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    for want_x, want_w in ((True, True), (True, False), (False, True)):
+        a, b = x.clone().requires_grad_(want_x), w.clone().requires_grad_(want_w)
+        rows = module.linear_distillation(a, b, teacher, given, reduction="none")
+        rows.backward(gout)
+        loss = check_lists((a.grad, b.grad), x, w, tokens, q, gout.double())
+        check_loss(rows.detach(), loss, x, w, 1.0)
+        a.grad = b.grad = None
+        module.linear_distillation(a, b, teacher, given).backward()
+        check_lists((a.grad, b.grad), x, w, tokens, q, torch.full((n,), 1.0 / int((~hole).sum()), dtype=torch.float64, device="cuda"))
+    assert check_kernels()
