@@ -8,7 +8,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import native as nv
-from ..utils.tensors import nccl_dtype, on_device, stream_of
+from ..utils.tensors import nccl_dtype, on_device, refuse_tangents, stream_of
 
 TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -116,6 +116,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, po
         raise ValueError(f"padding_idx {padding_idx} outside a table of {weight.shape[0]} rows")
     if ids.numel() > 2 ** 31 - 4096:
         raise ValueError(f"{ids.numel()} tokens in one call, more than 31 bits count")
+    refuse_tangents(weight, position_weight)
     if not here:
         raise ValueError("the embedding runs on tensors of one GPU")
     ids, scale = ids.contiguous(), float(scale)

@@ -8,7 +8,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import native as nv
-from ..utils.tensors import nccl_dtype, on_device, stream_of
+from ..utils.tensors import nccl_dtype, on_device, refuse_tangents, stream_of
 from .block import packed
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -47,6 +47,7 @@ def _check(x: torch.Tensor, weight: torch.Tensor, index: torch.Tensor, name: str
         raise ValueError(f"{name} are int64 or int32, got {index.dtype}")
     if max(x.numel() // d, v) > 2 ** 31 - 4096:
         raise ValueError("more rows or entries than 31 bits count")
+    refuse_tangents(x, weight)
 
 
 def _on_one_gpu(device: torch.device, *tensors: torch.Tensor) -> None:
@@ -206,7 +207,7 @@ def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_logits: t
     ``x`` and ``weight`` as in ``linear_cross_entropy``; ``teacher_logits`` [..., k] fp32, bf16 or fp16 and ``teacher_tokens`` [..., k]
     int64 or int32, k up to 256 in any order.  Entries of token -1 or of logit -inf are left out; a row without any has no loss and
     gives no gradient.  A token that stands in a row twice counts as two entries.  ``"mean"`` is over the rows with entries, 0 where
-    there is none.  No gradient reaches the teacher.  Any other token outside the vocabulary makes its row NaN."""
+    there is none.  No gradient (and no tangent) reaches the teacher.  Any other token outside the vocabulary makes its row NaN."""
     _check(x, weight, teacher_tokens, "teacher_tokens", reduction)
     if teacher_tokens.dim() != x.dim() or teacher_tokens.shape[:-1] != x.shape[:-1] or teacher_logits.shape != teacher_tokens.shape:
         raise ValueError(f"teacher_logits of {tuple(teacher_logits.shape)} and teacher_tokens of {tuple(teacher_tokens.shape)} for x of {tuple(x.shape)}")

@@ -7,6 +7,7 @@ from typing import Sequence
 
 import numpy as np
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from .. import native as nv
 
@@ -42,6 +43,14 @@ def on_device(device: torch.device):
     """Makes ``device`` the current one for a launch on its stream, where it is not already (a launch on another device's
     stream is refused by the runtime)."""
     return _HERE if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device.index)
+
+
+def refuse_tangents(*tensors) -> None:
+    """Kernels that read by address would leave a forward-mode tangent behind without a word; tensors may be None."""
+    if forward_ad._current_level < 0:                   # tangents live inside a level only (asked of each tensor, it is 1 us of a launch)
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("no forward-mode derivative of this operator; its gradients come from a backward pass")
 
 
 class _CudaBlob:

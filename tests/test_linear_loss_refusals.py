@@ -140,3 +140,22 @@ def test_long_entries(native):
     for bad in ((1.5,), (None,), (1, 1.0, 2.0), (1, "x"), tuple([1] * 26), ()):
         with pytest.raises(TypeError):
             call(*bad)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("which", range(6))
+def test_tangents_are_refused(which, grad):
+    """A forward-mode derivative is not computed, and not dropped either: of every operand that has a derivative, in and out of no_grad."""
+    import torch.autograd.forward_ad as fw
+    from dfccl_b200.ops.embedding import embedding
+    from dfccl_b200.ops.loss import linear_cross_entropy, linear_distillation
+    with fw.dual_level(), torch.set_grad_enabled(grad):
+        a, w = x(4, 16), x(9, 16)
+        with_tangent = fw.make_dual(x(4, 16) if which in (0, 2) else x(9, 16), torch.ones(4 if which in (0, 2) else 9, 16, dtype=BF))
+        call = [lambda t: linear_cross_entropy(t, w, i(4)), lambda t: linear_cross_entropy(a, t, i(4)),
+                lambda t: linear_distillation(t, w, x(4, 2), i(4, 2)), lambda t: linear_distillation(a, t, x(4, 2), i(4, 2)),
+                lambda t: embedding(i(4), t), lambda t: embedding(i(4), w, positions=i(4), position_weight=t)][which]
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(with_tangent)
+        with pytest.raises(ValueError, match="GPU"):
+            call(fw.unpack_dual(with_tangent).primal)
