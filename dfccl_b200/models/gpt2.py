@@ -26,7 +26,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ..ops.block import norm_residual, unhooked
-from ..ops.embedding import embedding
+from ..ops.embedding import embedding, lookup_supported
 from ..ops.fused_linear import TpGroup
 from ..ops.loss import linear_cross_entropy, linear_loss_supported
 from ..parallel.tp import ColumnParallelLinear, RowParallelLinear, gelu_mlp
@@ -99,7 +99,8 @@ class ParallelBlock(nn.Module):
 class GPT2Stage(nn.Module):
     """Blocks ``[first_layer, first_layer + n_layers)`` of the model for micro-batches of
     ``micro_batch`` sequences.  ``fused_ends``: token and position embedding in one kernel, and the loss without the logits,
-    whose rounding to bf16 it leaves out (on GPUs; elsewhere the stage computes as without it)."""
+    whose rounding to bf16 it leaves out (on GPUs and with
+    embeddings that only look up; elsewhere the stage computes as without it)."""
 
     def __init__(self, cfg: GPT2Config, tp: TpGroup, stage: int, n_stages: int, micro_batch: int, seed: int = 1234, fused_ends: bool = False):
         super().__init__()
@@ -135,7 +136,7 @@ class GPT2Stage(nn.Module):
         to the micro-batch's loss); the others return their hidden rows."""
         if self.is_first:
             ids = self.my_rows(x.reshape(-1))
-            if self.fused_ends and ids.is_cuda and unhooked(self.wte, nn.Embedding) and unhooked(self.wpe, nn.Embedding):
+            if self.fused_ends and ids.is_cuda and lookup_supported(self.wte, self.wpe):
                 h = embedding(ids, self.wte.weight, positions=self.pos, position_weight=self.wpe.weight)
             else:
                 h = self.wte(ids) + self.wpe(self.pos)

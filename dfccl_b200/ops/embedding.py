@@ -5,10 +5,12 @@ import functools
 from typing import Optional
 
 import torch
+import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from .. import native as nv
 from ..utils.tensors import nccl_dtype, on_device, refuse_tangents, stream_of
+from .block import unhooked
 
 TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -87,6 +89,15 @@ class _EmbeddingFn(torch.autograd.Function):
                                                                  ctx.scale, None if gw is None else gw.data_ptr(), ctx.rows, *second, work.data_ptr(), stream_of(g)),
                          "dfcclEmbeddingBackward")
         return None, gw, None, gp, None, None
+
+
+def lookup_supported(tokens: nn.Module, positions: nn.Module) -> bool:
+    """True if ``embedding`` of the two modules' tables is what calling them and adding their results gives: modules that look up and
+    do nothing else (no row without a gradient, renormalised, scaled by its count or of a sparse gradient), tables of one kind."""
+    a, b = tokens, positions
+    return (all(unhooked(m, nn.Embedding) and m.padding_idx is None and m.max_norm is None and not m.scale_grad_by_freq and not m.sparse for m in (a, b))
+            and a.weight.dtype == b.weight.dtype and a.weight.dtype in TYPES and a.weight.device == b.weight.device
+            and a.weight.shape[1] == b.weight.shape[1])
 
 
 def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, positions: Optional[torch.Tensor] = None,

@@ -184,3 +184,37 @@ def test_other_stream_and_graph():
             graph.replay()
         for k, (_, _, out) in enumerate(graphs):
             assert all(torch.equal(a, b) for a, b in zip(out, want[(turn + k) % 3]))
+
+
+@pytest.mark.parametrize("end", ["wte", "wpe"])
+@pytest.mark.parametrize("option", ["padding_idx", "max_norm", "scale_grad_by_freq", "sparse", "dtype"])
+def test_a_stage_respects_its_embeddings_options(option, end):
+    """A table that does more than look up keeps doing it where the stage's ends are fused."""
+    from dfccl_b200 import native as nv
+    from dfccl_b200.models.gpt2 import GPT2Config, GPT2Stage
+    from dfccl_b200.ops.fused_linear import TpGroup
+    (comm,) = nv.Comm.init_loopback(1, torch.cuda.current_device())
+    cfg = GPT2Config(n_layer=2, d_model=256, n_head=4, seq_len=128, vocab=300)
+    tp = TpGroup(comm, None, torch.device("cuda", torch.cuda.current_device()))
+    tokens = torch.randint(0, 40, (4, 129), device="cuda")
+    tokens[0, 0] = 7
+    results = []
+    for fused in (False, True):
+        stage = GPT2Stage(cfg, tp, 0, 2, 4, fused_ends=fused)
+        old = getattr(stage, end)
+        kind = {"padding_idx": {"padding_idx": 7}, "max_norm": {"max_norm": 0.125}, "scale_grad_by_freq": {"scale_grad_by_freq": True}, "sparse": {"sparse": True}}.get(option, {})
+        new = torch.nn.Embedding(old.num_embeddings, old.embedding_dim, device="cuda", dtype=torch.float32 if option == "dtype" else torch.bfloat16, **kind)
+        with torch.no_grad():
+            new.weight.copy_(old.weight)
+        setattr(stage, end, new)
+        stage.blocks = torch.nn.ModuleList()                 # what the first stage hands on is the embedding
+        h = stage(tokens[:, :-1])
+        grad = torch.linspace(-1, 1, h.numel(), device="cuda").view_as(h).to(h.dtype)
+        grads = torch.autograd.grad(h, [stage.wte.weight, stage.wpe.weight], grad)
+        results.append([h.detach(), new.weight.detach().clone()] + [torch.sparse_coo_tensor(g._indices(), g._values().double(), g.shape).to_dense() if g.is_sparse
+                                                                    else g.double() for g in grads])
+    comm.destroy()
+    (h0, w0, *g0), (h1, w1, *g1) = results
+    assert h0.dtype == h1.dtype and torch.equal(h0, h1) and torch.equal(w0, w1)
+    for a, b in zip(g0, g1):                                 # (sums in another order, rounded once: bf16 tables)
+        assert bool(((a - b).abs() <= 2.0 ** -7 * a.abs().clamp(min=a.abs().mean().item())).all())
