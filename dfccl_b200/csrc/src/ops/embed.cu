@@ -494,6 +494,7 @@ void setKeys(Table* t, const void* idx, int wide, int64_t rows, int64_t padding,
   t->buf[0] = (uint2*)at; t->buf[1] = (uint2*)(at + l.items); t->sums = (float*)(at + 2 * l.items);
 }
 
+constexpr int MOST_TOKENS = 0x7fffffff - 4095;      // loops over them step up to 2048 past their end
 int typeBytes(int t) { return t == ncclFloat32 ? 4 : t == ncclBfloat16 || t == ncclFloat16 ? 2 : 0; }
 
 }  // namespace
@@ -534,7 +535,7 @@ using namespace dfccl;
 DF_API ncclResult_t dfcclEmbeddingForward(const void* ids, int wideIds, int n, const void* w, int64_t rows, int64_t ldw, const void* positions, int widePositions,
                                           const void* p, int64_t prows, int64_t ldp, void* out, int d, int type, float scale, cudaStream_t stream) {
   const int bytes = typeBytes(type);
-  if (n <= 0 || d <= 0 || rows <= 0 || !bytes || !ids || !w || !out || ldw < d || (positions && (!p || prows <= 0 || ldp < d))) return ncclInvalidArgument;
+  if (n <= 0 || n > MOST_TOKENS || d <= 0 || rows <= 0 || !bytes || !ids || !w || !out || ldw < d || (positions && (!p || prows <= 0 || ldp < d))) return ncclInvalidArgument;
   Forward a{ids, positions, w, p, out, wideIds, widePositions, n, 0, 0, 0, rows, prows, ldw, ldp, scale};
   const uintptr_t grid = (uintptr_t)w | (uintptr_t)out | (uintptr_t)(ldw * bytes) | (uintptr_t)((size_t)d * bytes) |
                          (positions ? (uintptr_t)p | (uintptr_t)(ldp * bytes) : 0);
@@ -549,7 +550,7 @@ DF_API ncclResult_t dfcclEmbeddingForward(const void* ids, int wideIds, int n, c
 }
 
 DF_API size_t dfcclEmbeddingBackwardWork(int n, int d, int tables) {
-  if (n <= 0 || d <= 0 || tables < 1 || tables > MAX_TABLES) return 0;
+  if (n <= 0 || n > MOST_TOKENS || d <= 0 || tables < 1 || tables > MAX_TABLES) return 0;
   const Layout l = layoutOf(n, d);
   return tables * (2 * l.items + l.sums);
 }
@@ -557,7 +558,7 @@ DF_API size_t dfcclEmbeddingBackwardWork(int n, int d, int tables) {
 DF_API ncclResult_t dfcclEmbeddingBackward(const void* g, int n, int d, int type, const void* ids, int wideIds, int64_t padding, float scale, void* gw, int64_t rows,
                                            const void* positions, int widePositions, void* gp, int64_t prows, void* work, cudaStream_t stream) {
   const int bytes = typeBytes(type);
-  if (n <= 0 || d <= 0 || !bytes || !g || !work || !(gw || gp) || (gw && (!ids || rows <= 0 || rows > 0x7ffffff0ll)) ||
+  if (n <= 0 || n > MOST_TOKENS || d <= 0 || !bytes || !g || !work || !(gw || gp) || (gw && (!ids || rows <= 0 || rows > 0x7ffffff0ll)) ||
       (gp && (!positions || prows <= 0 || prows > 0x7ffffff0ll)) || (((uintptr_t)gw | (uintptr_t)gp | (uintptr_t)work) & 15))
     return ncclInvalidArgument;
   const Layout l = layoutOf(n, d);

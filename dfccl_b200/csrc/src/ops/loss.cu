@@ -570,7 +570,12 @@ BackwardPlan backwardPlan(int n, int v, int d, int k, bool wantX, bool wantW) {
   return p;
 }
 
-bool sizesOk(int n, int v, int d, int k) { return n > 0 && v > 0 && v <= VOCAB_NO_TOKEN - 512 && d > 0 && d % 8 == 0 && k > 0 && k <= MAX_LIST; }
+// Loops over pieces end at the first number of rows or columns that is not below the size: at most a piece behind it, and at most 256 for each of
+// the pieces, of which the smaller is 742 000 at 2^31.
+constexpr int MOST_ROWS = 0x7fffffff - (1 << 20);
+bool sizesOk(int n, int v, int d, int k) {
+  return n > 0 && n <= MOST_ROWS && v > 0 && v <= MOST_ROWS && d > 0 && d <= MOST_ROWS && d % 8 == 0 && k > 0 && k <= MAX_LIST;
+}
 
 }  // namespace
 }  // namespace dfccl

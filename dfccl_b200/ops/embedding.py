@@ -25,8 +25,8 @@ def _table(name: str, t: torch.Tensor) -> None:
         raise ValueError(f"{name} is [rows, columns], got {tuple(t.shape)}")
     if t.dtype not in TYPES:
         raise ValueError(f"{name} is bf16, fp16 or fp32, got {t.dtype}")
-    if t.shape[0] > 2 ** 31 - 16:
-        raise ValueError(f"{name} has {t.shape[0]} rows, more than 31 bits count")
+    if t.shape[0] > 2 ** 31 - 16 or t.shape[1] > 2 ** 31 - 4096:
+        raise ValueError(f"{name} is {t.shape[0]} x {t.shape[1]}, more than 31 bits count")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:

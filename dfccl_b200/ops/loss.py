@@ -24,6 +24,7 @@ ONE_GO_FROM = 2 ** 25
 SMALL_VOCABULARY = 14000            # of 2400 rows
 LARGE_HEAD = 0.8                     # of 2 ** 25 / 0.8 elements
 LIST_SHARE = 2 ** 14                 # an entry of a list: of 2048 entries
+MOST_ROWS = 2 ** 31 - 1 - 2 ** 20     # 31 bits, less what loops over pieces of them go past their end
 MOST_ENTRIES = 2 ** 31 - 4097        # of all lists together, as their sorting counts them
 
 
@@ -45,8 +46,8 @@ def _check(x: torch.Tensor, weight: torch.Tensor, index: torch.Tensor, name: str
         raise ValueError(f"the width is a multiple of 8 and the vocabulary not empty, got {v} x {d}")
     if index.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"{name} are int64 or int32, got {index.dtype}")
-    if max(x.numel() // d, v) > 2 ** 31 - 4096:
-        raise ValueError("more rows or entries than 31 bits count")
+    if max(x.numel() // d, v, d) > MOST_ROWS:
+        raise ValueError(f"at most {MOST_ROWS} rows, entries of the vocabulary and columns, got {x.numel() // d} x {v} x {d}")
     refuse_tangents(x, weight)
 
 

@@ -159,3 +159,28 @@ def test_tangents_are_refused(which, grad):
             call(with_tangent)
         with pytest.raises(ValueError, match="GPU"):
             call(fw.unpack_dual(with_tangent).primal)
+
+
+def test_sizes_at_the_end_of_31_bits(native):
+    """Loops over pieces of rows or columns count past their end by up to a piece: sizes whose count would not fit are refused."""
+    from dfccl_b200.ops.embedding import embedding
+    from dfccl_b200.ops.loss import MOST_ROWS, linear_cross_entropy, linear_distillation
+    L, top = native.lib(), 2 ** 31
+    assert top - 2 ** 21 < MOST_ROWS < top - 742000
+    for n, v, d in ((MOST_ROWS + 1, 9, 8), (4, MOST_ROWS + 1, 8), (top - 4096, 9, 8), (100, top - 4096, 8), (4, 9, top - 8)):
+        assert L.dfcclLinearLossWithGradientsWork(n, v, d, 1, 1, 1) == 0 and L.dfcclLinearLossBackwardWork(n, v, d, 0, 1, 1) == 0
+        assert d > 8 or L.dfcclLinearLossForwardWork(n, v, 1) == 0
+        rows, head = x(1, 1).expand(n, d), x(1, 1).expand(v, d)
+        with pytest.raises(ValueError, match="at most"):
+            linear_cross_entropy(rows, head, i(1).expand(n))
+        with pytest.raises(ValueError, match="at most"):
+            linear_distillation(rows, head, x(1, 1).expand(n, 2), i(1, 1).expand(n, 2))
+    assert L.dfcclLinearLossForwardWork(MOST_ROWS, 9, 1) > 0
+    assert L.dfcclEmbeddingBackwardWork(top - 4095, 8, 1) == 0 and L.dfcclEmbeddingBackwardWork(top - 4096, 8, 1) > 0
+    p = 4096
+    assert L.dfcclEmbeddingForward(p, 1, top - 1, p, 9, 16, None, 0, None, 0, 0, p, 16, native.BFLOAT16, 1.0, None) == native.INVALID_ARGUMENT
+    assert L.dfcclEmbeddingBackward(p, top - 1, 16, native.BFLOAT16, p, 1, -1, 1.0, p, 9, None, 0, None, 0, p, None) == native.INVALID_ARGUMENT
+    with pytest.raises(ValueError, match="31 bits"):
+        embedding(i(4), x(1, 1).expand(9, top + 8))
+    with pytest.raises(ValueError, match="31 bits"):
+        embedding(i(1).expand(top - 4095), x(9, 16))
