@@ -64,7 +64,7 @@ ncclResult_t dfcclEmbeddingForward(const void* ids, int wideIds, int n, const vo
                                    const void* p, int64_t prows, int64_t ldp, void* out, int d, int type, float scale, cudaStream_t stream);
 /* Gradients of the tables (contiguous, 16-byte aligned; either may be null) from that of `out`, g [n, d]: every row is written, rows
  * without tokens with zeros.  Tokens outside a table and tokens `padding` (-1: none) give no gradient.  Sums in fp32 in the order of the
- * tokens.  work: dfcclEmbeddingBackwardWork bytes for the number of tables that get a gradient. */
+ * tokens.  work: dfcclEmbeddingBackwardWork bytes, 32-byte aligned, for the number of tables that get a gradient. */
 ncclResult_t dfcclEmbeddingBackward(const void* g, int n, int d, int type, const void* ids, int wideIds, int64_t padding, float scale, void* gw, int64_t rows,
                                     const void* positions, int widePositions, void* gp, int64_t prows, void* work, cudaStream_t stream);
 size_t dfcclEmbeddingBackwardWork(int n, int d, int tables);
@@ -72,7 +72,8 @@ size_t dfcclEmbeddingBackwardWork(int n, int d, int tables);
 /* ---- losses of z = x w^T, x [n, d], w [v, d] (bf16, contiguous, 16-byte aligned, d % 8 == 0), without keeping z.
  * Every row is compared with a target (`targets`: 64-bit integers where `wide` is set, 32-bit otherwise; `ignore`: no target; k = 1) or,
  * with targets null, with a list of k <= dfcclLinearLossMaxList() vocabulary entries whose weights q add up to 1 (dfcclTeacherRows):
- * loss = T^2 sum q (ln q - ln softmax(z / T)).  A target outside the vocabulary makes its row's loss and gradients NaN. */
+ * loss = T^2 sum q (ln q - ln softmax(z / T)).  A target outside the vocabulary makes its row's loss and gradients NaN.
+ * work: as many bytes as the entry point's ...Work says, 32-byte aligned. */
 /* Lists from a teacher's logits: q = softmax(logits / temperature) over the entries of a row whose token is not -1 and whose logit is not
  * -inf, in the order of their tokens.  logitType: ncclFloat32, ncclBfloat16 or ncclFloat16.  state: 0 a row without an entry (loss 0, no
  * gradient), 1 a row with some, 2 a row with a token outside the vocabulary (NaN). */

@@ -559,7 +559,7 @@ DF_API ncclResult_t dfcclEmbeddingBackward(const void* g, int n, int d, int type
                                            const void* positions, int widePositions, void* gp, int64_t prows, void* work, cudaStream_t stream) {
   const int bytes = typeBytes(type);
   if (n <= 0 || n > MOST_TOKENS || d <= 0 || !bytes || !g || !work || !(gw || gp) || (gw && (!ids || rows <= 0 || rows > 0x7ffffff0ll)) ||
-      (gp && (!positions || prows <= 0 || prows > 0x7ffffff0ll)) || (((uintptr_t)gw | (uintptr_t)gp | (uintptr_t)work) & 15))
+      (gp && (!positions || prows <= 0 || prows > 0x7ffffff0ll)) || (((uintptr_t)gw | (uintptr_t)gp) & 15) || ((uintptr_t)work & 31))
     return ncclInvalidArgument;
   const Layout l = layoutOf(n, d);
   Backward a = {};

@@ -573,6 +573,8 @@ BackwardPlan backwardPlan(int n, int v, int d, int k, bool wantX, bool wantW) {
 // Loops over pieces end at the first number of rows or columns that is not below the size: at most a piece behind it, and at most 256 for each of
 // the pieces, of which the smaller is 742 000 at 2^31.
 constexpr int MOST_ROWS = 0x7fffffff - (1 << 20);
+// A workspace's parts lie at multiples of 256 bytes behind its beginning, and are accessed 32 bytes at a time.
+bool workOk(const void* work) { return work && ((uintptr_t)work & 31) == 0; }
 bool sizesOk(int n, int v, int d, int k) {
   return n > 0 && n <= MOST_ROWS && v > 0 && v <= MOST_ROWS && d > 0 && d <= MOST_ROWS && d % 8 == 0 && k > 0 && k <= MAX_LIST;
 }
@@ -619,7 +621,7 @@ DF_API size_t dfcclLinearLossForwardWork(int n, int v, int k) {
 DF_API ncclResult_t dfcclLinearLossForward(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, const void* tokens,
                                            const void* weights, const void* state, int k, float temperature, int reduction, void* work, void* lse, void* rest,
                                            void* rowLoss, void* loss, void* count, cudaStream_t stream) {
-  if (!sizesOk(n, v, d, k) || !x || !w || !rowsOk(targets, tokens, weights, state, k, temperature) || !work || !lse || !rest || reduction < 0 || reduction > 2) return ncclInvalidArgument;
+  if (!sizesOk(n, v, d, k) || !x || !w || !rowsOk(targets, tokens, weights, state, k, temperature) || !workOk(work) || !lse || !rest || reduction < 0 || reduction > 2) return ncclInvalidArgument;
   if ((((uintptr_t)x | (uintptr_t)w) & 15) || (reduction ? !loss || !count : !rowLoss)) return ncclInvalidArgument;
   const ForwardLayout l = forwardLayout(n, v, k);
   JoinArgs j = {};
@@ -654,7 +656,7 @@ DF_API size_t dfcclLinearLossBackwardWork(int n, int v, int d, int k, int wantX,
 DF_API ncclResult_t dfcclLinearLossBackward(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, const void* tokens,
                                             const void* weights, const void* state, int k, float temperature, const void* lse, const void* rest,
                                             const void* gout, int goutStride, const void* count, void* dx, void* dw, void* work, size_t workBytes, cudaStream_t stream) {
-  if (!sizesOk(n, v, d, k) || !x || !w || !rowsOk(targets, tokens, weights, state, k, temperature) || !lse || !rest || !gout || !work || !(dx || dw) || goutStride < 0) return ncclInvalidArgument;
+  if (!sizesOk(n, v, d, k) || !x || !w || !rowsOk(targets, tokens, weights, state, k, temperature) || !lse || !rest || !gout || !workOk(work) || !(dx || dw) || goutStride < 0) return ncclInvalidArgument;
   if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw) & 15) return ncclInvalidArgument;
   const BackwardPlan p = backwardPlan(n, v, d, targets ? 0 : k, dx != nullptr, dw != nullptr);
   if (p.all() > workBytes) return ncclInvalidArgument;          // (the setting has changed since the size was asked for)
@@ -750,7 +752,7 @@ DF_API size_t dfcclLinearLossWithGradientsWork(int n, int v, int d, int k, int w
 DF_API ncclResult_t dfcclLinearLossWithGradients(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, const void* tokens,
                                                  const void* weights, const void* state, int k, float temperature, int reduction, void* work, size_t workBytes,
                                                  void* lse, void* rest, void* loss, void* count, void* dx, void* dw, cudaStream_t stream) {
-  if (!sizesOk(n, v, d, k) || (int64_t)n * k > MOST_SORTED || !x || !w || !rowsOk(targets, tokens, weights, state, k, temperature) || !work || !lse ||
+  if (!sizesOk(n, v, d, k) || (int64_t)n * k > MOST_SORTED || !x || !w || !rowsOk(targets, tokens, weights, state, k, temperature) || !workOk(work) || !lse ||
       !rest || !loss || !count || !(dx || dw) || reduction < 1 || reduction > 2)
     return ncclInvalidArgument;
   if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw) & 15) return ncclInvalidArgument;

@@ -184,3 +184,15 @@ def test_sizes_at_the_end_of_31_bits(native):
         embedding(i(4), x(1, 1).expand(9, top + 8))
     with pytest.raises(ValueError, match="31 bits"):
         embedding(i(1).expand(top - 4095), x(9, 16))
+
+
+def test_entries_refuse_misaligned_workspaces(native):
+    """A workspace is accessed 32 bytes at a time: one that starts elsewhere is an invalid argument, not a fault."""
+    L, bad, p = native.lib(), native.INVALID_ARGUMENT, 4096
+    entries = [(L.dfcclLinearLossForward, [p, p, 4, 9, 16, p, 1, -100, None, None, None, 1, 1.0, 0, p, p, p, p, None, None, None], 14),
+               (L.dfcclLinearLossBackward, [p, p, 4, 9, 16, p, 1, -100, None, None, None, 1, 1.0, p, p, p, 0, None, p, p, p, 1 << 30, None], 20),
+               (L.dfcclLinearLossWithGradients, [p, p, 4, 9, 16, p, 1, -100, None, None, None, 1, 1.0, 1, p, 1 << 30, p, p, p, p, p, p, None], 14),
+               (L.dfcclEmbeddingBackward, [p, 4, 16, native.BFLOAT16, p, 1, -1, 1.0, p, 9, None, 0, None, 0, p, None], 14)]
+    for entry, args, work in entries:
+        for off in (4, 8, 16, 31):
+            assert entry(*args[:work], p + off, *args[work + 1:]) == bad, (entry, off)
