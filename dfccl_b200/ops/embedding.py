@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import functools
+import operator
 from typing import Optional
 
 import torch
@@ -123,7 +124,8 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, po
             raise ValueError(f"position_weight of {tuple(position_weight.shape)} {position_weight.dtype} beside weight of {tuple(weight.shape)} {weight.dtype}")
         here = here and positions.device == device and position_weight.device == device
         positions = positions.contiguous()
-    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+    padding = -1 if padding_idx is None else operator.index(padding_idx)
+    if padding_idx is not None and not 0 <= padding < weight.shape[0]:
         raise ValueError(f"padding_idx {padding_idx} outside a table of {weight.shape[0]} rows")
     if ids.numel() > 2 ** 31 - 4096:
         raise ValueError(f"{ids.numel()} tokens in one call, more than 31 bits count")
@@ -132,5 +134,5 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, po
         raise ValueError("the embedding runs on tensors of one GPU")
     ids, scale = ids.contiguous(), float(scale)
     if torch.is_grad_enabled() and (weight.requires_grad or (position_weight is not None and position_weight.requires_grad)):
-        return _EmbeddingFn.apply(ids, weight, positions, position_weight, scale, -1 if padding_idx is None else int(padding_idx))
+        return _EmbeddingFn.apply(ids, weight, positions, position_weight, scale, padding)
     return _forward(ids, weight, positions, position_weight, scale)

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import functools
+import operator
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -195,6 +196,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     _check(x, weight, targets, "targets", reduction)
     if targets.shape != x.shape[:-1]:
         raise ValueError(f"targets of {tuple(targets.shape)} for x of {tuple(x.shape)}")
+    ignore_index = operator.index(ignore_index)
+    if not -2 ** 63 <= ignore_index < 2 ** 63:
+        raise ValueError(f"ignore_index {ignore_index} is no token of 64 bits")
     _on_one_gpu(x.device, weight, targets)
     return _loss(x, weight, _Rows(targets.contiguous(), ignore_index, None, targets.numel(), 1, 1.0), reduction)
 

@@ -196,3 +196,25 @@ def test_entries_refuse_misaligned_workspaces(native):
     for entry, args, work in entries:
         for off in (4, 8, 16, 31):
             assert entry(*args[:work], p + off, *args[work + 1:]) == bad, (entry, off)
+
+
+def test_what_is_no_token():
+    """An ignored token or a padding token is a whole number that the kernels' 64 bits hold; None, a float or more bits are not read as token 0."""
+    import numpy as np
+    from dfccl_b200.ops.embedding import embedding
+    from dfccl_b200.ops.loss import linear_cross_entropy
+    for bad in (None, 0.0, -100.0, "0"):
+        with pytest.raises(TypeError):
+            linear_cross_entropy(x(4, 16), x(9, 16), i(4), ignore_index=bad)
+    for bad in (2 ** 63, 2 ** 64, -2 ** 63 - 1):
+        with pytest.raises(ValueError, match="64 bits"):
+            linear_cross_entropy(x(4, 16), x(9, 16), i(4), ignore_index=bad)
+    for good in (-2 ** 63, 2 ** 63 - 1, np.int32(3), torch.tensor(5)):
+        with pytest.raises(ValueError, match="GPU"):
+            linear_cross_entropy(x(4, 16), x(9, 16), i(4), ignore_index=good)
+    for bad in (2.0, 2.5, "0"):
+        with pytest.raises(TypeError):
+            embedding(i(4), x(9, 16), padding_idx=bad)
+    for good in (np.int64(3), 8):
+        with pytest.raises(ValueError, match="GPU"):
+            embedding(i(4), x(9, 16), padding_idx=good)
