@@ -72,7 +72,7 @@ size_t dfcclEmbeddingBackwardWork(int n, int d, int tables);
 /* ---- losses of z = x w^T, x [n, d], w [v, d] (bf16, contiguous, 16-byte aligned, d % 8 == 0), without keeping z.
  * Every row is compared with a target (`targets`: 64-bit integers where `wide` is set, 32-bit otherwise; `ignore`: no target; k = 1) or,
  * with targets null, with a list of k <= dfcclLinearLossMaxList() vocabulary entries whose weights q add up to 1 (dfcclTeacherRows):
- * loss = T^2 sum q (ln q - ln softmax(z / T)).  A target outside the vocabulary makes its row's loss and gradients NaN.
+ * loss = T^2 sum q (ln q - ln softmax(z / T)), T from 2^-20 to 2^20 (1 beside targets).  A target outside the vocabulary makes its row's loss and gradients NaN.
  * work: as many bytes as the entry point's ...Work says, 32-byte aligned. */
 /* Lists from a teacher's logits: q = softmax(logits / temperature) over the entries of a row whose token is not -1 and whose logit is not
  * -inf, in the order of their tokens.  logitType: ncclFloat32, ncclBfloat16 or ncclFloat16.  state: 0 a row without an entry (loss 0, no

@@ -575,6 +575,9 @@ BackwardPlan backwardPlan(int n, int v, int d, int k, bool wantX, bool wantW) {
 constexpr int MOST_ROWS = 0x7fffffff - (1 << 20);
 // A workspace's parts lie at multiples of 256 bytes behind its beginning, and are accessed 32 bytes at a time.
 bool workOk(const void* work) { return work && ((uintptr_t)work & 31) == 0; }
+// Below, ordinary logits (hundreds) would leave the exponents that fp32 tells apart by less than a power's range, 2^31; above, T^2 is more than
+// what a rounding of fp32 leaves of the loss.
+bool temperatureOk(float t) { return t >= 0x1p-20f && t <= 0x1p20f; }
 bool sizesOk(int n, int v, int d, int k) {
   return n > 0 && n <= MOST_ROWS && v > 0 && v <= MOST_ROWS && d > 0 && d <= MOST_ROWS && d % 8 == 0 && k > 0 && k <= MAX_LIST;
 }
@@ -590,7 +593,7 @@ DF_API int dfcclLinearLossMaxList(void) { return MAX_LIST; }
 DF_API ncclResult_t dfcclTeacherRows(const void* logits, int logitType, const void* tokens, int wide, int n, int k, int v, float temperature, void* outTokens,
                                      void* outWeights, void* state, cudaStream_t stream) {
   const int type = logitType == ncclFloat32 ? 0 : logitType == ncclBfloat16 ? 1 : logitType == ncclFloat16 ? 2 : -1;
-  if (!logits || !tokens || !outTokens || !outWeights || !state || type < 0 || !sizesOk(n, v, 8, k) || !(temperature > 0.f)) return ncclInvalidArgument;
+  if (!logits || !tokens || !outTokens || !outWeights || !state || type < 0 || !sizesOk(n, v, 8, k) || !temperatureOk(temperature)) return ncclInvalidArgument;
   CUDACHECK(launchBehind(teacherRowsKernel, (n + 3) / 4, 128, stream, logits, type, tokens, wide, n, k, v, 1.f / temperature, (int*)outTokens, (float*)outWeights,
                          (int*)state));
   return ncclSuccess;
@@ -608,7 +611,7 @@ VocabRows rowsOf(const void* targets, int wide, int v, int64_t ignore, const voi
                    weights ? (const float*)weights + at : nullptr, state ? (const int*)state + r : nullptr, k, LOG2E / temperature};
 }
 bool rowsOk(const void* targets, const void* tokens, const void* weights, const void* state, int k, float temperature) {
-  return (targets ? k == 1 : tokens && weights && state) && temperature > 0.f;
+  return (targets ? k == 1 : tokens && weights && state) && temperatureOk(temperature);
 }
 }  // namespace
 

@@ -189,7 +189,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
 
     ``x`` [..., d] and ``weight`` [vocabulary, d] are bf16, d a multiple of 8; ``targets`` [...] int64 or int32.  Rows of target
     ``ignore_index`` have no loss and give no gradient, whatever ``x`` holds there; ``"mean"`` is over the other rows, and 0 where
-    there is none.  Logits and sums are fp32; the probabilities are rounded to bf16 on their way into the products that make the
+    there is none.  Logits (up to 2**30 in size) and sums are fp32; the probabilities are rounded to bf16 on their way into the products that make the
     gradients of ``x`` and ``weight``, what the targets add to them is not.  They exist for as many columns or rows at a time as
     ``DFCCL_LOSS_WORKSPACE_BYTES`` (1 GiB) hold.  Large reduced losses make their gradients with the loss and keep them until the
     first backward pass.  There is no check of the targets' values on the host: one outside the vocabulary makes its row's loss and gradients NaN."""
@@ -209,7 +209,7 @@ def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_logits: t
     softmax of ``teacher_logits / T`` over the row's entries, p that of ``x @ weight.T / T`` over the whole vocabulary, read at
     ``teacher_tokens``.
 
-    ``x`` and ``weight`` as in ``linear_cross_entropy``; ``teacher_logits`` [..., k] fp32, bf16 or fp16 and ``teacher_tokens`` [..., k]
+    ``x`` and ``weight`` as in ``linear_cross_entropy``, T 2**-20 to 2**20 (a loss is exact to T^2 times a rounding or two of fp32); ``teacher_logits`` [..., k] fp32, bf16 or fp16 and ``teacher_tokens`` [..., k]
     int64 or int32, k up to 256 in any order.  Entries of token -1 or of logit -inf are left out; a row without any has no loss and
     gives no gradient.  A token that stands in a row twice counts as two entries.  ``"mean"`` is over the rows with entries, 0 where
     there is none.  No gradient (and no tangent) reaches the teacher.  Any other token outside the vocabulary makes its row NaN."""
@@ -221,8 +221,8 @@ def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_logits: t
     k = teacher_tokens.shape[-1]
     if not 1 <= k <= MAX_LIST:
         raise ValueError(f"lists of 1 to {MAX_LIST} entries, got {k}")
-    if not (temperature > 0.0 and temperature < float("inf")):
-        raise ValueError(f"the temperature is positive, got {temperature}")
+    if not 2.0 ** -20 <= temperature <= 2.0 ** 20:
+        raise ValueError(f"the temperature is 2**-20 to 2**20, got {temperature}")
     device, temperature = x.device, float(temperature)
     _on_one_gpu(device, weight, teacher_logits, teacher_tokens)
     n, v = teacher_tokens.numel() // k, weight.shape[0]

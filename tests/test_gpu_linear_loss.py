@@ -701,3 +701,25 @@ def test_what_lists_add_keeps_its_digits(n, v, d, k, limit, monkeypatch):
         module.linear_distillation(a, b, teacher, given).backward()
         check_lists((a.grad, b.grad), x, w, tokens, q, torch.full((n,), 1.0 / int((~hole).sum()), dtype=torch.float64, device="cuda"))
     assert check_kernels()
+
+
+def test_coldest_and_hottest_teachers():
+    """The ends of the temperatures: at 2**-20 logits of +-300 are exponents of 4e8, which fp32 tells apart by 32; at 2**20 the loss, some units, is what a
+    few roundings leave of T^2 = 1e12: only its gradient is of use."""
+    from dfccl_b200.ops.loss import linear_distillation
+    n, v, d = 100, 600, 64
+    x, w, gen = problem(n, v, d, 3, spread=4.0)
+    t = torch.randint(0, v, (n, 3), generator=gen, device="cuda")
+    t[:, 1], t[:, 2] = (t[:, 0] + 1) % v, (t[:, 0] + 2) % v
+    teacher = torch.randn(n, 3, generator=gen, device="cuda")
+    for temp in (2.0 ** -20, 2.0 ** 20):
+        q = torch.softmax(teacher.double() / temp, dim=1)
+        loss, dz = reference(x, w, t, q, temp)
+        a = x.clone().requires_grad_(True)
+        rows = linear_distillation(a, w, teacher, t, temperature=temp, reduction="none")
+        rows.sum().backward()
+        err = 2 * temp * logit_error(x, w).amax(dim=1) + 2.0 ** -22 * 3 * temp * (x.double() @ w.double().t()).abs().amax(dim=1)
+        assert bool(((rows.detach().double() - loss).abs() <= err + LN * (loss.abs() + temp * temp)).all())
+        assert a.grad.isfinite().all()
+        if temp > 1:                                     # (at 2**-20 a logit's error is a thousand steps of an exponent)
+            assert (a.grad.double() - dz @ w.double()).norm() <= 2.0 ** -8 * (dz @ w.double()).norm() + temp * 2.0 ** -22 * 8 * w.double().norm() * n ** 0.5

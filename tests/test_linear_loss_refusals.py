@@ -218,3 +218,17 @@ def test_what_is_no_token():
     for good in (np.int64(3), 8):
         with pytest.raises(ValueError, match="GPU"):
             embedding(i(4), x(9, 16), padding_idx=good)
+
+
+@pytest.mark.parametrize("temperature", [1e-45, 1e-25, 1e-7, 2.0 ** -20 * 0.99, 2.0 ** 20 * 1.01, 1e20, 1e39])
+def test_temperatures_out_of_range(native, temperature):
+    """Whose square, inverse or exponents fp32 does not hold: an error, not NaN."""
+    from dfccl_b200.ops.loss import linear_distillation
+    with pytest.raises(ValueError, match="temperature"):
+        linear_distillation(x(4, 16), x(9, 16), x(4, 2), i(4, 2), temperature=temperature)
+    for ok in (2.0 ** -20, 2.0 ** 20):
+        with pytest.raises(ValueError, match="GPU"):
+            linear_distillation(x(4, 16), x(9, 16), x(4, 2), i(4, 2), temperature=ok)
+    L, p = native.lib(), 4096
+    assert L.dfcclTeacherRows(p, native.FLOAT32, p, 1, 4, 2, 9, temperature, p, p, p, None) == native.INVALID_ARGUMENT
+    assert L.dfcclLinearLossForward(p, p, 4, 9, 16, None, 0, 0, p, p, p, 2, temperature, 0, p, p, p, p, None, None, None) == native.INVALID_ARGUMENT
