@@ -224,9 +224,11 @@ __global__ void __launch_bounds__(1024) joinRowsKernel(const JoinArgs a) {
         for (int i = lane; i < a.rows.k; i += 32) {
           const float q = a.rows.targets || tokenAt(i) == VOCAB_NO_TOKEN ? 1.f : weightAt(i);
           if (q != 0.f) sum += q * logf(q);             // (of entries that share the token)
-          a.rest[list + i] = i ? 0.f : others.y * exp2f(others.x - l);
+          a.rest[list + i] = 0.f;
         }
-        sum = warpSum(sum) + (ratio < 1e30f ? log1pf(ratio) : (l - u) * LN2);
+        sum = warpSum(sum);
+        if (lane == 0) a.rest[list] = sum != sum ? sum : others.y * exp2f(others.x - l);      // (the teacher's weights are not numbers)
+        sum += (ratio < 1e30f ? log1pf(ratio) : (l - u) * LN2);
       } else {
         for (int i = lane; i < a.rows.k; i += 32) {
           float rest = 0.f;

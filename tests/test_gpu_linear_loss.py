@@ -723,3 +723,23 @@ def test_coldest_and_hottest_teachers():
         assert a.grad.isfinite().all()
         if temp > 1:                                     # (at 2**-20 a logit's error is a thousand steps of an exponent)
             assert (a.grad.double() - dz @ w.double()).norm() <= 2.0 ** -8 * (dz @ w.double()).norm() + temp * 2.0 ** -22 * 8 * w.double().norm() * n ** 0.5
+
+
+@pytest.mark.parametrize("one_go", [False, True])
+@pytest.mark.parametrize("odd", [float("nan"), float("inf")])
+@pytest.mark.parametrize("k", [1, 2, 3])
+def test_a_teacher_that_is_no_number(k, odd, one_go, monkeypatch):
+    """Weights of NaN make their row's loss and gradient NaN, of one token as of several, and no other row's."""
+    from dfccl_b200.ops import loss as module
+    monkeypatch.setattr(module, "ONE_GO_FROM", 0 if one_go else 1 << 60)
+    n, v, d = 40, 300, 64
+    x, w, gen = problem(n, v, d, 83)
+    t = torch.randint(0, v, (n, 1), generator=gen, device="cuda")
+    t = torch.cat([t, t, (t + 1) % v], dim=1)[:, :k]        # (twice the same token, and another)
+    teacher = torch.randn(n, k, generator=gen, device="cuda")
+    teacher[7, 0] = odd
+    a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    assert module.linear_distillation(a, b, teacher, t, reduction="none").isnan().nonzero()[:, 0].tolist() == [7]
+    module.linear_distillation(a, b, teacher, t, reduction="sum").backward()
+    assert a.grad.isnan().all(dim=1).nonzero()[:, 0].tolist() == [7] and int(a.grad.isnan().sum()) == d
+    assert sorted(b.grad.isnan().all(dim=1).nonzero()[:, 0].tolist()) == sorted(set(t[7].tolist()))
