@@ -487,21 +487,34 @@ ncclResult_t makeMap(CUtensorMap* m, const void* base, uint64_t rows, uint64_t c
 std::atomic<int> g_reservedSms{0};
 
 struct ErrWords { uint32_t* dev = nullptr; volatile uint32_t* host = nullptr; };
-ErrWords errWords() {                       // one pair per device, created on first use
+// One pair per device, created on first use: also where that is a launch that is being captured (a relaxed capture mode, a stream of their own).
+ncclResult_t errWords(ErrWords* out) {
   static ErrWords w[64];
   static std::mutex mu;
   int dev = 0;
-  cudaGetDevice(&dev);
+  CUDACHECK(cudaGetDevice(&dev));
+  if (dev >= 64) return ncclInvalidUsage;
   std::lock_guard<std::mutex> l(mu);
-  if (!w[dev].dev) {
-    cudaMalloc((void**)&w[dev].dev, 4);
-    cudaMemset(w[dev].dev, 0, 4);
-    uint32_t* h = nullptr;
-    cudaHostAlloc((void**)&h, 4, cudaHostAllocMapped | cudaHostAllocPortable);
+  if (!w[dev].host) {
+    uint32_t *d = nullptr, *h = nullptr;
+    cudaStream_t s = nullptr;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    CUDACHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    cudaError_t e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMalloc((void**)&d, 4);
+    if (e == cudaSuccess) e = cudaMemsetAsync(d, 0, 4, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (e == cudaSuccess) e = cudaHostAlloc((void**)&h, 4, cudaHostAllocMapped | cudaHostAllocPortable);
+    if (s) cudaStreamDestroy(s);
+    if (e != cudaSuccess && d) cudaFree(d);
+    (void)cudaThreadExchangeStreamCaptureMode(&mode);
+    CUDACHECK(e);
     *h = 0;
+    w[dev].dev = d;
     w[dev].host = h;
   }
-  return w[dev];
+  *out = w[dev];
+  return ncclSuccess;
 }
 
 ncclResult_t launch(const void* A, const void* B, void* C, int M, int N, int K, const FusedArgs* f, cudaStream_t stream,
@@ -511,7 +524,8 @@ ncclResult_t launch(const void* A, const void* B, void* C, int M, int N, int K, 
     return ncclInvalidArgument;
   }
   if (((uintptr_t)A | (uintptr_t)B | (uintptr_t)C) & 15) return ncclInvalidArgument;
-  const ErrWords ew = errWords();
+  ErrWords ew;
+  DFCHECK(errWords(&ew));
   if (*ew.host) { DF_WARN("an earlier tensor-core kernel on this device gave up on a bounded wait; call dfcclGemmCheck to clear"); return dfcclTimeout; }
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
@@ -560,7 +574,8 @@ ncclResult_t gemmEncodeMap3(CUtensorMap* m, const void* base, uint64_t rows, uin
   return encodeMap(m, map3Key(base, rows, k, mnMajor, boxRows, boxK));
 }
 ncclResult_t gemmErrorWords(uint32_t** dev, uint32_t** host) {
-  const ErrWords ew = errWords();
+  ErrWords ew;
+  DFCHECK(errWords(&ew));
   if (*ew.host) { DF_WARN("an earlier tensor-core kernel on this device gave up on a bounded wait; call dfcclGemmCheck to clear"); return dfcclTimeout; }
   *dev = ew.dev; *host = (uint32_t*)ew.host;
   return ncclSuccess;
@@ -568,7 +583,7 @@ ncclResult_t gemmErrorWords(uint32_t** dev, uint32_t** host) {
 ncclResult_t gemmLaunch(const void* A, const void* B, void* C, int M, int N, int K, const FusedArgs* f, cudaStream_t stream, int aMn, int bMn) {
   return launch(A, B, C, M, N, K, f, stream, aMn, bMn);
 }
-bool gemmGaveUp() { return *errWords().host != 0; }
+bool gemmGaveUp() { ErrWords ew; return errWords(&ew) == ncclSuccess && *ew.host != 0; }
 void gemmReserveSmsAtLeast(int n) {
   int cur = g_reservedSms.load();
   while (cur < n && !g_reservedSms.compare_exchange_weak(cur, n)) {}
@@ -638,7 +653,8 @@ DF_API ncclResult_t dfcclGemmReserveSms(int n) {
 // Non-zero after a kernel of this file gave up on a bounded wait (reads and clears the word).
 DF_API ncclResult_t dfcclGemmCheck(int* failed) {
   uint32_t v = 0;
-  const ErrWords ew = errWords();
+  ErrWords ew;
+  DFCHECK(errWords(&ew));
   CUDACHECK(cudaMemcpy(&v, ew.dev, 4, cudaMemcpyDeviceToHost));
   if (v) { CUDACHECK(cudaMemset(ew.dev, 0, 4)); *ew.host = 0; }
   if (failed) *failed = (int)v;

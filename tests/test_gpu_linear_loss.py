@@ -743,3 +743,38 @@ def test_a_teacher_that_is_no_number(k, odd, one_go, monkeypatch):
     module.linear_distillation(a, b, teacher, t, reduction="sum").backward()
     assert a.grad.isnan().all(dim=1).nonzero()[:, 0].tolist() == [7] and int(a.grad.isnan().sum()) == d
     assert sorted(b.grad.isnan().all(dim=1).nonzero()[:, 0].tolist()) == sorted(set(t[7].tolist()))
+
+
+@pytest.mark.parametrize("first", ["targets", "targets, one go", "lists", "lists, one go", "embedding", "gradient of x alone"])
+def test_first_calls_of_a_process_are_captured(first):
+    """Nothing of this package has run before the capture: what it makes once per device is made beside it."""
+    code = f"""
+import torch
+from dfccl_b200.ops import loss as module
+from dfccl_b200.ops.embedding import embedding
+from dfccl_b200.ops.gemm import check_kernels
+first = {first!r}
+module.ONE_GO_FROM = 0 if "one go" in first else 1 << 60
+gen = torch.Generator(device="cuda").manual_seed(1)
+x, w = torch.randn(50, 64, generator=gen, device="cuda").to(torch.bfloat16), torch.randn(300, 64, generator=gen, device="cuda").to(torch.bfloat16)
+t, teacher = torch.randint(0, 300, (50, 3), generator=gen, device="cuda"), torch.randn(50, 3, generator=gen, device="cuda")
+leaves = [x.requires_grad_(True)] + ([w] if "alone" in first else [w.requires_grad_(True)])
+
+def step():
+    if first == "embedding":
+        out = embedding(t, w)
+        return (out.detach(),) + torch.autograd.grad(out, [w], torch.ones_like(out))
+    out = module.linear_distillation(x, w, teacher, t) if "lists" in first else module.linear_cross_entropy(x, w, t[:, 0])
+    return (out.detach(),) + torch.autograd.grad(out, [a for a in leaves if a.requires_grad])
+
+graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+with torch.cuda.graph(graph, stream=side):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+for a, b in zip(got, step()):
+    assert torch.equal(a, b)
+assert check_kernels()
+"""
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=pathlib.Path(__file__).parents[1])
+    assert run.returncode == 0, run.stderr[-2000:]
