@@ -213,7 +213,7 @@ def main(argv=None):
                "model_tflops_per_gpu": flops / (ms / 1e3) / 1e12 / w,
                "config": {"model": f"GPT-2 {a.model}", "parallelism": f"tp{a.tp} x pp{a.pp} x dp{a.dp}", "micro_batch": a.micro_batch,
                           "n_micro": a.n_micro, "global_batch": a.dp * a.n_micro * a.micro_batch, "seq_len": cfg.seq_len, "cuda_graph": bool(a.graph),
-                          "fused_ends": stage.fused_ends,
+                          "fused_ends": stage.ran_fused_ends,
                           "schedule": "1F1B, receives posted one micro-batch ahead" if tr.schedule == "1f1b" else "GPipe",
                           "pipeline_link_ctas": hyb.PP_CTAS, "optimizer": "SGD momentum 0.9, fp32 master weights" if a.impl == "dfccl" else "SGD momentum 0.9 (bf16)"},
                "clocks": clk.summary(),

@@ -106,6 +106,7 @@ class GPT2Stage(nn.Module):
         super().__init__()
         assert cfg.n_layer % n_stages == 0
         self.cfg, self.tp, self.fused_ends = cfg, tp, fused_ends
+        self._ends: dict = {}                            # of this stage: whether the last pass ran them on this package's kernels
         self.is_first, self.is_last = stage == 0, stage == n_stages - 1
         self.tokens = micro_batch * cfg.seq_len
         self.rows = self.tokens // tp.n
@@ -127,6 +128,11 @@ class GPT2Stage(nn.Module):
             self.head = nn.Parameter(_full((cfg.vocab, d), cfg.init_std, seed + 9, dev).to(torch.bfloat16))
             self.head.tp_replicated = True
 
+    @property
+    def ran_fused_ends(self) -> bool:
+        """True if the last forward pass ran every end that this stage has (one at least) on this package's kernels."""
+        return bool(self._ends) and all(self._ends.values())
+
     def my_rows(self, flat: torch.Tensor) -> torch.Tensor:
         return flat[self.tp.rank * self.rows:(self.tp.rank + 1) * self.rows]
 
@@ -136,7 +142,8 @@ class GPT2Stage(nn.Module):
         to the micro-batch's loss); the others return their hidden rows."""
         if self.is_first:
             ids = self.my_rows(x.reshape(-1))
-            if self.fused_ends and ids.is_cuda and lookup_supported(self.wte, self.wpe):
+            self._ends["embedding"] = self.fused_ends and ids.is_cuda and lookup_supported(self.wte, self.wpe)
+            if self._ends["embedding"]:
                 h = embedding(ids, self.wte.weight, positions=self.pos, position_weight=self.wpe.weight)
             else:
                 h = self.wte(ids) + self.wpe(self.pos)
@@ -147,6 +154,7 @@ class GPT2Stage(nn.Module):
         if not self.is_last:
             return h
         y, mine = norm_residual(self.ln_f, h)[1], self.my_rows(targets.reshape(-1))
-        if self.fused_ends and linear_loss_supported(y, self.head):
+        self._ends["loss"] = self.fused_ends and linear_loss_supported(y, self.head)
+        if self._ends["loss"]:
             return linear_cross_entropy(y, self.head, mine, reduction="sum") / self.tokens
         return F.cross_entropy((y @ self.head.t()).float(), mine, reduction="sum") / self.tokens

@@ -778,3 +778,21 @@ assert check_kernels()
 """
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=pathlib.Path(__file__).parents[1])
     assert run.returncode == 0, run.stderr[-2000:]
+
+
+def test_a_stage_says_what_ran(monkeypatch):
+    """Asked for is not run: a head that the loss does not take (its width, its type) leaves the stage's loss to the framework."""
+    from dfccl_b200 import native as nv
+    from dfccl_b200.models import gpt2
+    from dfccl_b200.ops.fused_linear import TpGroup
+    (comm,) = nv.Comm.init_loopback(1, torch.cuda.current_device())
+    tp = TpGroup(comm, None, torch.device("cuda", torch.cuda.current_device()))
+    tokens = torch.randint(0, 300, (2, 129), device="cuda")
+    for fused, typed, want in ((False, torch.bfloat16, False), (True, torch.bfloat16, True), (True, torch.float32, False)):
+        stage = gpt2.GPT2Stage(gpt2.GPT2Config(n_layer=1, d_model=256, n_head=4, seq_len=128, vocab=300), tp, 0, 1, 2, fused_ends=fused)
+        assert not stage.ran_fused_ends
+        if typed != torch.bfloat16:
+            stage.head = torch.nn.Parameter(stage.head.detach().float())
+            monkeypatch.setattr(gpt2, "norm_residual", lambda ln, x: (x, ln(x).float()))
+        assert stage(tokens[:, :-1], tokens[:, 1:]).isfinite().item() and stage.ran_fused_ends == want
+    comm.destroy()
