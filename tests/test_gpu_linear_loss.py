@@ -796,3 +796,91 @@ def test_a_stage_says_what_ran(monkeypatch):
             monkeypatch.setattr(gpt2, "norm_residual", lambda ln, x: (x, ln(x).float()))
         assert stage(tokens[:, :-1], tokens[:, 1:]).isfinite().item() and stage.ran_fused_ends == want
     comm.destroy()
+
+
+# more targets than ownSumsKernel takes: sums by sorted tokens, in pieces of the vocabulary; with dw cut into slices (few tiles, long
+# contraction) and without (many tiles)
+@pytest.mark.parametrize("narrow", [False, True])
+@pytest.mark.parametrize("n,v,d,limit", [(6000, 700, 64, 1 << 20), (2500, 9001, 520, 8 << 20), (2100, 20003, 1024, 16 << 20), (4500, 1300, 128, 3 << 20)])
+def test_pieces_of_the_vocabulary_by_sorted_targets(n, v, d, limit, narrow, monkeypatch):
+    """As test_pieces_of_the_vocabulary, for targets of 64 and of 32 bits and an ignored token of the vocabulary's own."""
+    from dfccl_b200.ops import loss as module
+    from dfccl_b200.ops.gemm import check_kernels
+    monkeypatch.setattr(module, "ONE_GO_FROM", 1 << 60)
+    monkeypatch.setenv("DFCCL_LOSS_WORKSPACE_BYTES", str(limit))
+    x, w, gen = problem(n, v, d, n + v + d)
+    t = (torch.rand(n, generator=gen, device="cuda") ** 3 * v).long().clamp_(max=v - 1)
+    ignored = int(t.mode().values)
+    keep = t != ignored
+    assert n - int(keep.sum()) > 20 and not bool((t[keep] == ignored).any())
+    loss, dz = reference(x, w, t[:, None], keep.double()[:, None], 1.0)
+    gout = torch.randn(n, generator=gen, device="cuda")
+    targets = t.int() if narrow else t
+    for want_x, want_w in ((True, True), (True, False), (False, True)):
+        a, b = x.clone().requires_grad_(want_x), w.clone().requires_grad_(want_w)
+        rows = module.linear_cross_entropy(a, b, targets, ignore_index=ignored, reduction="none")
+        check_loss(rows.detach(), loss, x, w, 1.0)
+        assert bool((rows.detach()[~keep] == 0).all())
+        rows.backward(gout)
+        check_gradients((a.grad, b.grad), x, w, dz, gout.double(), 1.0)
+        assert not want_x or bool((a.grad[~keep] == 0).all())
+        a.grad = b.grad = None
+        module.linear_cross_entropy(a, b, targets, ignore_index=ignored, reduction="sum").backward()
+        check_gradients((a.grad, b.grad), x, w, dz, torch.ones(n, dtype=torch.float64, device="cuda"), 1.0)
+        assert not want_w or bool((b.grad[ignored] != 0).any())          # (the other rows' probabilities of it)
+    assert check_kernels()
+
+
+@pytest.mark.parametrize("limit", [1 << 20, 1 << 30])
+@pytest.mark.parametrize("one_go", [False, True])
+@pytest.mark.parametrize("n,v,d", [(40, 300, 64), (700, 3001, 136), (3000, 700, 72)])
+def test_narrow_targets_and_an_ignored_token_of_the_vocabulary(n, v, d, one_go, limit, monkeypatch):
+    """Targets of 32 bits give what those of 64 give, in every piece; a token that is ignored has its share of the others' rows."""
+    from dfccl_b200.ops import loss as module
+    monkeypatch.setattr(module, "ONE_GO_FROM", 0 if one_go else 1 << 60)
+    monkeypatch.setenv("DFCCL_LOSS_WORKSPACE_BYTES", str(limit))
+    x, w, gen = problem(n, v, d, 7 * n + v)
+    t = torch.randint(0, v, (n,), generator=gen, device="cuda")
+    t[::5] = 11
+    keep = t != 11
+    loss, dz = reference(x, w, t[:, None], keep.double()[:, None], 1.0)
+    results = []
+    for targets in (t, t.int()):
+        a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        value = module.linear_cross_entropy(a, b, targets, ignore_index=11)
+        value.backward()
+        count = int(keep.sum())
+        assert abs(value.item() - loss.sum().item() / count) <= 2 * logit_error(x, w).max().item() + 2 * LN * (1 + loss.abs().max().item())
+        check_gradients((a.grad, b.grad), x, w, dz, torch.full((n,), 1.0 / count, dtype=torch.float64, device="cuda"), 1.0, more=2.0 ** -8 * (1 + 2.0 ** -8) if one_go else 0.0)
+        assert bool((a.grad[~keep] == 0).all()) and bool((b.grad[11] != 0).any())
+        results.append((value.detach(), a.grad, b.grad))
+    assert all(torch.equal(p, q) for p, q in zip(*results))
+
+
+@pytest.mark.parametrize("one_go", [False, True])
+@pytest.mark.parametrize("lists", [False, True])
+def test_checkpointed_and_moved_to_the_host(lists, one_go, monkeypatch):
+    """Inside a checkpoint (the loss runs again in the backward pass), and with what the backward pass needs kept on the host."""
+    from torch.utils.checkpoint import checkpoint
+    from dfccl_b200.ops import loss as module
+    monkeypatch.setattr(module, "ONE_GO_FROM", 0 if one_go else 1 << 60)
+    x, w, gen = problem(300, 2001, 128, 91)
+    t = torch.randint(0, 2001, (300, 3), generator=gen, device="cuda")
+    teacher = torch.randn(300, 3, generator=gen, device="cuda")
+
+    def value(a, b):
+        return module.linear_distillation(a, b, teacher, t) if lists else module.linear_cross_entropy(a, b, t[:, 0])
+
+    def gradients(call):
+        a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        out = call(a, b)
+        out.backward()
+        return out.detach(), a.grad, b.grad
+
+    def on_host(a, b):
+        with torch.autograd.graph.save_on_cpu():
+            return value(a, b)
+
+    want = gradients(value)
+    for call in (lambda a, b: checkpoint(value, a, b, use_reentrant=False), lambda a, b: checkpoint(value, a, b, use_reentrant=True), on_host):
+        assert all(torch.equal(p, q) for p, q in zip(want, gradients(call)))
