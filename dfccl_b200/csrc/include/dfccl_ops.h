@@ -63,8 +63,8 @@ ncclResult_t dfcclOpsWarm(void);   /* load these kernels now (before any stream 
 ncclResult_t dfcclEmbeddingForward(const void* ids, int wideIds, int n, const void* w, int64_t rows, int64_t ldw, const void* positions, int widePositions,
                                    const void* p, int64_t prows, int64_t ldp, void* out, int d, int type, float scale, cudaStream_t stream);
 /* Gradients of the tables (contiguous, 16-byte aligned; either may be null) from that of `out`, g [n, d]: every row is written, rows
- * without tokens with zeros.  Tokens outside a table and tokens `padding` (-1: none) give no gradient.  Sums in fp32 in the order of the
- * tokens.  work: dfcclEmbeddingBackwardWork bytes, 32-byte aligned, for the number of tables that get a gradient. */
+ * without tokens with zeros.  Tokens outside a table and tokens `padding` (-1: none) give no gradient.  Sums in fp32, in the order of the
+ * tokens within stretches of them.  work: dfcclEmbeddingBackwardWork bytes, 32-byte aligned, for the number of tables that get a gradient. */
 ncclResult_t dfcclEmbeddingBackward(const void* g, int n, int d, int type, const void* ids, int wideIds, int64_t padding, float scale, void* gw, int64_t rows,
                                     const void* positions, int widePositions, void* gp, int64_t prows, void* work, cudaStream_t stream);
 size_t dfcclEmbeddingBackwardWork(int n, int d, int tables);

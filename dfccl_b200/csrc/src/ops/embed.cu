@@ -3,13 +3,14 @@
 //
 // Forward: a gather, bound by memory (or by its launch, for few tokens): 16 bytes per thread and access where rows allow it.  131072 tokens of
 // 1024 bf16 with positions: 60 us, 537 MB to and from L2 and 300 of DRAM; 8192: 6.7; one: 2.
-// Backward: dw[v] = scale sum over tokens with id v of g, in fp32, in the order of the tokens, rounded once.  Three launches:
-//   1. one cluster of eight blocks per table sorts (id, token) by id - a stable radix sort, eight bits a pass, whose counts meet in
+// Backward: dw[v] = scale sum over tokens with id v of g, in fp32, in the order of the tokens within a stretch of them, then of the stretches (by eight
+// warps where there are more than eight of them, each a share in its order), rounded once.  Four launches:
+//   1. and 2. one cluster of eight blocks per table sorts (id, token) by id - a stable radix sort, eight bits a pass, whose counts meet in
 //      distributed shared memory - while another launch clears the gradients, which is what the time goes into: most rows of a
 //      large table have no token (50257 x 1024 bf16: 17 us; the sort of 8192 tokens 15, of 131072 49);
-//   2. the sorted tokens in stretches: rows whose tokens lie inside one are summed and stored, others leave one or two sums (8192 x 1024 and
+//   3. the sorted tokens in stretches: rows whose tokens lie inside one are summed and stored, others leave one or two sums (8192 x 1024 and
 //      positions: 9 us; 131072: 90, 600 MB at 6.7 TB/s: g is read once per table);
-//   3. those are added up, stretch by stretch (8 us; 16).
+//   4. those are added up, stretch by stretch (8 us; 16).
 // No result is added to by atomics, so a call repeats itself bit by bit.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>

@@ -2,8 +2,9 @@
 // the logits z = x w^T: softmax cross entropy with a target per row, and distillation from a teacher's list of logits per row.
 // Both are a divergence from a distribution q over a row's list of entries (one entry of weight 1: a target),
 //     loss = T^2 sum_k q_k (ln q_k - ln p_k),   p = softmax(z / T),   dz = T g (p - q),
-// so both run on the same products (gemm/tcgen05_vocab.cu); here are the passes around them.  They move n (k + 1) words and, behind the
-// forward product, 8 bytes per row and stretch of 256 columns: microseconds beside the products'.
+// so both run on the same products (gemm/tcgen05_vocab.cu); here are the passes around them.  Behind the forward product they move 8 bytes per
+// row and stretch of 256 columns; for the lists a row of w per entry twice (their logits, what they add to dx) and one of x twice (what they add
+// to dw, its sums).  Beside targets that is microseconds; 8192 lists of 32 over 50257 x 1024 take 270 us of 1997.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -505,7 +506,7 @@ __global__ void __launch_bounds__(256) joinSlicesKernel(const float* part, int s
   for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < packs; i += (size_t)gridDim.x * 256) {
     float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-    for (int s = 0; s < slices; ++s) {                  // (eight on their way at a time: few rows leave few threads, and up to 49 slices)
+    for (int s = 0; s < slices; ++s) {                  // (eight on their way at a time: few rows leave few threads and many slices, 49 at 50257 columns)
       const float4* src = (const float4*)part + ((size_t)s * packs + i) * 2;
       const float4 x = src[0], y = src[1];
       f[0] += x.x; f[1] += x.y; f[2] += x.z; f[3] += x.w; f[4] += y.x; f[5] += y.y; f[6] += y.z; f[7] += y.w;
@@ -753,7 +754,8 @@ DF_API size_t dfcclLinearLossWithGradientsWork(int n, int v, int d, int k, int w
 // Per piece of rows: powers of the logits relative to the largest of the row's list (vocabPowers), their sums, x times the rows' shares, the two
 // products.  What the lists themselves add to the gradients does not go through bf16 (VocabExact).  Rows with a power that is too
 // large send their piece through statistics and powers once more, with the logarithms of the sums as bases: launches that find nothing
-// to do otherwise (2 us each).
+// to do otherwise (2 us each).  That is 10 n v d of such a piece, more than the 8 of gradients apart from the loss: 8192 x 50257 x 1024 1806 us without
+// such a row, 2919 with one, 2630 apart.  It takes a loss above 41.6 (60 ln 2), four times that of a uniform guess among 50257.
 DF_API ncclResult_t dfcclLinearLossWithGradients(const void* x, const void* w, int n, int v, int d, const void* targets, int wide, int64_t ignore, const void* tokens,
                                                  const void* weights, const void* state, int k, float temperature, int reduction, void* work, size_t workBytes,
                                                  void* lse, void* rest, void* loss, void* count, void* dx, void* dw, cudaStream_t stream) {

@@ -107,7 +107,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, po
 
     ``weight`` and ``position_weight`` (both or neither of the position arguments) are bf16, fp16 or fp32 of one type, ``ids``
     and ``positions`` int64 or int32 of one shape.  The gradients of both tables are dense; each row of them is the fp32 sum over
-    its tokens in their order, rounded once, the same in every run.  Tokens ``padding_idx`` give ``weight`` none.  There is no check of the
+    its tokens (in their order within stretches of 16 to 128, whose sums are added up behind that), rounded once, the same in every run.  Tokens ``padding_idx`` give ``weight`` none.  There is no check of the
     ids' values on the host: a token outside its table gives a row of NaN and no gradient of that table."""
     _index("ids", ids)
     _table("weight", weight)

@@ -185,14 +185,20 @@ def _loss(x, weight, rows, reduction):
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
-    """Softmax cross entropy of the logits ``x @ weight.T`` with ``targets``, in fp32; the logits are never stored.
+    """Softmax cross entropy of the logits ``x @ weight.T`` with ``targets``, in fp32; the logits are not stored.
 
     ``x`` [..., d] and ``weight`` [vocabulary, d] are bf16, d a multiple of 8; ``targets`` [...] int64 or int32.  Rows of target
     ``ignore_index`` have no loss and give no gradient, whatever ``x`` holds there; ``"mean"`` is over the other rows, and 0 where
     there is none.  Logits (up to 2**30 in size) and sums are fp32; the probabilities are rounded to bf16 on their way into the products that make the
     gradients of ``x`` and ``weight``, what the targets add to them is not.  They exist for as many columns or rows at a time as
-    ``DFCCL_LOSS_WORKSPACE_BYTES`` (1 GiB) hold.  Large reduced losses make their gradients with the loss and keep them until the
-    first backward pass.  There is no check of the targets' values on the host: one outside the vocabulary makes its row's loss and gradients NaN."""
+    ``DFCCL_LOSS_WORKSPACE_BYTES`` (1 GiB) hold, 256 at least; beside them sums in fp32 take up to 8 bytes an element of ``weight`` and 10 an
+    element of ``x``, and up to 0.2 GB (8192 rows over 128256 x 4096: 3.4 GB in all).
+
+    Large reduced losses make their gradients with the loss and keep them until the first backward pass, which multiplies them by the
+    gradient of the loss where that is not 1.  If it is no power of two, they are rounded to bf16 a second time there (1.7e-3 off in the
+    2-norm becomes 2.3e-3); small losses take it into the first rounding.  A row whose loss is above 41 makes such a pass half as long again.
+
+    There is no check of the targets' values on the host: one outside the vocabulary makes its row's loss and gradients NaN."""
     _check(x, weight, targets, "targets", reduction)
     if targets.shape != x.shape[:-1]:
         raise ValueError(f"targets of {tuple(targets.shape)} for x of {tuple(x.shape)}")

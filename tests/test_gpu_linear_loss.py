@@ -884,3 +884,18 @@ def test_checkpointed_and_moved_to_the_host(lists, one_go, monkeypatch):
     want = gradients(value)
     for call in (lambda a, b: checkpoint(value, a, b, use_reentrant=False), lambda a, b: checkpoint(value, a, b, use_reentrant=True), on_host):
         assert all(torch.equal(p, q) for p, q in zip(want, gradients(call)))
+
+
+@pytest.mark.parametrize("n,v,d,k", [(8192, 128256, 4096, 0), (8192, 128256, 4096, 32), (32768, 50257, 1024, 0), (8192, 50257, 1024, 32), (77, 50257, 768, 0), (100000, 512, 64, 8),
+                                     (3, 1000000, 8192, 0), (2000, 30011, 640, 17)])
+def test_workspaces_have_the_size_that_is_said(n, v, d, k, monkeypatch):
+    """The limit for the probabilities (256 rows or columns at least), 8 bytes an element of the head and 10 of x; beside that 24 bytes and a sixteenth of a row
+    an entry, and what does not grow: a few hundred slices of 256 x 256, some stretches of sorted tokens."""
+    from dfccl_b200 import native as nv
+    L, entries = nv.lib(), n * max(1, k)
+    for limit in (1 << 24, 1 << 30):
+        monkeypatch.setenv("DFCCL_LOSS_WORKSPACE_BYTES", str(limit))
+        least = 256 * 2 * max(v + 64, n)
+        most = max(limit, least) * 33 // 32 + 8 * v * d + 10 * n * d + entries * (24 + d // 16) + 2049 * 8 * d + 16 * n + 4 * v + 600 * 2 ** 18 + (1 << 14)
+        assert 0 < L.dfcclLinearLossWithGradientsWork(n, v, d, max(1, k), 1, 1) <= most
+        assert 0 < L.dfcclLinearLossBackwardWork(n, v, d, k, 1, 1) <= most
